@@ -301,6 +301,140 @@ int vgpu_flat_last_ms(const vgpu_flat *h, float *ms_gemm, float *ms_total);
  * exact either way). */
 int vgpu_flat_last_fallbacks(const vgpu_flat *h, uint32_t *queries);
 
+/* ---- attention memory -------------------------------------------------------
+ * The keys and values of a model's tokens, held in HBM in 8 bits with one scale
+ * for each block of tokens and head, and softmax attention over them.  No
+ * counterpart in the reference: it stands beside the indexes as the memory that
+ * a model reads exactly, and what leaves it can go into an index, which scores
+ * by the same inner product (flat metric 1).
+ *
+ * A cache has num_seqs sequences, each with the slots 0..len-1 for its tokens in
+ * the order they came.  Sequences take blocks of block_tokens slots from a common
+ * pool as they grow.  In every block each head's keys have one float32 scale, and
+ * so have its values; a slot stands for code * scale:
+ *   s = amax * (1 / Z), amax over the new elements of the block and head, Z = 127
+ *       or 448 for e4m3 (0 when amax < 2^-100), but never below what the block has:
+ *       when it grows, the codes there become round(code * (s_old / s));
+ *   code = round(clamp(x * (1 / s), -Z, Z)), ties to even (e4m3: the nearest
+ *       e4m3 number), every step in float32.
+ * A NaN or an infinity makes the block's scale of that head NaN, and so every
+ * slot of it: attention that sees one of these slots returns NaN, attention that
+ * does not is unaffected.
+ *
+ * All pointers marked "device" are device memory of the cache's device, which
+ * must be current; host arrays (seqs, counts, ...) are read before the call
+ * returns.  The calls queue their work on `stream` (a hipStream_t, NULL the
+ * device's default stream) and return without waiting; calls on one cache that
+ * use different streams are put in order by the caller.  Lengths are host state
+ * and change when the call returns.  Under stream capture the calls are
+ * VGPU_ERR_UNSUPPORTED: a graph would replay with the lengths of its recording. */
+typedef struct vgpu_kv vgpu_kv;
+
+#define VGPU_KV_INT8 0
+#define VGPU_KV_FP8 1 /* e4m3 without infinities */
+
+#define VGPU_F32 0
+#define VGPU_F16 1
+#define VGPU_BF16 2
+
+typedef struct vgpu_kv_params {
+    size_t num_seqs;     /* sequences the cache can hold */
+    size_t num_heads;    /* key/value heads */
+    size_t head_dim;     /* 1..256 */
+    size_t num_blocks;   /* blocks in the pool */
+    size_t block_tokens; /* 32, 64, 128 or 256 */
+    size_t max_blocks;   /* blocks one sequence may take; 0 = num_blocks */
+    int code;            /* VGPU_KV_INT8 or VGPU_KV_FP8 */
+} vgpu_kv_params;
+
+typedef struct vgpu_kv_info {
+    size_t free_blocks;
+    size_t device_bytes; /* HBM the cache and its workspaces hold */
+} vgpu_kv_info;
+
+/* A tensor [tokens, heads, dim] in device memory, strides in elements. */
+typedef struct vgpu_tensor3 {
+    const void *data;
+    int dtype; /* VGPU_F32, VGPU_F16 or VGPU_BF16 */
+    int64_t stride_token, stride_head, stride_dim;
+} vgpu_tensor3;
+
+/* Attention of one batch; see vgpu_kv_attend. */
+typedef struct vgpu_kv_query {
+    vgpu_tensor3 q;       /* [tokens, num_q_heads, head_dim] */
+    size_t num_q_heads;   /* a multiple of the cache's heads */
+    float scale;          /* of the products q.k */
+    int causal;
+    size_t window;        /* 0 = none */
+    const uint8_t *mask;  /* device [tokens, slots], 0 hides the slot; or NULL */
+    int64_t mask_stride_token, mask_stride_slot;
+    size_t mask_slots;    /* slots of a mask row: at least the longest sequence */
+    int track;            /* nonzero: update the accumulated weights */
+    float decay;
+    void *out;            /* device [tokens, num_q_heads, head_dim], q's dtype, contiguous */
+    float *lse;           /* device [tokens, num_q_heads], or NULL */
+} vgpu_kv_query;
+
+int vgpu_kv_new(const vgpu_kv_params *params, vgpu_kv **out);
+void vgpu_kv_free(vgpu_kv *h); /* waits for the device */
+int vgpu_kv_get_info(const vgpu_kv *h, vgpu_kv_info *out);
+/* Slots in use: lengths i64[num_seqs]. */
+int vgpu_kv_lengths(const vgpu_kv *h, int64_t *lengths);
+
+/* In every call below the batch is the n distinct sequences seqs[0..n) with
+ * counts[i] tokens each, which follow one another in the tensors. */
+
+/* Quantise new tokens into the cache, after the last slot of each sequence.
+ * k, v [tokens, num_heads, head_dim].  positions (device i32 [tokens, num_heads];
+ * NULL: the count of tokens appended to the sequence so far, those that truncate
+ * took back left out) and weights (device f32 [tokens, num_heads], NULL: 0) are
+ * kept beside each slot and head.  Without enough free blocks
+ * VGPU_ERR_OUT_OF_MEMORY, beyond max_blocks VGPU_ERR_INVALID_PARAMETER; nothing
+ * is appended then. */
+int vgpu_kv_append(vgpu_kv *h, const int32_t *seqs, const int64_t *counts, size_t n,
+                   const vgpu_tensor3 *k, const vgpu_tensor3 *v, const int32_t *positions,
+                   const float *weights, void *stream);
+
+/* softmax(scale * q.k) v over the cached slots, accumulated in float32.  Token i
+ * of sequence s (of counts[s], the last ones appended) stands at slot
+ * p = len - counts[s] + i.  It sees the slots j <= p (causal; else all of them),
+ * of them those with j > p - window (window != 0), of them those whose mask is
+ * not 0.  Query heads g*G..g*G+G-1 share the key/value head g.  A token that sees
+ * nothing gets 0, and -inf in lse (the natural logarithm of the softmax
+ * denominator).  track: weight[slot, head] = decay * weight + the sum of the
+ * probabilities that the slot got from the call's tokens and the heads that share
+ * it (decay 0: that sum alone). */
+int vgpu_kv_attend(vgpu_kv *h, const int32_t *seqs, const int64_t *counts, size_t n,
+                   const vgpu_kv_query *query, void *stream);
+
+/* Cut each sequence longer than `budget` down to it.  Every head keeps its last
+ * `recent` slots and those of largest weight among the others (a NaN counts as
+ * larger than any number; of equal weights the lower slot stays), in their order,
+ * with their positions and weights.  They are laid out in blocks anew: a block's
+ * scale is the largest of its slots' old scales and a code becomes
+ * round(code * (s_old / s)).  into (NULL: in place) names n other sequences, empty
+ * ones, that receive the result while seqs stay as they are.  Either way the new
+ * blocks come from the pool; in place the old ones return to it sequence by
+ * sequence.  Where they do not suffice VGPU_ERR_OUT_OF_MEMORY, and nothing is cut.
+ * What leaves, as values (each NULL, or for num_dropped slots per sequence and
+ * head, at least the longest sequence's len - budget; rows past a sequence's own
+ * are position -1 and zeros): positions i32 [n, num_dropped, num_heads], k and v
+ * f32 [n, num_dropped, num_heads, head_dim], all device memory. */
+int vgpu_kv_evict(vgpu_kv *h, const int32_t *seqs, const int32_t *into, size_t n, size_t budget,
+                  size_t recent, size_t num_dropped, int32_t *dropped_positions, float *dropped_k,
+                  float *dropped_v, void *stream);
+
+/* The slots first[i] .. first[i]+counts[i]-1 of each sequence: k, v [tokens,
+ * num_heads, head_dim] in dtype (code * scale, rounded once), positions i32 and
+ * weights f32 [tokens, num_heads]; device memory, each may be NULL. */
+int vgpu_kv_read(vgpu_kv *h, const int32_t *seqs, const int64_t *first, const int64_t *counts,
+                 size_t n, int dtype, void *k, void *v, int32_t *positions, float *weights,
+                 void *stream);
+
+/* Forget the slots from lengths[i] on (0 empties the sequence); blocks that hold
+ * nothing any more return to the pool.  A block keeps its scales. */
+int vgpu_kv_truncate(vgpu_kv *h, const int32_t *seqs, const int64_t *lengths, size_t n);
+
 /* ---- per-kernel test entry points (host buffers) -------------------------- */
 /* Host steps of the build, no device needed.  Inverted lists from list
  * labels (search.rs:624-657): offsets u64[L+1], list_ids u32[n]; a label >= L

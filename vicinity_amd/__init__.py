@@ -9,12 +9,14 @@ from .filtering import MetadataFilter
 from .file_searcher import IVFPQFileSearcher
 from .flat import FlatIndex
 from . import datagen
+from .kv_cache import KVCache
 from .ivf_pq import MISSING_DISTANCE, MISSING_LABEL, IVFPQIndex, default_codebooks
 
 __all__ = [
     "IVFPQIndex",
     "IVFPQFileSearcher",
     "FlatIndex",
+    "KVCache",
     "MetadataFilter",
     "MISSING_LABEL",
     "MISSING_DISTANCE",

@@ -91,6 +91,31 @@ class Stats(ctypes.Structure):
         return {name: getattr(self, name) for name, _ in self._fields_}
 
 
+class KvParams(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_size_t) for name in (
+        "num_seqs", "num_heads", "head_dim", "num_blocks", "block_tokens", "max_blocks")] + [
+        ("code", ctypes.c_int)]
+
+
+class KvInfo(ctypes.Structure):
+    _fields_ = [("free_blocks", ctypes.c_size_t), ("device_bytes", ctypes.c_size_t)]
+
+
+class KvTensor(ctypes.Structure):
+    """vgpu_tensor3: [tokens, heads, dim], strides in elements."""
+    _fields_ = [("data", ctypes.c_void_p), ("dtype", ctypes.c_int),
+                ("stride_token", ctypes.c_int64), ("stride_head", ctypes.c_int64),
+                ("stride_dim", ctypes.c_int64)]
+
+
+class KvQuery(ctypes.Structure):
+    _fields_ = [("q", KvTensor), ("num_q_heads", ctypes.c_size_t), ("scale", ctypes.c_float),
+                ("causal", ctypes.c_int), ("window", ctypes.c_size_t), ("mask", ctypes.c_void_p),
+                ("mask_stride_token", ctypes.c_int64), ("mask_stride_slot", ctypes.c_int64),
+                ("mask_slots", ctypes.c_size_t), ("track", ctypes.c_int),
+                ("decay", ctypes.c_float), ("out", ctypes.c_void_p), ("lse", ctypes.c_void_p)]
+
+
 _sz = ctypes.c_size_t
 _vp = ctypes.c_void_p
 _H = ctypes.c_void_p
@@ -145,6 +170,16 @@ SIGNATURES = {
     "vgpu_flat_search_batch_device": (_i, [_H, _vp, _sz, _sz, _sz, _vp, _vp, _vp]),
     "vgpu_flat_last_ms": (_i, [_H, ctypes.POINTER(ctypes.c_float), ctypes.POINTER(ctypes.c_float)]),
     "vgpu_flat_last_fallbacks": (_i, [_H, ctypes.POINTER(ctypes.c_uint32)]),
+    "vgpu_kv_new": (_i, [ctypes.POINTER(KvParams), ctypes.POINTER(_H)]),
+    "vgpu_kv_free": (None, [_H]),
+    "vgpu_kv_get_info": (_i, [_H, ctypes.POINTER(KvInfo)]),
+    "vgpu_kv_lengths": (_i, [_H, _vp]),
+    "vgpu_kv_append": (_i, [_H, _vp, _vp, _sz, ctypes.POINTER(KvTensor), ctypes.POINTER(KvTensor), _vp, _vp,
+                            _vp]),
+    "vgpu_kv_attend": (_i, [_H, _vp, _vp, _sz, ctypes.POINTER(KvQuery), _vp]),
+    "vgpu_kv_evict": (_i, [_H, _vp, _vp, _sz, _sz, _sz, _sz, _vp, _vp, _vp, _vp]),
+    "vgpu_kv_read": (_i, [_H, _vp, _vp, _vp, _sz, _i, _vp, _vp, _vp, _vp, _vp]),
+    "vgpu_kv_truncate": (_i, [_H, _vp, _vp, _sz]),
     "vgpu_test_host_lists": (_i, [_vp, _sz, _sz, _vp, _vp]),
     "vgpu_test_host_centroid_update": (_i, [_vp, _sz, _sz, _vp, _sz, _vp]),
     "vgpu_test_polar_factor": (_i, [_vp, _sz, _vp]),

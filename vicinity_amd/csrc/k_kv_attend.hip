@@ -1,0 +1,567 @@
+// Softmax attention over the 8-bit cache.
+//
+// For a row r (a query token and head) and slot j:  u_j = scale * log2(e) * q_r.k_j,
+// o = sum 2^(u_j) v_j / sum 2^(u_j).  One pass over the tiles with a running
+// reference m: the value scale s_b of a block goes into the exponent,
+// p_j = 2^(u_j + log2 s_b - m), so o's accumulators add p_j * code directly in the
+// matrix instruction and the denominator adds p_j / s_b.
+//
+// Products: codes are integers up to 127 or e4m3 numbers, both exact in half
+// precision.  A query row is scaled by a power of two to a largest element of 2^14
+// and split into 1 (bf16, f16: exact) or 2 (f32: 22 bits) halves, so the scores are
+// float32 sums of exact products.  p is rounded to half precision (2^-12) for 16-bit
+// results and to two halves for float32 ones; p is held near 2^6 .. 2^14 at the top,
+// so what is below 2^-30 of the largest rounds to zero.
+// m only moves when a score exceeds it by 2^8: a step that costs a scaling of the
+// accumulators, taken by a whole wave, nearly always in the first tile only.
+#include "vgpu_kv.h"
+#include "vgpu_launch.h"
+
+#include <hip/hip_bf16.h>
+
+namespace vgpu {
+
+namespace {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float KV_TOP = 6.f;    // p of the reference is 2^KV_TOP
+constexpr float KV_SLACK = 8.f;  // and may grow to 2^(KV_TOP + KV_SLACK)
+#define KV_NEG (-__builtin_huge_valf())
+
+// Two halves of 8 codes.
+template <int CODE>
+__device__ __forceinline__ half8 kv_half8(uint32_t w0, uint32_t w1) {
+    u32x4 r;
+    if (CODE == KV_INT8) {
+        // 1024 + (code + 128) by its bits, less 1152
+        const half2v off = {(_Float16)-1152.f, (_Float16)-1152.f};
+        const uint32_t magic = 0x64646464u;
+        r.x = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, __builtin_amdgcn_perm(magic, w0, 0x04010400u)) + off);
+        r.y = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, __builtin_amdgcn_perm(magic, w0, 0x04030402u)) + off);
+        r.z = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, __builtin_amdgcn_perm(magic, w1, 0x04010400u)) + off);
+        r.w = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, __builtin_amdgcn_perm(magic, w1, 0x04030402u)) + off);
+    } else {
+        r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.f, false));
+        r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.f, true));
+        r.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.f, false));
+        r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.f, true));
+    }
+    return __builtin_bit_cast(half8, r);
+}
+
+__device__ __forceinline__ float kv_load(const KvTensor& x, int64_t i) {
+    if (x.type == KV_F32) return ((const float*)x.p)[i];
+    if (x.type == KV_F16) return (float)((const _Float16*)x.p)[i];
+    return __uint_as_float((uint32_t)((const uint16_t*)x.p)[i] << 16);
+}
+
+__device__ __forceinline__ void kv_store(void* p, size_t i, float v, int type) {
+    if (type == KV_F32)
+        ((float*)p)[i] = v;
+    else if (type == KV_F16)
+        ((_Float16*)p)[i] = (_Float16)v;
+    else
+        ((__hip_bfloat16*)p)[i] = __float2bfloat16(v);
+}
+
+// Largest over the four lanes that hold one row's slots.
+__device__ __forceinline__ float kv_max4(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float kv_sum4(float v) {
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+
+// Slots lo .. hi - 1 that row `row` (of count * G) of a sequence may see.
+__device__ __forceinline__ void kv_range(const KvAttend& a, int len, int count, int row, int& lo, int& hi) {
+    const int p = len - count + row / a.G;  // its own slot
+    hi = a.causal ? max(p + 1, 0) : len;
+    lo = a.window ? max(p + 1 - a.window, 0) : 0;
+}
+
+// The running state of a wave: NC column tiles of 16 rows.
+template <int S, int CODE, int PARTS, int NC>
+struct KvWave {
+    half8 q[NC][PARTS][S];
+    float qs[NC];          // 2^-(the row's scaling) * scale * log2(e)
+    int lo[NC], hi[NC];    // slots that the row sees
+    int row[NC];
+    float m[NC], l[NC], bad[NC];
+    floatx4 o[NC][2 * S];
+};
+
+template <int S, int CODE, int PARTS, int NC>
+__device__ __forceinline__ void kv_load_rows(KvWave<S, CODE, PARTS, NC>& w, const KvDev& c, const KvBatch& b,
+                                             const KvAttend& a, int i, int h, int row0) {
+    const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+    const int rows = b.count[i] * a.G, len = b.len[i];
+#pragma unroll
+    for (int n = 0; n < NC; n++) {
+        const int row = row0 + n * 16 + col;
+        w.row[n] = row < rows ? row : -1;
+        w.lo[n] = 0, w.hi[n] = 0;  // rows past the end see nothing
+        w.m[n] = KV_NEG, w.l[n] = 0.f, w.bad[n] = 0.f;
+        float big = 0.f;
+        const int64_t base = row < rows ? (int64_t)(b.tok0[i] + row / a.G) * a.q.st + (int64_t)(h * a.G + row % a.G) * a.q.sh : 0;
+        if (row < rows) kv_range(a, len, b.count[i], row, w.lo[n], w.hi[n]);
+        float x[S][8];
+#pragma unroll
+        for (int s = 0; s < S; s++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int d = 32 * s + 8 * g + e;
+                x[s][e] = row < rows && d < c.D ? kv_load(a.q, base + d * a.q.sd) : 0.f;
+                big = fmaxf(big, fabsf(x[s][e]));
+            }
+        big = kv_max4(big);
+        int ex = 0;
+        if (big > 0.f && big < __builtin_huge_valf()) (void)frexpf(big, &ex), ex -= 15;
+        w.qs[n] = ldexpf(a.scale2, ex);
+#pragma unroll
+        for (int s = 0; s < S; s++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float y = ldexpf(x[s][e], -ex);
+                const _Float16 y0 = (_Float16)y;
+                w.q[n][0][s][e] = y0;
+                if (PARTS > 1) w.q[n][PARTS - 1][s][e] = (_Float16)(y - (float)y0);
+            }
+#pragma unroll
+        for (int j = 0; j < 2 * S; j++) w.o[n][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+}
+
+// One tile of 32 slots from `slot0` on; ks, vs: its block's scales; inside: every row
+// sees all of it.
+template <int S, int CODE, int PARTS, int NC>
+__device__ __forceinline__ void kv_tile_step(KvWave<S, CODE, PARTS, NC>& w, const uint4 (&kc)[S], const uint4 (&vc)[S],
+                                             float ks, float vs, int slot0, bool inside, const KvAttend& a,
+                                             int tok0, float* scores, int64_t score_row) {
+    const int lane = threadIdx.x & 63, g = lane >> 4;
+    floatx4 u[NC][2];
+#pragma unroll
+    for (int n = 0; n < NC; n++) u[n][0] = u[n][1] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int o = 0; o < 2 * S; o++) {
+        const uint4 r = kc[o >> 1];
+        const half8 k = o & 1 ? kv_half8<CODE>(r.z, r.w) : kv_half8<CODE>(r.x, r.y);
+#pragma unroll
+        for (int n = 0; n < NC; n++)
+#pragma unroll
+            for (int p = 0; p < PARTS; p++)
+                u[n][o / S] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, w.q[n][p][o % S], u[n][o / S], 0, 0, 0);
+    }
+    // A scale of 0 stands for codes of 0: any number does.  NaN is kept apart.
+    const float sv = vs > 0.f ? vs : 1.f;
+    const float lv = __log2f(sv);
+    const float rv = 1.f / sv;
+    half8 p0[NC], p1[NC];
+#pragma unroll
+    for (int n = 0; n < NC; n++) {
+        const float f = w.qs[n] * ks;
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = u[n][j >> 2][j & 3] * f;
+        if (!inside) {
+            bool any = false;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int slot = slot0 + (j >> 2) * 16 + 4 * g + (j & 3);
+                bool see = slot >= w.lo[n] && slot < w.hi[n];
+                if (see && a.mask) see = a.mask[(int64_t)(tok0 + w.row[n] / a.G) * a.mask_st + slot * a.mask_ss] != 0;
+                x[j] = see ? x[j] : KV_NEG;
+                any |= see;
+            }
+            if (vs != vs && any) w.bad[n] = vs;
+        } else if (vs != vs) {
+            w.bad[n] = vs;
+        }
+        if (scores && w.row[n] >= 0) {
+            float4* at = (float4*)(scores + (int64_t)w.row[n] * score_row + slot0);
+            at[g] = make_float4(x[0], x[1], x[2], x[3]);
+            at[4 + g] = make_float4(x[4], x[5], x[6], x[7]);
+        }
+        float top = KV_NEG;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            x[j] += lv;
+            top = fmaxf(top, x[j]);
+        }
+        if (__any(top > w.m[n] + KV_SLACK)) {
+            const float m1 = fmaxf(w.m[n], kv_max4(top));
+            const float f1 = w.m[n] == KV_NEG ? 0.f : exp2f(w.m[n] - m1);
+            w.m[n] = m1;
+            w.l[n] *= f1;
+#pragma unroll
+            for (int j = 0; j < 2 * S; j++) w.o[n][j] *= f1;
+        }
+        const float m = w.m[n] == KV_NEG ? 0.f : w.m[n] - KV_TOP;
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float p = __builtin_amdgcn_exp2f(x[j] - m);
+            sum += p;
+            const _Float16 ph = (_Float16)p;
+            p0[n][j] = ph;
+            if (PARTS > 1) p1[n][j] = (_Float16)(p - (float)ph);
+        }
+        w.l[n] += sum * rv;
+    }
+#pragma unroll
+    for (int o = 0; o < 2 * S; o++) {
+        const uint4 r = vc[o >> 1];
+        const half8 v = o & 1 ? kv_half8<CODE>(r.z, r.w) : kv_half8<CODE>(r.x, r.y);
+#pragma unroll
+        for (int n = 0; n < NC; n++) {
+            w.o[n][o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p0[n], w.o[n][o], 0, 0, 0);
+            if (PARTS > 1) w.o[n][o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p1[n], w.o[n][o], 0, 0, 0);
+        }
+    }
+}
+
+template <int S>
+__device__ __forceinline__ void kv_fetch(uint4 (&k)[S], uint4 (&v)[S], const uint8_t* tile) {
+    const uint4* p = (const uint4*)tile + (threadIdx.x & 63);
+#pragma unroll
+    for (int s = 0; s < S; s++) k[s] = p[s * 64];
+#pragma unroll
+    for (int s = 0; s < S; s++) v[s] = p[(S + s) * 64];
+}
+
+// What a part with reference m and sum l is multiplied with under reference mx.  A part
+// without a score has m -inf and l 0, or l NaN where its scores were NaN.
+__device__ __forceinline__ float kv_join_factor(float m, float l, float mx) {
+    return m == KV_NEG ? 0.f * l : exp2f(m - mx);
+}
+
+// A finished row: o / l and the logarithm.
+__device__ __forceinline__ void kv_finish(const KvDev& c, const KvBatch& b, const KvAttend& a, int i, int h, int row,
+                                          float m, float l, size_t& at) {
+    at = (size_t)(b.tok0[i] + row / a.G) * c.H * a.G + h * a.G + row % a.G;
+    const float lse2 = l == 0.f ? KV_NEG : m - KV_TOP + log2f(l);
+    if (a.lse) a.lse[at] = lse2 * 0.69314718055994531f;
+    if (a.lse2) a.lse2[at] = lse2;
+}
+
+// BY_ROWS: the four waves take 4 * NC * 16 rows and every tile; else the same NC * 16
+// rows and every fourth tile, joined at the end.
+template <int S, int CODE, int PARTS, int NC, bool BY_ROWS>
+__global__ __launch_bounds__(256, 2) void kv_attend_kernel(KvDev c, KvBatch b, KvAttend a) {
+    extern __shared__ __align__(16) float lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, g = lane >> 4;
+    const int h = blockIdx.x % c.H, split = blockIdx.x / c.H % a.splits, unit = blockIdx.x / c.H / a.splits;
+    const int i = kv_find(b, unit);
+    const int len = b.len[i], rows = b.count[i] * a.G;
+    const int wg_rows = 16 * NC * (BY_ROWS ? 4 : 1);
+    const int wg_row0 = (unit - b.unit0[i]) * wg_rows;
+    const int row0 = wg_row0 + (BY_ROWS ? wave * 16 * NC : 0);
+
+    // tiles that some row of the workgroup sees
+    int lo0, hi0, lo1, hi1;
+    kv_range(a, len, b.count[i], wg_row0, lo0, hi0);
+    kv_range(a, len, b.count[i], min(wg_row0 + wg_rows, rows) - 1, lo1, hi1);
+    const int first = lo0 / KV_TILE, last = (hi1 + KV_TILE - 1) / KV_TILE;
+    const int t0 = first + split * a.split_tiles, t1 = min(t0 + a.split_tiles, last);
+    if (split > 0 && t0 >= t1) return;
+    const bool whole = first + a.split_tiles >= last;  // no other split has tiles
+
+    KvWave<S, CODE, PARTS, NC> w;
+    kv_load_rows(w, c, b, a, i, h, row0);
+    // slots that every row of this wave sees, and those that any does
+    int all_lo = 0, all_hi = 0, any_lo = 0, any_hi = 0;
+    if (row0 < rows) {
+        kv_range(a, len, b.count[i], row0, any_lo, all_hi);
+        kv_range(a, len, b.count[i], min(row0 + 16 * NC, rows) - 1, all_lo, any_hi);
+    }
+    const int* table = c.table + (size_t)b.seq[i] * c.W;
+    const int step = BY_ROWS ? 1 : 4;
+    const int64_t score_row = (int64_t)((len + KV_TILE - 1) / KV_TILE) * KV_TILE;
+    float* scores = a.scores ? a.scores + (int64_t)b.aux[i] * KV_TILE * c.H + h * score_row * rows : nullptr;
+    const int per_block = c.shift - 5;
+    for (int t = t0 + (BY_ROWS ? 0 : wave); t < t1; t += step) {
+        if (BY_ROWS && (t * KV_TILE >= any_hi || (t + 1) * KV_TILE <= any_lo)) continue;
+        const int block = __builtin_amdgcn_readfirstlane(table[t >> per_block]);
+        const size_t part = (size_t)block * c.H + h;
+        uint4 kc[S], vc[S];
+        kv_fetch<S>(kc, vc, c.pool + kv_tile_offset(c, block, h, t & ((1 << per_block) - 1)));
+        const bool inside = t * KV_TILE >= all_lo && (t + 1) * KV_TILE <= all_hi && !a.mask;
+        kv_tile_step(w, kc, vc, c.kscale[part], c.vscale[part], t * KV_TILE, inside, a, b.tok0[i], scores, score_row);
+    }
+#pragma unroll
+    for (int n = 0; n < NC; n++) w.l[n] = kv_sum4(w.l[n]), w.bad[n] = kv_sum4(w.bad[n]);
+
+    if (BY_ROWS) {
+#pragma unroll
+        for (int n = 0; n < NC; n++) {
+            if (w.row[n] < 0) continue;
+            if (whole) {
+                size_t at;
+                kv_finish(c, b, a, i, h, w.row[n], w.m[n], w.l[n], at);
+                const float inv = w.l[n] == 0.f ? 0.f : 1.f / w.l[n];
+#pragma unroll
+                for (int j = 0; j < 2 * S; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int d = 16 * j + 4 * g + e;
+                        if (d < c.D) kv_store(a.out, at * c.D + d, w.o[n][j][e] * inv + w.bad[n], a.q.type);
+                    }
+            } else {
+                const size_t at = (size_t)blockIdx.x * wg_rows + (w.row[n] - wg_row0);
+                if (g == 0) a.part_ml[at] = make_float2(w.m[n], w.l[n]);
+#pragma unroll
+                for (int j = 0; j < 2 * S; j++) {
+                    const floatx4 v = w.o[n][j] + w.bad[n];
+                    *(floatx4*)(a.part_o + at * (32 * S) + 16 * j + 4 * g) = v;
+                }
+            }
+        }
+        return;
+    }
+
+    // join the four waves: rows of [wave][row][32 S + 4] floats, then (m, l, bad)
+    constexpr int LDO = 32 * S + 4;
+    float* ml = lds + 4 * 16 * NC * LDO;
+#pragma unroll
+    for (int n = 0; n < NC; n++) {
+        const int r = wave * 16 * NC + n * 16 + col;
+#pragma unroll
+        for (int j = 0; j < 2 * S; j++) *(floatx4*)(lds + r * LDO + 16 * j + 4 * g) = w.o[n][j] + w.bad[n];
+        if (g == 0) ml[2 * r] = w.m[n], ml[2 * r + 1] = w.l[n];
+    }
+    __syncthreads();
+    for (int u = threadIdx.x; u < 16 * NC * 8 * S; u += 256) {
+        const int r = u / (8 * S), d = u % (8 * S) * 4;
+        const int row = row0 + r;
+        if (row >= rows) break;
+        float mx = KV_NEG;
+#pragma unroll
+        for (int x = 0; x < 4; x++) mx = fmaxf(mx, ml[2 * (x * 16 * NC + r)]);
+        floatx4 o = {0.f, 0.f, 0.f, 0.f};
+        float l = 0.f;
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+            const int rr = x * 16 * NC + r;
+            const float m = ml[2 * rr];
+            const float f = kv_join_factor(m, ml[2 * rr + 1], mx);
+            l += f * ml[2 * rr + 1];
+            o += *(const floatx4*)(lds + rr * LDO + d) * f;
+        }
+        if (whole) {
+            size_t at;
+            if (d == 0)
+                kv_finish(c, b, a, i, h, row, mx, l, at);
+            else
+                at = (size_t)(b.tok0[i] + row / a.G) * c.H * a.G + h * a.G + row % a.G;
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (d + e < c.D) kv_store(a.out, at * c.D + d + e, o[e] * inv, a.q.type);
+        } else {
+            const size_t at = (size_t)blockIdx.x * wg_rows + r;
+            if (d == 0) a.part_ml[at] = make_float2(mx, l);
+            *(floatx4*)(a.part_o + at * (32 * S) + d) = o;
+        }
+    }
+}
+
+// Joins the splits of rows whose tiles went to several workgroups: a wave per row.
+__global__ __launch_bounds__(256) void kv_join_kernel(KvDev c, KvBatch b, KvAttend a, int wg_rows) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int groups = (wg_rows + 3) / 4;
+    const int h = blockIdx.x % c.H, rg = blockIdx.x / c.H % groups, unit = blockIdx.x / c.H / groups;
+    const int i = kv_find(b, unit);
+    const int rows = b.count[i] * a.G, wg_row0 = (unit - b.unit0[i]) * wg_rows;
+    const int r = rg * 4 + wave, row = wg_row0 + r;
+    if (r >= wg_rows || row >= rows) return;
+    int lo0, hi0, lo1, hi1;
+    kv_range(a, b.len[i], b.count[i], wg_row0, lo0, hi0);
+    kv_range(a, b.len[i], b.count[i], min(wg_row0 + wg_rows, rows) - 1, lo1, hi1);
+    const int tiles = (hi1 + KV_TILE - 1) / KV_TILE - lo0 / KV_TILE;
+    const int splits = (tiles + a.split_tiles - 1) / a.split_tiles;
+    if (splits <= 1) return;  // the one workgroup has written the row
+    const size_t stride = (size_t)c.H * wg_rows;
+    const size_t base = ((size_t)unit * a.splits * c.H + h) * wg_rows + r;
+    float mx = KV_NEG;
+    for (int s = 0; s < splits; s++) mx = fmaxf(mx, a.part_ml[base + s * stride].x);
+    float l = 0.f;
+    float o[KV_MAX_DIM / 64] = {};
+    for (int s = 0; s < splits; s++) {
+        const float2 ml = a.part_ml[base + s * stride];
+        const float f = kv_join_factor(ml.x, ml.y, mx);
+        l += f * ml.y;
+        const float* po = a.part_o + (base + s * stride) * c.Dp;
+#pragma unroll
+        for (int k = 0; k < KV_MAX_DIM / 64; k++)
+            if (k * 64 + lane < c.Dp) o[k] += f * po[k * 64 + lane];
+    }
+    size_t at;
+    kv_finish(c, b, a, i, h, row, mx, l, at);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int k = 0; k < KV_MAX_DIM / 64; k++)
+        if (k * 64 + lane < c.D) kv_store(a.out, at * c.D + k * 64 + lane, o[k] * inv, a.q.type);
+}
+
+// Weights from the kept scores of a step: a thread per slot.
+__global__ __launch_bounds__(256) void kv_score_weights_kernel(KvDev c, KvBatch b, KvAttend a) {
+    const int h = blockIdx.x % c.H, unit = blockIdx.x / c.H;
+    const int i = kv_find(b, unit);
+    const int slot = (unit - b.unit0[i]) * 256 + threadIdx.x;
+    const int len = b.len[i], rows = b.count[i] * a.G;
+    if (slot >= len) return;
+    const int64_t score_row = (int64_t)((len + KV_TILE - 1) / KV_TILE) * KV_TILE;
+    const float* scores = a.scores + (int64_t)b.aux[i] * KV_TILE * c.H + h * score_row * rows;
+    float sum = 0.f;
+    for (int r = 0; r < rows; r++) {
+        int lo, hi;
+        kv_range(a, len, b.count[i], r, lo, hi);
+        if (slot < lo || slot >= hi) continue;
+        const float lse = a.lse2[(size_t)(b.tok0[i] + r / a.G) * c.H * a.G + h * a.G + r % a.G];
+        if (lse == KV_NEG) continue;  // the mask hides every slot of the row
+        sum += exp2f(scores[(int64_t)r * score_row + slot] - lse);
+    }
+    const int block = c.table[(size_t)b.seq[i] * c.W + (slot >> c.shift)];
+    float* w = c.weights + ((size_t)block * c.H + h) * c.B + (slot & (c.B - 1));
+    *w = a.decay == 0.f ? sum : a.decay * *w + sum;
+}
+
+// Weights by a second pass over the keys: a wave per tile, every row of the head.
+template <int S, int CODE, int PARTS>
+__global__ __launch_bounds__(256) void kv_tile_weights_kernel(KvDev c, KvBatch b, KvAttend a) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, col = lane & 15;
+    const int h = blockIdx.x % c.H, unit = blockIdx.x / c.H;
+    const int i = kv_find(b, unit);
+    const int len = b.len[i], rows = b.count[i] * a.G;
+    const int t = (unit - b.unit0[i]) * 4 + wave;
+    if (t * KV_TILE >= len) return;
+    const int* table = c.table + (size_t)b.seq[i] * c.W;
+    const int per_block = c.shift - 5;
+    const int block = __builtin_amdgcn_readfirstlane(table[t >> per_block]);
+    const size_t part = (size_t)block * c.H + h;
+    const float ks = c.kscale[part];
+    const uint4* p = (const uint4*)(c.pool + kv_tile_offset(c, block, h, t & ((1 << per_block) - 1))) + lane;
+    half8 k[2 * S];
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+        const uint4 r = p[s * 64];
+        k[2 * s] = kv_half8<CODE>(r.x, r.y);
+        k[2 * s + 1] = kv_half8<CODE>(r.z, r.w);
+    }
+    floatx4 sum[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    for (int row0 = 0; row0 < rows; row0 += 16) {
+        int lo0, hi0, lo1, hi1;
+        kv_range(a, len, b.count[i], row0, lo0, hi0);
+        kv_range(a, len, b.count[i], min(row0 + 16, rows) - 1, lo1, hi1);
+        if (hi1 <= t * KV_TILE || lo0 >= (t + 1) * KV_TILE) continue;
+        KvWave<S, CODE, PARTS, 1> w;
+        kv_load_rows(w, c, b, a, i, h, row0);
+        const int row = row0 + col;
+        const float lse = row < rows ? a.lse2[(size_t)(b.tok0[i] + row / a.G) * c.H * a.G + h * a.G + row % a.G] : KV_NEG;
+        floatx4 u[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int o = 0; o < 2 * S; o++)
+#pragma unroll
+            for (int x = 0; x < PARTS; x++)
+                u[o / S] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[o], w.q[0][x][o % S], u[o / S], 0, 0, 0);
+        const float f = w.qs[0] * ks;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int slot = t * KV_TILE + (j >> 2) * 16 + 4 * g + (j & 3);
+            bool see = slot >= w.lo[0] && slot < w.hi[0] && lse != KV_NEG;
+            if (see && a.mask) see = a.mask[(int64_t)(b.tok0[i] + row / a.G) * a.mask_st + slot * a.mask_ss] != 0;
+            sum[j >> 2][j & 3] += see ? exp2f(u[j >> 2][j & 3] * f - lse) : 0.f;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        float v = sum[j >> 2][j & 3];
+#pragma unroll
+        for (int x = 1; x < 16; x <<= 1) v += __shfl_xor(v, x);
+        const int slot = t * KV_TILE + (j >> 2) * 16 + 4 * g + (j & 3);
+        if (col == j && slot < len) {
+            float* wt = c.weights + part * c.B + (slot & (c.B - 1));
+            *wt = a.decay == 0.f ? v : a.decay * *wt + v;
+        }
+    }
+}
+
+template <int S, int CODE, int PARTS, int NC, bool BY_ROWS>
+void attend_one(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s) {
+    const unsigned grid = (unsigned)b.unit0[b.n] * c.H * a.splits;
+    const size_t lds = BY_ROWS ? 0 : (size_t)4 * 16 * NC * (32 * S + 4 + 2) * 4;
+    const auto kernel = kv_attend_kernel<S, CODE, PARTS, NC, BY_ROWS>;
+    if (lds > 65536) ensure_dyn_lds((const void*)kernel, lds);
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), lds, s, c, b, a);
+}
+
+template <int S, int CODE, int PARTS>
+void attend_s(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s) {
+    if (a.by_rows && a.nc == 2)
+        attend_one<S, CODE, PARTS, (S <= 4 ? 2 : 1), true>(c, b, a, s);
+    else if (a.by_rows)
+        attend_one<S, CODE, PARTS, 1, true>(c, b, a, s);
+    else
+        attend_one<S, CODE, PARTS, 1, false>(c, b, a, s);
+}
+
+template <int S, int CODE, int PARTS>
+void weights_s(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s) {
+    hipLaunchKernelGGL((kv_tile_weights_kernel<S, CODE, PARTS>), dim3((unsigned)b.unit0[b.n] * c.H), dim3(256), 0, s, c, b, a);
+}
+
+template <int CODE, int PARTS, bool WEIGHTS>
+void by_dim(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s) {
+    switch (c.Dp / 32) {
+#define KV_CASE(S)                                  \
+    case S:                                         \
+        if (WEIGHTS)                                \
+            weights_s<S, CODE, PARTS>(c, b, a, s);  \
+        else                                        \
+            attend_s<S, CODE, PARTS>(c, b, a, s);   \
+        break;
+        KV_CASE(2)
+        KV_CASE(3)
+        KV_CASE(4)
+        KV_CASE(6)
+        KV_CASE(8)
+#undef KV_CASE
+    }
+}
+
+template <bool WEIGHTS>
+void by_type(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s) {
+    const bool two = a.q.type == KV_F32;
+    if (c.code == KV_INT8)
+        two ? by_dim<KV_INT8, 2, WEIGHTS>(c, b, a, s) : by_dim<KV_INT8, 1, WEIGHTS>(c, b, a, s);
+    else
+        two ? by_dim<KV_FP8, 2, WEIGHTS>(c, b, a, s) : by_dim<KV_FP8, 1, WEIGHTS>(c, b, a, s);
+}
+
+}  // namespace
+
+void launch_kv_attend(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s) {
+    if (!b.unit0[b.n]) return;
+    by_type<false>(c, b, a, s);
+    if (a.splits > 1) {
+        const int rows = kv_attend_rows(a);
+        hipLaunchKernelGGL(kv_join_kernel, dim3((unsigned)b.unit0[b.n] * c.H * ((rows + 3) / 4)), dim3(256), 0, s, c, b, a, rows);
+    }
+}
+
+void launch_kv_weights(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s) {
+    if (!b.unit0[b.n]) return;
+    if (a.scores)
+        hipLaunchKernelGGL(kv_score_weights_kernel, dim3((unsigned)b.unit0[b.n] * c.H), dim3(256), 0, s, c, b, a);
+    else
+        by_type<true>(c, b, a, s);
+}
+
+}  // namespace vgpu

@@ -14,12 +14,16 @@
 using vgpu::Error;
 using vgpu::FlatIndex;
 using vgpu::IvfpqIndex;
+using vgpu::KvCache;
 
 struct vgpu_ivfpq {
     IvfpqIndex* ix;
 };
 struct vgpu_flat {
     FlatIndex* fx;
+};
+struct vgpu_kv {
+    KvCache* kv;
 };
 
 namespace {
@@ -528,6 +532,84 @@ int vgpu_flat_last_fallbacks(const vgpu_flat* h, uint32_t* queries) {
         need(h && queries, VGPU_ERR_INVALID_PARAMETER, "null argument");
         std::lock_guard<std::mutex> lk(h->fx->mu);
         *queries = h->fx->fallbacks;
+    });
+}
+
+int vgpu_kv_new(const vgpu_kv_params* params, vgpu_kv** out) {
+    return guard([&] {
+        need(params && out, VGPU_ERR_INVALID_PARAMETER, "null argument");
+        *out = nullptr;
+        std::unique_ptr<KvCache> kv(new KvCache(*params));
+        *out = new vgpu_kv{kv.get()};
+        kv.release();
+    });
+}
+
+void vgpu_kv_free(vgpu_kv* h) {
+    if (!h) return;
+    delete h->kv;
+    delete h;
+}
+
+int vgpu_kv_get_info(const vgpu_kv* h, vgpu_kv_info* out) {
+    return guard([&] {
+        need(h && out, VGPU_ERR_INVALID_PARAMETER, "null argument");
+        std::lock_guard<std::mutex> lk(h->kv->mu);
+        out->free_blocks = h->kv->free_blocks.size();
+        out->device_bytes = h->kv->device_bytes();
+    });
+}
+
+int vgpu_kv_lengths(const vgpu_kv* h, int64_t* lengths) {
+    return guard([&] {
+        need(h && lengths, VGPU_ERR_INVALID_PARAMETER, "null argument");
+        std::lock_guard<std::mutex> lk(h->kv->mu);
+        for (size_t i = 0; i < h->kv->seqs.size(); i++) lengths[i] = h->kv->seqs[i].len;
+    });
+}
+
+int vgpu_kv_append(vgpu_kv* h, const int32_t* seqs, const int64_t* counts, size_t n, const vgpu_tensor3* k,
+                   const vgpu_tensor3* v, const int32_t* positions, const float* weights, void* stream) {
+    return guard([&] {
+        need(h && k && v && (n == 0 || (seqs && counts)), VGPU_ERR_INVALID_PARAMETER, "null argument");
+        std::lock_guard<std::mutex> lk(h->kv->mu);
+        h->kv->append(seqs, counts, n, *k, *v, positions, weights, (hipStream_t)stream);
+    });
+}
+
+int vgpu_kv_attend(vgpu_kv* h, const int32_t* seqs, const int64_t* counts, size_t n, const vgpu_kv_query* query,
+                   void* stream) {
+    return guard([&] {
+        need(h && query && (n == 0 || (seqs && counts)), VGPU_ERR_INVALID_PARAMETER, "null argument");
+        std::lock_guard<std::mutex> lk(h->kv->mu);
+        h->kv->attend(seqs, counts, n, *query, (hipStream_t)stream);
+    });
+}
+
+int vgpu_kv_evict(vgpu_kv* h, const int32_t* seqs, const int32_t* into, size_t n, size_t budget, size_t recent,
+                  size_t num_dropped, int32_t* dropped_positions, float* dropped_k, float* dropped_v, void* stream) {
+    return guard([&] {
+        need(h && (n == 0 || seqs), VGPU_ERR_INVALID_PARAMETER, "null argument");
+        std::lock_guard<std::mutex> lk(h->kv->mu);
+        h->kv->evict(seqs, into, n, budget, recent, num_dropped, dropped_positions, dropped_k, dropped_v,
+                     (hipStream_t)stream);
+    });
+}
+
+int vgpu_kv_read(vgpu_kv* h, const int32_t* seqs, const int64_t* first, const int64_t* counts, size_t n, int dtype,
+                 void* k, void* v, int32_t* positions, float* weights, void* stream) {
+    return guard([&] {
+        need(h && (n == 0 || (seqs && first && counts)), VGPU_ERR_INVALID_PARAMETER, "null argument");
+        std::lock_guard<std::mutex> lk(h->kv->mu);
+        h->kv->read(seqs, first, counts, n, dtype, k, v, positions, weights, (hipStream_t)stream);
+    });
+}
+
+int vgpu_kv_truncate(vgpu_kv* h, const int32_t* seqs, const int64_t* lengths, size_t n) {
+    return guard([&] {
+        need(h && (n == 0 || (seqs && lengths)), VGPU_ERR_INVALID_PARAMETER, "null argument");
+        std::lock_guard<std::mutex> lk(h->kv->mu);
+        h->kv->truncate(seqs, lengths, n);
     });
 }
 

@@ -1,0 +1,466 @@
+// The attention memory's host side: argument checks, blocks and lengths, and the
+// launches of one call.
+#include <algorithm>
+#include <climits>
+#include <cmath>
+
+#include "vgpu_runtime.h"
+
+namespace vgpu {
+
+namespace {
+
+void need(bool ok, const std::string& msg, int code = VGPU_ERR_INVALID_PARAMETER) {
+    if (!ok) throw Error(code, msg);
+}
+
+size_t item_size(int type) { return type == KV_F32 ? 4 : 2; }
+
+// Workgroups that a step is cut into: three for each of the 256 compute units, so
+// that sequences of different lengths even out.
+constexpr int64_t kStepWorkgroups = 768;
+// Bytes of partial results of one launch.
+constexpr int64_t kPartBytes = (int64_t)256 << 20;
+// Steps of at most this many rows per head keep their scores for the weights.
+constexpr int64_t kScoreRows = 64;
+
+// A workspace that grows in large steps.
+template <typename T>
+void grow(DevBuf<T>& b, size_t count) {
+    if (count > b.n) b.reserve(std::max(count, b.n + b.n / 2));
+}
+
+}  // namespace
+
+KvCache::KvCache(const vgpu_kv_params& p) : params(p) {
+    const auto cfg = [](bool ok, const char* msg) { need(ok, msg, VGPU_ERR_INVALID_CONFIG); };
+    cfg(p.num_seqs > 0 && p.num_seqs <= (1u << 24), "num_seqs must be in the range 1..=2^24");
+    cfg(p.num_heads > 0 && p.num_heads <= 4096, "num_heads must be in the range 1..=4096");
+    cfg(p.head_dim > 0 && p.head_dim <= (size_t)KV_MAX_DIM, "head_dim must be in the range 1..=256");
+    cfg(p.block_tokens == 32 || p.block_tokens == 64 || p.block_tokens == 128 || p.block_tokens == 256,
+        "block_tokens must be 32, 64, 128 or 256");
+    cfg(p.code == VGPU_KV_INT8 || p.code == VGPU_KV_FP8, "code must be 0 (int8) or 1 (fp8 e4m3)");
+    cfg(p.num_blocks > 0 && p.num_blocks <= (size_t)1 << 30, "num_blocks must be in the range 1..=2^30");
+    if (!params.max_blocks || params.max_blocks > p.num_blocks) params.max_blocks = p.num_blocks;
+    // slots and score rows of a sequence are 32-bit numbers
+    cfg(params.max_blocks <= (size_t)(INT_MAX / 2) / p.block_tokens, "a sequence's slots must stay below 2^30");
+    VGPU_HIP(hipGetDevice(&device));
+    dev.H = (int)p.num_heads;
+    dev.D = (int)p.head_dim;
+    // padded dimensions the kernels are compiled for
+    dev.Dp = dev.D <= 64 ? 64 : dev.D <= 96 ? 96 : dev.D <= 128 ? 128 : dev.D <= 192 ? 192 : 256;
+    dev.B = (int)p.block_tokens;
+    dev.shift = __builtin_ctz((unsigned)dev.B);
+    dev.W = (int)params.max_blocks;
+    dev.code = p.code;
+    const size_t parts = p.num_blocks * p.num_heads, slots = parts * p.block_tokens;
+    pool.reserve(slots * 2 * dev.Dp);
+    kscale.reserve(parts);
+    vscale.reserve(parts);
+    positions.reserve(slots);
+    weights.reserve(slots);
+    table.reserve(p.num_seqs * params.max_blocks);
+    dev.pool = pool.p, dev.kscale = kscale.p, dev.vscale = vscale.p;
+    dev.positions = positions.p, dev.weights = weights.p, dev.table = table.p;
+    seqs.resize(p.num_seqs);
+    seen.assign(p.num_seqs, 0);
+    free_blocks.resize(p.num_blocks);
+    for (size_t i = 0; i < p.num_blocks; i++) free_blocks[i] = (int)(p.num_blocks - 1 - i);
+}
+
+KvCache::~KvCache() {
+    // queued work still reads the buffers
+    int cur = device;
+    (void)hipGetDevice(&cur);
+    if (cur != device) (void)hipSetDevice(device);
+    (void)hipDeviceSynchronize();
+    if (cur != device) (void)hipSetDevice(cur);
+}
+
+size_t KvCache::device_bytes() const {
+    return pool.bytes() + kscale.bytes() + vscale.bytes() + weights.bytes() + positions.bytes() + table.bytes() +
+           table2.bytes() + w_kept.bytes() + w_gone.bytes() + w_part.bytes() + w_scores.bytes() + w_lse2.bytes() +
+           w_ml.bytes();
+}
+
+void KvCache::check_call(const int32_t* ids, size_t n, hipStream_t s) {
+    int cur = -1;
+    VGPU_HIP(hipGetDevice(&cur));
+    need(cur == device, "the cache's device (" + std::to_string(device) + ") must be current, not device " +
+                            std::to_string(cur));
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    VGPU_HIP(hipStreamIsCapturing(s, &st));
+    need(st == hipStreamCaptureStatusNone, "the cache's lengths cannot follow a captured stream", VGPU_ERR_UNSUPPORTED);
+    (void)ids, (void)n;
+}
+
+static void check_ids(const KvCache& c, std::vector<uint8_t>& seen, const int32_t* ids, size_t n) {
+    std::string bad;
+    size_t i = 0;
+    for (; i < n && bad.empty(); i++) {
+        if (ids[i] < 0 || (size_t)ids[i] >= c.seqs.size())
+            bad = "sequence " + std::to_string(ids[i]) + " out of range [0, " + std::to_string(c.seqs.size()) + ")";
+        else if (seen[ids[i]])
+            bad = "sequence " + std::to_string(ids[i]) + " appears twice in the batch";
+        else
+            seen[ids[i]] = 1;
+    }
+    for (size_t j = 0; j < i; j++)
+        if (ids[j] >= 0 && (size_t)ids[j] < c.seqs.size()) seen[ids[j]] = 0;
+    need(bad.empty(), bad);
+}
+
+KvTensor KvCache::tensor(const vgpu_tensor3& t, const char* name) const {
+    need(t.dtype == VGPU_F32 || t.dtype == VGPU_F16 || t.dtype == VGPU_BF16,
+         std::string(name) + ": dtype must be float32, float16 or bfloat16");
+    KvTensor x;
+    x.p = t.data;
+    x.type = t.dtype;
+    x.st = t.stride_token, x.sh = t.stride_head, x.sd = t.stride_dim;
+    const size_t item = item_size(t.dtype);
+    need((uintptr_t)t.data % item == 0, std::string(name) + ": data must be aligned to its dtype");
+    // 8 dims as one or two 16-byte loads
+    const int64_t unit = 16 / (int64_t)item;
+    x.vec = x.sd == 1 && dev.D % 8 == 0 && (uintptr_t)t.data % 16 == 0 && x.st % unit == 0 && x.sh % unit == 0;
+    return x;
+}
+
+void KvCache::take_blocks(std::vector<int>& out, size_t count, size_t row, int* tab, KvRuns& runs, hipStream_t s) {
+    for (size_t j = 0; j < count; j++) {
+        const int block = free_blocks.back();
+        const size_t at = row * (size_t)dev.W + out.size();
+        if (runs.n && runs.at[runs.n - 1] + runs.count[runs.n - 1] == at &&
+            runs.block[runs.n - 1] + runs.count[runs.n - 1] == block) {
+            runs.count[runs.n - 1]++;
+        } else {
+            if (runs.n == KvRuns::MAX) {
+                launch_kv_table(tab, runs, s);
+                runs.n = 0;
+            }
+            runs.at[runs.n] = at, runs.block[runs.n] = block, runs.count[runs.n] = 1;
+            runs.n++;
+        }
+        out.push_back(block);
+        free_blocks.pop_back();
+    }
+}
+
+void KvCache::release_blocks(std::vector<int>& blocks, size_t keep) {
+    while (blocks.size() > keep) {
+        free_blocks.push_back(blocks.back());
+        blocks.pop_back();
+    }
+}
+
+void KvCache::append(const int32_t* ids, const int64_t* counts, size_t n, const vgpu_tensor3& k, const vgpu_tensor3& v,
+                     const int32_t* pos, const float* wts, hipStream_t s) {
+    check_call(ids, n, s);
+    check_ids(*this, seen, ids, n);
+    need(k.dtype == v.dtype, "k and v must have the same dtype");
+    const KvTensor kt = tensor(k, "k"), vt = tensor(v, "v");
+    int64_t tokens = 0;
+    size_t want = 0;
+    for (size_t i = 0; i < n; i++) {
+        const Seq& q = seqs[ids[i]];
+        need(counts[i] >= 0 && counts[i] <= INT_MAX / 2, "counts must not be negative, nor above 2^30");
+        tokens += counts[i];
+        need(tokens <= INT_MAX / 2, "more than 2^30 tokens in one call");
+        const size_t total = blocks_of(q.len + counts[i]);
+        need(total <= (size_t)dev.W, "sequence " + std::to_string(ids[i]) + " would need " + std::to_string(total) +
+                                         " blocks, more than max_blocks (" + std::to_string(dev.W) + ")");
+        need(pos || q.next + counts[i] <= INT_MAX, "positions must stay below 2^31");
+        want += total - q.blocks.size();
+    }
+    need(!tokens || (k.data && v.data), "null argument");
+    need(want <= free_blocks.size(),
+         "the cache needs " + std::to_string(want) + " more blocks and has " + std::to_string(free_blocks.size()),
+         VGPU_ERR_OUT_OF_MEMORY);
+    for (size_t i = 0; i < n; i++) seqs[ids[i]].blocks.reserve(blocks_of(seqs[ids[i]].len + counts[i]));
+    KvRuns runs;
+    for (size_t i = 0; i < n; i++) {
+        Seq& q = seqs[ids[i]];
+        take_blocks(q.blocks, blocks_of(q.len + counts[i]) - q.blocks.size(), ids[i], table.p, runs, s);
+    }
+    launch_kv_table(table.p, runs, s);
+    int64_t tok = 0;
+    for (size_t i0 = 0; i0 < n; i0 += KV_BATCH) {
+        KvBatch b;
+        b.n = 0;
+        b.unit0[0] = 0;
+        for (size_t i = i0; i < std::min(n, i0 + KV_BATCH); i++) {
+            Seq& q = seqs[ids[i]];
+            const int j = b.n;
+            b.seq[j] = ids[i];
+            b.len[j] = (int)q.len;
+            b.tok0[j] = (int)tok;
+            b.count[j] = (int)counts[i];
+            b.aux[j] = (int)q.next;
+            // blocks that the new tokens enter
+            const int64_t first = q.len >> dev.shift;
+            b.unit0[j + 1] = b.unit0[j] + (counts[i] ? (int)((int64_t)blocks_of(q.len + counts[i]) - first) : 0);
+            b.n++;
+            tok += counts[i];
+            q.len += counts[i];
+            q.next += counts[i];
+        }
+        launch_kv_append(dev, b, kt, vt, pos, wts, s);
+    }
+    VGPU_HIP(hipGetLastError());
+}
+
+void KvCache::read(const int32_t* ids, const int64_t* first, const int64_t* counts, size_t n, int dtype, void* k,
+                   void* v, int32_t* pos, float* wts, hipStream_t s) {
+    check_call(ids, n, s);
+    check_ids(*this, seen, ids, n);
+    need(dtype == VGPU_F32 || dtype == VGPU_F16 || dtype == VGPU_BF16, "dtype must be float32, float16 or bfloat16");
+    int64_t tok = 0;
+    for (size_t i = 0; i < n; i++) {
+        need(first[i] >= 0 && counts[i] >= 0 && first[i] <= seqs[ids[i]].len && counts[i] <= seqs[ids[i]].len - first[i],
+             "slots outside sequence " + std::to_string(ids[i]) + " of length " + std::to_string(seqs[ids[i]].len));
+        tok += counts[i];
+        need(tok <= INT_MAX / 2, "more than 2^30 tokens in one call");
+    }
+    KvReadOut o;
+    o.k = k, o.v = v, o.positions = pos, o.weights = wts, o.type = dtype;
+    tok = 0;
+    for (size_t i0 = 0; i0 < n; i0 += KV_BATCH) {
+        KvBatch b;
+        b.n = 0;
+        b.unit0[0] = 0;
+        for (size_t i = i0; i < std::min(n, i0 + KV_BATCH); i++) {
+            const int j = b.n;
+            b.seq[j] = ids[i];
+            b.len[j] = (int)seqs[ids[i]].len;
+            b.tok0[j] = (int)tok;
+            b.count[j] = (int)counts[i];
+            b.aux[j] = (int)first[i];
+            const int64_t last = first[i] + counts[i];
+            b.unit0[j + 1] = b.unit0[j] + (counts[i] ? (int)((last + KV_TILE - 1) / KV_TILE - first[i] / KV_TILE) : 0);
+            b.n++;
+            tok += counts[i];
+        }
+        if (k || v || pos || wts) launch_kv_read(dev, b, o, s);
+    }
+    VGPU_HIP(hipGetLastError());
+}
+
+void KvCache::truncate(const int32_t* ids, const int64_t* lengths, size_t n) {
+    check_ids(*this, seen, ids, n);
+    for (size_t i = 0; i < n; i++)
+        need(lengths[i] >= 0 && lengths[i] <= seqs[ids[i]].len,
+             "length " + std::to_string(lengths[i]) + " outside sequence " + std::to_string(ids[i]) + " of length " +
+                 std::to_string(seqs[ids[i]].len));
+    for (size_t i = 0; i < n; i++) {
+        Seq& q = seqs[ids[i]];
+        q.next = lengths[i] ? q.next - (q.len - lengths[i]) : 0;
+        q.len = lengths[i];
+        release_blocks(q.blocks, blocks_of(q.len));
+    }
+}
+
+void KvCache::evict(const int32_t* ids, const int32_t* into, size_t n, size_t budget, size_t recent,
+                    size_t num_dropped, int32_t* dpos, float* dk, float* dv, hipStream_t s) {
+    check_call(ids, n, s);
+    check_ids(*this, seen, ids, n);
+    need(budget <= (size_t)INT_MAX / 2, "budget must not exceed 2^30");
+    need(recent <= budget, "recent must not exceed budget");
+    const bool drops = dpos || dk || dv;
+    need(!drops || num_dropped <= (size_t)INT_MAX / 2, "num_dropped must not exceed 2^30");
+    if (into) {
+        std::vector<int32_t> both(ids, ids + n);
+        both.insert(both.end(), into, into + n);
+        check_ids(*this, seen, both.data(), both.size());
+        for (size_t i = 0; i < n; i++)
+            need(seqs[into[i]].len == 0, "sequence " + std::to_string(into[i]) + " is not empty");
+    }
+    const auto stays = [&](size_t i) { return std::min<int64_t>(seqs[ids[i]].len, (int64_t)budget); };
+    // does the pool hold the new blocks, given what comes back on the way?
+    size_t have = free_blocks.size();
+    for (size_t i = 0; i < n; i++) {
+        const Seq& q = seqs[ids[i]];
+        need(!drops || q.len - stays(i) <= (int64_t)num_dropped,
+             "num_dropped is below what leaves sequence " + std::to_string(ids[i]));
+        if (!into && q.len <= (int64_t)budget) continue;
+        const size_t take = blocks_of(stays(i));
+        need(take <= have, "the cut sequences need " + std::to_string(take) + " free blocks and find " +
+                               std::to_string(have), VGPU_ERR_OUT_OF_MEMORY);
+        have -= take;
+        if (!into) have += q.blocks.size();
+    }
+    const int drop = drops ? (int)num_dropped : 0;
+    need((int64_t)dev.H * ((drop + 7) / 8) <= INT_MAX / KV_BATCH && (int64_t)n * drop <= INT_MAX,
+         "too many dropped slots in one call");
+    const size_t group = std::min<size_t>(n, KV_BATCH);
+    if (!into) table2.reserve(table.n);
+    grow(w_kept, group * dev.H * std::max<size_t>(budget, 1));
+    if (drop) grow(w_gone, group * dev.H * (size_t)drop);
+    std::vector<std::vector<int>> fresh(n);
+    for (size_t i = 0; i < n; i++) fresh[i].reserve(blocks_of(stays(i)));
+    if (into)
+        for (size_t i = 0; i < n; i++) seqs[into[i]].blocks.reserve(blocks_of(stays(i)));
+    else
+        free_blocks.reserve(params.num_blocks);
+
+    KvEvict e;
+    e.budget = (int)std::max<size_t>(budget, 1), e.recent = (int)recent, e.drop = drop;
+    e.kept = w_kept.p, e.gone = drop ? w_gone.p : nullptr;
+    e.dst = into ? table.p : table2.p;
+    e.dpos = dpos, e.dk = dk, e.dv = dv;
+    for (size_t i0 = 0; i0 < n;) {
+        KvBatch b;
+        KvRuns runs;
+        b.n = 0;
+        b.unit0[0] = 0;
+        size_t i = i0;
+        for (; i < n && b.n < KV_BATCH; i++) {
+            Seq& q = seqs[ids[i]];
+            const int64_t stay = stays(i);
+            const bool cut = into || q.len > stay;
+            const size_t take = cut ? blocks_of(stay) : 0;
+            if (take > free_blocks.size()) break;  // the blocks of those before come back first
+            const int j = b.n++;
+            b.seq[j] = ids[i];
+            b.len[j] = (int)q.len;
+            b.count[j] = (int)stay;
+            b.tok0[j] = (int)(i * (size_t)drop);
+            b.aux[j] = into ? into[i] : ids[i];
+            b.unit0[j + 1] = b.unit0[j] + (int)take;
+            take_blocks(fresh[i], take, b.aux[j], into ? table.p : table2.p, runs, s);
+        }
+        launch_kv_table(into ? table.p : table2.p, runs, s);
+        launch_kv_evict(dev, b, e, s);
+        // the sequences' new state
+        for (size_t x = i0; x < i; x++) {
+            Seq& q = seqs[ids[x]];
+            const int64_t stay = stays(x);
+            if (into) {
+                Seq& r = seqs[into[x]];
+                r.blocks.assign(fresh[x].begin(), fresh[x].end());
+                r.len = stay;
+                r.next = q.next;
+            } else if (q.len > stay) {
+                KvRuns back;
+                release_blocks(q.blocks, 0);
+                for (size_t y = 0; y < fresh[x].size(); y++) {
+                    const size_t at = (size_t)ids[x] * dev.W + y;
+                    if (back.n && back.block[back.n - 1] + back.count[back.n - 1] == fresh[x][y]) {
+                        back.count[back.n - 1]++;
+                    } else {
+                        if (back.n == KvRuns::MAX) {
+                            launch_kv_table(table.p, back, s);
+                            back.n = 0;
+                        }
+                        back.at[back.n] = at, back.block[back.n] = fresh[x][y], back.count[back.n] = 1;
+                        back.n++;
+                    }
+                }
+                launch_kv_table(table.p, back, s);
+                q.blocks.assign(fresh[x].begin(), fresh[x].end());
+                q.len = stay;
+            }
+        }
+        i0 = i;
+    }
+    VGPU_HIP(hipGetLastError());
+}
+
+void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const vgpu_kv_query& q, hipStream_t s) {
+    check_call(ids, n, s);
+    check_ids(*this, seen, ids, n);
+    need(q.num_q_heads > 0 && q.num_q_heads % (size_t)dev.H == 0 && q.num_q_heads <= 65536,
+         "num_q_heads must be a multiple of the cache's heads (" + std::to_string(dev.H) + ")");
+    need(std::isfinite(q.scale), "scale must be finite");
+    need(!q.track || std::isfinite(q.decay), "decay must be finite");
+    KvAttend a;
+    a.q = tensor(q.q, "q");
+    a.G = (int)(q.num_q_heads / (size_t)dev.H);
+    a.scale2 = q.scale * 1.44269504088896341f;
+    a.causal = q.causal != 0;
+    a.window = (int)std::min<size_t>(q.window, (size_t)INT_MAX / 2);
+    a.mask = q.mask;
+    a.mask_st = q.mask_stride_token, a.mask_ss = q.mask_stride_slot;
+    a.track = q.track != 0;
+    a.decay = q.decay;
+    a.out = q.out;
+    a.lse = q.lse;
+    int64_t tokens = 0, longest = 0, most = 0;
+    for (size_t i = 0; i < n; i++) {
+        need(counts[i] >= 0, "counts must not be negative");
+        tokens += counts[i];
+        need(tokens * (int64_t)q.num_q_heads <= INT_MAX / 2, "more than 2^30 query rows in one call");
+        longest = std::max(longest, seqs[ids[i]].len);
+        most = std::max(most, counts[i] * a.G);
+    }
+    need(!q.mask || (int64_t)q.mask_slots >= longest, "a mask row must cover the longest sequence (" +
+                                                          std::to_string(longest) + " slots)");
+    need(!tokens || (q.q.data && q.out), "null argument");
+    need((uintptr_t)q.out % item_size(a.q.type) == 0 && (uintptr_t)q.lse % 4 == 0, "outputs must be aligned to their dtype");
+
+    // Many rows: each wave has its own; few: the waves share them and split the tiles.
+    a.by_rows = most >= 64;
+    a.nc = a.by_rows && dev.Dp <= 128 ? 2 : 1;
+    const bool keep_scores = a.track && !a.by_rows && most <= kScoreRows;
+    if (a.track) {
+        grow(w_lse2, (size_t)tokens * q.num_q_heads);
+        a.lse2 = w_lse2.p;
+    }
+    const int rows = kv_attend_rows(a);
+    int64_t tok = 0;
+    for (size_t i0 = 0; i0 < n; i0 += KV_BATCH) {
+        KvBatch b;
+        b.n = 0;
+        b.unit0[0] = 0;
+        int64_t work = 0, score_tiles = 0, tiles_max = 1;
+        for (size_t i = i0; i < std::min(n, i0 + KV_BATCH); i++) {
+            const int64_t len = seqs[ids[i]].len;
+            const int j = b.n++;
+            b.seq[j] = ids[i];
+            b.len[j] = (int)len;
+            b.tok0[j] = (int)tok;
+            b.count[j] = (int)counts[i];
+            const int64_t units = (counts[i] * a.G + rows - 1) / rows;
+            need(b.unit0[j] + units <= INT_MAX / 2, "too many query rows in one call");
+            b.unit0[j + 1] = b.unit0[j] + (int)units;
+            tok += counts[i];
+            int64_t tiles = (len + KV_TILE - 1) / KV_TILE;
+            need(score_tiles <= INT_MAX / 2, "too many scores in one call");
+            b.aux[j] = (int)score_tiles;
+            if (keep_scores) score_tiles += tiles * counts[i] * a.G;
+            // tiles that a row tile can see
+            if (a.window && a.causal) tiles = std::min<int64_t>(tiles, (a.window + rows / a.G + 2 * KV_TILE) / KV_TILE + 1);
+            tiles_max = std::max(tiles_max, tiles);
+            work += units * dev.H * tiles;
+        }
+        if (b.unit0[b.n]) {
+            const int64_t units = (int64_t)b.unit0[b.n] * dev.H;
+            int64_t per = std::max<int64_t>((work + kStepWorkgroups - 1) / kStepWorkgroups, a.by_rows ? 16 : 8);
+            const int64_t row_bytes = (int64_t)dev.Dp * 4 + 8;
+            int64_t splits = (tiles_max + per - 1) / per;
+            splits = std::min(splits, std::max<int64_t>(kPartBytes / (units * rows * row_bytes), 1));
+            per = (tiles_max + splits - 1) / splits;
+            splits = (tiles_max + per - 1) / per;
+            need(units * splits <= INT_MAX / 64, "too many query rows in one call");
+            a.split_tiles = (int)per;
+            a.splits = (int)splits;
+            a.part_o = nullptr, a.part_ml = nullptr, a.scores = nullptr;
+            if (splits > 1) {
+                grow(w_part, (size_t)(units * splits * rows) * dev.Dp);
+                grow(w_ml, (size_t)(units * splits * rows));
+                a.part_o = w_part.p, a.part_ml = w_ml.p;
+            }
+            if (keep_scores) {
+                grow(w_scores, (size_t)score_tiles * KV_TILE * dev.H);
+                a.scores = w_scores.p;
+            }
+            launch_kv_attend(dev, b, a, s);
+        }
+        if (a.track) {
+            const int per = keep_scores ? 256 : 4 * KV_TILE;
+            for (int j = 0; j < b.n; j++) b.unit0[j + 1] = b.unit0[j] + (b.len[j] + per - 1) / per;
+            launch_kv_weights(dev, b, a, s);
+        }
+    }
+    VGPU_HIP(hipGetLastError());
+}
+
+}  // namespace vgpu

@@ -1,0 +1,153 @@
+// The attention memory's device layout and the launchers of its kernels.
+//
+// The pool is made of blocks of B slots; a block holds every head's part one
+// after the other, and a part is B / 32 tiles of 32 slots.  A tile is 32 * Dp
+// bytes of key codes, then 32 * Dp bytes of value codes (Dp: the head dimension
+// padded to 32), in the order in which the lanes of a wave take them as operands
+// of the 16x16x32 matrix instruction, so every load of the attention is 16
+// contiguous bytes per lane and no element changes lanes between the two products:
+//
+//   keys    operand (j, s) = slots 16 j .. 16 j + 15 x dims 32 s .. 32 s + 31;
+//           lane 16 g + r holds slot 16 j + r, dims 32 s + 8 g .. + 7.
+//   values  operand i = dims 16 i .. 16 i + 15 x the 32 slots;
+//           lane 16 g + r holds dim 16 i + r, slots 4 g .. 4 g + 3 and
+//           16 + 4 g .. 16 + 4 g + 3: the slots whose scores that lane gets from
+//           the key products j = 0 and j = 1.
+//
+// Operands 2 p and 2 p + 1 (keys: number j * Dp / 32 + s) share 16 bytes of a lane.
+// int8 codes are stored with 128 added; e4m3 codes as they are.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace vgpu {
+
+constexpr int KV_TILE = 32;
+constexpr int KV_MAX_DIM = 256;
+// sequences of one launch: their batch description is a kernel argument
+constexpr int KV_BATCH = 128;
+
+enum KvCode { KV_INT8 = 0, KV_FP8 = 1 };
+enum KvType { KV_F32 = 0, KV_F16 = 1, KV_BF16 = 2 };
+
+struct KvDev {
+    uint8_t* pool = nullptr;
+    float* kscale = nullptr;   // [block * H + head]
+    float* vscale = nullptr;
+    int* positions = nullptr;  // [(block * H + head) * B + slot]
+    float* weights = nullptr;
+    int* table = nullptr;      // [seq * W + i]: the block of the sequence's slots i * B ..
+    int H = 0, D = 0, Dp = 0, B = 0, W = 0;
+    int shift = 0;             // log2 B
+    int code = KV_INT8;
+};
+
+// n sequences of one launch.  Workgroups unit0[i] .. unit0[i + 1] - 1 (times what
+// the kernel multiplies them by) belong to sequence i.
+struct KvBatch {
+    int n = 0;
+    int seq[KV_BATCH];
+    int len[KV_BATCH];    // slots in use (append: before it)
+    int tok0[KV_BATCH];   // row of its first token in the call's tensors
+    int count[KV_BATCH];  // its tokens
+    int aux[KV_BATCH];    // append: position of the first token; read: first slot;
+                          // evict: sequence that receives the result; attend: see there
+    int unit0[KV_BATCH + 1];
+};
+
+struct KvTensor {
+    const void* p = nullptr;
+    int64_t st = 0, sh = 0, sd = 0;  // strides in elements
+    int type = KV_F32;
+    bool vec = false;  // 8 dims of a row are one aligned 16- or 32-byte piece
+};
+
+// Bytes of a tile's key (or value) half.
+__host__ __device__ inline int kv_half(int Dp) { return KV_TILE * Dp; }
+
+#ifdef __HIPCC__
+__device__ inline size_t kv_tile_offset(const KvDev& c, int block, int head, int tile) {
+    const size_t part = (size_t)block * c.H + head;
+    return (part * (size_t)(c.B / KV_TILE) + tile) * (size_t)(2 * kv_half(c.Dp));
+}
+// Byte of (slot r, dims 8 m .. 8 m + 7) in the key half.
+__device__ inline int kv_key_byte(int r, int m, int S) {
+    const int o = (r >> 4) * S + (m >> 2);
+    return (o >> 1) * 1024 + ((m & 3) * 16 + (r & 15)) * 16 + (o & 1) * 8;
+}
+// Byte of (slot r, dim d) in the value half.
+__device__ inline int kv_value_byte(int r, int d) {
+    const int i = d >> 4;
+    const int lane = ((r & 15) >> 2) * 16 + (d & 15);
+    return (i >> 1) * 1024 + lane * 16 + (i & 1) * 8 + (r >> 4) * 4 + (r & 3);
+}
+// The batch entry of a workgroup: how many unit0 are not above it, less one.
+__device__ inline int kv_find(const KvBatch& b, int unit) {
+    const int lane = threadIdx.x & 63;
+    const int e0 = lane < b.n && b.unit0[lane] <= unit;
+    const int e1 = lane + 64 < b.n && b.unit0[lane + 64] <= unit;
+    return __builtin_amdgcn_readfirstlane(__popcll(__ballot(e0)) + __popcll(__ballot(e1)) - 1);
+}
+#endif
+
+// Entries of the block table: runs of consecutive blocks.
+struct KvRuns {
+    static constexpr int MAX = 200;
+    int n = 0;
+    size_t at[MAX];
+    int block[MAX], count[MAX];
+};
+void launch_kv_table(int* table, const KvRuns& r, hipStream_t s);
+
+void launch_kv_append(const KvDev& c, const KvBatch& b, const KvTensor& k, const KvTensor& v,
+                      const int* positions, const float* weights, hipStream_t s);
+
+struct KvReadOut {
+    void *k = nullptr, *v = nullptr;
+    int* positions = nullptr;
+    float* weights = nullptr;
+    int type = KV_F32;
+};
+void launch_kv_read(const KvDev& c, const KvBatch& b, const KvReadOut& o, hipStream_t s);
+
+// Eviction of the batch's sequences (count: the slots that stay, len above it).
+struct KvEvict {
+    int budget = 0, recent = 0, drop = 0;  // drop: rows of a sequence's dropped arrays (0: none)
+    int* kept = nullptr;     // [n, H, budget] slots that stay, ascending
+    int* gone = nullptr;     // [n, H, drop] slots that leave, ascending; null without them
+    const int* dst = nullptr;  // [seq * W + i] table with the new blocks of aux[i]
+    int* dpos = nullptr;     // the caller's arrays, [n, drop, H] and [n, drop, H, D]
+    float *dk = nullptr, *dv = nullptr;
+};
+void launch_kv_evict(const KvDev& c, const KvBatch& b, const KvEvict& e, hipStream_t s);
+
+struct KvAttend {
+    KvTensor q;
+    int G = 1;              // query heads per key/value head
+    float scale2 = 0.f;     // scale * log2(e)
+    int causal = 1, window = 0;
+    const uint8_t* mask = nullptr;
+    int64_t mask_st = 0, mask_ss = 0;
+    int track = 0;
+    float decay = 0.f;
+    void* out = nullptr;       // [tokens, H * G, D] in q's type
+    float* lse = nullptr;      // [tokens, H * G]
+    float* lse2 = nullptr;     // tracked: base-2 lse of the same rows (-inf: sees nothing)
+    float* part_o = nullptr;   // split attention: partial rows [workgroup, rows, Dp]
+    float2* part_ml = nullptr; // and their (max, sum), base 2
+    float* scores = nullptr;   // tracked steps: base-2 scores [row, tile, 32] of each (sequence, head)
+    int split_tiles = 0;       // tiles of one split
+    int splits = 0;            // splits of every row tile
+    int by_rows = 0;           // waves of a workgroup take different rows (else different tiles)
+    int nc = 1;                // 16-row column tiles of a wave: 1, or 2 where Dp <= 128 and by_rows
+};
+// Rows that one workgroup takes.
+inline int kv_attend_rows(const KvAttend& a) { return 16 * a.nc * (a.by_rows ? 4 : 1); }
+// unit0 counts row tiles of the sequences (of one head); the launch is unit0[n] * H * splits.
+void launch_kv_attend(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s);
+// With scores, aux: tiles of the score rows of the sequences before (of one head);
+// unit0 counts 256 slots, without scores 128.
+void launch_kv_weights(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s);
+
+}  // namespace vgpu

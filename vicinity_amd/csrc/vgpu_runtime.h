@@ -14,6 +14,7 @@
 #include <vector>
 
 #include "../../include/vicinity_gpu.h"
+#include "vgpu_kv.h"
 #include "vgpu_launch.h"
 
 namespace vgpu {
@@ -332,6 +333,51 @@ struct FlatIndex {
     // One pass: the ranking path's (rank) queries are bounded by flat_rank_chunk.
     void search_pass(const float* d_q, size_t nq, size_t k, bool rank, int64_t* d_ids, float* d_dists,
                      hipStream_t s);
+};
+
+// The attention memory: a pool of blocks in HBM, each sequence's blocks and length on
+// the host.  The calls queue kernels on the caller's stream and do not wait; the host
+// state changes with them, under the lock.
+struct KvCache {
+    vgpu_kv_params params{};
+    int device = 0;
+    KvDev dev;
+    DevBuf<uint8_t> pool;
+    DevBuf<float> kscale, vscale, weights;
+    DevBuf<int> positions, table;
+    DevBuf<int> table2;              // eviction in place: the new blocks
+    DevBuf<int> w_kept, w_gone;      // eviction: slots that stay, slots that leave
+    DevBuf<float> w_part, w_scores, w_lse2;
+    DevBuf<float2> w_ml;
+
+    struct Seq {
+        int64_t len = 0, next = 0;   // slots in use; position of the next token
+        std::vector<int> blocks;
+    };
+    std::vector<Seq> seqs;
+    std::vector<int> free_blocks;    // taken from the back
+    std::vector<uint8_t> seen;       // batch checks
+    std::mutex mu;
+
+    explicit KvCache(const vgpu_kv_params& p);
+    ~KvCache();
+    void append(const int32_t* ids, const int64_t* counts, size_t n, const vgpu_tensor3& k, const vgpu_tensor3& v,
+                const int32_t* pos, const float* wts, hipStream_t s);
+    void attend(const int32_t* ids, const int64_t* counts, size_t n, const vgpu_kv_query& q, hipStream_t s);
+    void evict(const int32_t* ids, const int32_t* into, size_t n, size_t budget, size_t recent, size_t num_dropped,
+               int32_t* dpos, float* dk, float* dv, hipStream_t s);
+    void read(const int32_t* ids, const int64_t* first, const int64_t* counts, size_t n, int dtype, void* k, void* v,
+              int32_t* pos, float* wts, hipStream_t s);
+    void truncate(const int32_t* ids, const int64_t* lengths, size_t n);
+    size_t device_bytes() const;
+
+  private:
+    size_t blocks_of(int64_t slots) const { return (size_t)((slots + dev.B - 1) >> dev.shift); }
+    void check_call(const int32_t* ids, size_t n, hipStream_t s);
+    KvTensor tensor(const vgpu_tensor3& t, const char* name) const;
+    // Blocks from the pool for `count` more of a sequence, written to `tab`'s row.
+    void take_blocks(std::vector<int>& out, size_t count, size_t row, int* tab, KvRuns& runs, hipStream_t s);
+    void release_blocks(std::vector<int>& blocks, size_t keep);
 };
 
 // A file descriptor closed with its owner (also when a constructor throws).

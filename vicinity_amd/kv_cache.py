@@ -1,0 +1,312 @@
+"""KVCache: a model's keys and values in HBM, in 8 bits with a scale for each block of
+tokens and head, softmax attention over them, and eviction by accumulated weight.
+
+It stands beside the indexes: what evict takes out of the cache are float32 keys and
+values, and ``FlatIndex(dim, "cosine")`` ranks keys by the same inner product that the
+attention takes them with.
+
+Tensors are torch tensors on the cache's GPU.  Calls are queued on the current torch
+stream, or on ``stream``, and return without waiting; a call on another stream than the
+one before it waits for that one on the GPU.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import numpy as np
+
+from . import _lib
+
+CODES = {"int8": 0, "fp8": 1}
+FIELDS = ("k", "v", "positions", "weights")
+
+
+def _dtypes():
+    import torch
+
+    return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+class KVCache:
+    """num_seqs sequences over a pool of num_blocks blocks of block_tokens slots.
+
+    code 'int8': value = code * scale, codes -127..127; 'fp8': e4m3 codes.  A sequence
+    takes at most max_blocks blocks (None: all of them)."""
+
+    def __init__(self, num_seqs: int, num_heads: int, head_dim: int, num_blocks: int,
+                 block_tokens: int = 64, code: str = "int8", max_blocks: int | None = None):
+        if code not in CODES:
+            raise ValueError(f"code must be one of {sorted(CODES)}, got {code!r}")
+        for name, value in (("num_seqs", num_seqs), ("num_heads", num_heads),
+                            ("head_dim", head_dim), ("num_blocks", num_blocks),
+                            ("block_tokens", block_tokens), ("max_blocks", max_blocks or 1)):
+            if not 0 < int(value) < 1 << 31:
+                raise ValueError(f"{name} must be in the range 1..2**31, got {value}")
+        self._h = None
+        self._L = _lib.load()
+        params = _lib.KvParams(num_seqs, num_heads, head_dim, num_blocks, block_tokens,
+                               max_blocks or 0, CODES[code])
+        h = ctypes.c_void_p()
+        _lib.check(self._L.vgpu_kv_new(ctypes.byref(params), ctypes.byref(h)))
+        self._h = h
+        self.num_seqs, self.num_heads, self.head_dim = num_seqs, num_heads, head_dim
+        self.num_blocks, self.block_tokens, self.code = num_blocks, block_tokens, code
+        import torch
+
+        self.device = torch.device("cuda", torch.cuda.current_device())
+        self._all = np.arange(num_seqs, dtype=np.int32)
+        self._last = None  # the stream of the last call
+
+    def __del__(self):
+        h = getattr(self, "_h", None)
+        if h is not None and h.value:
+            self._L.vgpu_kv_free(h)
+            self._h = None
+
+    # ---- state ------------------------------------------------------------
+    @property
+    def lengths(self) -> np.ndarray:
+        """Slots in use of every sequence, int64 [num_seqs]."""
+        out = np.empty(self.num_seqs, np.int64)
+        _lib.check(self._L.vgpu_kv_lengths(self._h, out.ctypes.data))
+        return out
+
+    def info(self) -> dict:
+        """free_blocks, and device_bytes: the HBM that the cache holds."""
+        out = _lib.KvInfo()
+        _lib.check(self._L.vgpu_kv_get_info(self._h, ctypes.byref(out)))
+        return {"free_blocks": out.free_blocks, "device_bytes": out.device_bytes}
+
+    def truncate(self, lengths, seqs=None) -> None:
+        """Forget each sequence's slots from lengths[i] on; 0 empties it."""
+        ids = self._seqs(seqs)
+        lens = self._ints(lengths, len(ids), "lengths")
+        _lib.check(self._L.vgpu_kv_truncate(self._h, ids.ctypes.data, lens.ctypes.data, len(ids)))
+
+    # ---- operators ----------------------------------------------------------
+    def append(self, k, v, seqs=None, counts=None, positions=None, weights=None,
+               stream=None) -> None:
+        """Quantise new tokens behind those that the sequences hold.
+
+        k, v [tokens, num_heads, head_dim], float32, float16 or bfloat16, any strides:
+        counts[i] tokens of seqs[i] after those of seqs[i - 1] (seqs None: every
+        sequence; counts None: the same number for each).  positions int32 and weights
+        float32 [tokens, num_heads] are kept beside the slots (None: tokens counted from
+        the sequence's start, and 0)."""
+        ids = self._seqs(seqs)
+        kt = self._tensor(k, "k", self.num_heads)
+        vt = self._tensor(v, "v", self.num_heads)
+        if k.shape != v.shape or k.dtype != v.dtype:
+            raise ValueError("k and v must have the same shape and dtype")
+        n = self._counts(counts, len(ids), k.shape[0])
+        pos = self._side(positions, "positions", k.shape[0], "int32")
+        wts = self._side(weights, "weights", k.shape[0], "float32")
+        s, _ = self._stream(stream, (k, v, positions, weights))
+        _lib.check(self._L.vgpu_kv_append(self._h, ids.ctypes.data, n.ctypes.data, len(ids),
+                                          ctypes.byref(kt), ctypes.byref(vt), pos, wts, s))
+
+    def attend(self, q, seqs=None, counts=None, scale: float | None = None, causal: bool = True,
+               window: int = 0, mask=None, decay: float | None = None, out=None,
+               return_lse: bool = False, stream=None):
+        """softmax(scale * q k^T) v over the cached slots, [tokens, heads, head_dim].
+
+        q [tokens, heads, head_dim] belongs to the last counts[i] tokens of seqs[i];
+        heads is a multiple of num_heads, consecutive query heads share a key/value head.
+        Token i stands at slot len - counts + i and sees the slots up to its own (causal;
+        else all), of them the last `window` (0: all), of them those where mask
+        [tokens, slots] (bool) is set.  A token that sees nothing gets 0 and lse -inf.
+        scale None: 1 / sqrt(head_dim).  decay: the accumulated weight of a slot and head
+        becomes decay * weight + what the call's tokens gave it (None: weights stay).
+        return_lse: also the float32 logarithms of the softmax denominators
+        [tokens, heads]."""
+        import torch
+
+        ids = self._seqs(seqs)
+        qt = self._tensor(q, "q", None)
+        tokens, heads = q.shape[0], q.shape[1]
+        if heads == 0 or heads % self.num_heads:
+            raise ValueError(f"q has {heads} heads, not a multiple of the cache's "
+                             f"{self.num_heads}")
+        n = self._counts(counts, len(ids), tokens)
+        if not isinstance(window, (int, np.integer)) or window < 0:
+            raise ValueError("window must be an int, 0 or more")
+        if out is not None and (out.shape != q.shape or out.dtype != q.dtype
+                                or out.device != q.device or not out.is_contiguous()):
+            raise ValueError("out must be contiguous, of q's shape, dtype and device")
+        if mask is not None:
+            if mask.dtype not in (torch.bool, torch.uint8) or mask.dim() != 2 \
+                    or mask.shape[0] != tokens or mask.device != self.device:
+                raise ValueError("mask must be a bool or uint8 tensor [tokens, slots] on the "
+                                 "cache's GPU")
+        s, ctx = self._stream(stream, (q, mask, out))
+        with ctx:
+            if out is None:
+                out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) \
+                if return_lse else None
+        query = _lib.KvQuery(
+            qt, heads, 1.0 / math.sqrt(self.head_dim) if scale is None else scale, int(causal),
+            int(window), mask.data_ptr() if mask is not None else None,
+            mask.stride(0) if mask is not None else 0, mask.stride(1) if mask is not None else 0,
+            mask.shape[1] if mask is not None else 0, int(decay is not None),
+            0.0 if decay is None else decay, out.data_ptr(),
+            lse.data_ptr() if lse is not None else None)
+        _lib.check(self._L.vgpu_kv_attend(self._h, ids.ctypes.data, n.ctypes.data, len(ids),
+                                          ctypes.byref(query), s))
+        return (out, lse) if return_lse else out
+
+    def evict(self, budget: int, recent: int = 0, seqs=None, into=None, dropped: bool = False,
+              stream=None):
+        """Cut each sequence longer than `budget` slots down to it.
+
+        Every head keeps its last `recent` slots and those of largest accumulated weight
+        among the others (of equal ones the lower slot), in their order.  into: empty
+        sequences that receive the result (seqs stay as they are); None: in place.
+        dropped: return what leaves as a dict, positions int32 [n, most, num_heads]
+        (-1 where a sequence lost fewer), k and v float32 [n, most, num_heads, head_dim]
+        (zeros there)."""
+        import torch
+
+        ids = self._seqs(seqs)
+        to = None if into is None else self._seqs(into)
+        if to is not None and len(to) != len(ids):
+            raise ValueError(f"into names {len(to)} sequences, seqs {len(ids)}")
+        for name, value in (("budget", budget), ("recent", recent)):
+            if not isinstance(value, (int, np.integer)) or value < 0:
+                raise ValueError(f"{name} must be an int, 0 or more")
+        s, ctx = self._stream(stream, ())
+        gone, most = None, 0
+        if dropped:
+            known = ids[(ids >= 0) & (ids < self.num_seqs)]  # the others are refused below
+            most = max(int(self.lengths[known].max(initial=0)) - int(budget), 0)
+            shape = (len(ids), most, self.num_heads)
+            with ctx:
+                gone = {"positions": torch.empty(shape, dtype=torch.int32, device=self.device),
+                        "k": torch.empty(shape + (self.head_dim,), device=self.device,
+                                         dtype=torch.float32)}
+                gone["v"] = torch.empty_like(gone["k"])
+        ptr = [gone[f].data_ptr() if gone and most else None for f in ("positions", "k", "v")]
+        _lib.check(self._L.vgpu_kv_evict(self._h, ids.ctypes.data,
+                                         None if to is None else to.ctypes.data, len(ids), budget,
+                                         recent, most, *ptr, s))
+        return gone
+
+    def read(self, seqs=None, first=None, counts=None, fields=FIELDS, dtype=None,
+             stream=None) -> dict:
+        """What the slots first[i] .. first[i] + counts[i] - 1 of seqs[i] hold (None: from
+        0, to the end), one sequence after the other: 'k' and 'v' [tokens, num_heads,
+        head_dim] in dtype (None: float32), 'positions' int32 and 'weights' float32
+        [tokens, num_heads]."""
+        import torch
+
+        dtype = torch.float32 if dtype is None else dtype
+        if dtype not in _dtypes():
+            raise TypeError("dtype must be float32, float16 or bfloat16")
+        if not set(fields) <= set(FIELDS):
+            raise ValueError(f"fields must be among {FIELDS}")
+        ids = self._seqs(seqs)
+        at = self._ints(0 if first is None else first, len(ids), "first")
+        if counts is None:
+            if ((ids < 0) | (ids >= self.num_seqs)).any():
+                raise ValueError(f"sequence out of range [0, {self.num_seqs})")
+            n = np.maximum(self.lengths[ids] - at, 0)
+        else:
+            n = self._ints(counts, len(ids), "counts")
+        tokens = max(int(n.sum()), 0)
+        s, ctx = self._stream(stream, ())
+        types = {"positions": torch.int32, "weights": torch.float32}
+        res = {}
+        with ctx:
+            for f in fields:
+                shape = (tokens, self.num_heads) + ((self.head_dim,) if f in "kv" else ())
+                res[f] = torch.empty(shape, dtype=types.get(f, dtype), device=self.device)
+        ptr = [res[f].data_ptr() if f in res else None for f in FIELDS]
+        _lib.check(self._L.vgpu_kv_read(self._h, ids.ctypes.data, at.ctypes.data, n.ctypes.data,
+                                        len(ids), _dtypes()[dtype], *ptr, s))
+        return res
+
+    # ---- arguments ------------------------------------------------------------
+    def _seqs(self, seqs) -> np.ndarray:
+        if seqs is None:
+            return self._all
+        a = np.asarray(list(seqs) if isinstance(seqs, range) else seqs)
+        if a.size == 0:
+            return np.zeros(0, np.int32)
+        if a.ndim != 1 or a.dtype.kind not in "iu":
+            raise ValueError("sequences must be a 1-D array of integers")
+        if int(a.min()) < 0 or int(a.max()) >= self.num_seqs:
+            raise ValueError(f"sequence out of range [0, {self.num_seqs})")
+        return np.ascontiguousarray(a, np.int32)
+
+    @staticmethod
+    def _ints(values, n: int, name: str) -> np.ndarray:
+        a = np.asarray(values)
+        if a.size and a.dtype.kind not in "iu":
+            raise ValueError(f"{name} must be integers")
+        if a.ndim == 0:
+            return np.full(n, int(a), np.int64)
+        if a.shape != (n,):
+            raise ValueError(f"{name} must have one entry for each of the {n} sequences")
+        return np.ascontiguousarray(a, np.int64)
+
+    def _counts(self, counts, n: int, tokens: int) -> np.ndarray:
+        if counts is None:
+            if n == 0 or tokens % n:
+                raise ValueError(f"{tokens} tokens cannot be shared out to {n} sequences: "
+                                 "counts is needed")
+            return np.full(n, tokens // n, np.int64)
+        a = self._ints(counts, n, "counts")
+        if (a < 0).any() or int(a.sum()) != tokens:
+            raise ValueError(f"counts must add up to the {tokens} tokens given")
+        return a
+
+    def _tensor(self, t, name: str, heads):
+        import torch
+
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch tensor")
+        if t.dtype not in _dtypes():
+            raise TypeError(f"{name} must be float32, float16 or bfloat16")
+        if t.dim() != 3 or t.shape[2] != self.head_dim or (heads and t.shape[1] != heads):
+            raise ValueError(f"{name} must have the shape [tokens, {heads or 'heads'}, "
+                             f"{self.head_dim}], got {list(t.shape)}")
+        if t.device != self.device:
+            raise ValueError(f"{name} must be on the cache's GPU ({self.device})")
+        return _lib.KvTensor(t.data_ptr() or None, _dtypes()[t.dtype], *t.stride())
+
+    def _side(self, t, name: str, tokens: int, dtype: str):
+        import torch
+
+        if t is None:
+            return None
+        if not isinstance(t, torch.Tensor) or t.dtype != getattr(torch, dtype):
+            raise TypeError(f"{name} must be a torch tensor of {dtype}")
+        if t.shape != (tokens, self.num_heads) or t.device != self.device \
+                or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous, [tokens, {self.num_heads}], on the "
+                             "cache's GPU")
+        return t.data_ptr()
+
+    def _stream(self, stream, tensors):
+        """The call's stream handle and a context that allocates on it.  Puts the call
+        behind the last one and keeps the tensors' memory until it has run."""
+        import contextlib
+
+        import torch
+
+        current = torch.cuda.current_stream(self.device)
+        use = current if stream is None else stream
+        with torch.cuda.stream(use):
+            capturing = torch.cuda.is_current_stream_capturing()  # refused by the library
+        if not capturing:
+            if self._last is not None and self._last != use:
+                use.wait_stream(self._last)
+            self._last = use
+        if use == current:
+            return use.cuda_stream or None, contextlib.nullcontext()
+        for t in tensors:
+            if t is not None:
+                t.record_stream(use)
+        return use.cuda_stream or None, torch.cuda.stream(use)
