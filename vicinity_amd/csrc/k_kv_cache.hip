@@ -6,6 +6,7 @@
 // Rounding: codes are the cache's format; every value before them is float32.
 #include "vgpu_kv.h"
 
+#include <climits>
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
@@ -71,12 +72,6 @@ __device__ __forceinline__ void decode4(uint32_t w, int code, float* v) {
     typedef float f2 __attribute__((ext_vector_type(2)));
     const f2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
     v[0] = lo.x, v[1] = lo.y, v[2] = hi.x, v[3] = hi.y;
-}
-
-__device__ __forceinline__ float decode1(uint8_t b, int code) {
-    float v[4];
-    decode4(b, code, v);
-    return v[0];
 }
 
 __device__ __forceinline__ uint32_t zero_codes(int code) { return code == KV_INT8 ? 0x80808080u : 0u; }
@@ -194,46 +189,107 @@ __device__ __forceinline__ void store1(void* p, size_t i, float v, int type) {
         ((__hip_bfloat16*)p)[i] = __float2bfloat16(v);
 }
 
-// One workgroup: one tile of one head, for the slots that are asked for.
-__global__ __launch_bounds__(256) void kv_read_kernel(KvDev c, KvBatch b, KvReadOut o) {
-    __shared__ __align__(16) uint8_t image[2 * KV_TILE * KV_MAX_DIM];
-    const int tid = threadIdx.x;
-    const int h = blockIdx.x % c.H, unit = blockIdx.x / c.H;
-    const int i = kv_find(b, unit);
-    const int first = b.aux[i], last = first + b.count[i];
-    const int slot0 = (first / KV_TILE + unit - b.unit0[i]) * KV_TILE;
-    const int lo = max(first - slot0, 0), hi = min(last - slot0, KV_TILE);
-    const int block = c.table[(size_t)b.seq[i] * c.W + (slot0 >> c.shift)];
-    const size_t part = (size_t)block * c.H + h;
-    const int in_block = slot0 & (c.B - 1);
-    const int64_t tok = (int64_t)b.tok0[i] + slot0 - first;
-    const int S = c.Dp / 32;
-    if (o.k || o.v) {
-        const uint4* tile = (const uint4*)(c.pool + kv_tile_offset(c, block, h, in_block / KV_TILE));
-        for (int u = tid; u < 2 * kv_half(c.Dp) / 16; u += 256) ((uint4*)image)[u] = tile[u];
-        __syncthreads();
-        const float ks = c.kscale[part], vs = c.vscale[part];
-        const int Md = (c.D + 7) / 8;
-        for (int u = tid; u < (hi - lo) * Md; u += 256) {
-            const int r = lo + u / Md, m = u % Md;
-            const size_t at = ((size_t)(tok + r) * c.H + h) * c.D + 8 * m;
-            float e[8];
-            if (o.k) {
-                const uint2 w = *(const uint2*)(image + kv_key_byte(r, m, S));
-                decode4(w.x, c.code, e);
-                decode4(w.y, c.code, e + 4);
-                for (int j = 0; j < 8 && 8 * m + j < c.D; j++) store1(o.k, at + j, e[j] * ks, o.type);
-            }
-            if (o.v) {
+// N values of a row from dim d on (those below D), rounded once.
+template <int T, int N>
+__device__ __forceinline__ void store_row(void* p, size_t row, int d, int D, bool vec, const float* v) {
+    if (vec && d + N <= D) {
+        if (T == KV_F32) {
+            float4* at = (float4*)((float*)p + row + d);
 #pragma unroll
-                for (int j = 0; j < 8; j++)
-                    e[j] = decode1(image[kv_half(c.Dp) + kv_value_byte(r, 8 * m + j)], c.code);
-                for (int j = 0; j < 8 && 8 * m + j < c.D; j++) store1(o.v, at + j, e[j] * vs, o.type);
+            for (int j = 0; j < N / 4; j++) at[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        } else {
+            uint32_t w[N / 2];
+#pragma unroll
+            for (int j = 0; j < N / 2; j++) {
+                uint16_t h[2];
+                store1(h, 0, v[2 * j], T), store1(h, 1, v[2 * j + 1], T);
+                w[j] = (uint32_t)h[0] | (uint32_t)h[1] << 16;
+            }
+#pragma unroll
+            for (int j = 0; j < N / 8; j++)
+                ((uint4*)((uint16_t*)p + row + d))[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < N; j++)
+        if (d + j < D) store1(p, row + d + j, v[j], T);
+}
+
+// The values of a tile, by one wave: a lane takes its 16 bytes of each piece, which are
+// 8 dims each of one slot and two operands (keys), or two dims of 8 slots (values).
+// row(slot): the element index of the slot's row in the outputs, or ~0.
+template <int T, typename Row>
+__device__ __forceinline__ void read_tile(const KvDev& c, const uint8_t* tile, float ks, float vs, void* ko, void* vo,
+                                          bool vec, Row row) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, x = lane & 15;
+    const int S = c.Dp / 32;
+    const uint4* at = (const uint4*)tile + lane;
+    if (ko) {
+        const size_t rows[2] = {row(x), row(16 + x)};
+        for (int p = 0; p < S; p++) {
+            const uint4 w = at[p * 64];
+#pragma unroll
+            for (int o = 0; o < 2; o++) {
+                const int j = (2 * p + o) / S, s = (2 * p + o) % S;
+                const size_t r = j ? rows[1] : rows[0];
+                float e[8];
+                decode4(o ? w.z : w.x, c.code, e);
+                decode4(o ? w.w : w.y, c.code, e + 4);
+#pragma unroll
+                for (int i = 0; i < 8; i++) e[i] *= ks;
+                if (r != ~(size_t)0) store_row<T, 8>(ko, r, 32 * s + 8 * g, c.D, vec, e);
             }
         }
     }
-    if (tid >= lo && tid < hi) {
-        const size_t at = (size_t)(tok + tid) * c.H + h, from = part * c.B + in_block + tid;
+    if (vo) {
+        size_t rows[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) rows[i] = row((i >> 2) * 16 + 4 * g + (i & 3));
+        for (int p = 0; p < S; p++) {
+            const uint4 w = at[(S + p) * 64];
+#pragma unroll
+            for (int o = 0; o < 2; o++) {
+                const int d = (2 * p + o) * 16 + x;
+                float e[8];
+                decode4(o ? w.z : w.x, c.code, e);
+                decode4(o ? w.w : w.y, c.code, e + 4);
+                if (d < c.D) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        if (rows[i] != ~(size_t)0) store1(vo, rows[i] + d, e[i] * vs, T);
+                }
+            }
+        }
+    }
+}
+
+// One workgroup: 128 slots of one head, a tile to a wave.  Bound by the bytes written:
+// no element passes through LDS, a key store is 32 contiguous bytes of a lane, a value
+// store 64 bytes of 16 lanes.
+template <int T>
+__global__ __launch_bounds__(256) void kv_read_kernel(KvDev c, KvBatch b, KvReadOut o) {
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int h = blockIdx.x % c.H, unit = blockIdx.x / c.H;
+    const int i = kv_find(b, unit);
+    const int first = b.aux[i], last = first + b.count[i];
+    const int group = (first / KV_READ + unit - b.unit0[i]) * KV_READ;
+    const int* table = c.table + (size_t)b.seq[i] * c.W;
+    const int64_t tok = (int64_t)b.tok0[i] - first;  // row of slot 0
+    const int slot0 = group + wave * KV_TILE;
+    if ((o.k || o.v) && slot0 < last && slot0 + KV_TILE > first) {
+        const int block = __builtin_amdgcn_readfirstlane(table[slot0 >> c.shift]);
+        const size_t part = (size_t)block * c.H + h;
+        const uint8_t* tile = c.pool + kv_tile_offset(c, block, h, (slot0 & (c.B - 1)) / KV_TILE);
+        read_tile<T>(c, tile, c.kscale[part], c.vscale[part], o.k, o.v, o.vec, [&](int r) -> size_t {
+            const int slot = slot0 + r;
+            return slot >= first && slot < last ? ((size_t)(tok + slot) * c.H + h) * c.D : ~(size_t)0;
+        });
+    }
+    const int slot = group + tid;
+    if (tid < KV_READ && slot >= first && slot < last && (o.positions || o.weights)) {
+        const size_t at = (size_t)(tok + slot) * c.H + h;
+        const size_t from = ((size_t)table[slot >> c.shift] * c.H + h) * c.B + (slot & (c.B - 1));
         if (o.positions) o.positions[at] = c.positions[from];
         if (o.weights) o.weights[at] = c.weights[from];
     }
@@ -264,7 +320,7 @@ __global__ __launch_bounds__(1024) void kv_select_kernel(KvDev c, KvBatch b, KvE
     const int* row = c.table + (size_t)b.seq[i] * c.W;
     const int len = b.len[i], stay = b.count[i];
     int* kept = e.kept + ((size_t)i * c.H + h) * e.budget;
-    int* gone = e.gone ? e.gone + ((size_t)i * c.H + h) * e.drop : nullptr;
+    int* gone = e.gone ? e.gone + ((size_t)i * c.H + h) * e.slots : nullptr;
     const int recent = stay < len ? min(e.recent, stay) : 0;
     const int old = len - recent, want = stay - recent;
     uint32_t prefix = 0, bits = 0, need = want;
@@ -315,14 +371,15 @@ __global__ __launch_bounds__(1024) void kv_select_kernel(KvDev c, KvBatch b, KvE
             kall += wsum[1][w];
         }
         at += (uint32_t)__popcll(kb & ((1ull << lane) - 1));
-        if (keep)
-            kept[at] = j;
-        else if (in && gone)
-            gone[j - at] = j;
+        if (keep) kept[at] = j;
+        if (in && gone) gone[j] = keep ? -1 : j - (int)at;
         equal += all, done += kall;
         __syncthreads();
     }
-    for (int j = tid; j < recent; j += 1024) kept[want + j] = old + j;
+    for (int j = tid; j < recent; j += 1024) {
+        kept[want + j] = old + j;
+        if (gone) gone[old + j] = -1;
+    }
 }
 
 // One workgroup: one block of one head of the result.
@@ -405,32 +462,45 @@ __global__ __launch_bounds__(256) void kv_move_kernel(KvDev c, KvBatch b, KvEvic
     }
 }
 
-// One workgroup: 8 rows of one head of what leaves; rows past the sequence's own are
-// position -1 and zeros.
-__global__ __launch_bounds__(256) void kv_dropped_kernel(KvDev c, KvBatch b, KvEvict e) {
-    const int groups = (e.drop + 7) / 8;
-    const int h = blockIdx.x % c.H, g = (blockIdx.x / c.H) % groups, i = blockIdx.x / c.H / groups;
-    const int* row = c.table + (size_t)b.seq[i] * c.W;
+// One workgroup: 128 slots of one head; those that leave are written to their rows.
+__global__ __launch_bounds__(256) void kv_dropped_kernel(KvDev c, KvBatch b, KvEvict e, int groups) {
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int h = blockIdx.x % c.H, g = blockIdx.x / c.H % groups, i = blockIdx.x / c.H / groups;
+    const int len = b.len[i], group = g * KV_READ;
+    const int* table = c.table + (size_t)b.seq[i] * c.W;
+    const int* gone = e.gone + ((size_t)i * c.H + h) * e.slots;
+    const int slot0 = group + wave * KV_TILE;
+    if ((e.dk || e.dv) && slot0 < len) {
+        const int block = __builtin_amdgcn_readfirstlane(table[slot0 >> c.shift]);
+        const size_t part = (size_t)block * c.H + h;
+        const uint8_t* tile = c.pool + kv_tile_offset(c, block, h, (slot0 & (c.B - 1)) / KV_TILE);
+        read_tile<KV_F32>(c, tile, c.kscale[part], c.vscale[part], e.dk, e.dv, e.vec, [&](int r) -> size_t {
+            const int to = slot0 + r < len ? gone[slot0 + r] : -1;
+            return to >= 0 ? ((size_t)(b.tok0[i] + to) * c.H + h) * c.D : ~(size_t)0;
+        });
+    }
+    const int slot = group + tid;
+    if (e.dpos && tid < KV_READ && slot < len) {
+        const int to = gone[slot];
+        if (to >= 0)
+            e.dpos[(size_t)(b.tok0[i] + to) * c.H + h] =
+                c.positions[((size_t)table[slot >> c.shift] * c.H + h) * c.B + (slot & (c.B - 1))];
+    }
+}
+
+// Rows past what a sequence lost: position -1 and zeros.
+__global__ __launch_bounds__(256) void kv_dropped_rest_kernel(KvDev c, KvBatch b, KvEvict e) {
+    const int i = blockIdx.y;
     const int n = b.len[i] - b.count[i];
-    const int S = c.Dp / 32;
-    for (int u = threadIdx.x; u < 8 * c.D; u += 256) {
-        const int j = g * 8 + u / c.D, d = u % c.D;
-        if (j >= e.drop) continue;
-        const size_t at = ((size_t)(b.tok0[i] + j) * c.H + h);
-        float kx = 0.f, vx = 0.f;
-        int pos = -1;
-        if (j < n) {
-            const int slot = e.gone[((size_t)i * c.H + h) * e.drop + j];
-            const int block = row[slot >> c.shift], s = slot & (c.B - 1);
-            const size_t part = (size_t)block * c.H + h;
-            const uint8_t* tile = c.pool + kv_tile_offset(c, block, h, s / KV_TILE);
-            kx = decode1(tile[kv_key_byte(s & 31, d / 8, S) + (d & 7)], c.code) * c.kscale[part];
-            vx = decode1(tile[kv_half(c.Dp) + kv_value_byte(s & 31, d)], c.code) * c.vscale[part];
-            pos = c.positions[part * c.B + s];
+    const size_t width = (size_t)c.H * c.D;
+    for (int j = n + blockIdx.x; j < e.drop; j += gridDim.x) {
+        const size_t row = (size_t)(b.tok0[i] + j);
+        for (size_t u = threadIdx.x; u < width; u += 256) {
+            if (e.dk) e.dk[row * width + u] = 0.f;
+            if (e.dv) e.dv[row * width + u] = 0.f;
         }
-        if (e.dk) e.dk[at * c.D + d] = kx;
-        if (e.dv) e.dv[at * c.D + d] = vx;
-        if (e.dpos && d == 0) e.dpos[at] = pos;
+        if (e.dpos)
+            for (int u = threadIdx.x; u < c.H; u += 256) e.dpos[row * c.H + u] = -1;
     }
 }
 
@@ -454,13 +524,30 @@ void launch_kv_append(const KvDev& c, const KvBatch& b, const KvTensor& k, const
 
 void launch_kv_read(const KvDev& c, const KvBatch& b, const KvReadOut& o, hipStream_t s) {
     const dim3 grid((unsigned)b.unit0[b.n] * c.H);
-    if (grid.x) hipLaunchKernelGGL(kv_read_kernel, grid, dim3(256), 0, s, c, b, o);
+    if (!grid.x) return;
+    if (o.type == KV_F32)
+        hipLaunchKernelGGL(kv_read_kernel<KV_F32>, grid, dim3(256), 0, s, c, b, o);
+    else if (o.type == KV_F16)
+        hipLaunchKernelGGL(kv_read_kernel<KV_F16>, grid, dim3(256), 0, s, c, b, o);
+    else
+        hipLaunchKernelGGL(kv_read_kernel<KV_BF16>, grid, dim3(256), 0, s, c, b, o);
 }
 
 void launch_kv_evict(const KvDev& c, const KvBatch& b, const KvEvict& e, hipStream_t s) {
     hipLaunchKernelGGL(kv_select_kernel, dim3(b.n * c.H), dim3(1024), 0, s, c, b, e);
-    if (e.drop > 0 && (e.dk || e.dv || e.dpos))
-        hipLaunchKernelGGL(kv_dropped_kernel, dim3((unsigned)b.n * c.H * ((e.drop + 7) / 8)), dim3(256), 0, s, c, b, e);
+    if (e.drop > 0) {
+        int longest = 0, least = INT_MAX;  // slots, and rows that leave
+        for (int i = 0; i < b.n; i++) {
+            longest = b.len[i] > longest ? b.len[i] : longest;
+            least = b.len[i] - b.count[i] < least ? b.len[i] - b.count[i] : least;
+        }
+        const int groups = (longest + KV_READ - 1) / KV_READ;
+        if (groups)
+            hipLaunchKernelGGL(kv_dropped_kernel, dim3((unsigned)b.n * c.H * groups), dim3(256), 0, s, c, b, e, groups);
+        if (least < e.drop)
+            hipLaunchKernelGGL(kv_dropped_rest_kernel, dim3(e.drop - least < 256 ? e.drop - least : 256, b.n), dim3(256),
+                               0, s, c, b, e);
+    }
     if (b.unit0[b.n])
         hipLaunchKernelGGL(kv_move_kernel, dim3((unsigned)b.unit0[b.n] * c.H), dim3(256), 0, s, c, b, e);
 }

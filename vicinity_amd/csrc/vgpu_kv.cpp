@@ -222,6 +222,7 @@ void KvCache::read(const int32_t* ids, const int64_t* first, const int64_t* coun
     }
     KvReadOut o;
     o.k = k, o.v = v, o.positions = pos, o.weights = wts, o.type = dtype;
+    o.vec = dev.D % 8 == 0 && ((uintptr_t)k | (uintptr_t)v) % 16 == 0;
     tok = 0;
     for (size_t i0 = 0; i0 < n; i0 += KV_BATCH) {
         KvBatch b;
@@ -235,7 +236,7 @@ void KvCache::read(const int32_t* ids, const int64_t* first, const int64_t* coun
             b.count[j] = (int)counts[i];
             b.aux[j] = (int)first[i];
             const int64_t last = first[i] + counts[i];
-            b.unit0[j + 1] = b.unit0[j] + (counts[i] ? (int)((last + KV_TILE - 1) / KV_TILE - first[i] / KV_TILE) : 0);
+            b.unit0[j + 1] = b.unit0[j] + (counts[i] ? (int)((last + KV_READ - 1) / KV_READ - first[i] / KV_READ) : 0);
             b.n++;
             tok += counts[i];
         }
@@ -288,12 +289,14 @@ void KvCache::evict(const int32_t* ids, const int32_t* into, size_t n, size_t bu
         if (!into) have += q.blocks.size();
     }
     const int drop = drops ? (int)num_dropped : 0;
-    need((int64_t)dev.H * ((drop + 7) / 8) <= INT_MAX / KV_BATCH && (int64_t)n * drop <= INT_MAX,
+    need((int64_t)dev.H * drop <= INT_MAX / KV_BATCH && (int64_t)n * drop <= INT_MAX,
          "too many dropped slots in one call");
     const size_t group = std::min<size_t>(n, KV_BATCH);
     if (!into) table2.reserve(table.n);
     grow(w_kept, group * dev.H * std::max<size_t>(budget, 1));
-    if (drop) grow(w_gone, group * dev.H * (size_t)drop);
+    int64_t longest = 0;
+    for (size_t i = 0; i < n; i++) longest = std::max(longest, seqs[ids[i]].len);
+    if (drop) grow(w_gone, group * dev.H * (size_t)longest);
     std::vector<std::vector<int>> fresh(n);
     for (size_t i = 0; i < n; i++) fresh[i].reserve(blocks_of(stays(i)));
     if (into)
@@ -306,6 +309,8 @@ void KvCache::evict(const int32_t* ids, const int32_t* into, size_t n, size_t bu
     e.kept = w_kept.p, e.gone = drop ? w_gone.p : nullptr;
     e.dst = into ? table.p : table2.p;
     e.dpos = dpos, e.dk = dk, e.dv = dv;
+    e.slots = (int)longest;
+    e.vec = dev.D % 8 == 0 && ((uintptr_t)dk | (uintptr_t)dv) % 16 == 0;
     for (size_t i0 = 0; i0 < n;) {
         KvBatch b;
         KvRuns runs;

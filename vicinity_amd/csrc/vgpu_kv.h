@@ -108,14 +108,19 @@ struct KvReadOut {
     int* positions = nullptr;
     float* weights = nullptr;
     int type = KV_F32;
+    bool vec = false;  // 8 dims of an output row are one aligned piece
 };
+// unit0 counts groups of KV_READ slots, from that of the first slot on.
+constexpr int KV_READ = 128;
 void launch_kv_read(const KvDev& c, const KvBatch& b, const KvReadOut& o, hipStream_t s);
 
 // Eviction of the batch's sequences (count: the slots that stay, len above it).
 struct KvEvict {
     int budget = 0, recent = 0, drop = 0;  // drop: rows of a sequence's dropped arrays (0: none)
     int* kept = nullptr;     // [n, H, budget] slots that stay, ascending
-    int* gone = nullptr;     // [n, H, drop] slots that leave, ascending; null without them
+    int* gone = nullptr;     // [n, H, slots] a slot's row among those that leave, or -1; null without them
+    int slots = 0;           // of the longest sequence
+    bool vec = false;        // 8 dims of a dropped row are one aligned piece
     const int* dst = nullptr;  // [seq * W + i] table with the new blocks of aux[i]
     int* dpos = nullptr;     // the caller's arrays, [n, drop, H] and [n, drop, H, D]
     float *dk = nullptr, *dv = nullptr;
