@@ -240,13 +240,20 @@ __device__ __forceinline__ float kv_join_factor(float m, float l, float mx) {
     return m == KV_NEG ? 0.f * l : exp2f(m - mx);
 }
 
-// A finished row: o / l and the logarithm.
+// Index of a row in the outputs, and in the arrays of one head after the other.
+__device__ __forceinline__ size_t kv_row(const KvDev& c, const KvBatch& b, const KvAttend& a, int i, int h, int row) {
+    return (size_t)(b.tok0[i] + row / a.G) * c.H * a.G + h * a.G + row % a.G;
+}
+__device__ __forceinline__ size_t kv_head_row(const KvDev& c, const KvBatch& b, const KvAttend& a, int i, int h, int row) {
+    return ((size_t)b.tok0[i] * c.H + (size_t)h * b.count[i]) * a.G + row;
+}
+
+// A finished row's logarithm.
 __device__ __forceinline__ void kv_finish(const KvDev& c, const KvBatch& b, const KvAttend& a, int i, int h, int row,
-                                          float m, float l, size_t& at) {
-    at = (size_t)(b.tok0[i] + row / a.G) * c.H * a.G + h * a.G + row % a.G;
+                                          float m, float l) {
     const float lse2 = l == 0.f ? KV_NEG : m - KV_TOP + log2f(l);
-    if (a.lse) a.lse[at] = lse2 * 0.69314718055994531f;
-    if (a.lse2) a.lse2[at] = lse2;
+    if (a.lse) a.lse[kv_row(c, b, a, i, h, row)] = lse2 * 0.69314718055994531f;
+    if (a.lse2) a.lse2[kv_head_row(c, b, a, i, h, row)] = lse2;
 }
 
 // BY_ROWS: the four waves take 4 * NC * 16 rows and every tile; else the same NC * 16
@@ -280,6 +287,17 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(KvDev c, KvBatch b, K
         kv_range(a, len, b.count[i], row0, any_lo, all_hi);
         kv_range(a, len, b.count[i], min(row0 + 16 * NC, rows) - 1, all_lo, any_hi);
     }
+    if (BY_ROWS && a.qop && split == 0) {
+#pragma unroll
+        for (int n = 0; n < NC; n++) {
+            const int tile = row0 / 16 + n;
+            if (tile * 16 >= rows) continue;
+            uint4* to = a.qop + ((size_t)b.aux[i] * c.H + (size_t)h * ((rows + 15) / 16) + tile) * (PARTS * S * 64);
+#pragma unroll
+            for (int x = 0; x < PARTS * S; x++) to[x * 64 + lane] = __builtin_bit_cast(uint4, w.q[n][x / S][x % S]);
+            if (g == 0 && w.row[n] >= 0) a.qs[kv_head_row(c, b, a, i, h, w.row[n])] = w.qs[n];
+        }
+    }
     const int* table = c.table + (size_t)b.seq[i] * c.W;
     const int step = BY_ROWS ? 1 : 4;
     const int64_t score_row = (int64_t)((len + KV_TILE - 1) / KV_TILE) * KV_TILE;
@@ -302,8 +320,8 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(KvDev c, KvBatch b, K
         for (int n = 0; n < NC; n++) {
             if (w.row[n] < 0) continue;
             if (whole) {
-                size_t at;
-                kv_finish(c, b, a, i, h, w.row[n], w.m[n], w.l[n], at);
+                const size_t at = kv_row(c, b, a, i, h, w.row[n]);
+                if (g == 0) kv_finish(c, b, a, i, h, w.row[n], w.m[n], w.l[n]);
                 const float inv = w.l[n] == 0.f ? 0.f : 1.f / w.l[n];
 #pragma unroll
                 for (int j = 0; j < 2 * S; j++)
@@ -354,11 +372,8 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(KvDev c, KvBatch b, K
             o += *(const floatx4*)(lds + rr * LDO + d) * f;
         }
         if (whole) {
-            size_t at;
-            if (d == 0)
-                kv_finish(c, b, a, i, h, row, mx, l, at);
-            else
-                at = (size_t)(b.tok0[i] + row / a.G) * c.H * a.G + h * a.G + row % a.G;
+            const size_t at = kv_row(c, b, a, i, h, row);
+            if (d == 0) kv_finish(c, b, a, i, h, row, mx, l);
             const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
             for (int e = 0; e < 4; e++)
@@ -371,15 +386,17 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(KvDev c, KvBatch b, K
     }
 }
 
-// Joins the splits of rows whose tiles went to several workgroups: a wave per row.
-__global__ __launch_bounds__(256) void kv_join_kernel(KvDev c, KvBatch b, KvAttend a, int wg_rows) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int groups = (wg_rows + 3) / 4;
-    const int h = blockIdx.x % c.H, rg = blockIdx.x / c.H % groups, unit = blockIdx.x / c.H / groups;
+// Joins the splits of a row whose tiles went to several workgroups: a workgroup per row,
+// its waves take every fourth split, then lane by lane in the waves' order.
+__global__ __launch_bounds__(256) void kv_join_kernel(KvDev c, KvBatch b, KvAttend a, int wg_rows, int used_rows) {
+    __shared__ float sh_o[4][KV_MAX_DIM];
+    __shared__ float sh_l[4];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int h = blockIdx.x % c.H, r = blockIdx.x / c.H % used_rows, unit = blockIdx.x / c.H / used_rows;
     const int i = kv_find(b, unit);
     const int rows = b.count[i] * a.G, wg_row0 = (unit - b.unit0[i]) * wg_rows;
-    const int r = rg * 4 + wave, row = wg_row0 + r;
-    if (r >= wg_rows || row >= rows) return;
+    const int row = wg_row0 + r;
+    if (row >= rows) return;
     int lo0, hi0, lo1, hi1;
     kv_range(a, b.len[i], b.count[i], wg_row0, lo0, hi0);
     kv_range(a, b.len[i], b.count[i], min(wg_row0 + wg_rows, rows) - 1, lo1, hi1);
@@ -389,24 +406,33 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvDev c, KvBatch b, KvAtte
     const size_t stride = (size_t)c.H * wg_rows;
     const size_t base = ((size_t)unit * a.splits * c.H + h) * wg_rows + r;
     float mx = KV_NEG;
-    for (int s = 0; s < splits; s++) mx = fmaxf(mx, a.part_ml[base + s * stride].x);
+    for (int s = lane; s < splits; s += 64) mx = fmaxf(mx, a.part_ml[base + s * stride].x);
+#pragma unroll
+    for (int x = 32; x; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
     float l = 0.f;
-    float o[KV_MAX_DIM / 64] = {};
-    for (int s = 0; s < splits; s++) {
+    constexpr int K = KV_MAX_DIM / 64;
+    float o[K] = {};
+#pragma unroll 4
+    for (int s = wave; s < splits; s += 4) {
         const float2 ml = a.part_ml[base + s * stride];
         const float f = kv_join_factor(ml.x, ml.y, mx);
         l += f * ml.y;
         const float* po = a.part_o + (base + s * stride) * c.Dp;
 #pragma unroll
-        for (int k = 0; k < KV_MAX_DIM / 64; k++)
+        for (int k = 0; k < K; k++)
             if (k * 64 + lane < c.Dp) o[k] += f * po[k * 64 + lane];
     }
-    size_t at;
-    kv_finish(c, b, a, i, h, row, mx, l, at);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-    for (int k = 0; k < KV_MAX_DIM / 64; k++)
-        if (k * 64 + lane < c.D) kv_store(a.out, at * c.D + k * 64 + lane, o[k] * inv, a.q.type);
+    for (int k = 0; k < K; k++) sh_o[wave][k * 64 + lane] = o[k];
+    if (lane == 0) sh_l[wave] = l;
+    __syncthreads();
+    const int d = threadIdx.x;
+    if (d >= c.D) return;
+    l = ((sh_l[0] + sh_l[1]) + sh_l[2]) + sh_l[3];
+    const float v = ((sh_o[0][d] + sh_o[1][d]) + sh_o[2][d]) + sh_o[3][d];
+    const size_t at = kv_row(c, b, a, i, h, row);
+    if (d == 0) kv_finish(c, b, a, i, h, row, mx, l);
+    kv_store(a.out, at * c.D + d, l == 0.f ? 0.f : v * (1.f / l), a.q.type);
 }
 
 // Weights from the kept scores of a step: a thread per slot.
@@ -423,7 +449,7 @@ __global__ __launch_bounds__(256) void kv_score_weights_kernel(KvDev c, KvBatch 
         int lo, hi;
         kv_range(a, len, b.count[i], r, lo, hi);
         if (slot < lo || slot >= hi) continue;
-        const float lse = a.lse2[(size_t)(b.tok0[i] + r / a.G) * c.H * a.G + h * a.G + r % a.G];
+        const float lse = a.lse2[kv_head_row(c, b, a, i, h, r)];
         if (lse == KV_NEG) continue;  // the mask hides every slot of the row
         sum += exp2f(scores[(int64_t)r * score_row + slot] - lse);
     }
@@ -432,66 +458,151 @@ __global__ __launch_bounds__(256) void kv_score_weights_kernel(KvDev c, KvBatch 
     *w = a.decay == 0.f ? sum : a.decay * *w + sum;
 }
 
-// Weights by a second pass over the keys: a wave per tile, every row of the head.
+// Weights of calls with many rows, by a second pass over the keys:  w_j = sum_r
+// 2^(u_rj - lse_r).  The attention left its query operands (a.qop) and each row's
+// factor (a.qs) and logarithm.  A wave holds the operands of KV_WT tiles and goes over
+// the rows of its chunk, 32 at a time through LDS, which the four waves share; the
+// chunks' sums are added in their order by kv_chunk_weights_kernel.  Bound by the
+// exponentials: 16 cycles of a SIMD for 64 of them, against 16 of the matrix unit for
+// the 512 multiply-adds of 4 scores of 128 dims.
+constexpr int KV_WT = 2;              // 32-slot tiles of a wave
+constexpr int KV_WG_SLOTS = 4 * KV_WT * KV_TILE;
+
 template <int S, int CODE, int PARTS>
-__global__ __launch_bounds__(256) void kv_tile_weights_kernel(KvDev c, KvBatch b, KvAttend a) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+__global__ __launch_bounds__(256, 2) void kv_tile_weights_kernel(KvDev c, KvBatch b, KvAttend a) {
+    extern __shared__ __align__(16) uint4 qbuf[];  // [2][2 row tiles][PARTS * S][64]
+    constexpr int QT = PARTS * S * 64;             // 16-byte pieces of a row tile
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, col = lane & 15;
-    const int h = blockIdx.x % c.H, unit = blockIdx.x / c.H;
+    const int h = blockIdx.x % c.H, chunk = blockIdx.x / c.H % a.chunks, unit = blockIdx.x / c.H / a.chunks;
     const int i = kv_find(b, unit);
     const int len = b.len[i], rows = b.count[i] * a.G;
-    const int t = (unit - b.unit0[i]) * 4 + wave;
-    if (t * KV_TILE >= len) return;
+    const int slots0 = (unit - b.unit0[i]) * KV_WG_SLOTS;
+    const int t0 = slots0 / KV_TILE + wave * KV_WT;
     const int* table = c.table + (size_t)b.seq[i] * c.W;
     const int per_block = c.shift - 5;
-    const int block = __builtin_amdgcn_readfirstlane(table[t >> per_block]);
-    const size_t part = (size_t)block * c.H + h;
-    const float ks = c.kscale[part];
-    const uint4* p = (const uint4*)(c.pool + kv_tile_offset(c, block, h, t & ((1 << per_block) - 1))) + lane;
-    half8 k[2 * S];
-#pragma unroll
-    for (int s = 0; s < S; s++) {
-        const uint4 r = p[s * 64];
-        k[2 * s] = kv_half8<CODE>(r.x, r.y);
-        k[2 * s + 1] = kv_half8<CODE>(r.z, r.w);
+    // rows of the chunk that see a slot of the workgroup
+    int r0 = chunk * a.chunk_rows, r1 = min(r0 + a.chunk_rows, rows);
+    if (a.causal) {
+        // token p sees slot0 from p = slot0 on: row (slot0 - (len - count)) * G
+        const int tok = slots0 - (len - b.count[i]);
+        if (tok > 0) r0 = max(r0, (int)min((int64_t)tok * a.G, (int64_t)rows) / 32 * 32);
     }
-    floatx4 sum[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-    for (int row0 = 0; row0 < rows; row0 += 16) {
-        int lo0, hi0, lo1, hi1;
-        kv_range(a, len, b.count[i], row0, lo0, hi0);
-        kv_range(a, len, b.count[i], min(row0 + 16, rows) - 1, lo1, hi1);
-        if (hi1 <= t * KV_TILE || lo0 >= (t + 1) * KV_TILE) continue;
-        KvWave<S, CODE, PARTS, 1> w;
-        kv_load_rows(w, c, b, a, i, h, row0);
-        const int row = row0 + col;
-        const float lse = row < rows ? a.lse2[(size_t)(b.tok0[i] + row / a.G) * c.H * a.G + h * a.G + row % a.G] : KV_NEG;
-        floatx4 u[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    if (a.window) {
+        const int64_t tok = (int64_t)min(slots0 + KV_WG_SLOTS, len) - 1 + a.window - (len - b.count[i]);
+        r1 = (int)min((int64_t)r1, max(tok, (int64_t)0) * a.G);
+    }
+    half8 k[KV_WT][2 * S];
+    float ks[KV_WT];
 #pragma unroll
-        for (int o = 0; o < 2 * S; o++)
+    for (int x = 0; x < KV_WT; x++) {
+        ks[x] = 0.f;
+        const bool in = (t0 + x) * KV_TILE < len;
+        const int t = in ? t0 + x : 0;  // a tile past the end: any that exists, unused
+        const int block = __builtin_amdgcn_readfirstlane(table[t >> per_block]);
+        ks[x] = c.kscale[(size_t)block * c.H + h];
+        const uint4* p = (const uint4*)(c.pool + kv_tile_offset(c, block, h, t & ((1 << per_block) - 1))) + lane;
 #pragma unroll
-            for (int x = 0; x < PARTS; x++)
-                u[o / S] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[o], w.q[0][x][o % S], u[o / S], 0, 0, 0);
-        const float f = w.qs[0] * ks;
+        for (int s = 0; s < S; s++) {
+            const uint4 r = p[s * 64];
+            k[x][2 * s] = kv_half8<CODE>(r.x, r.y);
+            k[x][2 * s + 1] = kv_half8<CODE>(r.z, r.w);
+        }
+    }
+    float sum[KV_WT][8] = {};
+    const size_t row_base = kv_head_row(c, b, a, i, h, 0);
+    const uint4* qop = a.qop + ((size_t)(b.aux[i]) * c.H + (size_t)h * ((rows + 15) / 16)) * QT;
+    const int last_piece = (rows + 15) / 16 * QT - 1;
+    constexpr int PIECES = (2 * QT + 255) / 256;  // of one thread and step
+    uint4 next[PIECES];
+    if (r0 < r1)
+#pragma unroll
+        for (int x = 0; x < PIECES; x++) next[x] = qop[min(r0 / 16 * QT + x * 256 + tid, last_piece)];
+    int buf = 0;
+    for (int r = r0; r < r1; r += 32, buf ^= 1) {
+        uint4* to = qbuf + buf * 2 * QT;
+#pragma unroll
+        for (int x = 0; x < PIECES; x++)
+            if (x * 256 + tid < 2 * QT) to[x * 256 + tid] = next[x];
+        __syncthreads();
+        if (r + 32 < r1)
+#pragma unroll
+            for (int x = 0; x < PIECES; x++) next[x] = qop[min((r + 32) / 16 * QT + x * 256 + tid, last_piece)];
+#pragma unroll
+        for (int y = 0; y < 2; y++) {
+            const int row0 = r + 16 * y, row = row0 + col;
+            if (row0 >= r1) break;
+            int lo0, hi0, lo1, hi1;
+            kv_range(a, len, b.count[i], row0, lo0, hi0);
+            kv_range(a, len, b.count[i], min(row0 + 16, rows) - 1, lo1, hi1);
+            if (hi1 <= t0 * KV_TILE || lo0 >= (t0 + KV_WT) * KV_TILE) continue;
+            const bool real = row < min(r1, rows);
+            float f = real ? a.qs[row_base + row] : 0.f;
+            float lse = real ? a.lse2[row_base + row] : -KV_NEG;
+            if (lse == KV_NEG) lse = -KV_NEG;  // sees nothing: every p is 0
+            floatx4 u[KV_WT][2];
+#pragma unroll
+            for (int x = 0; x < KV_WT; x++) u[x][0] = u[x][1] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < S; s++)
+#pragma unroll
+                for (int p = 0; p < PARTS; p++) {
+                    const half8 q = __builtin_bit_cast(half8, to[y * QT + (p * S + s) * 64 + lane]);
+#pragma unroll
+                    for (int x = 0; x < KV_WT; x++)
+#pragma unroll
+                        for (int j = 0; j < 2; j++)
+                            u[x][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[x][j * S + s], q, u[x][j], 0, 0, 0);
+                }
+            const bool inside = !a.mask && lo1 <= t0 * KV_TILE && hi0 >= (t0 + KV_WT) * KV_TILE;
+            if (inside) {
+#pragma unroll
+                for (int x = 0; x < KV_WT; x++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        sum[x][j] += __builtin_amdgcn_exp2f(__builtin_fmaf(u[x][j >> 2][j & 3], f * ks[x], -lse));
+            } else {
+                int lo = 0, hi = 0;
+                if (real) kv_range(a, len, b.count[i], row, lo, hi);
+#pragma unroll
+                for (int x = 0; x < KV_WT; x++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const int slot = (t0 + x) * KV_TILE + (j >> 2) * 16 + 4 * g + (j & 3);
+                        bool see = slot >= lo && slot < hi;
+                        if (see && a.mask) see = a.mask[(int64_t)(b.tok0[i] + row / a.G) * a.mask_st + slot * a.mask_ss] != 0;
+                        sum[x][j] += see ? __builtin_amdgcn_exp2f(__builtin_fmaf(u[x][j >> 2][j & 3], f * ks[x], -lse)) : 0.f;
+                    }
+            }
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < KV_WT; x++)
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const int slot = t * KV_TILE + (j >> 2) * 16 + 4 * g + (j & 3);
-            bool see = slot >= w.lo[0] && slot < w.hi[0] && lse != KV_NEG;
-            if (see && a.mask) see = a.mask[(int64_t)(b.tok0[i] + row / a.G) * a.mask_st + slot * a.mask_ss] != 0;
-            sum[j >> 2][j & 3] += see ? exp2f(u[j >> 2][j & 3] * f - lse) : 0.f;
-        }
-    }
+            float v = sum[x][j];
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        float v = sum[j >> 2][j & 3];
-#pragma unroll
-        for (int x = 1; x < 16; x <<= 1) v += __shfl_xor(v, x);
-        const int slot = t * KV_TILE + (j >> 2) * 16 + 4 * g + (j & 3);
-        if (col == j && slot < len) {
-            float* wt = c.weights + part * c.B + (slot & (c.B - 1));
-            *wt = a.decay == 0.f ? v : a.decay * *wt + v;
+            for (int y = 1; y < 16; y <<= 1) v += __shfl_xor(v, y);
+            // partial sums of the chunk: [unit, H, chunk, slot of the workgroup]
+            const int slot = (wave * KV_WT + x) * KV_TILE + (j >> 2) * 16 + 4 * g + (j & 3);
+            if (col == j) a.wpart[(((size_t)unit * c.H + h) * a.chunks + chunk) * KV_WG_SLOTS + slot] = v;
         }
-    }
 }
+
+// A thread per slot: the chunks' sums, and the weight.
+__global__ __launch_bounds__(256) void kv_chunk_weights_kernel(KvDev c, KvBatch b, KvAttend a) {
+    const int h = blockIdx.x % c.H, unit = blockIdx.x / c.H;
+    const int i = kv_find(b, unit);
+    const int slot = (unit - b.unit0[i]) * KV_WG_SLOTS + threadIdx.x;
+    if (slot >= b.len[i]) return;
+    float sum = 0.f;
+    for (int x = 0; x < a.chunks; x++)
+        sum += a.wpart[(((size_t)unit * c.H + h) * a.chunks + x) * KV_WG_SLOTS + threadIdx.x];
+    const int block = c.table[(size_t)b.seq[i] * c.W + (slot >> c.shift)];
+    float* w = c.weights + ((size_t)block * c.H + h) * c.B + (slot & (c.B - 1));
+    *w = a.decay == 0.f ? sum : a.decay * *w + sum;
+}
+static_assert(KV_WG_SLOTS == 256, "one thread per slot of a workgroup");
 
 template <int S, int CODE, int PARTS, int NC, bool BY_ROWS>
 void attend_one(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s) {
@@ -514,7 +625,10 @@ void attend_s(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s
 
 template <int S, int CODE, int PARTS>
 void weights_s(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s) {
-    hipLaunchKernelGGL((kv_tile_weights_kernel<S, CODE, PARTS>), dim3((unsigned)b.unit0[b.n] * c.H), dim3(256), 0, s, c, b, a);
+    const size_t lds = (size_t)2 * 2 * PARTS * S * 1024;
+    const auto kernel = kv_tile_weights_kernel<S, CODE, PARTS>;
+    if (lds > 65536) ensure_dyn_lds((const void*)kernel, lds);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)b.unit0[b.n] * c.H * a.chunks), dim3(256), lds, s, c, b, a);
 }
 
 template <int CODE, int PARTS, bool WEIGHTS>
@@ -552,16 +666,22 @@ void launch_kv_attend(const KvDev& c, const KvBatch& b, const KvAttend& a, hipSt
     by_type<false>(c, b, a, s);
     if (a.splits > 1) {
         const int rows = kv_attend_rows(a);
-        hipLaunchKernelGGL(kv_join_kernel, dim3((unsigned)b.unit0[b.n] * c.H * ((rows + 3) / 4)), dim3(256), 0, s, c, b, a, rows);
+        int most = 1;
+        for (int i = 0; i < b.n; i++) most = b.count[i] * a.G > most ? b.count[i] * a.G : most;
+        const int used = most < rows ? most : rows;
+        hipLaunchKernelGGL(kv_join_kernel, dim3((unsigned)b.unit0[b.n] * c.H * used), dim3(256), 0, s, c, b, a, rows, used);
     }
 }
 
 void launch_kv_weights(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s) {
     if (!b.unit0[b.n]) return;
-    if (a.scores)
-        hipLaunchKernelGGL(kv_score_weights_kernel, dim3((unsigned)b.unit0[b.n] * c.H), dim3(256), 0, s, c, b, a);
-    else
-        by_type<true>(c, b, a, s);
+    const dim3 grid((unsigned)b.unit0[b.n] * c.H);
+    if (a.scores) {
+        hipLaunchKernelGGL(kv_score_weights_kernel, grid, dim3(256), 0, s, c, b, a);
+        return;
+    }
+    by_type<true>(c, b, a, s);
+    hipLaunchKernelGGL(kv_chunk_weights_kernel, grid, dim3(256), 0, s, c, b, a);
 }
 
 }  // namespace vgpu

@@ -19,6 +19,7 @@ size_t item_size(int type) { return type == KV_F32 ? 4 : 2; }
 // Workgroups that a step is cut into: three for each of the 256 compute units, so
 // that sequences of different lengths even out.
 constexpr int64_t kStepWorkgroups = 768;
+constexpr int64_t kWeightWorkgroups = 1024;
 // Bytes of partial results of one launch.
 constexpr int64_t kPartBytes = (int64_t)256 << 20;
 // Steps of at most this many rows per head keep their scores for the weights.
@@ -80,7 +81,7 @@ KvCache::~KvCache() {
 size_t KvCache::device_bytes() const {
     return pool.bytes() + kscale.bytes() + vscale.bytes() + weights.bytes() + positions.bytes() + table.bytes() +
            table2.bytes() + w_kept.bytes() + w_gone.bytes() + w_part.bytes() + w_scores.bytes() + w_lse2.bytes() +
-           w_ml.bytes();
+           w_ml.bytes() + w_qop.bytes() + w_qs.bytes() + w_wpart.bytes();
 }
 
 void KvCache::check_call(const int32_t* ids, size_t n, hipStream_t s) {
@@ -405,9 +406,14 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
     a.by_rows = most >= 64;
     a.nc = a.by_rows && dev.Dp <= 128 ? 2 : 1;
     const bool keep_scores = a.track && !a.by_rows && most <= kScoreRows;
+    const int parts = a.q.type == KV_F32 ? 2 : 1;
     if (a.track) {
         grow(w_lse2, (size_t)tokens * q.num_q_heads);
         a.lse2 = w_lse2.p;
+        if (!keep_scores) {
+            grow(w_qs, (size_t)tokens * q.num_q_heads);
+            a.qs = w_qs.p;
+        }
     }
     const int rows = kv_attend_rows(a);
     int64_t tok = 0;
@@ -415,7 +421,7 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
         KvBatch b;
         b.n = 0;
         b.unit0[0] = 0;
-        int64_t work = 0, score_tiles = 0, tiles_max = 1;
+        int64_t work = 0, score_tiles = 0, row_tiles = 0, tiles_max = 1;
         for (size_t i = i0; i < std::min(n, i0 + KV_BATCH); i++) {
             const int64_t len = seqs[ids[i]].len;
             const int j = b.n++;
@@ -429,8 +435,9 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
             tok += counts[i];
             int64_t tiles = (len + KV_TILE - 1) / KV_TILE;
             need(score_tiles <= INT_MAX / 2, "too many scores in one call");
-            b.aux[j] = (int)score_tiles;
+            b.aux[j] = (int)(keep_scores ? score_tiles : row_tiles);
             if (keep_scores) score_tiles += tiles * counts[i] * a.G;
+            row_tiles += (counts[i] * a.G + 15) / 16;
             // tiles that a row tile can see
             if (a.window && a.causal) tiles = std::min<int64_t>(tiles, (a.window + rows / a.G + 2 * KV_TILE) / KV_TILE + 1);
             tiles_max = std::max(tiles_max, tiles);
@@ -457,11 +464,23 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
                 grow(w_scores, (size_t)score_tiles * KV_TILE * dev.H);
                 a.scores = w_scores.p;
             }
+            if (a.track && !keep_scores) {
+                grow(w_qop, (size_t)row_tiles * dev.H * parts * (dev.Dp / 32) * 64);
+                a.qop = w_qop.p;
+            }
             launch_kv_attend(dev, b, a, s);
         }
         if (a.track) {
-            const int per = keep_scores ? 256 : 4 * KV_TILE;
-            for (int j = 0; j < b.n; j++) b.unit0[j + 1] = b.unit0[j] + (b.len[j] + per - 1) / per;
+            for (int j = 0; j < b.n; j++) b.unit0[j + 1] = b.unit0[j] + (b.len[j] + 255) / 256;
+            if (!keep_scores) {
+                // chunks of at least 256 rows, until there are four workgroups to a compute unit
+                const int64_t units = std::max<int64_t>((int64_t)b.unit0[b.n] * dev.H, 1);
+                const int64_t chunks = std::min((most + 255) / 256, (kWeightWorkgroups + units - 1) / units);
+                a.chunk_rows = (int)(((most + chunks - 1) / chunks + 31) / 32 * 32);
+                a.chunks = (int)((most + a.chunk_rows - 1) / a.chunk_rows);
+                grow(w_wpart, (size_t)(units * a.chunks * 256));
+                a.wpart = w_wpart.p;
+            }
             launch_kv_weights(dev, b, a, s);
         }
     }

@@ -138,7 +138,14 @@ struct KvAttend {
     float decay = 0.f;
     void* out = nullptr;       // [tokens, H * G, D] in q's type
     float* lse = nullptr;      // [tokens, H * G]
-    float* lse2 = nullptr;     // tracked: base-2 lse of the same rows (-inf: sees nothing)
+    // tracked: base-2 lse of the rows, [sequence][head][row] (-inf: sees nothing)
+    float* lse2 = nullptr;
+    // tracked chunks: the query operands of 16-row tiles, [tile of the sequences before and of
+    // the heads before][part][32-dim step][lane], and the factor of each row, as lse2
+    uint4* qop = nullptr;
+    float* qs = nullptr;
+    float* wpart = nullptr;    // sums of `chunks` chunks of chunk_rows rows
+    int chunks = 1, chunk_rows = 0;
     float* part_o = nullptr;   // split attention: partial rows [workgroup, rows, Dp]
     float2* part_ml = nullptr; // and their (max, sum), base 2
     float* scores = nullptr;   // tracked steps: base-2 scores [row, tile, 32] of each (sequence, head)
@@ -151,8 +158,8 @@ struct KvAttend {
 inline int kv_attend_rows(const KvAttend& a) { return 16 * a.nc * (a.by_rows ? 4 : 1); }
 // unit0 counts row tiles of the sequences (of one head); the launch is unit0[n] * H * splits.
 void launch_kv_attend(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s);
-// With scores, aux: tiles of the score rows of the sequences before (of one head);
-// unit0 counts 256 slots, without scores 128.
+// unit0 counts 256 slots.  aux: with scores the tiles of the score rows of the sequences
+// before (of one head), without them the 16-row tiles of the sequences before.
 void launch_kv_weights(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s);
 
 }  // namespace vgpu

@@ -347,7 +347,8 @@ struct KvCache {
     DevBuf<int> positions, table;
     DevBuf<int> table2;              // eviction in place: the new blocks
     DevBuf<int> w_kept, w_gone;      // eviction: slots that stay, slots that leave
-    DevBuf<float> w_part, w_scores, w_lse2;
+    DevBuf<float> w_part, w_scores, w_lse2, w_qs, w_wpart;
+    DevBuf<uint4> w_qop;
     DevBuf<float2> w_ml;
 
     struct Seq {
