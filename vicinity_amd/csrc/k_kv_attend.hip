@@ -137,101 +137,145 @@ __device__ __forceinline__ void kv_load_rows(KvWave<S, CODE, PARTS, NC>& w, cons
     }
 }
 
-// One tile of 32 slots from `slot0` on; ks, vs: its block's scales; inside: every row
-// sees all of it.
+// What a wave needs to know of 64 tiles, one to a lane: refilled every 64 tiles, so no
+// step waits for the block table or a scale.
+struct KvTiles {
+    int block;
+    float ks, lv, rv;  // key scale, log2 and inverse of the value scale
+    uint64_t bad;      // tiles whose value scale is NaN
+};
+
+// Tiles first, first + step, ... below last, for lanes 0, 1, ...
+__device__ __forceinline__ KvTiles kv_tile_infos(const KvDev& c, const int* table, int h, int first, int step, int last) {
+    const int t = first + (threadIdx.x & 63) * step;
+    KvTiles r;
+    const bool in = t < last;
+    r.block = in ? table[t >> (c.shift - 5)] : 0;
+    const size_t part = (size_t)r.block * c.H + h;
+    r.ks = in ? c.kscale[part] : 0.f;
+    const float vs = in ? c.vscale[part] : 1.f;
+    r.bad = __ballot(vs != vs);
+    const float sv = vs > 0.f ? vs : 1.f;  // a scale of 0 stands for codes of 0: any number does
+    r.lv = log2f(sv);
+    r.rv = 1.f / sv;
+    return r;
+}
+__device__ __forceinline__ float kv_lane(float v, int lane) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), lane));
+}
+
+__device__ __forceinline__ float kv_max8(const float (&x)[8]) {
+    return fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+}
+
+// The softmax of a tile: u are its products with the rows, p0 (and p1) the probabilities
+// in operand order.  inside: every row sees all 32 slots.
 template <int S, int CODE, int PARTS, int NC>
-__device__ __forceinline__ void kv_tile_step(KvWave<S, CODE, PARTS, NC>& w, const uint4 (&kc)[S], const uint4 (&vc)[S],
-                                             float ks, float vs, int slot0, bool inside, const KvAttend& a,
-                                             int tok0, float* scores, int64_t score_row) {
-    const int lane = threadIdx.x & 63, g = lane >> 4;
-    floatx4 u[NC][2];
+__device__ __forceinline__ void kv_softmax(KvWave<S, CODE, PARTS, NC>& w, const floatx4 (&u)[NC][2], float ks, float lv,
+                                           float rv, bool bad, int slot0, bool inside, const KvAttend& a, int tok0,
+                                           float* scores, int64_t score_row, half8 (&p0)[NC], half8 (&p1)[NC]) {
+    const int g = (threadIdx.x & 63) >> 4;
+    float x[NC][8];  // scores above m - KV_TOP (above 0 while there is no m)
+    bool over = false;
+    if (inside && !scores) {
 #pragma unroll
-    for (int n = 0; n < NC; n++) u[n][0] = u[n][1] = floatx4{0.f, 0.f, 0.f, 0.f};
+        for (int n = 0; n < NC; n++) {
+            const float f = w.qs[n] * ks, base = w.m[n] == KV_NEG ? lv : lv - (w.m[n] - KV_TOP);
 #pragma unroll
-    for (int o = 0; o < 2 * S; o++) {
-        const uint4 r = kc[o >> 1];
-        const half8 k = o & 1 ? kv_half8<CODE>(r.z, r.w) : kv_half8<CODE>(r.x, r.y);
+            for (int j = 0; j < 8; j++) x[n][j] = __builtin_fmaf(u[n][j >> 2][j & 3], f, base);
+        }
+        if (bad)
 #pragma unroll
-        for (int n = 0; n < NC; n++)
+            for (int n = 0; n < NC; n++) w.bad[n] = __uint_as_float(0x7fc00000u);
+    } else {
 #pragma unroll
-            for (int p = 0; p < PARTS; p++)
-                u[n][o / S] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, w.q[n][p][o % S], u[n][o / S], 0, 0, 0);
-    }
-    // A scale of 0 stands for codes of 0: any number does.  NaN is kept apart.
-    const float sv = vs > 0.f ? vs : 1.f;
-    const float lv = __log2f(sv);
-    const float rv = 1.f / sv;
-    half8 p0[NC], p1[NC];
-#pragma unroll
-    for (int n = 0; n < NC; n++) {
-        const float f = w.qs[n] * ks;
-        float x[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = u[n][j >> 2][j & 3] * f;
-        if (!inside) {
-            bool any = false;
+        for (int n = 0; n < NC; n++) {
+            const float f = w.qs[n] * ks, base = w.m[n] == KV_NEG ? lv : lv - (w.m[n] - KV_TOP);
+            bool any = inside;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const int slot = slot0 + (j >> 2) * 16 + 4 * g + (j & 3);
-                bool see = slot >= w.lo[n] && slot < w.hi[n];
-                if (see && a.mask) see = a.mask[(int64_t)(tok0 + w.row[n] / a.G) * a.mask_st + slot * a.mask_ss] != 0;
-                x[j] = see ? x[j] : KV_NEG;
-                any |= see;
+                x[n][j] = u[n][j >> 2][j & 3] * f;
+                if (!inside) {
+                    const int slot = slot0 + (j >> 2) * 16 + 4 * g + (j & 3);
+                    bool see = slot >= w.lo[n] && slot < w.hi[n];
+                    if (see && a.mask) see = a.mask[(int64_t)(tok0 + w.row[n] / a.G) * a.mask_st + slot * a.mask_ss] != 0;
+                    x[n][j] = see ? x[n][j] : KV_NEG;
+                    any |= see;
+                }
             }
-            if (vs != vs && any) w.bad[n] = vs;
-        } else if (vs != vs) {
-            w.bad[n] = vs;
-        }
-        if (scores && w.row[n] >= 0) {
-            float4* at = (float4*)(scores + (int64_t)w.row[n] * score_row + slot0);
-            at[g] = make_float4(x[0], x[1], x[2], x[3]);
-            at[4 + g] = make_float4(x[4], x[5], x[6], x[7]);
-        }
-        float top = KV_NEG;
+            if (bad && any) w.bad[n] = __uint_as_float(0x7fc00000u);
+            if (scores && w.row[n] >= 0) {
+                float4* at = (float4*)(scores + (int64_t)w.row[n] * score_row + slot0);
+                at[g] = make_float4(x[n][0], x[n][1], x[n][2], x[n][3]);
+                at[4 + g] = make_float4(x[n][4], x[n][5], x[n][6], x[n][7]);
+            }
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            x[j] += lv;
-            top = fmaxf(top, x[j]);
+            for (int j = 0; j < 8; j++) x[n][j] += base;
         }
-        if (__any(top > w.m[n] + KV_SLACK)) {
-            const float m1 = fmaxf(w.m[n], kv_max4(top));
+    }
+#pragma unroll
+    for (int n = 0; n < NC; n++) over |= kv_max8(x[n]) > (w.m[n] == KV_NEG ? KV_NEG : KV_TOP + KV_SLACK);
+    if (__any(over)) {
+#pragma unroll
+        for (int n = 0; n < NC; n++) {
+            const float was = w.m[n] == KV_NEG ? 0.f : w.m[n] - KV_TOP;
+            const float m1 = fmaxf(w.m[n], kv_max4(kv_max8(x[n])) + was);
+            const float now = m1 == KV_NEG ? 0.f : m1 - KV_TOP;
             const float f1 = w.m[n] == KV_NEG ? 0.f : exp2f(w.m[n] - m1);
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[n][j] += was - now;
             w.m[n] = m1;
             w.l[n] *= f1;
 #pragma unroll
             for (int j = 0; j < 2 * S; j++) w.o[n][j] *= f1;
         }
-        const float m = w.m[n] == KV_NEG ? 0.f : w.m[n] - KV_TOP;
+    }
+#pragma unroll
+    for (int n = 0; n < NC; n++) {
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float p = __builtin_amdgcn_exp2f(x[j] - m);
+            const float p = __builtin_amdgcn_exp2f(x[n][j]);
             sum += p;
             const _Float16 ph = (_Float16)p;
             p0[n][j] = ph;
             if (PARTS > 1) p1[n][j] = (_Float16)(p - (float)ph);
         }
-        w.l[n] += sum * rv;
+        w.l[n] = __builtin_fmaf(sum, rv, w.l[n]);
     }
+}
+
+// Products of a tile's keys with the rows.
+template <int S, int CODE, int PARTS>
+__device__ __forceinline__ void kv_scores(const KvWave<S, CODE, PARTS, 1>& w, const uint4 (&kc)[S], floatx4 (&u)[1][2]) {
+    u[0][0] = u[0][1] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int o = 0; o < 2 * S; o++) {
+        const uint4 r = kc[o >> 1];
+        const half8 k = o & 1 ? kv_half8<CODE>(r.z, r.w) : kv_half8<CODE>(r.x, r.y);
+#pragma unroll
+        for (int p = 0; p < PARTS; p++)
+            u[0][o / S] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, w.q[0][p][o % S], u[0][o / S], 0, 0, 0);
+    }
+}
+
+template <int S, int CODE, int PARTS>
+__device__ __forceinline__ void kv_add_values(KvWave<S, CODE, PARTS, 1>& w, const uint4 (&vc)[S], const half8& p0, const half8& p1) {
 #pragma unroll
     for (int o = 0; o < 2 * S; o++) {
         const uint4 r = vc[o >> 1];
         const half8 v = o & 1 ? kv_half8<CODE>(r.z, r.w) : kv_half8<CODE>(r.x, r.y);
-#pragma unroll
-        for (int n = 0; n < NC; n++) {
-            w.o[n][o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p0[n], w.o[n][o], 0, 0, 0);
-            if (PARTS > 1) w.o[n][o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p1[n], w.o[n][o], 0, 0, 0);
-        }
+        w.o[0][o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p0, w.o[0][o], 0, 0, 0);
+        if (PARTS > 1) w.o[0][o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p1, w.o[0][o], 0, 0, 0);
     }
 }
 
+// A half of a tile, 16 contiguous bytes of a lane at a time.
 template <int S>
-__device__ __forceinline__ void kv_fetch(uint4 (&k)[S], uint4 (&v)[S], const uint8_t* tile) {
-    const uint4* p = (const uint4*)tile + (threadIdx.x & 63);
+__device__ __forceinline__ void kv_fetch(uint4 (&k)[S], const uint8_t* half) {
+    const uint4* p = (const uint4*)half + (threadIdx.x & 63);
 #pragma unroll
     for (int s = 0; s < S; s++) k[s] = p[s * 64];
-#pragma unroll
-    for (int s = 0; s < S; s++) v[s] = p[(S + s) * 64];
 }
 
 // What a part with reference m and sum l is multiplied with under reference mx.  A part
@@ -256,38 +300,142 @@ __device__ __forceinline__ void kv_finish(const KvDev& c, const KvBatch& b, cons
     if (a.lse2) a.lse2[kv_head_row(c, b, a, i, h, row)] = lse2;
 }
 
-// BY_ROWS: the four waves take 4 * NC * 16 rows and every tile; else the same NC * 16
-// rows and every fourth tile, joined at the end.
-template <int S, int CODE, int PARTS, int NC, bool BY_ROWS>
-__global__ __launch_bounds__(256, 2) void kv_attend_kernel(KvDev c, KvBatch b, KvAttend a) {
+// First row of a workgroup: the last rows, which see most, start first.
+__device__ __forceinline__ int kv_unit_row0(const KvBatch& b, int i, int unit, int wg_rows) {
+    return (b.unit0[i + 1] - 1 - unit) * wg_rows;
+}
+
+// The tiles that some row of a workgroup sees (first .. last - 1), and its split's share.
+struct KvSpan {
+    int first, last, t0, t1;
+    bool whole;  // no other split has tiles
+};
+__device__ __forceinline__ KvSpan kv_span(const KvAttend& a, int len, int count, int row0, int row1, int split) {
+    int lo0, hi0, lo1, hi1;
+    kv_range(a, len, count, row0, lo0, hi0);
+    kv_range(a, len, count, row1 - 1, lo1, hi1);
+    KvSpan p;
+    p.first = lo0 / KV_TILE, p.last = (hi1 + KV_TILE - 1) / KV_TILE;
+    p.t0 = p.first + split * a.split_tiles, p.t1 = min(p.t0 + a.split_tiles, p.last);
+    p.whole = p.first + a.split_tiles >= p.last;
+    return p;
+}
+
+// Few rows: the four waves of a workgroup take the same 16 rows and every fourth tile,
+// joined at the end.  The next tile's keys are loaded when this one's are used up, under
+// its softmax and values, and its values under the next one's keys: one tile of registers.  Bound by the cache's bytes: a tile's 64 Dp bytes against 4 Dp / 16
+// matrix instructions of 16 cycles.
+template <int S, int CODE, int PARTS>
+__global__ __launch_bounds__(256, S <= 4 ? 3 : 2) void kv_step_kernel(KvDev c, KvBatch b, KvAttend a) {
     extern __shared__ __align__(16) float lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
     const int h = blockIdx.x % c.H, split = blockIdx.x / c.H % a.splits, unit = blockIdx.x / c.H / a.splits;
     const int i = kv_find(b, unit);
     const int len = b.len[i], rows = b.count[i] * a.G;
-    const int wg_rows = 16 * NC * (BY_ROWS ? 4 : 1);
-    const int wg_row0 = (unit - b.unit0[i]) * wg_rows;
-    const int row0 = wg_row0 + (BY_ROWS ? wave * 16 * NC : 0);
+    const int row0 = kv_unit_row0(b, i, unit, 16), row1 = min(row0 + 16, rows);
+    const KvSpan sp = kv_span(a, len, b.count[i], row0, row1, split);
+    if (split > 0 && sp.t0 >= sp.t1) return;
 
-    // tiles that some row of the workgroup sees
-    int lo0, hi0, lo1, hi1;
-    kv_range(a, len, b.count[i], wg_row0, lo0, hi0);
-    kv_range(a, len, b.count[i], min(wg_row0 + wg_rows, rows) - 1, lo1, hi1);
-    const int first = lo0 / KV_TILE, last = (hi1 + KV_TILE - 1) / KV_TILE;
-    const int t0 = first + split * a.split_tiles, t1 = min(t0 + a.split_tiles, last);
-    if (split > 0 && t0 >= t1) return;
-    const bool whole = first + a.split_tiles >= last;  // no other split has tiles
+    const int* table = c.table + (size_t)b.seq[i] * c.W;
+    const int per_block = c.shift - 5, in_block = (1 << per_block) - 1;
+    const int64_t score_row = (int64_t)((len + KV_TILE - 1) / KV_TILE) * KV_TILE;
+    float* scores = a.scores ? a.scores + (int64_t)b.aux[i] * KV_TILE * c.H + h * score_row * rows : nullptr;
+    int all_lo, all_hi, x0, x1;  // slots that every row sees
+    kv_range(a, len, b.count[i], row0, x0, all_hi);
+    kv_range(a, len, b.count[i], row1 - 1, all_lo, x1);
+
+    const int n = max((sp.t1 - sp.t0 - wave + 3) / 4, 0);  // tiles of this wave
+    const int tw = sp.t0 + wave;
+    KvTiles info = kv_tile_infos(c, table, h, tw, 4, sp.t1);
+    const auto tile = [&](const KvTiles& f, int x) {
+        return c.pool + kv_tile_offset(c, __builtin_amdgcn_readlane(f.block, x & 63), h, (tw + 4 * x) & in_block);
+    };
+    uint4 kc[S], vc[S];
+    if (n > 0) kv_fetch<S>(kc, tile(info, 0)), kv_fetch<S>(vc, tile(info, 0) + kv_half(32 * S));
+    KvWave<S, CODE, PARTS, 1> w;
+    kv_load_rows(w, c, b, a, i, h, row0);
+    for (int x = 0; x < n; x++) {
+        const int t = tw + 4 * x, y = x & 63;
+        const float ks = kv_lane(info.ks, y), lv = kv_lane(info.lv, y), rv = kv_lane(info.rv, y);
+        const bool bad = info.bad >> y & 1;
+        if (y == 63 && x + 1 < n) info = kv_tile_infos(c, table, h, t + 4, 4, sp.t1);
+        const uint8_t* next = tile(info, x + 1 < n ? x + 1 : x);
+        floatx4 u[1][2];
+        kv_scores(w, kc, u);
+        if (x + 1 < n) kv_fetch<S>(kc, next);
+        half8 p0[1], p1[1];
+        const bool inside = t * KV_TILE >= all_lo && (t + 1) * KV_TILE <= all_hi && !a.mask;
+        kv_softmax(w, u, ks, lv, rv, bad, t * KV_TILE, inside, a, b.tok0[i], scores, score_row, p0, p1);
+        kv_add_values(w, vc, p0[0], p1[0]);
+        if (x + 1 < n) kv_fetch<S>(vc, next + kv_half(32 * S));
+    }
+    w.l[0] = kv_sum4(w.l[0]), w.bad[0] = kv_sum4(w.bad[0]);
+
+    // join the four waves: rows of [wave][row][32 S + 4] floats, then (m, l)
+    constexpr int LDO = 32 * S + 4;
+    float* ml = lds + 4 * 16 * LDO;
+    const int r4 = wave * 16 + col;
+#pragma unroll
+    for (int j = 0; j < 2 * S; j++) *(floatx4*)(lds + r4 * LDO + 16 * j + 4 * g) = w.o[0][j] + w.bad[0];
+    if (g == 0) ml[2 * r4] = w.m[0], ml[2 * r4 + 1] = w.l[0];
+    __syncthreads();
+    for (int u = threadIdx.x; u < 16 * 8 * S; u += 256) {
+        const int r = u / (8 * S), d = u % (8 * S) * 4;
+        const int row = row0 + r;
+        if (row >= rows) break;
+        float mx = KV_NEG;
+#pragma unroll
+        for (int x = 0; x < 4; x++) mx = fmaxf(mx, ml[2 * (x * 16 + r)]);
+        floatx4 o = {0.f, 0.f, 0.f, 0.f};
+        float l = 0.f;
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+            const int rr = x * 16 + r;
+            const float f = kv_join_factor(ml[2 * rr], ml[2 * rr + 1], mx);
+            l += f * ml[2 * rr + 1];
+            o += *(const floatx4*)(lds + rr * LDO + d) * f;
+        }
+        if (sp.whole) {
+            const size_t at = kv_row(c, b, a, i, h, row);
+            if (d == 0) kv_finish(c, b, a, i, h, row, mx, l);
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (d + e < c.D) kv_store(a.out, at * c.D + d + e, o[e] * inv, a.q.type);
+        } else {
+            const size_t at = (size_t)blockIdx.x * 16 + r;
+            if (d == 0) a.part_ml[at] = make_float2(mx, l);
+            *(floatx4*)(a.part_o + at * (32 * S) + d) = o;
+        }
+    }
+}
+
+// Many rows: the four waves of a workgroup take 4 * NC * 16 rows and every tile.  A tile's
+// codes are converted once, a quarter by each wave, and shared as half-precision operands
+// through LDS (two buffers, one barrier to a tile); an operand read feeds NC products.
+template <int S, int CODE, int PARTS, int NC>
+__global__ __launch_bounds__(256, 2) void kv_chunk_kernel(KvDev c, KvBatch b, KvAttend a) {
+    __shared__ half8 tiles[2][4 * S][64];  // operands of keys, then of values
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4;
+    const int h = blockIdx.x % c.H, split = blockIdx.x / c.H % a.splits, unit = blockIdx.x / c.H / a.splits;
+    const int i = kv_find(b, unit);
+    const int len = b.len[i], rows = b.count[i] * a.G;
+    constexpr int WG_ROWS = 64 * NC;
+    const int wg_row0 = kv_unit_row0(b, i, unit, WG_ROWS);
+    const int row0 = wg_row0 + wave * 16 * NC;
+    const KvSpan sp = kv_span(a, len, b.count[i], wg_row0, min(wg_row0 + WG_ROWS, rows), split);
+    if (split > 0 && sp.t0 >= sp.t1) return;
 
     KvWave<S, CODE, PARTS, NC> w;
     kv_load_rows(w, c, b, a, i, h, row0);
-    // slots that every row of this wave sees, and those that any does
-    int all_lo = 0, all_hi = 0, any_lo = 0, any_hi = 0;
+    int all_lo = 0, all_hi = 0, x0, x1;  // slots that every row of this wave sees
     if (row0 < rows) {
-        kv_range(a, len, b.count[i], row0, any_lo, all_hi);
-        kv_range(a, len, b.count[i], min(row0 + 16 * NC, rows) - 1, all_lo, any_hi);
+        kv_range(a, len, b.count[i], row0, x0, all_hi);
+        kv_range(a, len, b.count[i], min(row0 + 16 * NC, rows) - 1, all_lo, x1);
     }
-    if (BY_ROWS && a.qop && split == 0) {
+    if (a.qop && split == 0) {
 #pragma unroll
         for (int n = 0; n < NC; n++) {
             const int tile = row0 / 16 + n;
@@ -299,89 +447,87 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(KvDev c, KvBatch b, K
         }
     }
     const int* table = c.table + (size_t)b.seq[i] * c.W;
-    const int step = BY_ROWS ? 1 : 4;
-    const int64_t score_row = (int64_t)((len + KV_TILE - 1) / KV_TILE) * KV_TILE;
-    float* scores = a.scores ? a.scores + (int64_t)b.aux[i] * KV_TILE * c.H + h * score_row * rows : nullptr;
-    const int per_block = c.shift - 5;
-    for (int t = t0 + (BY_ROWS ? 0 : wave); t < t1; t += step) {
-        if (BY_ROWS && (t * KV_TILE >= any_hi || (t + 1) * KV_TILE <= any_lo)) continue;
-        const int block = __builtin_amdgcn_readfirstlane(table[t >> per_block]);
-        const size_t part = (size_t)block * c.H + h;
-        uint4 kc[S], vc[S];
-        kv_fetch<S>(kc, vc, c.pool + kv_tile_offset(c, block, h, t & ((1 << per_block) - 1)));
-        const bool inside = t * KV_TILE >= all_lo && (t + 1) * KV_TILE <= all_hi && !a.mask;
-        kv_tile_step(w, kc, vc, c.kscale[part], c.vscale[part], t * KV_TILE, inside, a, b.tok0[i], scores, score_row);
-    }
+    const int per_block = c.shift - 5, in_block = (1 << per_block) - 1;
+    constexpr int PIECES = (2 * S * 64 + 255) / 256;  // 16-byte pieces of a tile for one thread
+    uint4 next[PIECES];
+    const auto fetch = [&](int t, int block) {
+        const uint4* p = (const uint4*)(c.pool + kv_tile_offset(c, block, h, t & in_block));
 #pragma unroll
-    for (int n = 0; n < NC; n++) w.l[n] = kv_sum4(w.l[n]), w.bad[n] = kv_sum4(w.bad[n]);
-
-    if (BY_ROWS) {
+        for (int x = 0; x < PIECES; x++)
+            if (x * 256 + tid < 2 * S * 64) next[x] = p[x * 256 + tid];
+    };
+    const auto stage = [&](int buf) {
 #pragma unroll
-        for (int n = 0; n < NC; n++) {
-            if (w.row[n] < 0) continue;
-            if (whole) {
-                const size_t at = kv_row(c, b, a, i, h, w.row[n]);
-                if (g == 0) kv_finish(c, b, a, i, h, w.row[n], w.m[n], w.l[n]);
-                const float inv = w.l[n] == 0.f ? 0.f : 1.f / w.l[n];
-#pragma unroll
-                for (int j = 0; j < 2 * S; j++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int d = 16 * j + 4 * g + e;
-                        if (d < c.D) kv_store(a.out, at * c.D + d, w.o[n][j][e] * inv + w.bad[n], a.q.type);
-                    }
-            } else {
-                const size_t at = (size_t)blockIdx.x * wg_rows + (w.row[n] - wg_row0);
-                if (g == 0) a.part_ml[at] = make_float2(w.m[n], w.l[n]);
-#pragma unroll
-                for (int j = 0; j < 2 * S; j++) {
-                    const floatx4 v = w.o[n][j] + w.bad[n];
-                    *(floatx4*)(a.part_o + at * (32 * S) + 16 * j + 4 * g) = v;
-                }
+        for (int x = 0; x < PIECES; x++)
+            if (x * 256 + tid < 2 * S * 64) {
+                const int piece = (x * 256 + tid) >> 6;
+                tiles[buf][2 * piece][lane] = kv_half8<CODE>(next[x].x, next[x].y);
+                tiles[buf][2 * piece + 1][lane] = kv_half8<CODE>(next[x].z, next[x].w);
             }
-        }
-        return;
-    }
-
-    // join the four waves: rows of [wave][row][32 S + 4] floats, then (m, l, bad)
-    constexpr int LDO = 32 * S + 4;
-    float* ml = lds + 4 * 16 * NC * LDO;
-#pragma unroll
-    for (int n = 0; n < NC; n++) {
-        const int r = wave * 16 * NC + n * 16 + col;
-#pragma unroll
-        for (int j = 0; j < 2 * S; j++) *(floatx4*)(lds + r * LDO + 16 * j + 4 * g) = w.o[n][j] + w.bad[n];
-        if (g == 0) ml[2 * r] = w.m[n], ml[2 * r + 1] = w.l[n];
+    };
+    KvTiles info = kv_tile_infos(c, table, h, sp.t0, 1, sp.t1), ahead = info;
+    if (sp.t0 < sp.t1) {
+        fetch(sp.t0, __builtin_amdgcn_readlane(info.block, 0));
+        stage(0);
+        if (sp.t0 + 1 < sp.t1) fetch(sp.t0 + 1, __builtin_amdgcn_readlane(info.block, 1));
     }
     __syncthreads();
-    for (int u = threadIdx.x; u < 16 * NC * 8 * S; u += 256) {
-        const int r = u / (8 * S), d = u % (8 * S) * 4;
-        const int row = row0 + r;
-        if (row >= rows) break;
-        float mx = KV_NEG;
-#pragma unroll
-        for (int x = 0; x < 4; x++) mx = fmaxf(mx, ml[2 * (x * 16 * NC + r)]);
-        floatx4 o = {0.f, 0.f, 0.f, 0.f};
-        float l = 0.f;
-#pragma unroll
-        for (int x = 0; x < 4; x++) {
-            const int rr = x * 16 * NC + r;
-            const float m = ml[2 * rr];
-            const float f = kv_join_factor(m, ml[2 * rr + 1], mx);
-            l += f * ml[2 * rr + 1];
-            o += *(const floatx4*)(lds + rr * LDO + d) * f;
+    for (int t = sp.t0; t < sp.t1; t++) {
+        const int x = t - sp.t0, buf = x & 1, y = x & 63;
+        if (y == 0) info = ahead;
+        if (t + 1 < sp.t1) stage(buf ^ 1);
+        if (t + 2 < sp.t1) {
+            // infos of the next 64 tiles two steps before the first of them
+            if (y == 62) ahead = kv_tile_infos(c, table, h, t + 2, 1, sp.t1);
+            fetch(t + 2, y >= 62 ? __builtin_amdgcn_readlane(ahead.block, y - 62) : __builtin_amdgcn_readlane(info.block, y + 2));
         }
-        if (whole) {
-            const size_t at = kv_row(c, b, a, i, h, row);
-            if (d == 0) kv_finish(c, b, a, i, h, row, mx, l);
-            const float inv = l == 0.f ? 0.f : 1.f / l;
+        const bool inside = t * KV_TILE >= all_lo && (t + 1) * KV_TILE <= all_hi && !a.mask;
+        floatx4 u[NC][2];
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (d + e < c.D) kv_store(a.out, at * c.D + d + e, o[e] * inv, a.q.type);
+        for (int n = 0; n < NC; n++) u[n][0] = u[n][1] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int o = 0; o < 2 * S; o++) {
+            const half8 k = tiles[buf][o][lane];
+#pragma unroll
+            for (int n = 0; n < NC; n++)
+#pragma unroll
+                for (int p = 0; p < PARTS; p++)
+                    u[n][o / S] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, w.q[n][p][o % S], u[n][o / S], 0, 0, 0);
+        }
+        half8 p0[NC], p1[NC];
+        kv_softmax(w, u, kv_lane(info.ks, y), kv_lane(info.lv, y), kv_lane(info.rv, y), info.bad >> y & 1, t * KV_TILE,
+                   inside, a, b.tok0[i], nullptr, 0, p0, p1);
+#pragma unroll
+        for (int o = 0; o < 2 * S; o++) {
+            const half8 v = tiles[buf][2 * S + o][lane];
+#pragma unroll
+            for (int n = 0; n < NC; n++) {
+                w.o[n][o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p0[n], w.o[n][o], 0, 0, 0);
+                if (PARTS > 1) w.o[n][o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p1[n], w.o[n][o], 0, 0, 0);
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int n = 0; n < NC; n++) {
+        w.l[n] = kv_sum4(w.l[n]), w.bad[n] = kv_sum4(w.bad[n]);
+        if (w.row[n] < 0) continue;
+        if (sp.whole) {
+            const size_t at = kv_row(c, b, a, i, h, w.row[n]);
+            if (g == 0) kv_finish(c, b, a, i, h, w.row[n], w.m[n], w.l[n]);
+            const float inv = w.l[n] == 0.f ? 0.f : 1.f / w.l[n];
+#pragma unroll
+            for (int j = 0; j < 2 * S; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int d = 16 * j + 4 * g + e;
+                    if (d < c.D) kv_store(a.out, at * c.D + d, w.o[n][j][e] * inv + w.bad[n], a.q.type);
+                }
         } else {
-            const size_t at = (size_t)blockIdx.x * wg_rows + r;
-            if (d == 0) a.part_ml[at] = make_float2(mx, l);
-            *(floatx4*)(a.part_o + at * (32 * S) + d) = o;
+            const size_t at = (size_t)blockIdx.x * WG_ROWS + (w.row[n] - wg_row0);
+            if (g == 0) a.part_ml[at] = make_float2(w.m[n], w.l[n]);
+#pragma unroll
+            for (int j = 0; j < 2 * S; j++) *(floatx4*)(a.part_o + at * (32 * S) + 16 * j + 4 * g) = w.o[n][j] + w.bad[n];
         }
     }
 }
@@ -394,7 +540,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvDev c, KvBatch b, KvAtte
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = blockIdx.x % c.H, r = blockIdx.x / c.H % used_rows, unit = blockIdx.x / c.H / used_rows;
     const int i = kv_find(b, unit);
-    const int rows = b.count[i] * a.G, wg_row0 = (unit - b.unit0[i]) * wg_rows;
+    const int rows = b.count[i] * a.G, wg_row0 = kv_unit_row0(b, i, unit, wg_rows);
     const int row = wg_row0 + r;
     if (row >= rows) return;
     int lo0, hi0, lo1, hi1;
@@ -604,23 +750,17 @@ __global__ __launch_bounds__(256) void kv_chunk_weights_kernel(KvDev c, KvBatch 
 }
 static_assert(KV_WG_SLOTS == 256, "one thread per slot of a workgroup");
 
-template <int S, int CODE, int PARTS, int NC, bool BY_ROWS>
-void attend_one(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s) {
-    const unsigned grid = (unsigned)b.unit0[b.n] * c.H * a.splits;
-    const size_t lds = BY_ROWS ? 0 : (size_t)4 * 16 * NC * (32 * S + 4 + 2) * 4;
-    const auto kernel = kv_attend_kernel<S, CODE, PARTS, NC, BY_ROWS>;
-    if (lds > 65536) ensure_dyn_lds((const void*)kernel, lds);
-    hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), lds, s, c, b, a);
-}
-
 template <int S, int CODE, int PARTS>
 void attend_s(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s) {
-    if (a.by_rows && a.nc == 2)
-        attend_one<S, CODE, PARTS, (S <= 4 ? 2 : 1), true>(c, b, a, s);
-    else if (a.by_rows)
-        attend_one<S, CODE, PARTS, 1, true>(c, b, a, s);
-    else
-        attend_one<S, CODE, PARTS, 1, false>(c, b, a, s);
+    const dim3 grid((unsigned)b.unit0[b.n] * c.H * a.splits);
+    if (a.by_rows) {
+        hipLaunchKernelGGL((kv_chunk_kernel<S, CODE, PARTS, kv_chunk_nc(S * 32, PARTS)>), grid, dim3(256), 0, s, c, b, a);
+        return;
+    }
+    const size_t lds = (size_t)4 * 16 * (32 * S + 4 + 2) * 4;
+    const auto kernel = kv_step_kernel<S, CODE, PARTS>;
+    if (lds > 65536) ensure_dyn_lds((const void*)kernel, lds);
+    hipLaunchKernelGGL(kernel, grid, dim3(256), lds, s, c, b, a);
 }
 
 template <int S, int CODE, int PARTS>
@@ -665,7 +805,7 @@ void launch_kv_attend(const KvDev& c, const KvBatch& b, const KvAttend& a, hipSt
     if (!b.unit0[b.n]) return;
     by_type<false>(c, b, a, s);
     if (a.splits > 1) {
-        const int rows = kv_attend_rows(a);
+        const int rows = kv_attend_rows(a, c.Dp);
         int most = 1;
         for (int i = 0; i < b.n; i++) most = b.count[i] * a.G > most ? b.count[i] * a.G : most;
         const int used = most < rows ? most : rows;

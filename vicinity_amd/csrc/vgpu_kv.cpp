@@ -19,6 +19,9 @@ size_t item_size(int type) { return type == KV_F32 ? 4 : 2; }
 // Workgroups that a step is cut into: three for each of the 256 compute units, so
 // that sequences of different lengths even out.
 constexpr int64_t kStepWorkgroups = 768;
+// Workgroups of a call with many rows, two to a compute unit: with fewer, the tiles are
+// split too, which costs a partial result for every row and split.
+constexpr int64_t kChunkWorkgroups = 512;
 constexpr int64_t kWeightWorkgroups = 1024;
 // Bytes of partial results of one launch.
 constexpr int64_t kPartBytes = (int64_t)256 << 20;
@@ -404,7 +407,6 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
 
     // Many rows: each wave has its own; few: the waves share them and split the tiles.
     a.by_rows = most >= 64;
-    a.nc = a.by_rows && dev.Dp <= 128 ? 2 : 1;
     const bool keep_scores = a.track && !a.by_rows && most <= kScoreRows;
     const int parts = a.q.type == KV_F32 ? 2 : 1;
     if (a.track) {
@@ -415,7 +417,7 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
             a.qs = w_qs.p;
         }
     }
-    const int rows = kv_attend_rows(a);
+    const int rows = kv_attend_rows(a, dev.Dp);
     int64_t tok = 0;
     for (size_t i0 = 0; i0 < n; i0 += KV_BATCH) {
         KvBatch b;
@@ -445,11 +447,16 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
         }
         if (b.unit0[b.n]) {
             const int64_t units = (int64_t)b.unit0[b.n] * dev.H;
-            int64_t per = std::max<int64_t>((work + kStepWorkgroups - 1) / kStepWorkgroups, a.by_rows ? 16 : 8);
+            int64_t splits;
+            if (a.by_rows) {
+                splits = units >= kChunkWorkgroups ? 1 : std::min((kChunkWorkgroups + units - 1) / units, (tiles_max + 15) / 16);
+            } else {
+                const int64_t each = std::max<int64_t>((work + kStepWorkgroups - 1) / kStepWorkgroups, 8);
+                splits = (tiles_max + each - 1) / each;
+            }
             const int64_t row_bytes = (int64_t)dev.Dp * 4 + 8;
-            int64_t splits = (tiles_max + per - 1) / per;
             splits = std::min(splits, std::max<int64_t>(kPartBytes / (units * rows * row_bytes), 1));
-            per = (tiles_max + splits - 1) / splits;
+            const int64_t per = (tiles_max + splits - 1) / splits;
             splits = (tiles_max + per - 1) / per;
             need(units * splits <= INT_MAX / 64, "too many query rows in one call");
             a.split_tiles = (int)per;

@@ -152,10 +152,14 @@ struct KvAttend {
     int split_tiles = 0;       // tiles of one split
     int splits = 0;            // splits of every row tile
     int by_rows = 0;           // waves of a workgroup take different rows (else different tiles)
-    int nc = 1;                // 16-row column tiles of a wave: 1, or 2 where Dp <= 128 and by_rows
 };
+// 16-row tiles of a wave of the many-row kernel, by what its registers hold: Dp / 4
+// accumulators and Dp * parts / 8 query operands for each.
+constexpr int kv_chunk_nc(int Dp, int parts) { return Dp * parts <= 64 ? 4 : Dp <= 192 && Dp * parts <= 256 ? 2 : 1; }
 // Rows that one workgroup takes.
-inline int kv_attend_rows(const KvAttend& a) { return 16 * a.nc * (a.by_rows ? 4 : 1); }
+inline int kv_attend_rows(const KvAttend& a, int Dp) {
+    return a.by_rows ? 64 * kv_chunk_nc(Dp, a.q.type == KV_F32 ? 2 : 1) : 16;
+}
 // unit0 counts row tiles of the sequences (of one head); the launch is unit0[n] * H * splits.
 void launch_kv_attend(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s);
 // unit0 counts 256 slots.  aux: with scores the tiles of the score rows of the sequences
