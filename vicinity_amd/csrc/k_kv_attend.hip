@@ -164,18 +164,24 @@ __device__ __forceinline__ float kv_lane(float v, int lane) {
     return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), lane));
 }
 
+// Largest of 8, a NaN only if all are (fmaxf would quiet each operand first).
 __device__ __forceinline__ float kv_max8(const float (&x)[8]) {
-    return fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x[0]), "v"(x[1]), "v"(x[2]));
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(r), "v"(x[3]), "v"(x[4]));
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(r), "v"(x[5]), "v"(x[6]));
+    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(r), "v"(x[7]));
+    return r;
 }
 
-// The softmax of a tile: u are its products with the rows, p0 (and p1) the probabilities
-// in operand order.  inside: every row sees all 32 slots.
+// A tile's base-2 scores above m - KV_TOP (above 0 while there is no m) from its products
+// u with the rows; m moves if one is too far above it.  inside: every row sees all 32
+// slots.
 template <int S, int CODE, int PARTS, int NC>
-__device__ __forceinline__ void kv_softmax(KvWave<S, CODE, PARTS, NC>& w, const floatx4 (&u)[NC][2], float ks, float lv,
-                                           float rv, bool bad, int slot0, bool inside, const KvAttend& a, int tok0,
-                                           float* scores, int64_t score_row, half8 (&p0)[NC], half8 (&p1)[NC]) {
+__device__ __forceinline__ void kv_reference(KvWave<S, CODE, PARTS, NC>& w, const floatx4 (&u)[NC][2], float ks, float lv,
+                                             bool bad, int slot0, bool inside, const KvAttend& a, int tok0, float* scores,
+                                             int64_t score_row, float (&x)[NC][8]) {
     const int g = (threadIdx.x & 63) >> 4;
-    float x[NC][8];  // scores above m - KV_TOP (above 0 while there is no m)
     bool over = false;
     if (inside && !scores) {
 #pragma unroll
@@ -230,16 +236,29 @@ __device__ __forceinline__ void kv_softmax(KvWave<S, CODE, PARTS, NC>& w, const 
             for (int j = 0; j < 2 * S; j++) w.o[n][j] *= f1;
         }
     }
+}
+
+// The probabilities of a tile in operand order (p1: their second halves), and the
+// denominators' sums.
+template <int S, int CODE, int PARTS, int NC>
+__device__ __forceinline__ void kv_exponents(KvWave<S, CODE, PARTS, NC>& w, const float (&x)[NC][8], float rv,
+                                             half8 (&p0)[NC], half8 (&p1)[NC]) {
 #pragma unroll
     for (int n = 0; n < NC; n++) {
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const float p = __builtin_amdgcn_exp2f(x[n][j]);
-            sum += p;
             const _Float16 ph = (_Float16)p;
             p0[n][j] = ph;
-            if (PARTS > 1) p1[n][j] = (_Float16)(p - (float)ph);
+            if (PARTS > 1) p1[n][j] = (_Float16)(p - (float)ph), sum += p;
+        }
+        if (PARTS == 1) {
+            // the sum of what the products take, two at a time
+            const half2v one = {(_Float16)1.f, (_Float16)1.f};
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                sum = __builtin_amdgcn_fdot2(half2v{p0[n][2 * j], p0[n][2 * j + 1]}, one, sum, false);
         }
         w.l[n] = __builtin_fmaf(sum, rv, w.l[n]);
     }
@@ -366,7 +385,9 @@ __global__ __launch_bounds__(256, S <= 4 ? 3 : 2) void kv_step_kernel(KvDev c, K
         if (x + 1 < n) kv_fetch<S>(kc, next);
         half8 p0[1], p1[1];
         const bool inside = t * KV_TILE >= all_lo && (t + 1) * KV_TILE <= all_hi && !a.mask;
-        kv_softmax(w, u, ks, lv, rv, bad, t * KV_TILE, inside, a, b.tok0[i], scores, score_row, p0, p1);
+        float z[1][8];
+        kv_reference(w, u, ks, lv, bad, t * KV_TILE, inside, a, b.tok0[i], scores, score_row, z);
+        kv_exponents(w, z, rv, p0, p1);
         kv_add_values(w, vc, p0[0], p1[0]);
         if (x + 1 < n) kv_fetch<S>(vc, next + kv_half(32 * S));
     }
@@ -413,10 +434,10 @@ __global__ __launch_bounds__(256, S <= 4 ? 3 : 2) void kv_step_kernel(KvDev c, K
 
 // Many rows: the four waves of a workgroup take 4 * NC * 16 rows and every tile.  A tile's
 // codes are converted once, a quarter by each wave, and shared as half-precision operands
-// through LDS (two buffers, one barrier to a tile); an operand read feeds NC products.
+// through LDS (three buffers, one barrier to a tile); an operand read feeds NC products.
 template <int S, int CODE, int PARTS, int NC>
-__global__ __launch_bounds__(256, 2) void kv_chunk_kernel(KvDev c, KvBatch b, KvAttend a) {
-    __shared__ half8 tiles[2][4 * S][64];  // operands of keys, then of values
+__global__ __launch_bounds__(256, S == 8 ? 1 : 2) void kv_chunk_kernel(KvDev c, KvBatch b, KvAttend a) {
+    __shared__ half8 tiles[3][4 * S][64];  // operands of keys, then of values
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4;
     const int h = blockIdx.x % c.H, split = blockIdx.x / c.H % a.splits, unit = blockIdx.x / c.H / a.splits;
@@ -448,65 +469,94 @@ __global__ __launch_bounds__(256, 2) void kv_chunk_kernel(KvDev c, KvBatch b, Kv
     }
     const int* table = c.table + (size_t)b.seq[i] * c.W;
     const int per_block = c.shift - 5, in_block = (1 << per_block) - 1;
-    constexpr int PIECES = (2 * S * 64 + 255) / 256;  // 16-byte pieces of a tile for one thread
+    constexpr int PIECES = (2 * S + 3) / 4;  // 16-byte pieces of a lane that a wave converts
     uint4 next[PIECES];
     const auto fetch = [&](int t, int block) {
-        const uint4* p = (const uint4*)(c.pool + kv_tile_offset(c, block, h, t & in_block));
+        const uint4* p = (const uint4*)(c.pool + kv_tile_offset(c, block, h, t & in_block)) + lane;
 #pragma unroll
         for (int x = 0; x < PIECES; x++)
-            if (x * 256 + tid < 2 * S * 64) next[x] = p[x * 256 + tid];
+            if ((x + 1) * 4 <= 2 * S || x * 4 + wave < 2 * S) next[x] = p[(x * 4 + wave) * 64];
     };
     const auto stage = [&](int buf) {
 #pragma unroll
         for (int x = 0; x < PIECES; x++)
-            if (x * 256 + tid < 2 * S * 64) {
-                const int piece = (x * 256 + tid) >> 6;
-                tiles[buf][2 * piece][lane] = kv_half8<CODE>(next[x].x, next[x].y);
-                tiles[buf][2 * piece + 1][lane] = kv_half8<CODE>(next[x].z, next[x].w);
+            if ((x + 1) * 4 <= 2 * S || x * 4 + wave < 2 * S) {
+                tiles[buf][2 * (x * 4 + wave)][lane] = kv_half8<CODE>(next[x].x, next[x].y);
+                tiles[buf][2 * (x * 4 + wave) + 1][lane] = kv_half8<CODE>(next[x].z, next[x].w);
             }
     };
+    // Step t: the exponentials and values of tile t stand beside the keys' products of
+    // tile t + 1, so the vector and the matrix unit have independent work; tile t + 2 goes
+    // to LDS, t + 3 to registers.  (Two buffers, values one step later, freed LDS that no
+    // wave could use and took 1311 us for 1218: two addresses to a step.)
+    const int n_tiles = max(sp.t1 - sp.t0, 0);
     KvTiles info = kv_tile_infos(c, table, h, sp.t0, 1, sp.t1), ahead = info;
-    if (sp.t0 < sp.t1) {
-        fetch(sp.t0, __builtin_amdgcn_readlane(info.block, 0));
-        stage(0);
-        if (sp.t0 + 1 < sp.t1) fetch(sp.t0 + 1, __builtin_amdgcn_readlane(info.block, 1));
-    }
-    __syncthreads();
-    for (int t = sp.t0; t < sp.t1; t++) {
-        const int x = t - sp.t0, buf = x & 1, y = x & 63;
-        if (y == 0) info = ahead;
-        if (t + 1 < sp.t1) stage(buf ^ 1);
-        if (t + 2 < sp.t1) {
-            // infos of the next 64 tiles two steps before the first of them
-            if (y == 62) ahead = kv_tile_infos(c, table, h, t + 2, 1, sp.t1);
-            fetch(t + 2, y >= 62 ? __builtin_amdgcn_readlane(ahead.block, y - 62) : __builtin_amdgcn_readlane(info.block, y + 2));
-        }
-        const bool inside = t * KV_TILE >= all_lo && (t + 1) * KV_TILE <= all_hi && !a.mask;
-        floatx4 u[NC][2];
+    const auto block_of = [&](int x) {  // of tile x, in info's 64 or the next
+        return x < 64 ? __builtin_amdgcn_readlane(info.block, x) : __builtin_amdgcn_readlane(ahead.block, x - 64);
+    };
+    const auto products = [&](const half8(&k)[2 * S], floatx4(&u)[NC][2]) {
 #pragma unroll
         for (int n = 0; n < NC; n++) u[n][0] = u[n][1] = floatx4{0.f, 0.f, 0.f, 0.f};
+        // 2 NC sums in turn, so that no product waits for the one before it
 #pragma unroll
-        for (int o = 0; o < 2 * S; o++) {
-            const half8 k = tiles[buf][o][lane];
+        for (int s = 0; s < S; s++)
 #pragma unroll
-            for (int n = 0; n < NC; n++)
+            for (int p = 0; p < PARTS; p++)
 #pragma unroll
-                for (int p = 0; p < PARTS; p++)
-                    u[n][o / S] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, w.q[n][p][o % S], u[n][o / S], 0, 0, 0);
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int n = 0; n < NC; n++)
+                        u[n][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[j * S + s], w.q[n][p][s], u[n][j], 0, 0, 0);
+    };
+    floatx4 u[NC][2];
+    if (n_tiles > 0) {
+        fetch(sp.t0, block_of(0));
+        stage(0);
+        if (n_tiles > 1) {
+            fetch(sp.t0 + 1, block_of(1));
+            stage(1);
         }
+        if (n_tiles > 2) fetch(sp.t0 + 2, block_of(2));
+    }
+    __syncthreads();
+    if (n_tiles > 0) {
+        half8 kop[2 * S];
+#pragma unroll
+        for (int o = 0; o < 2 * S; o++) kop[o] = tiles[0][o][lane];
+        products(kop, u);
+    }
+    int b0 = 0, b1 = 1, b2 = 2;  // buffers of tiles t, t + 1, t + 2
+    for (int xt = 0; xt < n_tiles; xt++) {
+        const int t = sp.t0 + xt, y = xt & 63;
+        if (y == 0 && xt > 0) info = ahead;
+        const bool inside = t * KV_TILE >= all_lo && (t + 1) * KV_TILE <= all_hi && !a.mask;
+        const float rv = kv_lane(info.rv, y);
+        float z[NC][8];
+        half8 kop[2 * S], vop[2 * S];
+#pragma unroll
+        for (int o = 0; o < 2 * S; o++) kop[o] = tiles[b1][o][lane];
+        kv_reference(w, u, kv_lane(info.ks, y), kv_lane(info.lv, y), info.bad >> y & 1, t * KV_TILE, inside, a, b.tok0[i],
+                     nullptr, 0, z);
+        if (y == 60) ahead = kv_tile_infos(c, table, h, t + 4, 1, sp.t1);
         half8 p0[NC], p1[NC];
-        kv_softmax(w, u, kv_lane(info.ks, y), kv_lane(info.lv, y), kv_lane(info.rv, y), info.bad >> y & 1, t * KV_TILE,
-                   inside, a, b.tok0[i], nullptr, 0, p0, p1);
+        // past the last tile this works on what lies there, and is not used
+#pragma unroll
+        for (int o = 0; o < 2 * S; o++) vop[o] = tiles[b0][2 * S + o][lane];
+        products(kop, u);
+        kv_exponents(w, z, rv, p0, p1);
 #pragma unroll
         for (int o = 0; o < 2 * S; o++) {
-            const half8 v = tiles[buf][2 * S + o][lane];
 #pragma unroll
             for (int n = 0; n < NC; n++) {
-                w.o[n][o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p0[n], w.o[n][o], 0, 0, 0);
-                if (PARTS > 1) w.o[n][o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p1[n], w.o[n][o], 0, 0, 0);
+                w.o[n][o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vop[o], p0[n], w.o[n][o], 0, 0, 0);
+                if (PARTS > 1) w.o[n][o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vop[o], p1[n], w.o[n][o], 0, 0, 0);
             }
         }
+        stage(b2);
+        if (xt + 3 < n_tiles) fetch(t + 3, block_of(y + 3));
         __syncthreads();
+        const int tmp = b0;
+        b0 = b1, b1 = b2, b2 = tmp;
     }
 #pragma unroll
     for (int n = 0; n < NC; n++) {
