@@ -12,6 +12,7 @@ one before it waits for that one on the GPU.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 
@@ -21,12 +22,11 @@ from . import _lib
 
 CODES = {"int8": 0, "fp8": 1}
 FIELDS = ("k", "v", "positions", "weights")
+_SAME = contextlib.nullcontext()  # the current stream
 
 
-def _dtypes():
-    import torch
-
-    return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+def _ptr(a: np.ndarray) -> int:
+    return a.__array_interface__["data"][0]
 
 
 class KVCache:
@@ -56,8 +56,10 @@ class KVCache:
         import torch
 
         self.device = torch.device("cuda", torch.cuda.current_device())
+        self._types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
         self._all = np.arange(num_seqs, dtype=np.int32)
-        self._last = None  # the stream of the last call
+        self._last = None      # the stream of the last call, and its handle
+        self._last_raw = None
 
     def __del__(self):
         h = getattr(self, "_h", None)
@@ -70,7 +72,7 @@ class KVCache:
     def lengths(self) -> np.ndarray:
         """Slots in use of every sequence, int64 [num_seqs]."""
         out = np.empty(self.num_seqs, np.int64)
-        _lib.check(self._L.vgpu_kv_lengths(self._h, out.ctypes.data))
+        _lib.check(self._L.vgpu_kv_lengths(self._h, _ptr(out)))
         return out
 
     def info(self) -> dict:
@@ -83,7 +85,7 @@ class KVCache:
         """Forget each sequence's slots from lengths[i] on; 0 empties it."""
         ids = self._seqs(seqs)
         lens = self._ints(lengths, len(ids), "lengths")
-        _lib.check(self._L.vgpu_kv_truncate(self._h, ids.ctypes.data, lens.ctypes.data, len(ids)))
+        _lib.check(self._L.vgpu_kv_truncate(self._h, _ptr(ids), _ptr(lens), len(ids)))
 
     # ---- operators ----------------------------------------------------------
     def append(self, k, v, seqs=None, counts=None, positions=None, weights=None,
@@ -104,7 +106,7 @@ class KVCache:
         pos = self._side(positions, "positions", k.shape[0], "int32")
         wts = self._side(weights, "weights", k.shape[0], "float32")
         s, _ = self._stream(stream, (k, v, positions, weights))
-        _lib.check(self._L.vgpu_kv_append(self._h, ids.ctypes.data, n.ctypes.data, len(ids),
+        _lib.check(self._L.vgpu_kv_append(self._h, _ptr(ids), _ptr(n), len(ids),
                                           ctypes.byref(kt), ctypes.byref(vt), pos, wts, s))
 
     def attend(self, q, seqs=None, counts=None, scale: float | None = None, causal: bool = True,
@@ -153,7 +155,7 @@ class KVCache:
             mask.shape[1] if mask is not None else 0, int(decay is not None),
             0.0 if decay is None else decay, out.data_ptr(),
             lse.data_ptr() if lse is not None else None)
-        _lib.check(self._L.vgpu_kv_attend(self._h, ids.ctypes.data, n.ctypes.data, len(ids),
+        _lib.check(self._L.vgpu_kv_attend(self._h, _ptr(ids), _ptr(n), len(ids),
                                           ctypes.byref(query), s))
         return (out, lse) if return_lse else out
 
@@ -188,8 +190,8 @@ class KVCache:
                                          dtype=torch.float32)}
                 gone["v"] = torch.empty_like(gone["k"])
         ptr = [gone[f].data_ptr() if gone and most else None for f in ("positions", "k", "v")]
-        _lib.check(self._L.vgpu_kv_evict(self._h, ids.ctypes.data,
-                                         None if to is None else to.ctypes.data, len(ids), budget,
+        _lib.check(self._L.vgpu_kv_evict(self._h, _ptr(ids),
+                                         None if to is None else _ptr(to), len(ids), budget,
                                          recent, most, *ptr, s))
         return gone
 
@@ -202,7 +204,7 @@ class KVCache:
         import torch
 
         dtype = torch.float32 if dtype is None else dtype
-        if dtype not in _dtypes():
+        if dtype not in self._types:
             raise TypeError("dtype must be float32, float16 or bfloat16")
         if not set(fields) <= set(FIELDS):
             raise ValueError(f"fields must be among {FIELDS}")
@@ -223,8 +225,8 @@ class KVCache:
                 shape = (tokens, self.num_heads) + ((self.head_dim,) if f in "kv" else ())
                 res[f] = torch.empty(shape, dtype=types.get(f, dtype), device=self.device)
         ptr = [res[f].data_ptr() if f in res else None for f in FIELDS]
-        _lib.check(self._L.vgpu_kv_read(self._h, ids.ctypes.data, at.ctypes.data, n.ctypes.data,
-                                        len(ids), _dtypes()[dtype], *ptr, s))
+        _lib.check(self._L.vgpu_kv_read(self._h, _ptr(ids), _ptr(at), _ptr(n),
+                                        len(ids), self._types[dtype], *ptr, s))
         return res
 
     # ---- arguments ------------------------------------------------------------
@@ -267,14 +269,14 @@ class KVCache:
 
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a torch tensor")
-        if t.dtype not in _dtypes():
+        if t.dtype not in self._types:
             raise TypeError(f"{name} must be float32, float16 or bfloat16")
         if t.dim() != 3 or t.shape[2] != self.head_dim or (heads and t.shape[1] != heads):
             raise ValueError(f"{name} must have the shape [tokens, {heads or 'heads'}, "
                              f"{self.head_dim}], got {list(t.shape)}")
         if t.device != self.device:
             raise ValueError(f"{name} must be on the cache's GPU ({self.device})")
-        return _lib.KvTensor(t.data_ptr() or None, _dtypes()[t.dtype], *t.stride())
+        return _lib.KvTensor(t.data_ptr() or None, self._types[t.dtype], *t.stride())
 
     def _side(self, t, name: str, tokens: int, dtype: str):
         import torch
@@ -292,21 +294,24 @@ class KVCache:
     def _stream(self, stream, tensors):
         """The call's stream handle and a context that allocates on it.  Puts the call
         behind the last one and keeps the tensors' memory until it has run."""
-        import contextlib
-
         import torch
 
-        current = torch.cuda.current_stream(self.device)
-        use = current if stream is None else stream
+        if stream is None:
+            raw = torch._C._cuda_getCurrentRawStream(self.device.index)
+            if raw == self._last_raw:
+                return raw or None, _SAME
+            use = torch.cuda.current_stream(self.device)
+        else:
+            use, raw = stream, stream.cuda_stream
         with torch.cuda.stream(use):
             capturing = torch.cuda.is_current_stream_capturing()  # refused by the library
         if not capturing:
-            if self._last is not None and self._last != use:
+            if self._last is not None and self._last_raw != raw:
                 use.wait_stream(self._last)
-            self._last = use
-        if use == current:
-            return use.cuda_stream or None, contextlib.nullcontext()
+            self._last, self._last_raw = use, raw
+        if stream is None or torch.cuda.current_stream(self.device) == use:
+            return raw or None, _SAME
         for t in tensors:
             if t is not None:
                 t.record_stream(use)
-        return use.cuda_stream or None, torch.cuda.stream(use)
+        return raw or None, torch.cuda.stream(use)
