@@ -53,10 +53,34 @@ __device__ __forceinline__ half8 kv_half8(uint32_t w0, uint32_t w1) {
     return __builtin_bit_cast(half8, r);
 }
 
-__device__ __forceinline__ float kv_load(const KvTensor& x, int64_t i) {
-    if (x.type == KV_F32) return ((const float*)x.p)[i];
-    if (x.type == KV_F16) return (float)((const _Float16*)x.p)[i];
-    return __uint_as_float((uint32_t)((const uint16_t*)x.p)[i] << 16);
+__device__ __forceinline__ float kv_half_bits(uint32_t h, int type) {
+    return type == KV_F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)h) : __uint_as_float(h << 16);
+}
+
+// dims d .. d + 7 of a row (0 from D on); PARTS 2: float32, else one of the 16-bit types
+template <int PARTS>
+__device__ __forceinline__ void kv_load8(const KvTensor& x, int64_t row, int d, int D, float (&v)[8]) {
+    if (x.vec) {
+        if (PARTS > 1) {
+            const float4* p = (const float4*)((const float*)x.p + row + d);
+            const float4 a = p[0], b = p[1];
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        } else {
+            const uint4 a = *(const uint4*)((const uint16_t*)x.p + row + d);
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = kv_half_bits(w[e >> 1] >> (16 * (e & 1)) & 0xffffu, x.type);
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const int64_t at = row + (int64_t)(d + e) * x.sd;
+        if (PARTS > 1)
+            v[e] = d + e < D ? ((const float*)x.p)[at] : 0.f;
+        else
+            v[e] = d + e < D ? kv_half_bits(((const uint16_t*)x.p)[at], x.type) : 0.f;
+    }
 }
 
 __device__ __forceinline__ void kv_store(void* p, size_t i, float v, int type) {
@@ -112,13 +136,16 @@ __device__ __forceinline__ void kv_load_rows(KvWave<S, CODE, PARTS, NC>& w, cons
         if (row < rows) kv_range(a, len, b.count[i], row, w.lo[n], w.hi[n]);
         float x[S][8];
 #pragma unroll
-        for (int s = 0; s < S; s++)
+        for (int s = 0; s < S; s++) {
+            if (row < rows && 32 * s + 8 * g < c.D) {
+                kv_load8<PARTS>(a.q, base, 32 * s + 8 * g, c.D, x[s]);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int d = 32 * s + 8 * g + e;
-                x[s][e] = row < rows && d < c.D ? kv_load(a.q, base + d * a.q.sd) : 0.f;
-                big = fmaxf(big, fabsf(x[s][e]));
+                for (int e = 0; e < 8; e++) x[s][e] = 0.f;
             }
+#pragma unroll
+            for (int e = 0; e < 8; e++) big = fmaxf(big, fabsf(x[s][e]));
+        }
         big = kv_max4(big);
         int ex = 0;
         if (big > 0.f && big < __builtin_huge_valf()) (void)frexpf(big, &ex), ex -= 15;
@@ -319,25 +346,31 @@ __device__ __forceinline__ void kv_finish(const KvDev& c, const KvBatch& b, cons
     if (a.lse2) a.lse2[kv_head_row(c, b, a, i, h, row)] = lse2;
 }
 
-// First row of a workgroup: the last rows, which see most, start first.
-__device__ __forceinline__ int kv_unit_row0(const KvBatch& b, int i, int unit, int wg_rows) {
-    return (b.unit0[i + 1] - 1 - unit) * wg_rows;
-}
-
-// The tiles that some row of a workgroup sees (first .. last - 1), and its split's share.
-struct KvSpan {
-    int first, last, t0, t1;
+// What a workgroup does: its sequence, split and first row (the last rows, which see
+// most, start first), and the tiles t0 .. t1 - 1 that its rows see in its split.
+struct KvJob {
+    int i, h, split, row0, row1;
+    int t0, t1;
     bool whole;  // no other split has tiles
+    bool none;   // this one has none
 };
-__device__ __forceinline__ KvSpan kv_span(const KvAttend& a, int len, int count, int row0, int row1, int split) {
+__device__ __forceinline__ KvJob kv_job(const KvDev& c, const KvBatch& b, const KvAttend& a, int wg_rows) {
+    KvJob j;
+    j.h = blockIdx.x % c.H;
+    const int unit = blockIdx.x / c.H;
+    j.i = kv_find(b, unit);
+    const int u = unit - b.unit0[j.i], splits = b.splits[j.i], rows = b.count[j.i] * a.G;
+    const int tile = (rows + wg_rows - 1) / wg_rows - 1 - u / splits;
+    j.split = u % splits;
+    j.row0 = tile * wg_rows, j.row1 = min(j.row0 + wg_rows, rows);
     int lo0, hi0, lo1, hi1;
-    kv_range(a, len, count, row0, lo0, hi0);
-    kv_range(a, len, count, row1 - 1, lo1, hi1);
-    KvSpan p;
-    p.first = lo0 / KV_TILE, p.last = (hi1 + KV_TILE - 1) / KV_TILE;
-    p.t0 = p.first + split * a.split_tiles, p.t1 = min(p.t0 + a.split_tiles, p.last);
-    p.whole = p.first + a.split_tiles >= p.last;
-    return p;
+    kv_range(a, b.len[j.i], b.count[j.i], j.row0, lo0, hi0);
+    kv_range(a, b.len[j.i], b.count[j.i], j.row1 - 1, lo1, hi1);
+    const int first = lo0 / KV_TILE, last = (hi1 + KV_TILE - 1) / KV_TILE;
+    j.t0 = first + j.split * b.per[j.i], j.t1 = min(j.t0 + b.per[j.i], last);
+    j.whole = first + b.per[j.i] >= last;
+    j.none = j.split > 0 && j.t0 >= j.t1;
+    return j;
 }
 
 // Few rows: the four waves of a workgroup take the same 16 rows and every fourth tile,
@@ -349,12 +382,10 @@ __global__ __launch_bounds__(256, S <= 4 ? 3 : 2) void kv_step_kernel(KvDev c, K
     extern __shared__ __align__(16) float lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
-    const int h = blockIdx.x % c.H, split = blockIdx.x / c.H % a.splits, unit = blockIdx.x / c.H / a.splits;
-    const int i = kv_find(b, unit);
+    const KvJob sp = kv_job(c, b, a, 16);
+    if (sp.none) return;
+    const int i = sp.i, h = sp.h, row0 = sp.row0, row1 = sp.row1;
     const int len = b.len[i], rows = b.count[i] * a.G;
-    const int row0 = kv_unit_row0(b, i, unit, 16), row1 = min(row0 + 16, rows);
-    const KvSpan sp = kv_span(a, len, b.count[i], row0, row1, split);
-    if (split > 0 && sp.t0 >= sp.t1) return;
 
     const int* table = c.table + (size_t)b.seq[i] * c.W;
     const int per_block = c.shift - 5, in_block = (1 << per_block) - 1;
@@ -440,14 +471,12 @@ __global__ __launch_bounds__(256, S == 8 ? 1 : 2) void kv_chunk_kernel(KvDev c, 
     __shared__ half8 tiles[3][4 * S][64];  // operands of keys, then of values
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4;
-    const int h = blockIdx.x % c.H, split = blockIdx.x / c.H % a.splits, unit = blockIdx.x / c.H / a.splits;
-    const int i = kv_find(b, unit);
-    const int len = b.len[i], rows = b.count[i] * a.G;
     constexpr int WG_ROWS = 64 * NC;
-    const int wg_row0 = kv_unit_row0(b, i, unit, WG_ROWS);
+    const KvJob sp = kv_job(c, b, a, WG_ROWS);
+    if (sp.none) return;
+    const int i = sp.i, h = sp.h, wg_row0 = sp.row0;
+    const int len = b.len[i], rows = b.count[i] * a.G;
     const int row0 = wg_row0 + wave * 16 * NC;
-    const KvSpan sp = kv_span(a, len, b.count[i], wg_row0, min(wg_row0 + WG_ROWS, rows), split);
-    if (split > 0 && sp.t0 >= sp.t1) return;
 
     KvWave<S, CODE, PARTS, NC> w;
     kv_load_rows(w, c, b, a, i, h, row0);
@@ -456,7 +485,7 @@ __global__ __launch_bounds__(256, S == 8 ? 1 : 2) void kv_chunk_kernel(KvDev c, 
         kv_range(a, len, b.count[i], row0, x0, all_hi);
         kv_range(a, len, b.count[i], min(row0 + 16 * NC, rows) - 1, all_lo, x1);
     }
-    if (a.qop && split == 0) {
+    if (a.qop && sp.split == 0) {
 #pragma unroll
         for (int n = 0; n < NC; n++) {
             const int tile = row0 / 16 + n;
@@ -583,75 +612,85 @@ __global__ __launch_bounds__(256, S == 8 ? 1 : 2) void kv_chunk_kernel(KvDev c, 
 }
 
 // Joins the splits of a row whose tiles went to several workgroups: a workgroup per row,
-// its waves take every fourth split, then lane by lane in the waves' order.
+// Dp / 4 threads to a split; each thread adds its splits in order, then the thread groups.
+// unit0 counts row tiles here, aux is the first of the sequence's units.
 __global__ __launch_bounds__(256) void kv_join_kernel(KvDev c, KvBatch b, KvAttend a, int wg_rows, int used_rows) {
-    __shared__ float sh_o[4][KV_MAX_DIM];
-    __shared__ float sh_l[4];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    __shared__ floatx4 sh_o[256];
+    __shared__ float sh_l[64];
+    const int tid = threadIdx.x;
     const int h = blockIdx.x % c.H, r = blockIdx.x / c.H % used_rows, unit = blockIdx.x / c.H / used_rows;
     const int i = kv_find(b, unit);
-    const int rows = b.count[i] * a.G, wg_row0 = kv_unit_row0(b, i, unit, wg_rows);
-    const int row = wg_row0 + r;
+    const int rows = b.count[i] * a.G, u = unit - b.unit0[i];
+    const int tile = b.unit0[i + 1] - b.unit0[i] - 1 - u;
+    const int row0 = tile * wg_rows, row = row0 + r;
     if (row >= rows) return;
     int lo0, hi0, lo1, hi1;
-    kv_range(a, b.len[i], b.count[i], wg_row0, lo0, hi0);
-    kv_range(a, b.len[i], b.count[i], min(wg_row0 + wg_rows, rows) - 1, lo1, hi1);
+    kv_range(a, b.len[i], b.count[i], row0, lo0, hi0);
+    kv_range(a, b.len[i], b.count[i], min(row0 + wg_rows, rows) - 1, lo1, hi1);
     const int tiles = (hi1 + KV_TILE - 1) / KV_TILE - lo0 / KV_TILE;
-    const int splits = (tiles + a.split_tiles - 1) / a.split_tiles;
+    const int splits = (tiles + b.per[i] - 1) / b.per[i];
     if (splits <= 1) return;  // the one workgroup has written the row
     const size_t stride = (size_t)c.H * wg_rows;
-    const size_t base = ((size_t)unit * a.splits * c.H + h) * wg_rows + r;
+    const size_t base = ((size_t)(b.aux[i] + u * b.splits[i]) * c.H + h) * wg_rows + r;
     float mx = KV_NEG;
-    for (int s = lane; s < splits; s += 64) mx = fmaxf(mx, a.part_ml[base + s * stride].x);
+    for (int s = tid & 63; s < splits; s += 64) mx = fmaxf(mx, a.part_ml[base + s * stride].x);
 #pragma unroll
     for (int x = 32; x; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
+    const int width = c.Dp / 4, groups = 256 / width, grp = tid / width, d4 = tid % width;
+    floatx4 o = {0.f, 0.f, 0.f, 0.f};
     float l = 0.f;
-    constexpr int K = KV_MAX_DIM / 64;
-    float o[K] = {};
+    if (grp < groups) {
 #pragma unroll 4
-    for (int s = wave; s < splits; s += 4) {
-        const float2 ml = a.part_ml[base + s * stride];
-        const float f = kv_join_factor(ml.x, ml.y, mx);
-        l += f * ml.y;
-        const float* po = a.part_o + (base + s * stride) * c.Dp;
-#pragma unroll
-        for (int k = 0; k < K; k++)
-            if (k * 64 + lane < c.Dp) o[k] += f * po[k * 64 + lane];
+        for (int s = grp; s < splits; s += groups) {
+            const float2 ml = a.part_ml[base + s * stride];
+            const float f = kv_join_factor(ml.x, ml.y, mx);
+            l += f * ml.y;
+            o += *(const floatx4*)(a.part_o + (base + s * stride) * c.Dp + d4 * 4) * f;
+        }
+        sh_o[tid] = o;
+        if (d4 == 0) sh_l[grp] = l;
     }
-#pragma unroll
-    for (int k = 0; k < K; k++) sh_o[wave][k * 64 + lane] = o[k];
-    if (lane == 0) sh_l[wave] = l;
     __syncthreads();
-    const int d = threadIdx.x;
-    if (d >= c.D) return;
-    l = ((sh_l[0] + sh_l[1]) + sh_l[2]) + sh_l[3];
-    const float v = ((sh_o[0][d] + sh_o[1][d]) + sh_o[2][d]) + sh_o[3][d];
-    const size_t at = kv_row(c, b, a, i, h, row);
-    if (d == 0) kv_finish(c, b, a, i, h, row, mx, l);
-    kv_store(a.out, at * c.D + d, l == 0.f ? 0.f : v * (1.f / l), a.q.type);
+    if (tid >= width) return;
+    for (int x = 1; x < groups; x++) o += sh_o[x * width + tid];
+    l = sh_l[0];
+    for (int x = 1; x < groups; x++) l += sh_l[x];
+    if (tid == 0) kv_finish(c, b, a, i, h, row, mx, l);
+    const size_t at = kv_row(c, b, a, i, h, row) * c.D;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (4 * tid + e < c.D) kv_store(a.out, at + 4 * tid + e, o[e] * inv, a.q.type);
 }
 
-// Weights from the kept scores of a step: a thread per slot.
+// Weights from the kept scores of a step: four slots to a thread, bound by the scores' bytes.
 __global__ __launch_bounds__(256) void kv_score_weights_kernel(KvDev c, KvBatch b, KvAttend a) {
     const int h = blockIdx.x % c.H, unit = blockIdx.x / c.H;
     const int i = kv_find(b, unit);
-    const int slot = (unit - b.unit0[i]) * 256 + threadIdx.x;
+    const int slot = (unit - b.unit0[i]) * KV_SCORE_SLOTS + threadIdx.x * 4;
     const int len = b.len[i], rows = b.count[i] * a.G;
     if (slot >= len) return;
     const int64_t score_row = (int64_t)((len + KV_TILE - 1) / KV_TILE) * KV_TILE;
-    const float* scores = a.scores + (int64_t)b.aux[i] * KV_TILE * c.H + h * score_row * rows;
-    float sum = 0.f;
+    const float* scores = a.scores + (int64_t)b.aux[i] * KV_TILE * c.H + h * score_row * rows + slot;
+    const float* lses = a.lse2 + kv_head_row(c, b, a, i, h, 0);
+    floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
     for (int r = 0; r < rows; r++) {
         int lo, hi;
         kv_range(a, len, b.count[i], r, lo, hi);
-        if (slot < lo || slot >= hi) continue;
-        const float lse = a.lse2[kv_head_row(c, b, a, i, h, r)];
-        if (lse == KV_NEG) continue;  // the mask hides every slot of the row
-        sum += exp2f(scores[(int64_t)r * score_row + slot] - lse);
+        const float lse = lses[r];
+        // scores exist for the tiles of the row's workgroup only; -inf: it sees nothing
+        if (slot + 3 < lo || slot >= hi || lse == KV_NEG) continue;
+        const floatx4 x = *(const floatx4*)(scores + (int64_t)r * score_row);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (slot + e >= lo && slot + e < hi) sum[e] += __builtin_amdgcn_exp2f(x[e] - lse);
     }
     const int block = c.table[(size_t)b.seq[i] * c.W + (slot >> c.shift)];
     float* w = c.weights + ((size_t)block * c.H + h) * c.B + (slot & (c.B - 1));
-    *w = a.decay == 0.f ? sum : a.decay * *w + sum;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (slot + e < len) w[e] = a.decay == 0.f ? sum[e] : a.decay * w[e] + sum[e];
 }
 
 // Weights of calls with many rows, by a second pass over the keys:  w_j = sum_r
@@ -662,7 +701,7 @@ __global__ __launch_bounds__(256) void kv_score_weights_kernel(KvDev c, KvBatch 
 // exponentials: 16 cycles of a SIMD for 64 of them, against 16 of the matrix unit for
 // the 512 multiply-adds of 4 scores of 128 dims.
 constexpr int KV_WT = 2;              // 32-slot tiles of a wave
-constexpr int KV_WG_SLOTS = 4 * KV_WT * KV_TILE;
+static_assert(KV_WEIGHT_SLOTS == 4 * KV_WT * KV_TILE, "four waves of KV_WT tiles");
 
 template <int S, int CODE, int PARTS>
 __global__ __launch_bounds__(256, 2) void kv_tile_weights_kernel(KvDev c, KvBatch b, KvAttend a) {
@@ -673,7 +712,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_weights_kernel(KvDev c, KvBatc
     const int h = blockIdx.x % c.H, chunk = blockIdx.x / c.H % a.chunks, unit = blockIdx.x / c.H / a.chunks;
     const int i = kv_find(b, unit);
     const int len = b.len[i], rows = b.count[i] * a.G;
-    const int slots0 = (unit - b.unit0[i]) * KV_WG_SLOTS;
+    const int slots0 = (unit - b.unit0[i]) * KV_WEIGHT_SLOTS;
     const int t0 = slots0 / KV_TILE + wave * KV_WT;
     const int* table = c.table + (size_t)b.seq[i] * c.W;
     const int per_block = c.shift - 5;
@@ -685,7 +724,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_weights_kernel(KvDev c, KvBatc
         if (tok > 0) r0 = max(r0, (int)min((int64_t)tok * a.G, (int64_t)rows) / 32 * 32);
     }
     if (a.window) {
-        const int64_t tok = (int64_t)min(slots0 + KV_WG_SLOTS, len) - 1 + a.window - (len - b.count[i]);
+        const int64_t tok = (int64_t)min(slots0 + KV_WEIGHT_SLOTS, len) - 1 + a.window - (len - b.count[i]);
         r1 = (int)min((int64_t)r1, max(tok, (int64_t)0) * a.G);
     }
     half8 k[KV_WT][2 * S];
@@ -781,7 +820,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_weights_kernel(KvDev c, KvBatc
             for (int y = 1; y < 16; y <<= 1) v += __shfl_xor(v, y);
             // partial sums of the chunk: [unit, H, chunk, slot of the workgroup]
             const int slot = (wave * KV_WT + x) * KV_TILE + (j >> 2) * 16 + 4 * g + (j & 3);
-            if (col == j) a.wpart[(((size_t)unit * c.H + h) * a.chunks + chunk) * KV_WG_SLOTS + slot] = v;
+            if (col == j) a.wpart[(((size_t)unit * c.H + h) * a.chunks + chunk) * KV_WEIGHT_SLOTS + slot] = v;
         }
 }
 
@@ -789,20 +828,20 @@ __global__ __launch_bounds__(256, 2) void kv_tile_weights_kernel(KvDev c, KvBatc
 __global__ __launch_bounds__(256) void kv_chunk_weights_kernel(KvDev c, KvBatch b, KvAttend a) {
     const int h = blockIdx.x % c.H, unit = blockIdx.x / c.H;
     const int i = kv_find(b, unit);
-    const int slot = (unit - b.unit0[i]) * KV_WG_SLOTS + threadIdx.x;
+    const int slot = (unit - b.unit0[i]) * KV_WEIGHT_SLOTS + threadIdx.x;
     if (slot >= b.len[i]) return;
     float sum = 0.f;
     for (int x = 0; x < a.chunks; x++)
-        sum += a.wpart[(((size_t)unit * c.H + h) * a.chunks + x) * KV_WG_SLOTS + threadIdx.x];
+        sum += a.wpart[(((size_t)unit * c.H + h) * a.chunks + x) * KV_WEIGHT_SLOTS + threadIdx.x];
     const int block = c.table[(size_t)b.seq[i] * c.W + (slot >> c.shift)];
     float* w = c.weights + ((size_t)block * c.H + h) * c.B + (slot & (c.B - 1));
     *w = a.decay == 0.f ? sum : a.decay * *w + sum;
 }
-static_assert(KV_WG_SLOTS == 256, "one thread per slot of a workgroup");
+static_assert(KV_WEIGHT_SLOTS == 256, "one thread per slot of a workgroup");
 
 template <int S, int CODE, int PARTS>
 void attend_s(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s) {
-    const dim3 grid((unsigned)b.unit0[b.n] * c.H * a.splits);
+    const dim3 grid((unsigned)b.unit0[b.n] * c.H);
     if (a.by_rows) {
         hipLaunchKernelGGL((kv_chunk_kernel<S, CODE, PARTS, kv_chunk_nc(S * 32, PARTS)>), grid, dim3(256), 0, s, c, b, a);
         return;
@@ -854,13 +893,18 @@ void by_type(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s)
 void launch_kv_attend(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s) {
     if (!b.unit0[b.n]) return;
     by_type<false>(c, b, a, s);
-    if (a.splits > 1) {
-        const int rows = kv_attend_rows(a, c.Dp);
-        int most = 1;
-        for (int i = 0; i < b.n; i++) most = b.count[i] * a.G > most ? b.count[i] * a.G : most;
-        const int used = most < rows ? most : rows;
-        hipLaunchKernelGGL(kv_join_kernel, dim3((unsigned)b.unit0[b.n] * c.H * used), dim3(256), 0, s, c, b, a, rows, used);
+    // the sequences with several splits, by row tiles
+    const int wg_rows = kv_attend_rows(a, c.Dp);
+    KvBatch j = b;
+    int used = 1;
+    for (int i = 0; i < b.n; i++) {
+        const int rows = b.count[i] * a.G, tiles = b.splits[i] > 1 ? (rows + wg_rows - 1) / wg_rows : 0;
+        j.aux[i] = b.unit0[i];
+        j.unit0[i + 1] = j.unit0[i] + tiles;
+        if (tiles && rows > used) used = rows < wg_rows ? rows : wg_rows;
     }
+    if (j.unit0[j.n])
+        hipLaunchKernelGGL(kv_join_kernel, dim3((unsigned)j.unit0[j.n] * c.H * used), dim3(256), 0, s, c, j, a, wg_rows, used);
 }
 
 void launch_kv_weights(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s) {

@@ -423,7 +423,8 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
         KvBatch b;
         b.n = 0;
         b.unit0[0] = 0;
-        int64_t work = 0, score_tiles = 0, row_tiles = 0, tiles_max = 1;
+        int64_t work = 0, units = 0, score_tiles = 0, row_tiles = 0;
+        int64_t tiles[KV_BATCH], row_units[KV_BATCH];  // that a row tile can see; row tiles
         for (size_t i = i0; i < std::min(n, i0 + KV_BATCH); i++) {
             const int64_t len = seqs[ids[i]].len;
             const int j = b.n++;
@@ -431,40 +432,42 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
             b.len[j] = (int)len;
             b.tok0[j] = (int)tok;
             b.count[j] = (int)counts[i];
-            const int64_t units = (counts[i] * a.G + rows - 1) / rows;
-            need(b.unit0[j] + units <= INT_MAX / 2, "too many query rows in one call");
-            b.unit0[j + 1] = b.unit0[j] + (int)units;
+            row_units[j] = (counts[i] * a.G + rows - 1) / rows;
+            units += row_units[j] * dev.H;
             tok += counts[i];
-            int64_t tiles = (len + KV_TILE - 1) / KV_TILE;
+            tiles[j] = (len + KV_TILE - 1) / KV_TILE;
             need(score_tiles <= INT_MAX / 2, "too many scores in one call");
             b.aux[j] = (int)(keep_scores ? score_tiles : row_tiles);
-            if (keep_scores) score_tiles += tiles * counts[i] * a.G;
+            if (keep_scores) score_tiles += tiles[j] * counts[i] * a.G;
             row_tiles += (counts[i] * a.G + 15) / 16;
-            // tiles that a row tile can see
-            if (a.window && a.causal) tiles = std::min<int64_t>(tiles, (a.window + rows / a.G + 2 * KV_TILE) / KV_TILE + 1);
-            tiles_max = std::max(tiles_max, tiles);
-            work += units * dev.H * tiles;
+            if (a.window && a.causal)
+                tiles[j] = std::min<int64_t>(tiles[j], (a.window + rows / a.G + 2 * KV_TILE) / KV_TILE + 1);
+            work += row_units[j] * dev.H * tiles[j];
         }
-        if (b.unit0[b.n]) {
-            const int64_t units = (int64_t)b.unit0[b.n] * dev.H;
-            int64_t splits;
-            if (a.by_rows) {
-                splits = units >= kChunkWorkgroups ? 1 : std::min((kChunkWorkgroups + units - 1) / units, (tiles_max + 15) / 16);
-            } else {
-                const int64_t each = std::max<int64_t>((work + kStepWorkgroups - 1) / kStepWorkgroups, 8);
-                splits = (tiles_max + each - 1) / each;
+        need(units <= INT_MAX / 64, "too many query rows in one call");
+        if (units) {
+            // Tiles of one workgroup: as few as keep all workgroups on the card at once
+            const int64_t target = a.by_rows ? kChunkWorkgroups : kStepWorkgroups;
+            const int64_t part_units = kPartBytes / (rows * ((int64_t)dev.Dp * 4 + 8));
+            int64_t each = std::max<int64_t>((work + target - 1) / target, a.by_rows ? 16 : 8), groups, split_units;
+            for (;; each += each / 8 + 1) {
+                groups = split_units = 0;
+                bool one = true;
+                for (int j = 0; j < b.n; j++) {
+                    const int64_t splits = a.by_rows && units >= target ? 1 : std::max<int64_t>((tiles[j] + each - 1) / each, 1);
+                    b.splits[j] = (int)splits;
+                    b.per[j] = (int)std::max<int64_t>((tiles[j] + splits - 1) / splits, 1);
+                    b.unit0[j + 1] = b.unit0[j] + (int)(row_units[j] * splits);
+                    groups += row_units[j] * splits * dev.H;
+                    one = one && splits == 1;
+                    if (splits > 1) split_units += row_units[j] * splits * dev.H;
+                }
+                if (one || (groups <= target + target / 8 && groups <= part_units)) break;
             }
-            const int64_t row_bytes = (int64_t)dev.Dp * 4 + 8;
-            splits = std::min(splits, std::max<int64_t>(kPartBytes / (units * rows * row_bytes), 1));
-            const int64_t per = (tiles_max + splits - 1) / splits;
-            splits = (tiles_max + per - 1) / per;
-            need(units * splits <= INT_MAX / 64, "too many query rows in one call");
-            a.split_tiles = (int)per;
-            a.splits = (int)splits;
             a.part_o = nullptr, a.part_ml = nullptr, a.scores = nullptr;
-            if (splits > 1) {
-                grow(w_part, (size_t)(units * splits * rows) * dev.Dp);
-                grow(w_ml, (size_t)(units * splits * rows));
+            if (split_units) {
+                grow(w_part, (size_t)(groups * rows) * dev.Dp);
+                grow(w_ml, (size_t)(groups * rows));
                 a.part_o = w_part.p, a.part_ml = w_ml.p;
             }
             if (keep_scores) {
@@ -478,14 +481,15 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
             launch_kv_attend(dev, b, a, s);
         }
         if (a.track) {
-            for (int j = 0; j < b.n; j++) b.unit0[j + 1] = b.unit0[j] + (b.len[j] + 255) / 256;
+            const int per = keep_scores ? KV_SCORE_SLOTS : KV_WEIGHT_SLOTS;
+            for (int j = 0; j < b.n; j++) b.unit0[j + 1] = b.unit0[j] + (b.len[j] + per - 1) / per;
             if (!keep_scores) {
                 // chunks of at least 256 rows, until there are four workgroups to a compute unit
-                const int64_t units = std::max<int64_t>((int64_t)b.unit0[b.n] * dev.H, 1);
-                const int64_t chunks = std::min((most + 255) / 256, (kWeightWorkgroups + units - 1) / units);
+                const int64_t groups = std::max<int64_t>((int64_t)b.unit0[b.n] * dev.H, 1);
+                const int64_t chunks = std::min((most + 255) / 256, (kWeightWorkgroups + groups - 1) / groups);
                 a.chunk_rows = (int)(((most + chunks - 1) / chunks + 31) / 32 * 32);
                 a.chunks = (int)((most + a.chunk_rows - 1) / a.chunk_rows);
-                grow(w_wpart, (size_t)(units * a.chunks * 256));
+                grow(w_wpart, (size_t)(groups * a.chunks * KV_WEIGHT_SLOTS));
                 a.wpart = w_wpart.p;
             }
             launch_kv_weights(dev, b, a, s);

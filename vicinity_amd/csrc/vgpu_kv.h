@@ -53,6 +53,8 @@ struct KvBatch {
     int count[KV_BATCH];  // its tokens
     int aux[KV_BATCH];    // append: position of the first token; read: first slot;
                           // evict: sequence that receives the result; attend: see there
+    int splits[KV_BATCH]; // attend: parts that the tiles of its rows go to, of per[i] tiles
+    int per[KV_BATCH];
     int unit0[KV_BATCH + 1];
 };
 
@@ -149,8 +151,6 @@ struct KvAttend {
     float* part_o = nullptr;   // split attention: partial rows [workgroup, rows, Dp]
     float2* part_ml = nullptr; // and their (max, sum), base 2
     float* scores = nullptr;   // tracked steps: base-2 scores [row, tile, 32] of each (sequence, head)
-    int split_tiles = 0;       // tiles of one split
-    int splits = 0;            // splits of every row tile
     int by_rows = 0;           // waves of a workgroup take different rows (else different tiles)
 };
 // 16-row tiles of a wave of the many-row kernel, by what its registers hold: Dp / 4
@@ -161,9 +161,11 @@ constexpr int kv_chunk_nc(int Dp, int parts) { return Dp * parts <= 64 ? 4 : Dp 
 inline int kv_attend_rows(const KvAttend& a, int Dp) {
     return a.by_rows ? 64 * kv_chunk_nc(Dp, a.q.type == KV_F32 ? 2 : 1) : 16;
 }
-// unit0 counts row tiles of the sequences (of one head); the launch is unit0[n] * H * splits.
+// unit0 counts row tiles times splits of the sequences (of one head).
 void launch_kv_attend(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s);
-// unit0 counts 256 slots.  aux: with scores the tiles of the score rows of the sequences
+// Slots of a workgroup that makes weights of kept scores, and of one that goes over the keys.
+constexpr int KV_SCORE_SLOTS = 1024, KV_WEIGHT_SLOTS = 256;
+// unit0 counts these.  aux: with scores the tiles of the score rows of the sequences
 // before (of one head), without them the 16-row tiles of the sequences before.
 void launch_kv_weights(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s);
 
