@@ -747,34 +747,45 @@ __global__ __launch_bounds__(256, 2) void kv_tile_weights_kernel(KvDev c, KvBatc
     float sum[KV_WT][8] = {};
     const size_t row_base = kv_head_row(c, b, a, i, h, 0);
     const uint4* qop = a.qop + ((size_t)(b.aux[i]) * c.H + (size_t)h * ((rows + 15) / 16)) * QT;
-    const int last_piece = (rows + 15) / 16 * QT - 1;
-    constexpr int PIECES = (2 * QT + 255) / 256;  // of one thread and step
-    uint4 next[PIECES];
-    if (r0 < r1)
+    const int end = min(r1, rows);
+    const int last_kib = (rows + 15) / 16 * PARTS * S - 1;  // of the head's operands
+    float next_f[2], next_lse[2];  // of this lane's row in the two row tiles
+    // straight to LDS, 1 KiB of a wave at a time
+    const auto fetch = [&](int r, uint4* to) {
+        for (int x = wave; x < 2 * PARTS * S; x += 4)
+            __builtin_amdgcn_global_load_lds(
+                (const __attribute__((address_space(1))) void*)(qop + min(r / 16 * PARTS * S + x, last_kib) * 64 + lane),
+                (__attribute__((address_space(3))) void*)(to + x * 64), 16, 0, 0);
 #pragma unroll
-        for (int x = 0; x < PIECES; x++) next[x] = qop[min(r0 / 16 * QT + x * 256 + tid, last_piece)];
+        for (int y = 0; y < 2; y++) {
+            const int row = r + 16 * y + col;
+            next_f[y] = row < end ? a.qs[row_base + row] : 0.f;
+            next_lse[y] = row < end ? a.lse2[row_base + row] : KV_NEG;
+        }
+    };
+    if (r0 < r1) fetch(r0, qbuf);
     int buf = 0;
     for (int r = r0; r < r1; r += 32, buf ^= 1) {
-        uint4* to = qbuf + buf * 2 * QT;
+        const uint4* to = qbuf + buf * 2 * QT;
+        float fs[2], ls[2];
 #pragma unroll
-        for (int x = 0; x < PIECES; x++)
-            if (x * 256 + tid < 2 * QT) to[x * 256 + tid] = next[x];
+        for (int y = 0; y < 2; y++) {
+            fs[y] = next_f[y];
+            ls[y] = next_lse[y] == KV_NEG ? -KV_NEG : next_lse[y];  // sees nothing: every p is 0
+        }
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the loads to LDS have landed
         __syncthreads();
-        if (r + 32 < r1)
-#pragma unroll
-            for (int x = 0; x < PIECES; x++) next[x] = qop[min((r + 32) / 16 * QT + x * 256 + tid, last_piece)];
+        if (r + 32 < r1) fetch(r + 32, qbuf + (buf ^ 1) * 2 * QT);
 #pragma unroll
         for (int y = 0; y < 2; y++) {
             const int row0 = r + 16 * y, row = row0 + col;
-            if (row0 >= r1) break;
+            if (row0 >= end) break;
             int lo0, hi0, lo1, hi1;
             kv_range(a, len, b.count[i], row0, lo0, hi0);
             kv_range(a, len, b.count[i], min(row0 + 16, rows) - 1, lo1, hi1);
             if (hi1 <= t0 * KV_TILE || lo0 >= (t0 + KV_WT) * KV_TILE) continue;
-            const bool real = row < min(r1, rows);
-            float f = real ? a.qs[row_base + row] : 0.f;
-            float lse = real ? a.lse2[row_base + row] : -KV_NEG;
-            if (lse == KV_NEG) lse = -KV_NEG;  // sees nothing: every p is 0
+            const bool real = row < end;
+            const float f = fs[y], lse = ls[y];
             floatx4 u[KV_WT][2];
 #pragma unroll
             for (int x = 0; x < KV_WT; x++) u[x][0] = u[x][1] = floatx4{0.f, 0.f, 0.f, 0.f};
