@@ -57,39 +57,75 @@ __device__ __forceinline__ float kv_half_bits(uint32_t h, int type) {
     return type == KV_F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)h) : __uint_as_float(h << 16);
 }
 
-// dims d .. d + 7 of a row (0 from D on); PARTS 2: float32, else one of the 16-bit types
-template <int PARTS>
-__device__ __forceinline__ void kv_load8(const KvTensor& x, int64_t row, int d, int D, float (&v)[8]) {
-    if (x.vec) {
-        if (PARTS > 1) {
-            const float4* p = (const float4*)((const float*)x.p + row + d);
-            const float4 a = p[0], b = p[1];
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        } else {
-            const uint4 a = *(const uint4*)((const uint16_t*)x.p + row + d);
-            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+// A lane's dims of a row, x[s][e] = dim 32 s + 8 g + e (0 from D on); PARTS 2: float32,
+// else one of the 16-bit types.  Rows of one aligned piece per 8 dims, or any strides.
+template <int S, int PARTS>
+__device__ __forceinline__ void kv_load_row(const KvTensor& t, int64_t row, int g, int D, float (&x)[S][8]) {
+    if (t.vec) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = kv_half_bits(w[e >> 1] >> (16 * (e & 1)) & 0xffffu, x.type);
+        for (int s = 0; s < S; s++) {
+            const int64_t at = row + min(32 * s + 8 * g, D - 8);
+            const bool in = 32 * s + 8 * g < D;
+            if (PARTS > 1) {
+                const float4* p = (const float4*)((const float*)t.p + at);
+                const float4 a = p[0], b = p[1];
+                x[s][0] = a.x, x[s][1] = a.y, x[s][2] = a.z, x[s][3] = a.w;
+                x[s][4] = b.x, x[s][5] = b.y, x[s][6] = b.z, x[s][7] = b.w;
+            } else {
+                const uint4 a = *(const uint4*)((const uint16_t*)t.p + at);
+                const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[s][e] = kv_half_bits(w[e >> 1] >> (16 * (e & 1)) & 0xffffu, t.type);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[s][e] = in ? x[s][e] : 0.f;
         }
         return;
     }
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const int64_t at = row + (int64_t)(d + e) * x.sd;
-        if (PARTS > 1)
-            v[e] = d + e < D ? ((const float*)x.p)[at] : 0.f;
-        else
-            v[e] = d + e < D ? kv_half_bits(((const uint16_t*)x.p)[at], x.type) : 0.f;
-    }
+    for (int s = 0; s < S; s++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int d = 32 * s + 8 * g + e;
+            const int64_t at = row + (int64_t)min(d, D - 1) * t.sd;
+            const float v = PARTS > 1 ? ((const float*)t.p)[at] : kv_half_bits(((const uint16_t*)t.p)[at], t.type);
+            x[s][e] = d < D ? v : 0.f;
+        }
 }
 
-__device__ __forceinline__ void kv_store(void* p, size_t i, float v, int type) {
-    if (type == KV_F32)
-        ((float*)p)[i] = v;
-    else if (type == KV_F16)
-        ((_Float16*)p)[i] = (_Float16)v;
-    else
-        ((__hip_bfloat16*)p)[i] = __float2bfloat16(v);
+// Dims d .. d + 3 of a result row (those below D), rounded once.
+template <int PARTS>
+__device__ __forceinline__ void kv_store4(const KvAttend& a, size_t row, int d, int D, floatx4 v) {
+    if (PARTS > 1) {
+        float* at = (float*)a.out + row + d;
+        if (a.vec_out && d < D) {
+            *(floatx4*)at = v;
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (d + e < D) at[e] = v[e];
+        return;
+    }
+    uint32_t w[2];
+    if (a.q.type == KV_F16) {
+#pragma unroll
+        for (int e = 0; e < 2; e++) w[e] = __builtin_bit_cast(uint32_t, half2v{(_Float16)v[2 * e], (_Float16)v[2 * e + 1]});
+    } else {
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const __hip_bfloat16 x = __float2bfloat16(v[2 * e]), y = __float2bfloat16(v[2 * e + 1]);
+            w[e] = (uint32_t)__builtin_bit_cast(uint16_t, x) | (uint32_t)__builtin_bit_cast(uint16_t, y) << 16;
+        }
+    }
+    uint16_t* at = (uint16_t*)a.out + row + d;
+    if (a.vec_out && d < D) {
+        *(uint2*)at = make_uint2(w[0], w[1]);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (d + e < D) at[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
 }
 
 // Largest over the four lanes that hold one row's slots.
@@ -132,20 +168,16 @@ __device__ __forceinline__ void kv_load_rows(KvWave<S, CODE, PARTS, NC>& w, cons
         w.lo[n] = 0, w.hi[n] = 0;  // rows past the end see nothing
         w.m[n] = KV_NEG, w.l[n] = 0.f, w.bad[n] = 0.f;
         float big = 0.f;
-        const int64_t base = row < rows ? (int64_t)(b.tok0[i] + row / a.G) * a.q.st + (int64_t)(h * a.G + row % a.G) * a.q.sh : 0;
+        // (a row past the end loads the last one's and is not used)
+        const int real = min(row, rows - 1);
+        const int64_t base = (int64_t)(b.tok0[i] + real / a.G) * a.q.st + (int64_t)(h * a.G + real % a.G) * a.q.sh;
         if (row < rows) kv_range(a, len, b.count[i], row, w.lo[n], w.hi[n]);
         float x[S][8];
+        kv_load_row<S, PARTS>(a.q, base, g, c.D, x);
 #pragma unroll
-        for (int s = 0; s < S; s++) {
-            if (row < rows && 32 * s + 8 * g < c.D) {
-                kv_load8<PARTS>(a.q, base, 32 * s + 8 * g, c.D, x[s]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; e++) x[s][e] = 0.f;
-            }
+        for (int s = 0; s < S; s++)
 #pragma unroll
             for (int e = 0; e < 8; e++) big = fmaxf(big, fabsf(x[s][e]));
-        }
         big = kv_max4(big);
         int ex = 0;
         if (big > 0.f && big < __builtin_huge_valf()) (void)frexpf(big, &ex), ex -= 15;
@@ -167,7 +199,7 @@ __device__ __forceinline__ void kv_load_rows(KvWave<S, CODE, PARTS, NC>& w, cons
 // What a wave needs to know of 64 tiles, one to a lane: refilled every 64 tiles, so no
 // step waits for the block table or a scale.
 struct KvTiles {
-    int block;
+    uint32_t lo, hi;   // its offset in the pool
     float ks, lv, rv;  // key scale, log2 and inverse of the value scale
     uint64_t bad;      // tiles whose value scale is NaN
 };
@@ -177,8 +209,10 @@ __device__ __forceinline__ KvTiles kv_tile_infos(const KvDev& c, const int* tabl
     const int t = first + (threadIdx.x & 63) * step;
     KvTiles r;
     const bool in = t < last;
-    r.block = in ? table[t >> (c.shift - 5)] : 0;
-    const size_t part = (size_t)r.block * c.H + h;
+    const int block = in ? table[t >> (c.shift - 5)] : 0;
+    const size_t part = (size_t)block * c.H + h;
+    const size_t at = kv_tile_offset(c, block, h, t & (c.B / KV_TILE - 1));
+    r.lo = (uint32_t)at, r.hi = (uint32_t)(at >> 32);
     r.ks = in ? c.kscale[part] : 0.f;
     const float vs = in ? c.vscale[part] : 1.f;
     r.bad = __ballot(vs != vs);
@@ -186,6 +220,11 @@ __device__ __forceinline__ KvTiles kv_tile_infos(const KvDev& c, const int* tabl
     r.lv = log2f(sv);
     r.rv = 1.f / sv;
     return r;
+}
+__device__ __forceinline__ const uint8_t* kv_tile_of(const KvDev& c, const KvTiles& f, int lane) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)f.lo, lane);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)f.hi, lane);
+    return c.pool + ((size_t)hi << 32 | lo);
 }
 __device__ __forceinline__ float kv_lane(float v, int lane) {
     return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), lane));
@@ -226,14 +265,26 @@ __device__ __forceinline__ void kv_reference(KvWave<S, CODE, PARTS, NC>& w, cons
             const float f = w.qs[n] * ks, base = w.m[n] == KV_NEG ? lv : lv - (w.m[n] - KV_TOP);
             bool any = inside;
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                x[n][j] = u[n][j >> 2][j & 3] * f;
-                if (!inside) {
-                    const int slot = slot0 + (j >> 2) * 16 + 4 * g + (j & 3);
-                    bool see = slot >= w.lo[n] && slot < w.hi[n];
-                    if (see && a.mask) see = a.mask[(int64_t)(tok0 + w.row[n] / a.G) * a.mask_st + slot * a.mask_ss] != 0;
+            for (int j = 0; j < 8; j++) x[n][j] = u[n][j >> 2][j & 3] * f;
+            if (!inside) {
+                // slot0 + 4 g + off sees: lo <= slot < hi
+                const int first = w.lo[n] - slot0 - 4 * g, count = w.hi[n] - w.lo[n];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const bool see = (unsigned)((j >> 2) * 16 + (j & 3) - first) < (unsigned)count && count > 0;
                     x[n][j] = see ? x[n][j] : KV_NEG;
                     any |= see;
+                }
+                if (a.mask && any) {
+                    any = false;
+                    const uint8_t* mask = a.mask + (int64_t)(tok0 + w.row[n] / a.G) * a.mask_st;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const int off = (j >> 2) * 16 + (j & 3);
+                        const bool see = (unsigned)(off - first) < (unsigned)count && mask[(slot0 + 4 * g + off) * a.mask_ss];
+                        x[n][j] = see ? x[n][j] : KV_NEG;
+                        any |= see;
+                    }
                 }
             }
             if (bad && any) w.bad[n] = __uint_as_float(0x7fc00000u);
@@ -283,9 +334,12 @@ __device__ __forceinline__ void kv_exponents(KvWave<S, CODE, PARTS, NC>& w, cons
         if (PARTS == 1) {
             // the sum of what the products take, two at a time
             const half2v one = {(_Float16)1.f, (_Float16)1.f};
+            const u32x4 two = __builtin_bit_cast(u32x4, p0[n]);
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                sum = __builtin_amdgcn_fdot2(half2v{p0[n][2 * j], p0[n][2 * j + 1]}, one, sum, false);
+            for (int j = 0; j < 4; j++) {
+                const uint32_t pair = two[j];
+                sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, pair), one, sum, false);
+            }
         }
         w.l[n] = __builtin_fmaf(sum, rv, w.l[n]);
     }
@@ -346,8 +400,9 @@ __device__ __forceinline__ void kv_finish(const KvDev& c, const KvBatch& b, cons
     if (a.lse2) a.lse2[kv_head_row(c, b, a, i, h, row)] = lse2;
 }
 
-// What a workgroup does: its sequence, split and first row (the last rows, which see
-// most, start first), and the tiles t0 .. t1 - 1 that its rows see in its split.
+// What a workgroup does: its sequence, split and first row (first splits before second
+// ones, and the last rows, which see most, before the first ones: long work starts
+// early), and the tiles t0 .. t1 - 1 that its rows see in its split.
 struct KvJob {
     int i, h, split, row0, row1;
     int t0, t1;
@@ -359,9 +414,9 @@ __device__ __forceinline__ KvJob kv_job(const KvDev& c, const KvBatch& b, const 
     j.h = blockIdx.x % c.H;
     const int unit = blockIdx.x / c.H;
     j.i = kv_find(b, unit);
-    const int u = unit - b.unit0[j.i], splits = b.splits[j.i], rows = b.count[j.i] * a.G;
-    const int tile = (rows + wg_rows - 1) / wg_rows - 1 - u / splits;
-    j.split = u % splits;
+    const int u = unit - b.unit0[j.i], rows = b.count[j.i] * a.G, row_tiles = (rows + wg_rows - 1) / wg_rows;
+    const int tile = row_tiles - 1 - u % row_tiles;
+    j.split = u / row_tiles;
     j.row0 = tile * wg_rows, j.row1 = min(j.row0 + wg_rows, rows);
     int lo0, hi0, lo1, hi1;
     kv_range(a, b.len[j.i], b.count[j.i], j.row0, lo0, hi0);
@@ -388,7 +443,6 @@ __global__ __launch_bounds__(256, S <= 4 ? 3 : 2) void kv_step_kernel(KvDev c, K
     const int len = b.len[i], rows = b.count[i] * a.G;
 
     const int* table = c.table + (size_t)b.seq[i] * c.W;
-    const int per_block = c.shift - 5, in_block = (1 << per_block) - 1;
     const int64_t score_row = (int64_t)((len + KV_TILE - 1) / KV_TILE) * KV_TILE;
     float* scores = a.scores ? a.scores + (int64_t)b.aux[i] * KV_TILE * c.H + h * score_row * rows : nullptr;
     int all_lo, all_hi, x0, x1;  // slots that every row sees
@@ -398,9 +452,7 @@ __global__ __launch_bounds__(256, S <= 4 ? 3 : 2) void kv_step_kernel(KvDev c, K
     const int n = max((sp.t1 - sp.t0 - wave + 3) / 4, 0);  // tiles of this wave
     const int tw = sp.t0 + wave;
     KvTiles info = kv_tile_infos(c, table, h, tw, 4, sp.t1);
-    const auto tile = [&](const KvTiles& f, int x) {
-        return c.pool + kv_tile_offset(c, __builtin_amdgcn_readlane(f.block, x & 63), h, (tw + 4 * x) & in_block);
-    };
+    const auto tile = [&](const KvTiles& f, int x) { return kv_tile_of(c, f, x & 63); };
     uint4 kc[S], vc[S];
     if (n > 0) kv_fetch<S>(kc, tile(info, 0)), kv_fetch<S>(vc, tile(info, 0) + kv_half(32 * S));
     KvWave<S, CODE, PARTS, 1> w;
@@ -452,9 +504,7 @@ __global__ __launch_bounds__(256, S <= 4 ? 3 : 2) void kv_step_kernel(KvDev c, K
             const size_t at = kv_row(c, b, a, i, h, row);
             if (d == 0) kv_finish(c, b, a, i, h, row, mx, l);
             const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (d + e < c.D) kv_store(a.out, at * c.D + d + e, o[e] * inv, a.q.type);
+            kv_store4<PARTS>(a, at * c.D, d, c.D, o * inv);
         } else {
             const size_t at = (size_t)blockIdx.x * 16 + r;
             if (d == 0) a.part_ml[at] = make_float2(mx, l);
@@ -478,8 +528,37 @@ __global__ __launch_bounds__(256, S == 8 ? 1 : 2) void kv_chunk_kernel(KvDev c, 
     const int len = b.len[i], rows = b.count[i] * a.G;
     const int row0 = wg_row0 + wave * 16 * NC;
 
+    const int n_tiles = max(sp.t1 - sp.t0, 0);
+    KvTiles info = kv_tile_infos(c, c.table + (size_t)b.seq[i] * c.W, h, sp.t0, 1, sp.t1), ahead = info;
+    constexpr int PIECES = (2 * S + 3) / 4;  // 16-byte pieces of a lane that a wave converts
+    const auto fetch = [&](uint4(&to)[PIECES], const uint8_t* tile) {
+        const uint4* p = (const uint4*)tile + lane;
+#pragma unroll
+        for (int x = 0; x < PIECES; x++)
+            if ((x + 1) * 4 <= 2 * S || x * 4 + wave < 2 * S) to[x] = p[(x * 4 + wave) * 64];
+    };
+    const auto stage = [&](int buf, const uint4(&from)[PIECES]) {
+#pragma unroll
+        for (int x = 0; x < PIECES; x++)
+            if ((x + 1) * 4 <= 2 * S || x * 4 + wave < 2 * S) {
+                tiles[buf][2 * (x * 4 + wave)][lane] = kv_half8<CODE>(from[x].x, from[x].y);
+                tiles[buf][2 * (x * 4 + wave) + 1][lane] = kv_half8<CODE>(from[x].z, from[x].w);
+            }
+    };
+    // the first three tiles and the rows are on the way together
+    uint4 next[PIECES];
     KvWave<S, CODE, PARTS, NC> w;
-    kv_load_rows(w, c, b, a, i, h, row0);
+    if (n_tiles > 0) {
+        uint4 tile0[PIECES], tile1[PIECES];
+        fetch(tile0, kv_tile_of(c, info, 0));
+        fetch(tile1, kv_tile_of(c, info, min(n_tiles - 1, 1)));
+        fetch(next, kv_tile_of(c, info, min(n_tiles - 1, 2)));
+        kv_load_rows(w, c, b, a, i, h, row0);
+        stage(0, tile0);
+        stage(1, tile1);
+    } else {
+        kv_load_rows(w, c, b, a, i, h, row0);
+    }
     int all_lo = 0, all_hi = 0, x0, x1;  // slots that every row of this wave sees
     if (row0 < rows) {
         kv_range(a, len, b.count[i], row0, x0, all_hi);
@@ -496,33 +575,10 @@ __global__ __launch_bounds__(256, S == 8 ? 1 : 2) void kv_chunk_kernel(KvDev c, 
             if (g == 0 && w.row[n] >= 0) a.qs[kv_head_row(c, b, a, i, h, w.row[n])] = w.qs[n];
         }
     }
-    const int* table = c.table + (size_t)b.seq[i] * c.W;
-    const int per_block = c.shift - 5, in_block = (1 << per_block) - 1;
-    constexpr int PIECES = (2 * S + 3) / 4;  // 16-byte pieces of a lane that a wave converts
-    uint4 next[PIECES];
-    const auto fetch = [&](int t, int block) {
-        const uint4* p = (const uint4*)(c.pool + kv_tile_offset(c, block, h, t & in_block)) + lane;
-#pragma unroll
-        for (int x = 0; x < PIECES; x++)
-            if ((x + 1) * 4 <= 2 * S || x * 4 + wave < 2 * S) next[x] = p[(x * 4 + wave) * 64];
-    };
-    const auto stage = [&](int buf) {
-#pragma unroll
-        for (int x = 0; x < PIECES; x++)
-            if ((x + 1) * 4 <= 2 * S || x * 4 + wave < 2 * S) {
-                tiles[buf][2 * (x * 4 + wave)][lane] = kv_half8<CODE>(next[x].x, next[x].y);
-                tiles[buf][2 * (x * 4 + wave) + 1][lane] = kv_half8<CODE>(next[x].z, next[x].w);
-            }
-    };
     // Step t: the exponentials and values of tile t stand beside the keys' products of
     // tile t + 1, so the vector and the matrix unit have independent work; tile t + 2 goes
     // to LDS, t + 3 to registers.  (Two buffers, values one step later, freed LDS that no
     // wave could use and took 1311 us for 1218: two addresses to a step.)
-    const int n_tiles = max(sp.t1 - sp.t0, 0);
-    KvTiles info = kv_tile_infos(c, table, h, sp.t0, 1, sp.t1), ahead = info;
-    const auto block_of = [&](int x) {  // of tile x, in info's 64 or the next
-        return x < 64 ? __builtin_amdgcn_readlane(info.block, x) : __builtin_amdgcn_readlane(ahead.block, x - 64);
-    };
     const auto products = [&](const half8(&k)[2 * S], floatx4(&u)[NC][2]) {
 #pragma unroll
         for (int n = 0; n < NC; n++) u[n][0] = u[n][1] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -538,15 +594,6 @@ __global__ __launch_bounds__(256, S == 8 ? 1 : 2) void kv_chunk_kernel(KvDev c, 
                         u[n][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[j * S + s], w.q[n][p][s], u[n][j], 0, 0, 0);
     };
     floatx4 u[NC][2];
-    if (n_tiles > 0) {
-        fetch(sp.t0, block_of(0));
-        stage(0);
-        if (n_tiles > 1) {
-            fetch(sp.t0 + 1, block_of(1));
-            stage(1);
-        }
-        if (n_tiles > 2) fetch(sp.t0 + 2, block_of(2));
-    }
     __syncthreads();
     if (n_tiles > 0) {
         half8 kop[2 * S];
@@ -566,11 +613,13 @@ __global__ __launch_bounds__(256, S == 8 ? 1 : 2) void kv_chunk_kernel(KvDev c, 
         for (int o = 0; o < 2 * S; o++) kop[o] = tiles[b1][o][lane];
         kv_reference(w, u, kv_lane(info.ks, y), kv_lane(info.lv, y), info.bad >> y & 1, t * KV_TILE, inside, a, b.tok0[i],
                      nullptr, 0, z);
-        if (y == 60) ahead = kv_tile_infos(c, table, h, t + 4, 1, sp.t1);
+        if (y == 60) ahead = kv_tile_infos(c, c.table + (size_t)b.seq[i] * c.W, h, t + 4, 1, sp.t1);
         half8 p0[NC], p1[NC];
         // past the last tile this works on what lies there, and is not used
 #pragma unroll
         for (int o = 0; o < 2 * S; o++) vop[o] = tiles[b0][2 * S + o][lane];
+        // the loads first: their use waits behind the keys' products (two halves: no registers for it)
+        if (PARTS == 1) __builtin_amdgcn_sched_barrier(0);
         products(kop, u);
         kv_exponents(w, z, rv, p0, p1);
 #pragma unroll
@@ -581,8 +630,8 @@ __global__ __launch_bounds__(256, S == 8 ? 1 : 2) void kv_chunk_kernel(KvDev c, 
                 if (PARTS > 1) w.o[n][o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vop[o], p1[n], w.o[n][o], 0, 0, 0);
             }
         }
-        stage(b2);
-        if (xt + 3 < n_tiles) fetch(t + 3, block_of(y + 3));
+        stage(b2, next);
+        if (xt + 3 < n_tiles) fetch(next, y + 3 < 64 ? kv_tile_of(c, info, y + 3) : kv_tile_of(c, ahead, y + 3 - 64));
         __syncthreads();
         const int tmp = b0;
         b0 = b1, b1 = b2, b2 = tmp;
@@ -596,12 +645,7 @@ __global__ __launch_bounds__(256, S == 8 ? 1 : 2) void kv_chunk_kernel(KvDev c, 
             if (g == 0) kv_finish(c, b, a, i, h, w.row[n], w.m[n], w.l[n]);
             const float inv = w.l[n] == 0.f ? 0.f : 1.f / w.l[n];
 #pragma unroll
-            for (int j = 0; j < 2 * S; j++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int d = 16 * j + 4 * g + e;
-                    if (d < c.D) kv_store(a.out, at * c.D + d, w.o[n][j][e] * inv + w.bad[n], a.q.type);
-                }
+            for (int j = 0; j < 2 * S; j++) kv_store4<PARTS>(a, at * c.D, 16 * j + 4 * g, c.D, w.o[n][j] * inv + w.bad[n]);
         } else {
             const size_t at = (size_t)blockIdx.x * WG_ROWS + (w.row[n] - wg_row0);
             if (g == 0) a.part_ml[at] = make_float2(w.m[n], w.l[n]);
@@ -611,56 +655,68 @@ __global__ __launch_bounds__(256, S == 8 ? 1 : 2) void kv_chunk_kernel(KvDev c, 
     }
 }
 
-// Joins the splits of a row whose tiles went to several workgroups: a workgroup per row,
-// Dp / 4 threads to a split; each thread adds its splits in order, then the thread groups.
-// unit0 counts row tiles here, aux is the first of the sequence's units.
+// Joins the splits of rows whose tiles went to several workgroups; Dp / 4 threads read a
+// partial row.  WIDE: a workgroup per row, its thread groups take splits in turn (steps of
+// many splits and few rows); else a thread group per row (chunks of few splits and many
+// rows).  unit0 counts row tiles here, aux is the first of the sequence's units.
+template <bool WIDE>
 __global__ __launch_bounds__(256) void kv_join_kernel(KvDev c, KvBatch b, KvAttend a, int wg_rows, int used_rows) {
     __shared__ floatx4 sh_o[256];
     __shared__ float sh_l[64];
     const int tid = threadIdx.x;
-    const int h = blockIdx.x % c.H, r = blockIdx.x / c.H % used_rows, unit = blockIdx.x / c.H / used_rows;
+    const int width = c.Dp / 4, groups = 256 / width, grp = tid / width, d4 = tid % width;
+    const int per_wg = WIDE ? 1 : groups, pieces = (used_rows + per_wg - 1) / per_wg;
+    const int h = blockIdx.x % c.H, piece = blockIdx.x / c.H % pieces, unit = blockIdx.x / c.H / pieces;
     const int i = kv_find(b, unit);
     const int rows = b.count[i] * a.G, u = unit - b.unit0[i];
-    const int tile = b.unit0[i + 1] - b.unit0[i] - 1 - u;
-    const int row0 = tile * wg_rows, row = row0 + r;
-    if (row >= rows) return;
+    const int row0 = (b.unit0[i + 1] - b.unit0[i] - 1 - u) * wg_rows;
+    const int r = WIDE ? piece : piece * groups + grp, row = row0 + r;
     int lo0, hi0, lo1, hi1;
     kv_range(a, b.len[i], b.count[i], row0, lo0, hi0);
     kv_range(a, b.len[i], b.count[i], min(row0 + wg_rows, rows) - 1, lo1, hi1);
     const int tiles = (hi1 + KV_TILE - 1) / KV_TILE - lo0 / KV_TILE;
     const int splits = (tiles + b.per[i] - 1) / b.per[i];
-    if (splits <= 1) return;  // the one workgroup has written the row
-    const size_t stride = (size_t)c.H * wg_rows;
-    const size_t base = ((size_t)(b.aux[i] + u * b.splits[i]) * c.H + h) * wg_rows + r;
+    if (splits <= 1) return;  // the one workgroup has written the rows
+    if (WIDE ? row >= rows : (grp >= groups || r >= wg_rows || row >= rows)) return;
+    const size_t stride = (size_t)(b.unit0[i + 1] - b.unit0[i]) * c.H * wg_rows;
+    const size_t base = ((size_t)(b.aux[i] + u) * c.H + h) * wg_rows + r;
     float mx = KV_NEG;
-    for (int s = tid & 63; s < splits; s += 64) mx = fmaxf(mx, a.part_ml[base + s * stride].x);
+    if (WIDE) {
+        for (int s = tid & 63; s < splits; s += 64) mx = fmaxf(mx, a.part_ml[base + s * stride].x);
 #pragma unroll
-    for (int x = 32; x; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
-    const int width = c.Dp / 4, groups = 256 / width, grp = tid / width, d4 = tid % width;
+        for (int x = 32; x; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
+    } else {
+        for (int s = 0; s < splits; s++) mx = fmaxf(mx, a.part_ml[base + s * stride].x);
+    }
     floatx4 o = {0.f, 0.f, 0.f, 0.f};
     float l = 0.f;
     if (grp < groups) {
 #pragma unroll 4
-        for (int s = grp; s < splits; s += groups) {
+        for (int s = WIDE ? grp : 0; s < splits; s += WIDE ? groups : 1) {
             const float2 ml = a.part_ml[base + s * stride];
             const float f = kv_join_factor(ml.x, ml.y, mx);
             l += f * ml.y;
             o += *(const floatx4*)(a.part_o + (base + s * stride) * c.Dp + d4 * 4) * f;
         }
-        sh_o[tid] = o;
-        if (d4 == 0) sh_l[grp] = l;
     }
-    __syncthreads();
-    if (tid >= width) return;
-    for (int x = 1; x < groups; x++) o += sh_o[x * width + tid];
-    l = sh_l[0];
-    for (int x = 1; x < groups; x++) l += sh_l[x];
-    if (tid == 0) kv_finish(c, b, a, i, h, row, mx, l);
+    if (WIDE) {
+        if (grp < groups) {
+            sh_o[tid] = o;
+            if (d4 == 0) sh_l[grp] = l;
+        }
+        __syncthreads();
+        if (tid >= width) return;
+        for (int x = 1; x < groups; x++) o += sh_o[x * width + tid];
+        l = sh_l[0];
+        for (int x = 1; x < groups; x++) l += sh_l[x];
+    }
+    if (d4 == 0) kv_finish(c, b, a, i, h, row, mx, l);
     const size_t at = kv_row(c, b, a, i, h, row) * c.D;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int e = 0; e < 4; e++)
-        if (4 * tid + e < c.D) kv_store(a.out, at + 4 * tid + e, o[e] * inv, a.q.type);
+    o = o * (l == 0.f ? 0.f : 1.f / l);
+    if (a.q.type == KV_F32)
+        kv_store4<2>(a, at, 4 * d4, c.D, o);
+    else
+        kv_store4<1>(a, at, 4 * d4, c.D, o);
 }
 
 // Weights from the kept scores of a step: four slots to a thread, bound by the scores' bytes.
@@ -914,8 +970,15 @@ void launch_kv_attend(const KvDev& c, const KvBatch& b, const KvAttend& a, hipSt
         j.unit0[i + 1] = j.unit0[i] + tiles;
         if (tiles && rows > used) used = rows < wg_rows ? rows : wg_rows;
     }
-    if (j.unit0[j.n])
-        hipLaunchKernelGGL(kv_join_kernel, dim3((unsigned)j.unit0[j.n] * c.H * used), dim3(256), 0, s, c, j, a, wg_rows, used);
+    if (!j.unit0[j.n]) return;
+    if (a.by_rows) {
+        const int per_wg = 256 / (c.Dp / 4);
+        hipLaunchKernelGGL(kv_join_kernel<false>, dim3((unsigned)j.unit0[j.n] * c.H * ((used + per_wg - 1) / per_wg)),
+                           dim3(256), 0, s, c, j, a, wg_rows, used);
+    } else {
+        hipLaunchKernelGGL(kv_join_kernel<true>, dim3((unsigned)j.unit0[j.n] * c.H * used), dim3(256), 0, s, c, j, a,
+                           wg_rows, used);
+    }
 }
 
 void launch_kv_weights(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s) {

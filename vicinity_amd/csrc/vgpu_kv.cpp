@@ -22,7 +22,7 @@ constexpr int64_t kStepWorkgroups = 768;
 // Workgroups of a call with many rows, two to a compute unit: with fewer, the tiles are
 // split too, which costs a partial result for every row and split.
 constexpr int64_t kChunkWorkgroups = 512;
-constexpr int64_t kWeightWorkgroups = 1024;
+constexpr int64_t kWeightWorkgroups = 3072;
 // Bytes of partial results of one launch.
 constexpr int64_t kPartBytes = (int64_t)256 << 20;
 // Steps of at most this many rows per head keep their scores for the weights.
@@ -392,6 +392,7 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
     a.decay = q.decay;
     a.out = q.out;
     a.lse = q.lse;
+    a.vec_out = dev.D % 4 == 0 && (uintptr_t)q.out % (4 * item_size(a.q.type)) == 0;
     int64_t tokens = 0, longest = 0, most = 0;
     for (size_t i = 0; i < n; i++) {
         need(counts[i] >= 0, "counts must not be negative");
@@ -442,7 +443,9 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
             row_tiles += (counts[i] * a.G + 15) / 16;
             if (a.window && a.causal)
                 tiles[j] = std::min<int64_t>(tiles[j], (a.window + rows / a.G + 2 * KV_TILE) / KV_TILE + 1);
-            work += row_units[j] * dev.H * tiles[j];
+            // (the first tokens of a chunk see less than the last)
+            const int64_t seen = a.causal && !a.window ? std::max<int64_t>(2 * len - counts[i], 0) : 2 * KV_TILE * tiles[j];
+            work += row_units[j] * dev.H * ((seen + 2 * KV_TILE - 1) / (2 * KV_TILE));
         }
         need(units <= INT_MAX / 64, "too many query rows in one call");
         if (units) {
@@ -454,7 +457,10 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
                 groups = split_units = 0;
                 bool one = true;
                 for (int j = 0; j < b.n; j++) {
-                    const int64_t splits = a.by_rows && units >= target ? 1 : std::max<int64_t>((tiles[j] + each - 1) / each, 1);
+                    // many rows: whole unless that would leave one workgroup at work alone
+                    const int64_t most_tiles = a.by_rows ? each + each / 4 : each;
+                    const int64_t splits = a.by_rows && units >= 4 * target
+                                               ? 1 : std::max<int64_t>((tiles[j] + most_tiles - 1) / most_tiles, 1);
                     b.splits[j] = (int)splits;
                     b.per[j] = (int)std::max<int64_t>((tiles[j] + splits - 1) / splits, 1);
                     b.unit0[j + 1] = b.unit0[j] + (int)(row_units[j] * splits);
@@ -462,7 +468,7 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
                     one = one && splits == 1;
                     if (splits > 1) split_units += row_units[j] * splits * dev.H;
                 }
-                if (one || (groups <= target + target / 8 && groups <= part_units)) break;
+                if (one || ((a.by_rows || groups <= target + target / 8) && groups <= part_units)) break;
             }
             a.part_o = nullptr, a.part_ml = nullptr, a.scores = nullptr;
             if (split_units) {

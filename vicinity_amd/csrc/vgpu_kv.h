@@ -139,6 +139,7 @@ struct KvAttend {
     int track = 0;
     float decay = 0.f;
     void* out = nullptr;       // [tokens, H * G, D] in q's type
+    bool vec_out = false;      // 4 dims of its rows are one aligned piece
     float* lse = nullptr;      // [tokens, H * G]
     // tracked: base-2 lse of the rows, [sequence][head][row] (-inf: sees nothing)
     float* lse2 = nullptr;
