@@ -51,13 +51,17 @@ __device__ __forceinline__ void load8(const KvTensor& x, int64_t row, int m, int
 }
 
 __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, int code) {
+    const float z = code == KV_INT8 ? 127.f : 448.f;
+    // (a NaN becomes some number: its block's scale is NaN)
+    a = __builtin_amdgcn_fmed3f(a, -z, z), b = __builtin_amdgcn_fmed3f(b, -z, z);
+    c = __builtin_amdgcn_fmed3f(c, -z, z), d = __builtin_amdgcn_fmed3f(d, -z, z);
     if (code == KV_INT8) {
-        const int i0 = (int)rintf(fminf(fmaxf(a, -127.f), 127.f)) + 128, i1 = (int)rintf(fminf(fmaxf(b, -127.f), 127.f)) + 128;
-        const int i2 = (int)rintf(fminf(fmaxf(c, -127.f), 127.f)) + 128, i3 = (int)rintf(fminf(fmaxf(d, -127.f), 127.f)) + 128;
-        return (uint32_t)i0 | (uint32_t)i1 << 8 | (uint32_t)i2 << 16 | (uint32_t)i3 << 24;
+        // 1.5 * 2^23 + 128: the sum's last byte is the integer, ties to even, plus 128
+        const float m = 12583040.f;
+        const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(b + m), __float_as_uint(a + m), 0x0c0c0400u);
+        const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(d + m), __float_as_uint(c + m), 0x04000c0cu);
+        return lo | hi;
     }
-    a = fminf(fmaxf(a, -448.f), 448.f), b = fminf(fmaxf(b, -448.f), 448.f);
-    c = fminf(fmaxf(c, -448.f), 448.f), d = fminf(fmaxf(d, -448.f), 448.f);
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
     w = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
     return (uint32_t)w;
@@ -82,17 +86,36 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float r, int code) {
     return encode4(v[0] * r, v[1] * r, v[2] * r, v[3] * r, code);
 }
 
+// Byte l & 3 of each of the quad's four lanes, in their order.
+__device__ __forceinline__ uint32_t quad_transpose(uint32_t w) {
+    const uint32_t q = threadIdx.x & 3;
+    const uint32_t a0 = (uint32_t)__builtin_amdgcn_mov_dpp((int)w, 0x00, 0xf, 0xf, true);
+    const uint32_t a1 = (uint32_t)__builtin_amdgcn_mov_dpp((int)w, 0x55, 0xf, 0xf, true);
+    const uint32_t a2 = (uint32_t)__builtin_amdgcn_mov_dpp((int)w, 0xaa, 0xf, 0xf, true);
+    const uint32_t a3 = (uint32_t)__builtin_amdgcn_mov_dpp((int)w, 0xff, 0xf, 0xf, true);
+    const uint32_t sel = q | (q + 4) << 8;  // byte q of the second operand, then of the first
+    const uint32_t lo = __builtin_amdgcn_perm(a1, a0, sel), hi = __builtin_amdgcn_perm(a3, a2, sel);
+    return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+}
+
 __global__ __launch_bounds__(256) void kv_table_kernel(int* table, KvRuns r) {
     const int i = blockIdx.x;
     for (int j = threadIdx.x; j < r.count[i]; j += blockDim.x) table[r.at[i] + j] = r.block[i] + j;
 }
 
-// One workgroup: the keys or the values of one (block, head) that new tokens enter.
+// One workgroup: the keys or the values of one (block, head) that new tokens enter.  Each
+// thread loads its pieces of 8 dims once and keeps them (HOLD of them; blocks with more are
+// read a second time, from L2) until the scale is known; the codes are put in order in LDS
+// and leave in 16-byte pieces.  A few tokens in a begun block that keeps its scale go to
+// their bytes directly.  Bound by the bytes in and out.
+constexpr int KV_HOLD = 8;
+constexpr int KV_FEW = 4;
+
 template <int T>
 __global__ __launch_bounds__(256) void kv_append_kernel(KvDev c, KvBatch b, KvTensor k, KvTensor v,
                                                         const int* __restrict__ positions,
                                                         const float* __restrict__ weights) {
-    __shared__ __align__(16) uint8_t image[KV_TILE * KV_MAX_DIM];
+    extern __shared__ __align__(16) uint8_t image[];  // the block's codes: B * Dp bytes
     __shared__ uint32_t red[4];
     const int tid = threadIdx.x;
     const bool vals = blockIdx.x & 1;
@@ -102,21 +125,64 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvDev c, KvBatch b, KvTe
     const int blk = (len0 >> c.shift) + unit - b.unit0[i];
     const int slot0 = blk << c.shift;
     const int held = max(len0 - slot0, 0), end = min(len1 - slot0, c.B);  // new slots held .. end - 1
-    const int block = c.table[(size_t)b.seq[i] * c.W + blk];
+    // a sequence that touches one block brings its number, and the table learns a new one here
+    int* entry = c.table + (size_t)b.seq[i] * c.W + blk;
+    const int block = b.splits[i] >= 0 ? b.splits[i] : *entry;
+    if (b.splits[i] >= 0 && !held && h == 0 && !vals && tid == 0) *entry = block;
     const size_t part = (size_t)block * c.H + h;
     const KvTensor& x = vals ? v : k;
     const int64_t tok0 = (int64_t)b.tok0[i] + slot0 - len0;  // token of slot 0 of the block
-    const int S = c.Dp / 32;
-    const int Md = (c.D + 7) / 8;
+    // piece u: 8 dims m of the new slot r.  Values go by quads of slots, aligned in the block
+    // (r may lie outside at its ends), so that a quad of lanes can exchange their codes.
+    const int S = c.Dp / 32, Md = (c.D + 7) / 8;
+    // u / Md of u < 256 Md, Md <= 32: the product's excess stays below 2^20
+    const uint32_t inv_m = ((1u << 20) + Md - 1) / Md;
+    const auto split = [&](int u, int& q, int& m) {
+        q = (int)((uint32_t)u * inv_m >> 20);
+        m = u - q * Md;
+    };
+    const int start = vals ? held & ~3 : held, units = (vals ? (end - start + 3 & ~3) : end - held) * Md;
+    const auto piece = [&](int u, int& r, int& m) {
+        int q;
+        split(vals ? u >> 2 : u, q, m);
+        r = start + (vals ? q * 4 + (u & 3) : q);
+        return r >= held && r < end;
+    };
+    const auto load = [&](int u, float(&y)[8]) {
+        int r, m;
+        if (piece(u, r, m)) {
+            load8<T>(x, (tok0 + r) * x.st + (int64_t)h * x.sh, m, c.D, y);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) y[j] = 0.f;
+        }
+    };
+    float* scale = (vals ? c.vscale : c.kscale) + part;
+    const float s_old = held ? *scale : 0.f;
+    uint8_t* base = c.pool + kv_tile_offset(c, block, h, 0) + (vals ? kv_half(c.Dp) : 0);
+    const int half = kv_half(c.Dp);
 
     // largest magnitude, as bits: infinities and NaN are above every number
     uint32_t big = 0;
-    for (int u = tid; u < (end - held) * Md; u += 256) {
-        const int r = held + u / Md, m = u % Md;
-        float e[8];
-        load8<T>(x, (tok0 + r) * x.st + (int64_t)h * x.sh, m, c.D, e);
+    float e[KV_HOLD][8];
+    const bool hold = units <= KV_HOLD * 256;
+    const auto magnitude = [&](const float(&y)[8]) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) big = max(big, __float_as_uint(e[j]) & 0x7fffffffu);
+        for (int j = 0; j < 8; j++) big = max(big, __float_as_uint(y[j]) & 0x7fffffffu);
+    };
+    if (hold) {
+#pragma unroll
+        for (int z = 0; z < KV_HOLD; z++) {
+            if (z * 256 + tid < units) load(z * 256 + tid, e[z]);
+        }
+#pragma unroll
+        for (int z = 0; z < KV_HOLD; z++)
+            if (z * 256 + tid < units) magnitude(e[z]);
+    } else {
+        for (int u = tid; u < units; u += 256) {
+            load(u, e[0]);
+            magnitude(e[0]);
+        }
     }
 #pragma unroll
     for (int o = 32; o; o >>= 1) big = max(big, (uint32_t)__shfl_xor((int)big, o));
@@ -125,25 +191,29 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvDev c, KvBatch b, KvTe
     big = max(max(red[0], red[1]), max(red[2], red[3]));
     const float rz = c.code == KV_INT8 ? 1.f / 127.f : 1.f / 448.f;
     const float amax = __uint_as_float(big);
-    float* scale = (vals ? c.vscale : c.kscale) + part;
-    const float s_old = held ? *scale : 0.f;
     float s = amax >= KV_TINY ? amax * rz : 0.f;
     s = s_old > s ? s_old : s;
     if (big >= 0x7f800000u || s_old != s_old) s = __uint_as_float(0x7fc00000u);
     const float inv = s > 0.f ? 1.f / s : 0.f;
     const float ratio = s > 0.f ? s_old / s : 0.f;
     const bool grown = held && s > s_old;  // (false for NaN: the old codes stay as they are)
-    __syncthreads();
-    if (tid == 0) *scale = s;
+    if (tid == 0 && !(s == s_old && held)) *scale = s;
+    if (!vals) {
+        for (int r = held + tid; r < end; r += 256) {
+            const int64_t at = (tok0 + r) * c.H + h;
+            c.positions[part * c.B + r] = positions ? positions[at] : b.aux[i] + slot0 + r - len0;
+            c.weights[part * c.B + r] = weights ? weights[at] : 0.f;
+        }
+    }
 
-    uint8_t* base = c.pool + kv_tile_offset(c, block, h, 0) + (vals ? kv_half(c.Dp) : 0);
-    for (int t = grown ? 0 : held / KV_TILE; t * KV_TILE < end; t++) {
-        uint8_t* tile = base + (size_t)t * 2 * kv_half(c.Dp);
-        const int r0 = t * KV_TILE;
-        for (int u = tid; u < kv_half(c.Dp) / 16; u += 256) {
+    const bool direct = held % KV_TILE && !grown && end - held <= KV_FEW && held / KV_TILE == (end - 1) / KV_TILE;
+    const int first = grown ? 0 : held / KV_TILE, last = (end + KV_TILE - 1) / KV_TILE;  // tiles that change
+    if (!direct) {
+        for (int u = tid; u < (last - first) * half / 16; u += 256) {
+            const int t = first + u * 16 / half, o = u % (half / 16);
             uint4 w = {zero_codes(c.code), zero_codes(c.code), zero_codes(c.code), zero_codes(c.code)};
-            if (r0 < held) {
-                w = ((const uint4*)tile)[u];
+            if (t * KV_TILE < held) {
+                w = ((const uint4*)(base + (size_t)t * 2 * half))[o];
                 if (grown) {
                     w.x = rescale4(w.x, ratio, c.code), w.y = rescale4(w.y, ratio, c.code);
                     w.z = rescale4(w.z, ratio, c.code), w.w = rescale4(w.w, ratio, c.code);
@@ -152,32 +222,47 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvDev c, KvBatch b, KvTe
             ((uint4*)image)[u] = w;
         }
         __syncthreads();
-        const int lo = max(held - r0, 0), hi = min(end - r0, KV_TILE);
-        for (int u = tid; u < (hi - lo) * Md; u += 256) {
-            const int r = lo + u / Md, m = u % Md;
-            float e[8];
-            load8<T>(x, (tok0 + r0 + r) * x.st + (int64_t)h * x.sh, m, c.D, e);
-            const uint32_t w0 = encode4(e[0] * inv, e[1] * inv, e[2] * inv, e[3] * inv, c.code);
-            const uint32_t w1 = encode4(e[4] * inv, e[5] * inv, e[6] * inv, e[7] * inv, c.code);
-            if (!vals) {
-                *(uint2*)(image + kv_key_byte(r, m, S)) = make_uint2(w0, w1);
+    }
+    const auto encode = [&](int u, const float(&y)[8]) {
+        int r, m;
+        (void)piece(u, r, m);
+        const int t = r / KV_TILE;
+        uint32_t w[2] = {encode4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv, c.code),
+                         encode4(y[4] * inv, y[5] * inv, y[6] * inv, y[7] * inv, c.code)};
+        uint8_t* to = direct ? base + (size_t)t * 2 * half : image + (t - first) * half;
+        if (!vals) {
+            *(uint2*)(to + kv_key_byte(r & 31, m, S)) = make_uint2(w[0], w[1]);
+            return;
+        }
+        // four slots of dim 8 m + (lane of the quad), and of that + 4
+        const int r0 = r & ~3, d = 8 * m + (u & 3);
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const uint32_t four = quad_transpose(w[j]);
+            uint8_t* at = to + kv_value_byte(r0 & 31, d + 4 * j);
+            if (r0 >= held && r0 + 3 < end) {
+                *(uint32_t*)at = four;
             } else {
 #pragma unroll
-                for (int j = 0; j < 8; j++)
-                    image[kv_value_byte(r, 8 * m + j)] = (uint8_t)((j < 4 ? w0 : w1) >> (8 * (j & 3)));
+                for (int z = 0; z < 4; z++)
+                    if (r0 + z >= held && r0 + z < end) at[z] = (uint8_t)(four >> (8 * z));
             }
         }
-        __syncthreads();
-        for (int u = tid; u < kv_half(c.Dp) / 16; u += 256) ((uint4*)tile)[u] = ((const uint4*)image)[u];
-        __syncthreads();
-    }
-    if (!vals) {
-        for (int r = held + tid; r < end; r += 256) {
-            const int64_t at = (tok0 + r) * c.H + h;
-            c.positions[part * c.B + r] = positions ? positions[at] : b.aux[i] + slot0 + r - len0;
-            c.weights[part * c.B + r] = weights ? weights[at] : 0.f;
+    };
+    if (hold) {
+#pragma unroll
+        for (int z = 0; z < KV_HOLD; z++)
+            if (z * 256 + tid < units) encode(z * 256 + tid, e[z]);
+    } else {
+        for (int u = tid; u < units; u += 256) {
+            load(u, e[0]);
+            encode(u, e[0]);
         }
     }
+    if (direct) return;
+    __syncthreads();
+    for (int u = tid; u < (last - first) * half / 16; u += 256)
+        ((uint4*)(base + (size_t)(first + u * 16 / half) * 2 * half))[u % (half / 16)] = ((const uint4*)image)[u];
 }
 
 __device__ __forceinline__ void store1(void* p, size_t i, float v, int type) {
@@ -205,9 +290,10 @@ __device__ __forceinline__ void store_row(void* p, size_t row, int d, int D, boo
                 store1(h, 0, v[2 * j], T), store1(h, 1, v[2 * j + 1], T);
                 w[j] = (uint32_t)h[0] | (uint32_t)h[1] << 16;
             }
-#pragma unroll
-            for (int j = 0; j < N / 8; j++)
-                ((uint4*)((uint16_t*)p + row + d))[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+            if (N == 4)
+                *(uint2*)((uint16_t*)p + row + d) = make_uint2(w[0], w[1]);
+            else
+                *(uint4*)((uint16_t*)p + row + d) = make_uint4(w[0], w[1], w[N / 2 - 2], w[N / 2 - 1]);
         }
         return;
     }
@@ -217,7 +303,7 @@ __device__ __forceinline__ void store_row(void* p, size_t row, int d, int D, boo
 }
 
 // The values of a tile, by one wave: a lane takes its 16 bytes of each piece, which are
-// 8 dims each of one slot and two operands (keys), or two dims of 8 slots (values).
+// 8 dims each of one slot and two operands (keys), or of 8 slots and two dims (values).
 // row(slot): the element index of the slot's row in the outputs, or ~0.
 template <int T, typename Row>
 __device__ __forceinline__ void read_tile(const KvDev& c, const uint8_t* tile, float ks, float vs, void* ko, void* vo,
@@ -243,21 +329,22 @@ __device__ __forceinline__ void read_tile(const KvDev& c, const uint8_t* tile, f
         }
     }
     if (vo) {
-        size_t rows[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) rows[i] = row((i >> 2) * 16 + 4 * g + (i & 3));
+        // a quad of lanes exchanges bytes, so that a lane has 4 dims of slots 4 g + (x & 3)
+        // and 16 above
+        const int r = 4 * g + (x & 3);
+        const size_t rows[2] = {row(r), row(16 + r)};
         for (int p = 0; p < S; p++) {
             const uint4 w = at[(S + p) * 64];
 #pragma unroll
             for (int o = 0; o < 2; o++) {
-                const int d = (2 * p + o) * 16 + x;
-                float e[8];
-                decode4(o ? w.z : w.x, c.code, e);
-                decode4(o ? w.w : w.y, c.code, e + 4);
-                if (d < c.D) {
+                const int d = (2 * p + o) * 16 + (x & ~3);
 #pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        if (rows[i] != ~(size_t)0) store1(vo, rows[i] + d, e[i] * vs, T);
+                for (int half = 0; half < 2; half++) {
+                    float e[4];
+                    decode4(quad_transpose(half ? (o ? w.w : w.y) : (o ? w.z : w.x)), c.code, e);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) e[i] *= vs;
+                    if (rows[half] != ~(size_t)0) store_row<T, 4>(vo, rows[half], d, c.D, vec, e);
                 }
             }
         }
@@ -265,8 +352,8 @@ __device__ __forceinline__ void read_tile(const KvDev& c, const uint8_t* tile, f
 }
 
 // One workgroup: 128 slots of one head, a tile to a wave.  Bound by the bytes written:
-// no element passes through LDS, a key store is 32 contiguous bytes of a lane, a value
-// store 64 bytes of 16 lanes.
+// no element passes through LDS; a key store is 32 contiguous bytes of a lane, a value
+// store 16 (64 of four lanes).
 template <int T>
 __global__ __launch_bounds__(256) void kv_read_kernel(KvDev c, KvBatch b, KvReadOut o) {
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -308,87 +395,226 @@ __device__ __forceinline__ size_t slot_at(const KvDev& c, const int* row, int h,
     return ((size_t)row[slot >> c.shift] * c.H + h) * c.B + (slot & (c.B - 1));
 }
 
-// One workgroup: which slots of one (sequence, head) stay.  The key of the last one
-// that does is found by its 8-bit digits, from the top; of the slots with that very
-// key the lowest stay.
-__global__ __launch_bounds__(1024) void kv_select_kernel(KvDev c, KvBatch b, KvEvict e) {
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t sh_prefix, sh_need;
-    __shared__ uint32_t wsum[2][16];
+// The weight of the last slot that stays is found by its key's digits of 11, 11 and 10
+// bits, from the top: a histogram of the slots that share the digits so far, and the digit
+// in which the count from above reaches what is needed.  Of the slots with that very key
+// the lowest stay.
+constexpr int KV_BINS = 2048;
+__device__ __forceinline__ int digit_shift(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
+__device__ __forceinline__ uint32_t digit_bits(int pass) { return pass == 0 ? 0xffe00000u : pass == 1 ? 0xfffffc00u : ~0u; }
+__device__ __forceinline__ uint32_t digit_of(uint32_t key, int pass) { return key >> digit_shift(pass) & (pass < 2 ? 2047u : 1023u); }
+
+struct KvCut {
+    uint32_t key, need;  // the digits so far; how many of the slots that share them stay
+};
+// By 1024 threads: adds the digit of a histogram (LDS or global).  scan: 18 words of LDS.
+__device__ void find_digit(const uint32_t* hist, int pass, uint32_t* scan, KvCut& cut) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int h = blockIdx.x % c.H, i = blockIdx.x / c.H;
-    const int* row = c.table + (size_t)b.seq[i] * c.W;
-    const int len = b.len[i], stay = b.count[i];
-    int* kept = e.kept + ((size_t)i * c.H + h) * e.budget;
-    int* gone = e.gone ? e.gone + ((size_t)i * c.H + h) * e.slots : nullptr;
-    const int recent = stay < len ? min(e.recent, stay) : 0;
-    const int old = len - recent, want = stay - recent;
-    uint32_t prefix = 0, bits = 0, need = want;
-    if (want > 0 && want < old) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int j = tid; j < 256; j += 1024) hist[j] = 0;
+    const int hi = KV_BINS - 1 - 2 * tid;  // this thread's two bins, from the top
+    const uint32_t c0 = hist[hi], c1 = hist[hi - 1];
+    uint32_t sum = c0 + c1;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t up = (uint32_t)__shfl_up((int)sum, o);
+        if (lane >= o) sum += up;
+    }
+    if (lane == 63) scan[wave] = sum;
+    __syncthreads();
+    for (int w = 0; w < wave; w++) sum += scan[w];
+    const uint32_t before = sum - c0 - c1;
+    if (before < cut.need && sum >= cut.need) {  // one thread
+        const bool first = before + c0 >= cut.need;
+        scan[16] = (uint32_t)(first ? hi : hi - 1);
+        scan[17] = cut.need - before - (first ? 0 : c0);
+    }
+    __syncthreads();
+    cut.key |= scan[16] << digit_shift(pass);
+    cut.need = scan[17];
+    __syncthreads();
+}
+
+// One (sequence, head): the slots before `old` compete for `want` places.
+struct KvSelect {
+    const int* row;
+    int h, old, want, recent;
+    int *kept, *gone;
+    bool compete;
+};
+__device__ __forceinline__ KvSelect select_job(const KvDev& c, const KvBatch& b, const KvEvict& e, int i, int h) {
+    KvSelect j;
+    j.row = c.table + (size_t)b.seq[i] * c.W;
+    j.h = h;
+    j.kept = e.kept + ((size_t)i * c.H + h) * e.budget;
+    j.gone = e.gone ? e.gone + ((size_t)i * c.H + h) * e.slots : nullptr;
+    j.recent = b.count[i] < b.len[i] ? min(e.recent, b.count[i]) : 0;
+    j.old = b.len[i] - j.recent, j.want = b.count[i] - j.recent;
+    j.compete = j.want > 0 && j.want < j.old;
+    return j;
+}
+
+// Whether each of 1024 threads' slots stays, and its place: done and equal count what the
+// slots before took and how many had the cut's key.
+__device__ __forceinline__ void place_slots(const KvSelect& s, const KvCut& cut, uint32_t key, int j, bool in,
+                                            uint32_t* scan, uint32_t& done, uint32_t& equal) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const bool eq = in && s.compete && key == cut.key;
+    const bool above = in && (s.want >= s.old || (s.compete && key > cut.key));
+    const uint64_t eb = __ballot(eq), ab = __ballot(above);
+    if (lane == 0) scan[wave] = (uint32_t)__popcll(eb) | (uint32_t)__popcll(ab) << 16;
+    __syncthreads();
+    uint32_t e0 = equal, a0 = 0, all_e = 0, all_a = 0;
+    for (int w = 0; w < 16; w++) {
+        const uint32_t x = scan[w];
+        if (w < wave) e0 += x & 0xffffu, a0 += x >> 16;
+        all_e += x & 0xffffu, all_a += x >> 16;
+    }
+    const uint64_t below = (1ull << lane) - 1;
+    e0 += (uint32_t)__popcll(eb & below), a0 += (uint32_t)__popcll(ab & below);
+    // kept so far: those above the cut, and of the equal ones at most cut.need
+    const uint32_t at = done - min(equal, cut.need) + a0 + min(e0, cut.need);
+    const bool keep = above || (eq && e0 < cut.need);
+    if (keep) s.kept[at] = j;
+    if (in && s.gone) s.gone[j] = keep ? -1 : j - (int)at;
+    done += all_a + min(equal + all_e, cut.need) - min(equal, cut.need);
+    equal += all_e;
+    __syncthreads();
+}
+
+// Up to 16384 slots: one workgroup, the keys in registers.
+constexpr int KV_SELECT = 16;
+__global__ __launch_bounds__(1024) void kv_select_kernel(KvDev c, KvBatch b, KvEvict e) {
+    __shared__ uint32_t hist[KV_BINS];
+    __shared__ uint32_t scan[18];
+    const int tid = threadIdx.x;
+    const KvSelect s = select_job(c, b, e, blockIdx.x / c.H, blockIdx.x % c.H);
+    uint32_t key[KV_SELECT];
+#pragma unroll
+    for (int x = 0; x < KV_SELECT; x++) {
+        const int j = x * 1024 + tid;
+        key[x] = s.compete && j < s.old ? weight_key(c.weights[slot_at(c, s.row, s.h, j)]) : 0;
+    }
+    KvCut cut = {0, (uint32_t)max(s.want, 0)};
+    if (s.compete) {
+        for (int pass = 0; pass < 3; pass++) {
+            hist[tid] = hist[tid + 1024] = 0;
             __syncthreads();
-            for (int j = tid; j < old; j += 1024) {
-                const uint32_t key = weight_key(c.weights[slot_at(c, row, h, j)]);
-                if ((key & bits) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1u);
-            }
+            const uint32_t bits = pass ? digit_bits(pass - 1) : 0;
+#pragma unroll
+            for (int x = 0; x < KV_SELECT; x++)
+                if (x * 1024 + tid < s.old && (key[x] & bits) == cut.key) atomicAdd(&hist[digit_of(key[x], pass)], 1u);
             __syncthreads();
-            if (tid == 0) {
-                uint32_t left = need;
-                int digit = 255;
-                for (; digit > 0 && hist[digit] < left; digit--) left -= hist[digit];
-                sh_prefix = prefix | (uint32_t)digit << shift;
-                sh_need = left;
-            }
-            __syncthreads();
-            prefix = sh_prefix, need = sh_need;
-            bits |= 255u << shift;
+            find_digit(hist, pass, scan, cut);
         }
     }
-    // prefix: the key of the last slot that stays, need: how many with that key do
     uint32_t done = 0, equal = 0;
-    for (int j0 = 0; j0 < old; j0 += 1024) {
-        const int j = j0 + tid;
-        const bool in = j < old;
-        const uint32_t key = in && want > 0 && want < old ? weight_key(c.weights[slot_at(c, row, h, j)]) : 0;
-        const bool eq = in && want > 0 && want < old && key == prefix;
-        const uint64_t eb = __ballot(eq);
-        if (lane == 0) wsum[0][wave] = (uint32_t)__popcll(eb);
-        __syncthreads();
-        uint32_t before = equal, all = 0;
-        for (int w = 0; w < 16; w++) {
-            if (w < wave) before += wsum[0][w];
-            all += wsum[0][w];
-        }
-        const uint32_t rank = before + (uint32_t)__popcll(eb & ((1ull << lane) - 1));
-        const bool keep = in && (want >= old || (want > 0 && (key > prefix || (eq && rank < need))));
-        const uint64_t kb = __ballot(keep);
-        if (lane == 0) wsum[1][wave] = (uint32_t)__popcll(kb);
-        __syncthreads();
-        uint32_t at = done, kall = 0;
-        for (int w = 0; w < 16; w++) {
-            if (w < wave) at += wsum[1][w];
-            kall += wsum[1][w];
-        }
-        at += (uint32_t)__popcll(kb & ((1ull << lane) - 1));
-        if (keep) kept[at] = j;
-        if (in && gone) gone[j] = keep ? -1 : j - (int)at;
-        equal += all, done += kall;
-        __syncthreads();
-    }
-    for (int j = tid; j < recent; j += 1024) {
-        kept[want + j] = old + j;
-        if (gone) gone[old + j] = -1;
+#pragma unroll
+    for (int x = 0; x < KV_SELECT; x++)
+        if (x * 1024 < s.old) place_slots(s, cut, key[x], x * 1024 + tid, x * 1024 + tid < s.old, scan, done, equal);
+    for (int j = tid; j < s.recent; j += 1024) {
+        s.kept[s.want + j] = s.old + j;
+        if (s.gone) s.gone[s.old + j] = -1;
     }
 }
 
-// One workgroup: one block of one head of the result.
+// Longer sequences: 4096 slots to a workgroup and a launch for each step, e.hist (three
+// histograms of each sequence and head, zero before) and e.counts between them.
+constexpr int KV_LONG = 4096;
+__device__ __forceinline__ KvCut long_cut(const KvDev& c, const KvEvict& e, const KvSelect& s, int i, int passes, uint32_t* scan) {
+    KvCut cut = {0, (uint32_t)max(s.want, 0)};
+    if (s.compete)
+        for (int p = 0; p < passes; p++) find_digit(e.hist + (((size_t)i * c.H + s.h) * 3 + p) * KV_BINS, p, scan, cut);
+    return cut;
+}
+
+__global__ __launch_bounds__(1024) void kv_long_hist_kernel(KvDev c, KvBatch b, KvEvict e, int groups, int pass) {
+    __shared__ uint32_t hist[KV_BINS];
+    __shared__ uint32_t scan[18];
+    const int tid = threadIdx.x, h = blockIdx.x % c.H, g = blockIdx.x / c.H % groups, i = blockIdx.x / c.H / groups;
+    const KvSelect s = select_job(c, b, e, i, h);
+    if (!s.compete || g * KV_LONG >= s.old) return;
+    uint32_t key[4];
+#pragma unroll
+    for (int x = 0; x < 4; x++) {
+        const int j = g * KV_LONG + x * 1024 + tid;
+        key[x] = j < s.old ? weight_key(c.weights[slot_at(c, s.row, h, j)]) : 0;
+    }
+    const KvCut cut = long_cut(c, e, s, i, pass, scan);
+    hist[tid] = hist[tid + 1024] = 0;
+    __syncthreads();
+    const uint32_t bits = pass ? digit_bits(pass - 1) : 0;
+#pragma unroll
+    for (int x = 0; x < 4; x++)
+        if (g * KV_LONG + x * 1024 + tid < s.old && (key[x] & bits) == cut.key)
+            atomicAdd(&hist[digit_of(key[x], pass)], 1u);
+    __syncthreads();
+    uint32_t* to = e.hist + (((size_t)i * c.H + h) * 3 + pass) * KV_BINS;
+    for (int x = tid; x < KV_BINS; x += 1024)
+        if (hist[x]) atomicAdd(&to[x], hist[x]);  // counts: the order does not matter
+}
+
+// place 0: how many of each group are above the cut and how many on it; 1: their places.
+__global__ __launch_bounds__(1024) void kv_long_place_kernel(KvDev c, KvBatch b, KvEvict e, int groups, int place) {
+    __shared__ uint32_t scan[18];
+    __shared__ uint32_t sums[2];
+    const int tid = threadIdx.x, h = blockIdx.x % c.H, g = blockIdx.x / c.H % groups, i = blockIdx.x / c.H / groups;
+    const KvSelect s = select_job(c, b, e, i, h);
+    if (place && g == 0)
+        for (int j = tid; j < s.recent; j += 1024) {
+            s.kept[s.want + j] = s.old + j;
+            if (s.gone) s.gone[s.old + j] = -1;
+        }
+    if (g * KV_LONG >= s.old) return;
+    uint32_t key[4];
+#pragma unroll
+    for (int x = 0; x < 4; x++) {
+        const int j = g * KV_LONG + x * 1024 + tid;
+        key[x] = s.compete && j < s.old ? weight_key(c.weights[slot_at(c, s.row, h, j)]) : 0;
+    }
+    const KvCut cut = long_cut(c, e, s, i, 3, scan);
+    uint2* counts = e.counts + ((size_t)i * c.H + h) * groups;
+    if (tid < 2) sums[tid] = 0;
+    __syncthreads();
+    if (!place) {
+        uint32_t above = 0, on = 0;
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+            const bool in = g * KV_LONG + x * 1024 + tid < s.old;
+            above += (uint32_t)__popcll(__ballot(in && (s.want >= s.old || (s.compete && key[x] > cut.key))));
+            on += (uint32_t)__popcll(__ballot(in && s.compete && key[x] == cut.key));
+        }
+        if ((tid & 63) == 0) atomicAdd(&sums[0], above), atomicAdd(&sums[1], on);
+        __syncthreads();
+        if (tid == 0) counts[g] = make_uint2(sums[0], sums[1]);
+        return;
+    }
+    uint32_t above = 0, on = 0;
+    for (int x = tid; x < g; x += 1024) above += counts[x].x, on += counts[x].y;
+    if (above) atomicAdd(&sums[0], above);
+    if (on) atomicAdd(&sums[1], on);
+    __syncthreads();
+    uint32_t equal = sums[1], done = sums[0] + min(equal, cut.need);
+#pragma unroll
+    for (int x = 0; x < 4; x++) {
+        const int j = g * KV_LONG + x * 1024 + tid;
+        place_slots(s, cut, key[x], j, j < s.old, scan, done, equal);
+    }
+}
+
+__global__ __launch_bounds__(256) void kv_zero_kernel(uint4* p, int n) {
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256) p[i] = make_uint4(0, 0, 0, 0);
+}
+
+// One workgroup: the keys or the values of one block of one head of the result, gathered
+// from L2, 8 bytes of a key or one byte of a value at a time.  (Source tiles brought to LDS
+// whole: 72 us for 61, and 113 for 71 where one slot in six stays.)
 __global__ __launch_bounds__(256) void kv_move_kernel(KvDev c, KvBatch b, KvEvict e) {
-    __shared__ int from_block[256], from_slot[256];
-    __shared__ float kr[256], vr[256];
-    __shared__ float red[2][4];
+    __shared__ const uint8_t* from[256];  // a slot's tile half
+    __shared__ int slots[256];            // and its place there
+    __shared__ float ratios[256];
+    __shared__ uint32_t red[4];
     const int tid = threadIdx.x, lane = tid & 63;
-    const int h = blockIdx.x % c.H, unit = blockIdx.x / c.H;
+    const bool vals = blockIdx.x & 1;
+    const int h = (blockIdx.x >> 1) % c.H, unit = (blockIdx.x >> 1) / c.H;
     const int i = kv_find(b, unit);
     const int blk = unit - b.unit0[i], slot0 = blk << c.shift;
     const int n = min(b.count[i] - slot0, c.B);
@@ -396,69 +622,57 @@ __global__ __launch_bounds__(256) void kv_move_kernel(KvDev c, KvBatch b, KvEvic
     const int* kept = e.kept + ((size_t)i * c.H + h) * e.budget + slot0;
     const int block = e.dst[(size_t)b.aux[i] * c.W + blk];
     const size_t part = (size_t)block * c.H + h;
-    float ks = 0.f, vs = 0.f;
+    const int S = c.Dp / 32, half = kv_half(c.Dp);
+    float s_old = 0.f;
     if (tid < n) {
-        const int slot = kept[tid];
-        const int fb = row[slot >> c.shift];
+        const int slot = kept[tid], in = slot & (c.B - 1), fb = row[slot >> c.shift];
         const size_t fp = (size_t)fb * c.H + h;
-        from_block[tid] = fb;
-        from_slot[tid] = slot & (c.B - 1);
-        ks = c.kscale[fp], vs = c.vscale[fp];
-        c.positions[part * c.B + tid] = c.positions[fp * c.B + (slot & (c.B - 1))];
-        c.weights[part * c.B + tid] = c.weights[fp * c.B + (slot & (c.B - 1))];
+        from[tid] = c.pool + kv_tile_offset(c, fb, h, in / KV_TILE) + (vals ? half : 0);
+        slots[tid] = in & 31;
+        s_old = vals ? c.vscale[fp] : c.kscale[fp];
+        if (vals)
+            c.weights[part * c.B + tid] = c.weights[fp * c.B + in];
+        else
+            c.positions[part * c.B + tid] = c.positions[fp * c.B + in];
     }
     // the largest scale, as bits (scales are not negative; NaN is above all)
-    uint32_t kb = __float_as_uint(ks), vb = __float_as_uint(vs);
+    uint32_t big = __float_as_uint(s_old);
 #pragma unroll
-    for (int o = 32; o; o >>= 1) {
-        kb = max(kb, (uint32_t)__shfl_xor((int)kb, o));
-        vb = max(vb, (uint32_t)__shfl_xor((int)vb, o));
-    }
-    if (lane == 0) red[0][tid >> 6] = __uint_as_float(kb), red[1][tid >> 6] = __uint_as_float(vb);
+    for (int o = 32; o; o >>= 1) big = max(big, (uint32_t)__shfl_xor((int)big, o));
+    if (lane == 0) red[tid >> 6] = big;
     __syncthreads();
-    for (int w = 0; w < 4; w++) {
-        kb = max(kb, __float_as_uint(red[0][w]));
-        vb = max(vb, __float_as_uint(red[1][w]));
-    }
-    const float kt = __uint_as_float(kb), vt = __uint_as_float(vb);
-    if (tid < n) {
-        kr[tid] = kt > 0.f ? ks / kt : 0.f;
-        vr[tid] = vt > 0.f ? vs / vt : 0.f;
-    }
-    if (tid == 0) c.kscale[part] = kt, c.vscale[part] = vt;
+    big = max(max(red[0], red[1]), max(red[2], red[3]));
+    const float s = __uint_as_float(big);
+    if (tid < n) ratios[tid] = s != s ? 1.f : s > 0.f ? s_old / s : 0.f;  // NaN: the codes stay
+    if (tid == 0) (vals ? c.vscale : c.kscale)[part] = s;
     __syncthreads();
-    const int S = c.Dp / 32, half = kv_half(c.Dp);
     const uint32_t zero = zero_codes(c.code);
-    for (int t = 0; t * KV_TILE < n; t++) {
-        uint8_t* tile = c.pool + kv_tile_offset(c, block, h, t);
-        for (int u = tid; u < half / 8; u += 256) {  // keys: 8 dims of one slot
-            const int p = u >> 7, l = (u & 127) >> 1, o = 2 * p + (u & 1);
-            const int r = (o / S) * 16 + (l & 15), m = (o % S) * 4 + (l >> 4);
-            const int q = t * KV_TILE + r;
-            uint2 w = make_uint2(zero, zero);
+    uint8_t* base = c.pool + kv_tile_offset(c, block, h, 0) + (vals ? half : 0);
+    for (int u = tid; u < (n + KV_TILE - 1) / KV_TILE * half / 8; u += 256) {
+        const int t = u * 8 / half, x = u % (half / 8), p = x >> 7, l = (x & 127) >> 1, o = 2 * p + (x & 1);
+        uint32_t w[2] = {zero, zero};
+        if (!vals) {  // 8 dims of one slot
+            const int q = t * KV_TILE + (o / S) * 16 + (l & 15), m = (o % S) * 4 + (l >> 4);
             if (q < n) {
-                const uint8_t* src = c.pool + kv_tile_offset(c, from_block[q], h, from_slot[q] / KV_TILE);
-                w = *(const uint2*)(src + kv_key_byte(from_slot[q] & 31, m, S));
-                if (kr[q] != 1.f && kt == kt) w.x = rescale4(w.x, kr[q], c.code), w.y = rescale4(w.y, kr[q], c.code);
+                const uint2 v = *(const uint2*)(from[q] + kv_key_byte(slots[q], m, S));
+                w[0] = v.x, w[1] = v.y;
+                if (ratios[q] != 1.f) w[0] = rescale4(w[0], ratios[q], c.code), w[1] = rescale4(w[1], ratios[q], c.code);
             }
-            ((uint2*)tile)[u] = w;
-        }
-        for (int u = tid; u < half / 8; u += 256) {  // values: 8 slots of one dim
-            const int p = u >> 7, l = (u & 127) >> 1, d = (2 * p + (u & 1)) * 16 + (l & 15);
-            uint32_t w[2] = {0, 0};
+        } else {  // 8 slots of one dim
+            const int d = o * 16 + (l & 15);
+            w[0] = w[1] = 0;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const int q = t * KV_TILE + (j >> 2) * 16 + (l >> 4) * 4 + (j & 3);
                 uint32_t byte = zero & 255u;
                 if (q < n) {
-                    const uint8_t* src = c.pool + kv_tile_offset(c, from_block[q], h, from_slot[q] / KV_TILE) + half;
-                    byte = src[kv_value_byte(from_slot[q] & 31, d)];
-                    if (vr[q] != 1.f && vt == vt) byte = rescale4(byte, vr[q], c.code) & 255u;
+                    byte = from[q][kv_value_byte(slots[q], d)];
+                    if (ratios[q] != 1.f) byte = rescale4(byte, ratios[q], c.code) & 255u;
                 }
                 w[j >> 2] |= byte << (8 * (j & 3));
             }
-            ((uint2*)(tile + half))[u] = make_uint2(w[0], w[1]);
         }
+        *(uint2*)(base + (size_t)t * 2 * half + x * 8) = make_uint2(w[0], w[1]);
     }
 }
 
@@ -513,13 +727,14 @@ void launch_kv_table(int* table, const KvRuns& r, hipStream_t s) {
 void launch_kv_append(const KvDev& c, const KvBatch& b, const KvTensor& k, const KvTensor& v,
                       const int* positions, const float* weights, hipStream_t s) {
     const dim3 grid((unsigned)b.unit0[b.n] * c.H * 2);
+    const size_t lds = (size_t)c.B * c.Dp;  // at most 64 KiB
     if (!grid.x) return;
     if (k.type == KV_F32)
-        hipLaunchKernelGGL(kv_append_kernel<KV_F32>, grid, dim3(256), 0, s, c, b, k, v, positions, weights);
+        hipLaunchKernelGGL(kv_append_kernel<KV_F32>, grid, dim3(256), lds, s, c, b, k, v, positions, weights);
     else if (k.type == KV_F16)
-        hipLaunchKernelGGL(kv_append_kernel<KV_F16>, grid, dim3(256), 0, s, c, b, k, v, positions, weights);
+        hipLaunchKernelGGL(kv_append_kernel<KV_F16>, grid, dim3(256), lds, s, c, b, k, v, positions, weights);
     else
-        hipLaunchKernelGGL(kv_append_kernel<KV_BF16>, grid, dim3(256), 0, s, c, b, k, v, positions, weights);
+        hipLaunchKernelGGL(kv_append_kernel<KV_BF16>, grid, dim3(256), lds, s, c, b, k, v, positions, weights);
 }
 
 void launch_kv_read(const KvDev& c, const KvBatch& b, const KvReadOut& o, hipStream_t s) {
@@ -534,13 +749,24 @@ void launch_kv_read(const KvDev& c, const KvBatch& b, const KvReadOut& o, hipStr
 }
 
 void launch_kv_evict(const KvDev& c, const KvBatch& b, const KvEvict& e, hipStream_t s) {
-    hipLaunchKernelGGL(kv_select_kernel, dim3(b.n * c.H), dim3(1024), 0, s, c, b, e);
+    int longest = 0, least = INT_MAX;  // slots, and rows that leave
+    for (int i = 0; i < b.n; i++) {
+        longest = b.len[i] > longest ? b.len[i] : longest;
+        least = b.len[i] - b.count[i] < least ? b.len[i] - b.count[i] : least;
+    }
+    if (longest <= KV_SELECT * 1024) {
+        hipLaunchKernelGGL(kv_select_kernel, dim3(b.n * c.H), dim3(1024), 0, s, c, b, e);
+    } else {
+        const int groups = (longest + KV_LONG - 1) / KV_LONG;
+        const dim3 grid((unsigned)b.n * c.H * groups);
+        const int words = b.n * c.H * 3 * KV_BINS / 4;
+        hipLaunchKernelGGL(kv_zero_kernel, dim3(words / 256 < 1024 ? (words + 255) / 256 : 1024), dim3(256), 0, s, (uint4*)e.hist, words);
+        for (int pass = 0; pass < 3; pass++)
+            hipLaunchKernelGGL(kv_long_hist_kernel, grid, dim3(1024), 0, s, c, b, e, groups, pass);
+        for (int place = 0; place < 2; place++)
+            hipLaunchKernelGGL(kv_long_place_kernel, grid, dim3(1024), 0, s, c, b, e, groups, place);
+    }
     if (e.drop > 0) {
-        int longest = 0, least = INT_MAX;  // slots, and rows that leave
-        for (int i = 0; i < b.n; i++) {
-            longest = b.len[i] > longest ? b.len[i] : longest;
-            least = b.len[i] - b.count[i] < least ? b.len[i] - b.count[i] : least;
-        }
         const int groups = (longest + KV_READ - 1) / KV_READ;
         if (groups)
             hipLaunchKernelGGL(kv_dropped_kernel, dim3((unsigned)b.n * c.H * groups), dim3(256), 0, s, c, b, e, groups);
@@ -549,7 +775,16 @@ void launch_kv_evict(const KvDev& c, const KvBatch& b, const KvEvict& e, hipStre
                                0, s, c, b, e);
     }
     if (b.unit0[b.n])
-        hipLaunchKernelGGL(kv_move_kernel, dim3((unsigned)b.unit0[b.n] * c.H), dim3(256), 0, s, c, b, e);
+        hipLaunchKernelGGL(kv_move_kernel, dim3((unsigned)b.unit0[b.n] * c.H * 2), dim3(256), 0, s, c, b, e);
+}
+
+KvSelectSpace kv_select_space(const KvDev& c, int n, int longest) {
+    KvSelectSpace r;
+    if (longest > KV_SELECT * 1024) {
+        r.hist = (size_t)n * c.H * 3 * KV_BINS;
+        r.counts = (size_t)n * c.H * ((longest + KV_LONG - 1) / KV_LONG);
+    }
+    return r;
 }
 
 }  // namespace vgpu

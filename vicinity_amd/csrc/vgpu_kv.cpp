@@ -84,7 +84,7 @@ KvCache::~KvCache() {
 size_t KvCache::device_bytes() const {
     return pool.bytes() + kscale.bytes() + vscale.bytes() + weights.bytes() + positions.bytes() + table.bytes() +
            table2.bytes() + w_kept.bytes() + w_gone.bytes() + w_part.bytes() + w_scores.bytes() + w_lse2.bytes() +
-           w_ml.bytes() + w_qop.bytes() + w_qs.bytes() + w_wpart.bytes();
+           w_ml.bytes() + w_hist.bytes() + w_counts.bytes() + w_qop.bytes() + w_qs.bytes() + w_wpart.bytes();
 }
 
 void KvCache::check_call(const int32_t* ids, size_t n, hipStream_t s) {
@@ -183,7 +183,14 @@ void KvCache::append(const int32_t* ids, const int64_t* counts, size_t n, const 
     KvRuns runs;
     for (size_t i = 0; i < n; i++) {
         Seq& q = seqs[ids[i]];
-        take_blocks(q.blocks, blocks_of(q.len + counts[i]) - q.blocks.size(), ids[i], table.p, runs, s);
+        const size_t more = blocks_of(q.len + counts[i]) - q.blocks.size();
+        // one block touched: the append itself writes the table
+        if (more == 1 && q.len % dev.B == 0 && counts[i] <= dev.B) {
+            q.blocks.push_back(free_blocks.back());
+            free_blocks.pop_back();
+        } else {
+            take_blocks(q.blocks, more, ids[i], table.p, runs, s);
+        }
     }
     launch_kv_table(table.p, runs, s);
     int64_t tok = 0;
@@ -201,7 +208,9 @@ void KvCache::append(const int32_t* ids, const int64_t* counts, size_t n, const 
             b.aux[j] = (int)q.next;
             // blocks that the new tokens enter
             const int64_t first = q.len >> dev.shift;
-            b.unit0[j + 1] = b.unit0[j] + (counts[i] ? (int)((int64_t)blocks_of(q.len + counts[i]) - first) : 0);
+            const int64_t touched = counts[i] ? (int64_t)blocks_of(q.len + counts[i]) - first : 0;
+            b.splits[j] = touched == 1 ? q.blocks[first] : -1;
+            b.unit0[j + 1] = b.unit0[j] + (int)touched;
             b.n++;
             tok += counts[i];
             q.len += counts[i];
@@ -301,6 +310,9 @@ void KvCache::evict(const int32_t* ids, const int32_t* into, size_t n, size_t bu
     int64_t longest = 0;
     for (size_t i = 0; i < n; i++) longest = std::max(longest, seqs[ids[i]].len);
     if (drop) grow(w_gone, group * dev.H * (size_t)longest);
+    const KvSelectSpace space = kv_select_space(dev, (int)group, (int)longest);
+    grow(w_hist, space.hist);
+    grow(w_counts, space.counts);
     std::vector<std::vector<int>> fresh(n);
     for (size_t i = 0; i < n; i++) fresh[i].reserve(blocks_of(stays(i)));
     if (into)
@@ -314,6 +326,7 @@ void KvCache::evict(const int32_t* ids, const int32_t* into, size_t n, size_t bu
     e.dst = into ? table.p : table2.p;
     e.dpos = dpos, e.dk = dk, e.dv = dv;
     e.slots = (int)longest;
+    e.hist = w_hist.p, e.counts = w_counts.p;
     e.vec = dev.D % 8 == 0 && ((uintptr_t)dk | (uintptr_t)dv) % 16 == 0;
     for (size_t i0 = 0; i0 < n;) {
         KvBatch b;

@@ -53,7 +53,8 @@ struct KvBatch {
     int count[KV_BATCH];  // its tokens
     int aux[KV_BATCH];    // append: position of the first token; read: first slot;
                           // evict: sequence that receives the result; attend: see there
-    int splits[KV_BATCH]; // attend: parts that the tiles of its rows go to, of per[i] tiles
+    int splits[KV_BATCH]; // attend: parts that the tiles of its rows go to, of per[i] tiles;
+                          // append: the one block it touches, or -1 (see the table)
     int per[KV_BATCH];
     int unit0[KV_BATCH + 1];
 };
@@ -123,10 +124,17 @@ struct KvEvict {
     int* gone = nullptr;     // [n, H, slots] a slot's row among those that leave, or -1; null without them
     int slots = 0;           // of the longest sequence
     bool vec = false;        // 8 dims of a dropped row are one aligned piece
+    uint32_t* hist = nullptr;  // selection from long sequences (kv_select_space)
+    uint2* counts = nullptr;
     const int* dst = nullptr;  // [seq * W + i] table with the new blocks of aux[i]
     int* dpos = nullptr;     // the caller's arrays, [n, drop, H] and [n, drop, H, D]
     float *dk = nullptr, *dv = nullptr;
 };
+// Elements of KvEvict's hist and counts for n sequences, the longest of them so long.
+struct KvSelectSpace {
+    size_t hist = 0, counts = 0;
+};
+KvSelectSpace kv_select_space(const KvDev& c, int n, int longest);
 void launch_kv_evict(const KvDev& c, const KvBatch& b, const KvEvict& e, hipStream_t s);
 
 struct KvAttend {

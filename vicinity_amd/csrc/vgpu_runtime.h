@@ -349,6 +349,8 @@ struct KvCache {
     DevBuf<int> w_kept, w_gone;      // eviction: slots that stay, slots that leave
     DevBuf<float> w_part, w_scores, w_lse2, w_qs, w_wpart;
     DevBuf<uint4> w_qop;
+    DevBuf<uint32_t> w_hist;
+    DevBuf<uint2> w_counts;
     DevBuf<float2> w_ml;
 
     struct Seq {
