@@ -17,37 +17,43 @@ namespace {
 // Scales are 0 below this largest magnitude, so 1 / s stays finite.
 constexpr float KV_TINY = 0x1p-100f;
 
-__device__ __forceinline__ float to_f32(const void* p, int64_t i, int type) {
-    if (type == KV_F32) return ((const float*)p)[i];
-    if (type == KV_F16) return (float)((const _Float16*)p)[i];
-    return __uint_as_float((uint32_t)((const uint16_t*)p)[i] << 16);
-}
+// Eight elements as they lie in memory.
+template <int T>
+struct Eight {
+    uint32_t w[T == KV_F32 ? 8 : 4];
+    __device__ __forceinline__ float at(int e) const {
+        if (T == KV_F32) return __uint_as_float(w[e]);
+        const uint32_t h = w[e >> 1] >> (16 * (e & 1)) & 0xffffu;
+        return T == KV_F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)h) : __uint_as_float(h << 16);
+    }
+};
 
 // dims 8 m .. 8 m + 7 of a row (0 from D on)
 template <int T>
-__device__ __forceinline__ void load8(const KvTensor& x, int64_t row, int m, int D, float* v) {
+__device__ __forceinline__ Eight<T> load8(const KvTensor& x, int64_t row, int m, int D) {
+    Eight<T> r;
+    constexpr int W = T == KV_F32 ? 8 : 4;
     if (x.vec) {
-        if (T == KV_F32) {
-            const float4* p = (const float4*)((const float*)x.p + row + 8 * m);
-            const float4 a = p[0], b = p[1];
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-            v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        } else {
-            const uint4 a = *(const uint4*)((const uint16_t*)x.p + row + 8 * m);
-            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+        const uint4* p = (const uint4*)((const uint8_t*)x.p + (row + 8 * m) * (T == KV_F32 ? 4 : 2));
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const uint16_t h = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
-                v[e] = T == KV_F16 ? (float)__builtin_bit_cast(_Float16, h) : __uint_as_float((uint32_t)h << 16);
-            }
+        for (int j = 0; j < W / 4; j++) {
+            const uint4 a = p[j];
+            r.w[4 * j] = a.x, r.w[4 * j + 1] = a.y, r.w[4 * j + 2] = a.z, r.w[4 * j + 3] = a.w;
         }
     } else {
 #pragma unroll
+        for (int j = 0; j < W; j++) r.w[j] = 0;
+#pragma unroll
         for (int e = 0; e < 8; e++) {
             const int d = 8 * m + e;
-            v[e] = d < D ? to_f32(x.p, row + d * x.sd, T) : 0.f;
+            if (d >= D) continue;
+            if (T == KV_F32)
+                r.w[e] = ((const uint32_t*)x.p)[row + d * x.sd];
+            else
+                r.w[e >> 1] |= (uint32_t)((const uint16_t*)x.p)[row + d * x.sd] << (16 * (e & 1));
         }
     }
+    return r;
 }
 
 __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, int code) {
@@ -148,14 +154,9 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvDev c, KvBatch b, KvTe
         r = start + (vals ? q * 4 + (u & 3) : q);
         return r >= held && r < end;
     };
-    const auto load = [&](int u, float(&y)[8]) {
+    const auto load = [&](int u) {
         int r, m;
-        if (piece(u, r, m)) {
-            load8<T>(x, (tok0 + r) * x.st + (int64_t)h * x.sh, m, c.D, y);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++) y[j] = 0.f;
-        }
+        return piece(u, r, m) ? load8<T>(x, (tok0 + r) * x.st + (int64_t)h * x.sh, m, c.D) : Eight<T>{};
     };
     float* scale = (vals ? c.vscale : c.kscale) + part;
     const float s_old = held ? *scale : 0.f;
@@ -164,23 +165,23 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvDev c, KvBatch b, KvTe
 
     // largest magnitude, as bits: infinities and NaN are above every number
     uint32_t big = 0;
-    float e[KV_HOLD][8];
+    Eight<T> e[KV_HOLD];
     const bool hold = units <= KV_HOLD * 256;
-    const auto magnitude = [&](const float(&y)[8]) {
+    const auto magnitude = [&](const Eight<T>& y) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) big = max(big, __float_as_uint(y[j]) & 0x7fffffffu);
+        for (int j = 0; j < 8; j++) big = max(big, __float_as_uint(y.at(j)) & 0x7fffffffu);
     };
     if (hold) {
 #pragma unroll
         for (int z = 0; z < KV_HOLD; z++) {
-            if (z * 256 + tid < units) load(z * 256 + tid, e[z]);
+            if (z * 256 + tid < units) e[z] = load(z * 256 + tid);
         }
 #pragma unroll
         for (int z = 0; z < KV_HOLD; z++)
             if (z * 256 + tid < units) magnitude(e[z]);
     } else {
         for (int u = tid; u < units; u += 256) {
-            load(u, e[0]);
+            e[0] = load(u);
             magnitude(e[0]);
         }
     }
@@ -209,26 +210,26 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvDev c, KvBatch b, KvTe
     const bool direct = held % KV_TILE && !grown && end - held <= KV_FEW && held / KV_TILE == (end - 1) / KV_TILE;
     const int first = grown ? 0 : held / KV_TILE, last = (end + KV_TILE - 1) / KV_TILE;  // tiles that change
     if (!direct) {
-        for (int u = tid; u < (last - first) * half / 16; u += 256) {
-            const int t = first + u * 16 / half, o = u % (half / 16);
-            uint4 w = {zero_codes(c.code), zero_codes(c.code), zero_codes(c.code), zero_codes(c.code)};
-            if (t * KV_TILE < held) {
-                w = ((const uint4*)(base + (size_t)t * 2 * half))[o];
-                if (grown) {
-                    w.x = rescale4(w.x, ratio, c.code), w.y = rescale4(w.y, ratio, c.code);
-                    w.z = rescale4(w.z, ratio, c.code), w.w = rescale4(w.w, ratio, c.code);
+        for (int t = first; t < last; t++)
+            for (int o = tid; o < half / 16; o += 256) {
+                uint4 w = {zero_codes(c.code), zero_codes(c.code), zero_codes(c.code), zero_codes(c.code)};
+                if (t * KV_TILE < held) {
+                    w = ((const uint4*)(base + (size_t)t * 2 * half))[o];
+                    if (grown) {
+                        w.x = rescale4(w.x, ratio, c.code), w.y = rescale4(w.y, ratio, c.code);
+                        w.z = rescale4(w.z, ratio, c.code), w.w = rescale4(w.w, ratio, c.code);
+                    }
                 }
+                ((uint4*)(image + (t - first) * half))[o] = w;
             }
-            ((uint4*)image)[u] = w;
-        }
         __syncthreads();
     }
-    const auto encode = [&](int u, const float(&y)[8]) {
+    const auto encode = [&](int u, const Eight<T>& y) {
         int r, m;
         (void)piece(u, r, m);
         const int t = r / KV_TILE;
-        uint32_t w[2] = {encode4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv, c.code),
-                         encode4(y[4] * inv, y[5] * inv, y[6] * inv, y[7] * inv, c.code)};
+        uint32_t w[2] = {encode4(y.at(0) * inv, y.at(1) * inv, y.at(2) * inv, y.at(3) * inv, c.code),
+                         encode4(y.at(4) * inv, y.at(5) * inv, y.at(6) * inv, y.at(7) * inv, c.code)};
         uint8_t* to = direct ? base + (size_t)t * 2 * half : image + (t - first) * half;
         if (!vals) {
             *(uint2*)(to + kv_key_byte(r & 31, m, S)) = make_uint2(w[0], w[1]);
@@ -255,14 +256,15 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvDev c, KvBatch b, KvTe
             if (z * 256 + tid < units) encode(z * 256 + tid, e[z]);
     } else {
         for (int u = tid; u < units; u += 256) {
-            load(u, e[0]);
+            e[0] = load(u);
             encode(u, e[0]);
         }
     }
     if (direct) return;
     __syncthreads();
-    for (int u = tid; u < (last - first) * half / 16; u += 256)
-        ((uint4*)(base + (size_t)(first + u * 16 / half) * 2 * half))[u % (half / 16)] = ((const uint4*)image)[u];
+    for (int t = first; t < last; t++)
+        for (int o = tid; o < half / 16; o += 256)
+            ((uint4*)(base + (size_t)t * 2 * half))[o] = ((const uint4*)(image + (t - first) * half))[o];
 }
 
 __device__ __forceinline__ void store1(void* p, size_t i, float v, int type) {
@@ -648,11 +650,13 @@ __global__ __launch_bounds__(256) void kv_move_kernel(KvDev c, KvBatch b, KvEvic
     __syncthreads();
     const uint32_t zero = zero_codes(c.code);
     uint8_t* base = c.pool + kv_tile_offset(c, block, h, 0) + (vals ? half : 0);
-    for (int u = tid; u < (n + KV_TILE - 1) / KV_TILE * half / 8; u += 256) {
-        const int t = u * 8 / half, x = u % (half / 8), p = x >> 7, l = (x & 127) >> 1, o = 2 * p + (x & 1);
+    const int tiles = (n + KV_TILE - 1) / KV_TILE;
+    for (int x = tid; x < half / 8; x += 256)
+    for (int t = 0; t < tiles; t++) {
+        const int p = x >> 7, l = (x & 127) >> 1, o = 2 * p + (x & 1);
         uint32_t w[2] = {zero, zero};
         if (!vals) {  // 8 dims of one slot
-            const int q = t * KV_TILE + (o / S) * 16 + (l & 15), m = (o % S) * 4 + (l >> 4);
+            const int upper = o >= S, q = t * KV_TILE + upper * 16 + (l & 15), m = (o - upper * S) * 4 + (l >> 4);
             if (q < n) {
                 const uint2 v = *(const uint2*)(from[q] + kv_key_byte(slots[q], m, S));
                 w[0] = v.x, w[1] = v.y;
