@@ -15,6 +15,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import math
+from array import array
 
 import numpy as np
 
@@ -25,8 +26,21 @@ FIELDS = ("k", "v", "positions", "weights")
 _SAME = contextlib.nullcontext()  # the current stream
 
 
-def _ptr(a: np.ndarray) -> int:
-    return a.__array_interface__["data"][0]
+def _ptr(a: array) -> int:
+    return a.buffer_info()[0]
+
+
+def _array(kind: str, values, name: str) -> array:
+    """Host integers for the library: a list, a range, an array ('i': 32 bits, 'q': 64)."""
+    if not isinstance(values, (list, tuple, range)):
+        values = np.asarray(values)
+        if values.ndim != 1 or (values.size and values.dtype.kind not in "iu"):
+            raise ValueError(f"{name} must be a 1-D array of integers")
+        values = values.tolist()
+    try:
+        return array(kind, values)
+    except (TypeError, OverflowError) as e:
+        raise ValueError(f"{name} must be a 1-D array of integers that fit the library") from e
 
 
 class KVCache:
@@ -57,7 +71,7 @@ class KVCache:
 
         self.device = torch.device("cuda", torch.cuda.current_device())
         self._types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-        self._all = np.arange(num_seqs, dtype=np.int32)
+        self._all = array("i", range(num_seqs))
         self._last = None      # the stream of the last call, and its handle
         self._last_raw = None
 
@@ -71,9 +85,7 @@ class KVCache:
     @property
     def lengths(self) -> np.ndarray:
         """Slots in use of every sequence, int64 [num_seqs]."""
-        out = np.empty(self.num_seqs, np.int64)
-        _lib.check(self._L.vgpu_kv_lengths(self._h, _ptr(out)))
-        return out
+        return np.array(self._lengths())
 
     def info(self) -> dict:
         """free_blocks, and device_bytes: the HBM that the cache holds."""
@@ -181,8 +193,8 @@ class KVCache:
         s, ctx = self._stream(stream, ())
         gone, most = None, 0
         if dropped:
-            known = ids[(ids >= 0) & (ids < self.num_seqs)]  # the others are refused below
-            most = max(int(self.lengths[known].max(initial=0)) - int(budget), 0)
+            lens = self._lengths()
+            most = max(max((lens[i] for i in ids), default=0) - int(budget), 0)
             shape = (len(ids), most, self.num_heads)
             with ctx:
                 gone = {"positions": torch.empty(shape, dtype=torch.int32, device=self.device),
@@ -206,17 +218,17 @@ class KVCache:
         dtype = torch.float32 if dtype is None else dtype
         if dtype not in self._types:
             raise TypeError("dtype must be float32, float16 or bfloat16")
-        if not set(fields) <= set(FIELDS):
-            raise ValueError(f"fields must be among {FIELDS}")
+        for f in fields:
+            if f not in FIELDS:
+                raise ValueError(f"fields must be among {FIELDS}")
         ids = self._seqs(seqs)
         at = self._ints(0 if first is None else first, len(ids), "first")
         if counts is None:
-            if ((ids < 0) | (ids >= self.num_seqs)).any():
-                raise ValueError(f"sequence out of range [0, {self.num_seqs})")
-            n = np.maximum(self.lengths[ids] - at, 0)
+            lens = self._lengths()
+            n = array("q", [max(lens[i] - f, 0) for i, f in zip(ids, at)])
         else:
             n = self._ints(counts, len(ids), "counts")
-        tokens = max(int(n.sum()), 0)
+        tokens = max(sum(n), 0)
         s, ctx = self._stream(stream, ())
         types = {"positions": torch.int32, "weights": torch.float32}
         res = {}
@@ -230,37 +242,36 @@ class KVCache:
         return res
 
     # ---- arguments ------------------------------------------------------------
-    def _seqs(self, seqs) -> np.ndarray:
+    def _lengths(self) -> array:
+        out = array("q", bytes(8 * self.num_seqs))
+        _lib.check(self._L.vgpu_kv_lengths(self._h, _ptr(out)))
+        return out
+
+    def _seqs(self, seqs) -> array:
         if seqs is None:
             return self._all
-        a = np.asarray(list(seqs) if isinstance(seqs, range) else seqs)
-        if a.size == 0:
-            return np.zeros(0, np.int32)
-        if a.ndim != 1 or a.dtype.kind not in "iu":
-            raise ValueError("sequences must be a 1-D array of integers")
-        if int(a.min()) < 0 or int(a.max()) >= self.num_seqs:
+        a = _array("i", seqs, "sequences")
+        if a and not 0 <= min(a) <= max(a) < self.num_seqs:
             raise ValueError(f"sequence out of range [0, {self.num_seqs})")
-        return np.ascontiguousarray(a, np.int32)
+        return a
 
     @staticmethod
-    def _ints(values, n: int, name: str) -> np.ndarray:
-        a = np.asarray(values)
-        if a.size and a.dtype.kind not in "iu":
-            raise ValueError(f"{name} must be integers")
-        if a.ndim == 0:
-            return np.full(n, int(a), np.int64)
-        if a.shape != (n,):
+    def _ints(values, n: int, name: str) -> array:
+        if isinstance(values, (int, np.integer)):
+            return _array("q", [int(values)] * n, name)
+        a = _array("q", values, name)
+        if len(a) != n:
             raise ValueError(f"{name} must have one entry for each of the {n} sequences")
-        return np.ascontiguousarray(a, np.int64)
+        return a
 
-    def _counts(self, counts, n: int, tokens: int) -> np.ndarray:
+    def _counts(self, counts, n: int, tokens: int) -> array:
         if counts is None:
             if n == 0 or tokens % n:
                 raise ValueError(f"{tokens} tokens cannot be shared out to {n} sequences: "
                                  "counts is needed")
-            return np.full(n, tokens // n, np.int64)
+            return array("q", [tokens // n]) * n
         a = self._ints(counts, n, "counts")
-        if (a < 0).any() or int(a.sum()) != tokens:
+        if (a and min(a) < 0) or sum(a) != tokens:
             raise ValueError(f"counts must add up to the {tokens} tokens given")
         return a
 
