@@ -321,12 +321,18 @@ __device__ __forceinline__ void read_tile(const KvDev& c, const uint8_t* tile, f
             for (int o = 0; o < 2; o++) {
                 const int j = (2 * p + o) / S, s = (2 * p + o) % S;
                 const size_t r = j ? rows[1] : rows[0];
-                float e[8];
-                decode4(o ? w.z : w.x, c.code, e);
-                decode4(o ? w.w : w.y, c.code, e + 4);
+                // dims 8 g .. + 3 and + 4 .. + 7 of lane group g become 4 g .. and 16 + 4 g ..,
+                // so that a store of the four groups is contiguous
+                const auto half = __builtin_amdgcn_permlane16_swap(o ? w.z : w.x, o ? w.w : w.y, false, false);
+                const auto two = __builtin_amdgcn_permlane32_swap(half[0], half[1], false, false);
 #pragma unroll
-                for (int i = 0; i < 8; i++) e[i] *= ks;
-                if (r != ~(size_t)0) store_row<T, 8>(ko, r, 32 * s + 8 * g, c.D, vec, e);
+                for (int y = 0; y < 2; y++) {
+                    float e[4];
+                    decode4(two[y], c.code, e);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) e[i] *= ks;
+                    if (r != ~(size_t)0) store_row<T, 4>(ko, r, 32 * s + 16 * y + 4 * g, c.D, vec, e);
+                }
             }
         }
     }
@@ -354,8 +360,7 @@ __device__ __forceinline__ void read_tile(const KvDev& c, const uint8_t* tile, f
 }
 
 // One workgroup: 128 slots of one head, a tile to a wave.  Bound by the bytes written:
-// no element passes through LDS; a key store is 32 contiguous bytes of a lane, a value
-// store 16 (64 of four lanes).
+// no element passes through LDS, and four lanes store 64 contiguous bytes.
 template <int T>
 __global__ __launch_bounds__(256) void kv_read_kernel(KvDev c, KvBatch b, KvReadOut o) {
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -663,17 +668,21 @@ __global__ __launch_bounds__(256) void kv_move_kernel(KvDev c, KvBatch b, KvEvic
                 if (ratios[q] != 1.f) w[0] = rescale4(w[0], ratios[q], c.code), w[1] = rescale4(w[1], ratios[q], c.code);
             }
         } else {  // 8 slots of one dim
-            const int d = o * 16 + (l & 15);
-            w[0] = w[1] = 0;
+            const int d = o * 16 + (l & 15), q0 = t * KV_TILE + (l >> 4) * 4;
+            uint32_t bytes[8];
+            float r[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const int q = t * KV_TILE + (j >> 2) * 16 + (l >> 4) * 4 + (j & 3);
-                uint32_t byte = zero & 255u;
-                if (q < n) {
-                    byte = from[q][kv_value_byte(slots[q], d)];
-                    if (ratios[q] != 1.f) byte = rescale4(byte, ratios[q], c.code) & 255u;
-                }
-                w[j >> 2] |= byte << (8 * (j & 3));
+                const int q = min(q0 + (j >> 2) * 16 + (j & 3), n - 1);  // past the end: any slot, unused
+                bytes[j] = from[q][kv_value_byte(slots[q], d)];
+                r[j] = ratios[q];
+            }
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+                float v[4];
+                decode4(bytes[4 * y] | bytes[4 * y + 1] << 8 | bytes[4 * y + 2] << 16 | bytes[4 * y + 3] << 24, c.code, v);
+                // (a ratio of 1 keeps the code)
+                w[y] = encode4(v[0] * r[4 * y], v[1] * r[4 * y + 1], v[2] * r[4 * y + 2], v[3] * r[4 * y + 3], c.code);
             }
         }
         *(uint2*)(base + (size_t)t * 2 * half + x * 8) = make_uint2(w[0], w[1]);
