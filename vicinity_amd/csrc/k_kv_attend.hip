@@ -277,13 +277,15 @@ __device__ __forceinline__ void kv_reference(KvWave<S, CODE, PARTS, NC>& w, cons
                 }
                 if (a.mask && any) {
                     any = false;
-                    const uint8_t* mask = a.mask + (int64_t)(tok0 + w.row[n] / a.G) * a.mask_st;
+                    const uint8_t* mask = a.mask + (int64_t)(tok0 + max(w.row[n], 0) / a.G) * a.mask_st;
+                    uint8_t see[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++)  // (slots past the row's last are hidden already)
+                        see[j] = mask[min(slot0 + 4 * g + (j >> 2) * 16 + (j & 3), w.hi[n] - 1) * a.mask_ss];
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
-                        const int off = (j >> 2) * 16 + (j & 3);
-                        const bool see = (unsigned)(off - first) < (unsigned)count && mask[(slot0 + 4 * g + off) * a.mask_ss];
-                        x[n][j] = see ? x[n][j] : KV_NEG;
-                        any |= see;
+                        x[n][j] = see[j] ? x[n][j] : KV_NEG;
+                        any |= see[j] && (unsigned)((j >> 2) * 16 + (j & 3) - first) < (unsigned)count;
                     }
                 }
             }
@@ -329,17 +331,8 @@ __device__ __forceinline__ void kv_exponents(KvWave<S, CODE, PARTS, NC>& w, cons
             const float p = __builtin_amdgcn_exp2f(x[n][j]);
             const _Float16 ph = (_Float16)p;
             p0[n][j] = ph;
-            if (PARTS > 1) p1[n][j] = (_Float16)(p - (float)ph), sum += p;
-        }
-        if (PARTS == 1) {
-            // the sum of what the products take, two at a time
-            const half2v one = {(_Float16)1.f, (_Float16)1.f};
-            const u32x4 two = __builtin_bit_cast(u32x4, p0[n]);
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const uint32_t pair = two[j];
-                sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2v, pair), one, sum, false);
-            }
+            if (PARTS > 1) p1[n][j] = (_Float16)(p - (float)ph);
+            sum += p;  // (the rounded ones' sum, by dot products, would cost the logarithm its float32)
         }
         w.l[n] = __builtin_fmaf(sum, rv, w.l[n]);
     }
@@ -756,7 +749,7 @@ __global__ __launch_bounds__(256) void kv_score_weights_kernel(KvDev c, KvBatch 
 // chunks' sums are added in their order by kv_chunk_weights_kernel.  Bound by the
 // exponentials: 16 cycles of a SIMD for 64 of them, against 16 of the matrix unit for
 // the 512 multiply-adds of 4 scores of 128 dims.
-constexpr int KV_WT = 2;              // 32-slot tiles of a wave
+constexpr int KV_WT = 1;              // 32-slot tiles of a wave
 static_assert(KV_WEIGHT_SLOTS == 4 * KV_WT * KV_TILE, "four waves of KV_WT tiles");
 
 template <int S, int CODE, int PARTS>
@@ -892,7 +885,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_weights_kernel(KvDev c, KvBatc
 }
 
 // A thread per slot: the chunks' sums, and the weight.
-__global__ __launch_bounds__(256) void kv_chunk_weights_kernel(KvDev c, KvBatch b, KvAttend a) {
+__global__ __launch_bounds__(KV_WEIGHT_SLOTS) void kv_chunk_weights_kernel(KvDev c, KvBatch b, KvAttend a) {
     const int h = blockIdx.x % c.H, unit = blockIdx.x / c.H;
     const int i = kv_find(b, unit);
     const int slot = (unit - b.unit0[i]) * KV_WEIGHT_SLOTS + threadIdx.x;
@@ -904,7 +897,6 @@ __global__ __launch_bounds__(256) void kv_chunk_weights_kernel(KvDev c, KvBatch 
     float* w = c.weights + ((size_t)block * c.H + h) * c.B + (slot & (c.B - 1));
     *w = a.decay == 0.f ? sum : a.decay * *w + sum;
 }
-static_assert(KV_WEIGHT_SLOTS == 256, "one thread per slot of a workgroup");
 
 template <int S, int CODE, int PARTS>
 void attend_s(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s) {
@@ -989,7 +981,7 @@ void launch_kv_weights(const KvDev& c, const KvBatch& b, const KvAttend& a, hipS
         return;
     }
     by_type<true>(c, b, a, s);
-    hipLaunchKernelGGL(kv_chunk_weights_kernel, grid, dim3(256), 0, s, c, b, a);
+    hipLaunchKernelGGL(kv_chunk_weights_kernel, grid, dim3(KV_WEIGHT_SLOTS), 0, s, c, b, a);
 }
 
 }  // namespace vgpu

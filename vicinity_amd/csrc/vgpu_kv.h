@@ -173,7 +173,7 @@ inline int kv_attend_rows(const KvAttend& a, int Dp) {
 // unit0 counts row tiles times splits of the sequences (of one head).
 void launch_kv_attend(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s);
 // Slots of a workgroup that makes weights of kept scores, and of one that goes over the keys.
-constexpr int KV_SCORE_SLOTS = 1024, KV_WEIGHT_SLOTS = 256;
+constexpr int KV_SCORE_SLOTS = 1024, KV_WEIGHT_SLOTS = 128;
 // unit0 counts these.  aux: with scores the tiles of the score rows of the sequences
 // before (of one head), without them the 16-row tiles of the sequences before.
 void launch_kv_weights(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s);
