@@ -115,19 +115,26 @@ def attend(q, k, v, see, scale):
     g = hq // h
     out, lse = np.zeros((t, hq, d)), np.full((t, hq), -np.inf)
     w = np.zeros((k.shape[0], h))
-    for i in range(t):
-        idx = np.nonzero(see[i])[0]
-        if not len(idx):
-            continue
-        for a in range(hq):
-            s = k[idx, a // g] @ q[i, a].astype(np.float64) * scale
-            m = s.max()
+    rows = see.any(axis=1)
+    if not rows.any():
+        return out, lse, w
+    q = q[rows].astype(np.float64)
+    hide = ~see[rows]
+    for a in range(h):
+        # slots that no row sees may hold NaN: they take no part
+        used = see[rows].any(axis=0)
+        ka, va = k[used, a], v[used, a]
+        for b in range(a * g, a * g + g):
+            s = q[:, b] @ ka.T * scale
+            s[hide[:, used]] = -np.inf
+            m = s.max(axis=1, keepdims=True)
             with np.errstate(invalid="ignore"):
                 e = np.exp(s - m)
-                total = e.sum()
-                out[i, a] = (e / total) @ v[idx, a // g]
-            lse[i, a] = m + np.log(total)
-            w[idx, a // g] += e / total
+                total = e.sum(axis=1, keepdims=True)
+                p = e / total
+            out[rows, b] = p @ va
+            lse[rows, b] = (m + np.log(total))[:, 0]
+            w[used, a] += p.sum(axis=0)
     return out, lse, w
 
 

@@ -339,6 +339,35 @@ def test_scores_far_apart_and_value_scales_far_apart():
         _check_attend(pair, q, [0], [3], decay=0.0)
 
 
+@pytest.mark.parametrize("code", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("group", [1, 40, 130])
+def test_logarithms_and_weights_keep_float32_whatever_the_query_type(code, dtype, group):
+    """One dimension and few slots: the bounds come down to some 2^-14, below what a half
+    precision probability in the denominator would cost."""
+    lens = [2, 3, 5, 9, 17]
+    _case(f"logarithms {code} {dtype} group {group}")
+    pair = Pair(5, 1, 1, 32, code)
+    pair.append(_rand((sum(lens), 1, 1), dtype, 86), _rand((sum(lens), 1, 1), dtype, 87), list(range(5)), lens)
+    q = _rand((5, group, 1), dtype, 88)
+    _check_attend(pair, q, list(range(5)), [1] * 5, decay=0.0, scale=0.5)
+    _check_attend(pair, q, list(range(5)), [1] * 5, scale=0.5)
+
+
+@pytest.mark.parametrize("n,group,counts", [(3000, 4, [120, 30]), (2100, 8, [70, 1]), (5000, 1, [300, 260])])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_many_rows_over_long_sequences(n, group, counts, dtype):
+    """Enough rows and tiles for the kernel of many rows, in one or several splits."""
+    _case(f"many rows: {n} slots group {group} counts {counts} {dtype}")
+    pair = Pair(2, 2, 64, 64, "fp8", blocks=200)
+    pair.append(_rand((n + 900, 2, 64), dtype, 74, 0.7), _rand((n + 900, 2, 64), dtype, 75), [0, 1], [n, 900])
+    q = _rand((sum(counts), 2 * group, 64), dtype, 76)
+    _check_attend(pair, q, [0, 1], counts)
+    _check_attend(pair, q, [0, 1], counts, window=1000, decay=1.0)
+    mask = (_torch().rand((sum(counts), n), generator=_torch().Generator().manual_seed(77)) < 0.5).to("cuda:0")
+    _check_attend(pair, q, [0, 1], counts, mask=mask)
+
+
 def test_rows_of_any_size():
     """Queries from 2^-60 to 2^60, and zero: the scale undoes it."""
     torch = _torch()

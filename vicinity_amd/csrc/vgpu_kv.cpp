@@ -25,8 +25,15 @@ constexpr int64_t kChunkWorkgroups = 512;
 constexpr int64_t kWeightWorkgroups = 3072;
 // Bytes of partial results of one launch.
 constexpr int64_t kPartBytes = (int64_t)256 << 20;
-// Steps of at most this many rows per head keep their scores for the weights.
-constexpr int64_t kScoreRows = 64;
+// Calls of at most this many rows per head keep their scores for the weights; with more a
+// second pass over the keys is cheaper (16 sequences of 4096, 8 x 128: 32 rows 70 and 93 us,
+// 48 rows 91 and 96, 64 rows 116 and 102).
+constexpr int64_t kScoreRows = 48;
+// The kernel of many rows takes over where its workgroups are filled to three quarters and
+// have this many 32-slot tiles to do in all (16 sequences of 4096, 8 x 128, 128 rows: 65 us
+// against 77 by row tiles of 16, 96 rows 67 and 58, 256 rows 106 and 139; 4 sequences of 1024,
+// 256 rows: 29 and 16 us).
+constexpr int64_t kChunkTiles = 4096;
 
 // A workspace that grows in large steps.
 template <typename T>
@@ -406,13 +413,16 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
     a.out = q.out;
     a.lse = q.lse;
     a.vec_out = dev.D % 4 == 0 && (uintptr_t)q.out % (4 * item_size(a.q.type)) == 0;
-    int64_t tokens = 0, longest = 0, most = 0;
+    const int parts = a.q.type == KV_F32 ? 2 : 1;
+    const int64_t chunk_rows = 64 * kv_chunk_nc(dev.Dp, parts);
+    int64_t tokens = 0, longest = 0, most = 0, chunk_tiles = 0;
     for (size_t i = 0; i < n; i++) {
         need(counts[i] >= 0, "counts must not be negative");
         tokens += counts[i];
         need(tokens * (int64_t)q.num_q_heads <= INT_MAX / 2, "more than 2^30 query rows in one call");
         longest = std::max(longest, seqs[ids[i]].len);
         most = std::max(most, counts[i] * a.G);
+        chunk_tiles += (counts[i] * a.G + chunk_rows - 1) / chunk_rows * dev.H * ((seqs[ids[i]].len + KV_TILE - 1) / KV_TILE);
     }
     need(!q.mask || (int64_t)q.mask_slots >= longest, "a mask row must cover the longest sequence (" +
                                                           std::to_string(longest) + " slots)");
@@ -420,9 +430,8 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
     need((uintptr_t)q.out % item_size(a.q.type) == 0 && (uintptr_t)q.lse % 4 == 0, "outputs must be aligned to their dtype");
 
     // Many rows: each wave has its own; few: the waves share them and split the tiles.
-    a.by_rows = most >= 64;
-    const bool keep_scores = a.track && !a.by_rows && most <= kScoreRows;
-    const int parts = a.q.type == KV_F32 ? 2 : 1;
+    a.by_rows = a.track ? most > kScoreRows : most > chunk_rows * 3 / 4 && chunk_tiles >= kChunkTiles;
+    const bool keep_scores = a.track && !a.by_rows;
     if (a.track) {
         grow(w_lse2, (size_t)tokens * q.num_q_heads);
         a.lse2 = w_lse2.p;
