@@ -140,7 +140,7 @@ __device__ __forceinline__ float kv_sum4(float v) {
 
 // Slots lo .. hi - 1 that row `row` (of count * G) of a sequence may see.
 __device__ __forceinline__ void kv_range(const KvAttend& a, int len, int count, int row, int& lo, int& hi) {
-    const int p = len - count + row / a.G;  // its own slot
+    const int p = len - count + kv_div(row, a.by_group);  // its own slot
     hi = a.causal ? max(p + 1, 0) : len;
     lo = a.window ? max(p + 1 - a.window, 0) : 0;
 }
@@ -170,7 +170,7 @@ __device__ __forceinline__ void kv_load_rows(KvWave<S, CODE, PARTS, NC>& w, cons
         float big = 0.f;
         // (a row past the end loads the last one's and is not used)
         const int real = min(row, rows - 1);
-        const int64_t base = (int64_t)(b.tok0[i] + real / a.G) * a.q.st + (int64_t)(h * a.G + real % a.G) * a.q.sh;
+        const int64_t base = (int64_t)(b.tok0[i] + kv_div(real, a.by_group)) * a.q.st + (int64_t)(h * a.G + kv_mod(real, a.by_group)) * a.q.sh;
         if (row < rows) kv_range(a, len, b.count[i], row, w.lo[n], w.hi[n]);
         float x[S][8];
         kv_load_row<S, PARTS>(a.q, base, g, c.D, x);
@@ -277,7 +277,7 @@ __device__ __forceinline__ void kv_reference(KvWave<S, CODE, PARTS, NC>& w, cons
                 }
                 if (a.mask && any) {
                     any = false;
-                    const uint8_t* mask = a.mask + (int64_t)(tok0 + max(w.row[n], 0) / a.G) * a.mask_st;
+                    const uint8_t* mask = a.mask + (int64_t)(tok0 + kv_div(max(w.row[n], 0), a.by_group)) * a.mask_st;
                     uint8_t see[8];
 #pragma unroll
                     for (int j = 0; j < 8; j++)  // (slots past the row's last are hidden already)
@@ -379,7 +379,7 @@ __device__ __forceinline__ float kv_join_factor(float m, float l, float mx) {
 
 // Index of a row in the outputs, and in the arrays of one head after the other.
 __device__ __forceinline__ size_t kv_row(const KvDev& c, const KvBatch& b, const KvAttend& a, int i, int h, int row) {
-    return (size_t)(b.tok0[i] + row / a.G) * c.H * a.G + h * a.G + row % a.G;
+    return (size_t)(b.tok0[i] + kv_div(row, a.by_group)) * c.H * a.G + h * a.G + kv_mod(row, a.by_group);
 }
 __device__ __forceinline__ size_t kv_head_row(const KvDev& c, const KvBatch& b, const KvAttend& a, int i, int h, int row) {
     return ((size_t)b.tok0[i] * c.H + (size_t)h * b.count[i]) * a.G + row;
@@ -404,8 +404,8 @@ struct KvJob {
 };
 __device__ __forceinline__ KvJob kv_job(const KvDev& c, const KvBatch& b, const KvAttend& a, int wg_rows) {
     KvJob j;
-    j.h = blockIdx.x % c.H;
-    const int unit = blockIdx.x / c.H;
+    j.h = kv_mod(blockIdx.x, c.by_heads);
+    const int unit = kv_div(blockIdx.x, c.by_heads);
     j.i = kv_find(b, unit);
     const int u = unit - b.unit0[j.i], rows = b.count[j.i] * a.G, row_tiles = (rows + wg_rows - 1) / wg_rows;
     const int tile = row_tiles - 1 - u % row_tiles;
@@ -659,7 +659,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvDev c, KvBatch b, KvAtte
     const int tid = threadIdx.x;
     const int width = c.Dp / 4, groups = 256 / width, grp = tid / width, d4 = tid % width;
     const int per_wg = WIDE ? 1 : groups, pieces = (used_rows + per_wg - 1) / per_wg;
-    const int h = blockIdx.x % c.H, piece = blockIdx.x / c.H % pieces, unit = blockIdx.x / c.H / pieces;
+    const int h = kv_mod(blockIdx.x, c.by_heads), piece = kv_div(blockIdx.x, c.by_heads) % pieces, unit = kv_div(blockIdx.x, c.by_heads) / pieces;
     const int i = kv_find(b, unit);
     const int rows = b.count[i] * a.G, u = unit - b.unit0[i];
     const int row0 = (b.unit0[i + 1] - b.unit0[i] - 1 - u) * wg_rows;
@@ -714,7 +714,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvDev c, KvBatch b, KvAtte
 
 // Weights from the kept scores of a step: four slots to a thread, bound by the scores' bytes.
 __global__ __launch_bounds__(256) void kv_score_weights_kernel(KvDev c, KvBatch b, KvAttend a) {
-    const int h = blockIdx.x % c.H, unit = blockIdx.x / c.H;
+    const int h = kv_mod(blockIdx.x, c.by_heads), unit = kv_div(blockIdx.x, c.by_heads);
     const int i = kv_find(b, unit);
     const int slot = (unit - b.unit0[i]) * KV_SCORE_SLOTS + threadIdx.x * 4;
     const int len = b.len[i], rows = b.count[i] * a.G;
@@ -758,7 +758,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_weights_kernel(KvDev c, KvBatc
     constexpr int QT = PARTS * S * 64;             // 16-byte pieces of a row tile
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, col = lane & 15;
-    const int h = blockIdx.x % c.H, chunk = blockIdx.x / c.H % a.chunks, unit = blockIdx.x / c.H / a.chunks;
+    const int h = kv_mod(blockIdx.x, c.by_heads), chunk = kv_div(blockIdx.x, c.by_heads) % a.chunks, unit = kv_div(blockIdx.x, c.by_heads) / a.chunks;
     const int i = kv_find(b, unit);
     const int len = b.len[i], rows = b.count[i] * a.G;
     const int slots0 = (unit - b.unit0[i]) * KV_WEIGHT_SLOTS;
@@ -865,7 +865,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_weights_kernel(KvDev c, KvBatc
                     for (int j = 0; j < 8; j++) {
                         const int slot = (t0 + x) * KV_TILE + (j >> 2) * 16 + 4 * g + (j & 3);
                         bool see = slot >= lo && slot < hi;
-                        if (see && a.mask) see = a.mask[(int64_t)(b.tok0[i] + row / a.G) * a.mask_st + slot * a.mask_ss] != 0;
+                        if (see && a.mask) see = a.mask[(int64_t)(b.tok0[i] + kv_div(row, a.by_group)) * a.mask_st + slot * a.mask_ss] != 0;
                         sum[x][j] += see ? __builtin_amdgcn_exp2f(__builtin_fmaf(u[x][j >> 2][j & 3], f * ks[x], -lse)) : 0.f;
                     }
             }
@@ -886,7 +886,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_weights_kernel(KvDev c, KvBatc
 
 // A thread per slot: the chunks' sums, and the weight.
 __global__ __launch_bounds__(KV_WEIGHT_SLOTS) void kv_chunk_weights_kernel(KvDev c, KvBatch b, KvAttend a) {
-    const int h = blockIdx.x % c.H, unit = blockIdx.x / c.H;
+    const int h = kv_mod(blockIdx.x, c.by_heads), unit = kv_div(blockIdx.x, c.by_heads);
     const int i = kv_find(b, unit);
     const int slot = (unit - b.unit0[i]) * KV_WEIGHT_SLOTS + threadIdx.x;
     if (slot >= b.len[i]) return;

@@ -125,7 +125,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvDev c, KvBatch b, KvTe
     __shared__ uint32_t red[4];
     const int tid = threadIdx.x;
     const bool vals = blockIdx.x & 1;
-    const int h = (blockIdx.x >> 1) % c.H, unit = (blockIdx.x >> 1) / c.H;
+    const int h = kv_mod(blockIdx.x >> 1, c.by_heads), unit = kv_div(blockIdx.x >> 1, c.by_heads);
     const int i = kv_find(b, unit);
     const int len0 = b.len[i], len1 = len0 + b.count[i];
     const int blk = (len0 >> c.shift) + unit - b.unit0[i];
@@ -364,7 +364,7 @@ __device__ __forceinline__ void read_tile(const KvDev& c, const uint8_t* tile, f
 template <int T>
 __global__ __launch_bounds__(256) void kv_read_kernel(KvDev c, KvBatch b, KvReadOut o) {
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int h = blockIdx.x % c.H, unit = blockIdx.x / c.H;
+    const int h = kv_mod(blockIdx.x, c.by_heads), unit = kv_div(blockIdx.x, c.by_heads);
     const int i = kv_find(b, unit);
     const int first = b.aux[i], last = first + b.count[i];
     const int group = (first / KV_READ + unit - b.unit0[i]) * KV_READ;
@@ -383,6 +383,24 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvDev c, KvBatch b, KvRead
     const int slot = group + tid;
     if (tid < KV_READ && slot >= first && slot < last && (o.positions || o.weights)) {
         const size_t at = (size_t)(tok + slot) * c.H + h;
+        const size_t from = ((size_t)table[slot >> c.shift] * c.H + h) * c.B + (slot & (c.B - 1));
+        if (o.positions) o.positions[at] = c.positions[from];
+        if (o.weights) o.weights[at] = c.weights[from];
+    }
+}
+
+// Positions and weights alone: 128 slots of every head to a workgroup, so that the outputs
+// [token, head] leave in one piece.
+__global__ __launch_bounds__(256) void kv_read_side_kernel(KvDev c, KvBatch b, KvReadOut o) {
+    const int unit = blockIdx.x, i = kv_find(b, unit);
+    const int first = b.aux[i], last = first + b.count[i];
+    const int group = (first / KV_READ + unit - b.unit0[i]) * KV_READ;
+    const int* table = c.table + (size_t)b.seq[i] * c.W;
+    const size_t tok = (size_t)b.tok0[i];
+    for (int u = threadIdx.x; u < KV_READ * c.H; u += 256) {
+        const int r = kv_div(u, c.by_heads), h = u - r * c.H, slot = group + r;
+        if (slot < first || slot >= last) continue;
+        const size_t at = (tok + (slot - first)) * c.H + h;
         const size_t from = ((size_t)table[slot >> c.shift] * c.H + h) * c.B + (slot & (c.B - 1));
         if (o.positions) o.positions[at] = c.positions[from];
         if (o.weights) o.weights[at] = c.weights[from];
@@ -493,7 +511,7 @@ __global__ __launch_bounds__(1024) void kv_select_kernel(KvDev c, KvBatch b, KvE
     __shared__ uint32_t hist[KV_BINS];
     __shared__ uint32_t scan[18];
     const int tid = threadIdx.x;
-    const KvSelect s = select_job(c, b, e, blockIdx.x / c.H, blockIdx.x % c.H);
+    const KvSelect s = select_job(c, b, e, kv_div(blockIdx.x, c.by_heads), kv_mod(blockIdx.x, c.by_heads));
     uint32_t key[KV_SELECT];
 #pragma unroll
     for (int x = 0; x < KV_SELECT; x++) {
@@ -536,7 +554,7 @@ __device__ __forceinline__ KvCut long_cut(const KvDev& c, const KvEvict& e, cons
 __global__ __launch_bounds__(1024) void kv_long_hist_kernel(KvDev c, KvBatch b, KvEvict e, int groups, int pass) {
     __shared__ uint32_t hist[KV_BINS];
     __shared__ uint32_t scan[18];
-    const int tid = threadIdx.x, h = blockIdx.x % c.H, g = blockIdx.x / c.H % groups, i = blockIdx.x / c.H / groups;
+    const int tid = threadIdx.x, h = kv_mod(blockIdx.x, c.by_heads), g = kv_div(blockIdx.x, c.by_heads) % groups, i = kv_div(blockIdx.x, c.by_heads) / groups;
     const KvSelect s = select_job(c, b, e, i, h);
     if (!s.compete || g * KV_LONG >= s.old) return;
     uint32_t key[4];
@@ -563,7 +581,7 @@ __global__ __launch_bounds__(1024) void kv_long_hist_kernel(KvDev c, KvBatch b, 
 __global__ __launch_bounds__(1024) void kv_long_place_kernel(KvDev c, KvBatch b, KvEvict e, int groups, int place) {
     __shared__ uint32_t scan[18];
     __shared__ uint32_t sums[2];
-    const int tid = threadIdx.x, h = blockIdx.x % c.H, g = blockIdx.x / c.H % groups, i = blockIdx.x / c.H / groups;
+    const int tid = threadIdx.x, h = kv_mod(blockIdx.x, c.by_heads), g = kv_div(blockIdx.x, c.by_heads) % groups, i = kv_div(blockIdx.x, c.by_heads) / groups;
     const KvSelect s = select_job(c, b, e, i, h);
     if (place && g == 0)
         for (int j = tid; j < s.recent; j += 1024) {
@@ -621,7 +639,7 @@ __global__ __launch_bounds__(256) void kv_move_kernel(KvDev c, KvBatch b, KvEvic
     __shared__ uint32_t red[4];
     const int tid = threadIdx.x, lane = tid & 63;
     const bool vals = blockIdx.x & 1;
-    const int h = (blockIdx.x >> 1) % c.H, unit = (blockIdx.x >> 1) / c.H;
+    const int h = kv_mod(blockIdx.x >> 1, c.by_heads), unit = kv_div(blockIdx.x >> 1, c.by_heads);
     const int i = kv_find(b, unit);
     const int blk = unit - b.unit0[i], slot0 = blk << c.shift;
     const int n = min(b.count[i] - slot0, c.B);
@@ -692,7 +710,7 @@ __global__ __launch_bounds__(256) void kv_move_kernel(KvDev c, KvBatch b, KvEvic
 // One workgroup: 128 slots of one head; those that leave are written to their rows.
 __global__ __launch_bounds__(256) void kv_dropped_kernel(KvDev c, KvBatch b, KvEvict e, int groups) {
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int h = blockIdx.x % c.H, g = blockIdx.x / c.H % groups, i = blockIdx.x / c.H / groups;
+    const int h = kv_mod(blockIdx.x, c.by_heads), g = kv_div(blockIdx.x, c.by_heads) % groups, i = kv_div(blockIdx.x, c.by_heads) / groups;
     const int len = b.len[i], group = g * KV_READ;
     const int* table = c.table + (size_t)b.seq[i] * c.W;
     const int* gone = e.gone + ((size_t)i * c.H + h) * e.slots;
@@ -753,7 +771,9 @@ void launch_kv_append(const KvDev& c, const KvBatch& b, const KvTensor& k, const
 void launch_kv_read(const KvDev& c, const KvBatch& b, const KvReadOut& o, hipStream_t s) {
     const dim3 grid((unsigned)b.unit0[b.n] * c.H);
     if (!grid.x) return;
-    if (o.type == KV_F32)
+    if (!o.k && !o.v)
+        hipLaunchKernelGGL(kv_read_side_kernel, dim3((unsigned)b.unit0[b.n]), dim3(256), 0, s, c, b, o);
+    else if (o.type == KV_F32)
         hipLaunchKernelGGL(kv_read_kernel<KV_F32>, grid, dim3(256), 0, s, c, b, o);
     else if (o.type == KV_F16)
         hipLaunchKernelGGL(kv_read_kernel<KV_F16>, grid, dim3(256), 0, s, c, b, o);

@@ -57,6 +57,7 @@ KvCache::KvCache(const vgpu_kv_params& p) : params(p) {
     cfg(params.max_blocks <= (size_t)(INT_MAX / 2) / p.block_tokens, "a sequence's slots must stay below 2^30");
     VGPU_HIP(hipGetDevice(&device));
     dev.H = (int)p.num_heads;
+    dev.by_heads = KvDiv(dev.H);
     dev.D = (int)p.head_dim;
     // padded dimensions the kernels are compiled for
     dev.Dp = dev.D <= 64 ? 64 : dev.D <= 96 ? 96 : dev.D <= 128 ? 128 : dev.D <= 192 ? 192 : 256;
@@ -403,6 +404,7 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
     KvAttend a;
     a.q = tensor(q.q, "q");
     a.G = (int)(q.num_q_heads / (size_t)dev.H);
+    a.by_group = KvDiv(a.G);
     a.scale2 = q.scale * 1.44269504088896341f;
     a.causal = q.causal != 0;
     a.window = (int)std::min<size_t>(q.window, (size_t)INT_MAX / 2);

@@ -31,6 +31,21 @@ constexpr int KV_BATCH = 128;
 enum KvCode { KV_INT8 = 0, KV_FP8 = 1 };
 enum KvType { KV_F32 = 0, KV_F16 = 1, KV_BF16 = 2 };
 
+// Division of numbers below 2^30 by a launch's constant d: with k = ceil(log2 d) and
+// m = ceil(2^(30 + k) / d), x / d is x m >> 30 + k (the product's excess, below x 2^k,
+// stays below 2^(30 + k)).
+struct KvDiv {
+    uint32_t m = 1u << 30;
+    int shift = 30, d = 1;
+    KvDiv() = default;
+    explicit KvDiv(int by) : d(by) {
+        int k = 0;
+        while ((1ll << k) < by) k++;
+        shift = 30 + k;
+        m = (uint32_t)(((1ull << shift) + (uint64_t)by - 1) / (uint64_t)by);
+    }
+};
+
 struct KvDev {
     uint8_t* pool = nullptr;
     float* kscale = nullptr;   // [block * H + head]
@@ -41,6 +56,7 @@ struct KvDev {
     int H = 0, D = 0, Dp = 0, B = 0, W = 0;
     int shift = 0;             // log2 B
     int code = KV_INT8;
+    KvDiv by_heads;            // H
 };
 
 // n sequences of one launch.  Workgroups unit0[i] .. unit0[i + 1] - 1 (times what
@@ -70,6 +86,8 @@ struct KvTensor {
 __host__ __device__ inline int kv_half(int Dp) { return KV_TILE * Dp; }
 
 #ifdef __HIPCC__
+__device__ inline int kv_div(int x, const KvDiv& by) { return (int)((uint64_t)(uint32_t)x * by.m >> by.shift); }
+__device__ inline int kv_mod(int x, const KvDiv& by) { return x - kv_div(x, by) * by.d; }
 __device__ inline size_t kv_tile_offset(const KvDev& c, int block, int head, int tile) {
     const size_t part = (size_t)block * c.H + head;
     return (part * (size_t)(c.B / KV_TILE) + tile) * (size_t)(2 * kv_half(c.Dp));
@@ -140,6 +158,7 @@ void launch_kv_evict(const KvDev& c, const KvBatch& b, const KvEvict& e, hipStre
 struct KvAttend {
     KvTensor q;
     int G = 1;              // query heads per key/value head
+    KvDiv by_group;         // G
     float scale2 = 0.f;     // scale * log2(e)
     int causal = 1, window = 0;
     const uint8_t* mask = nullptr;
