@@ -760,7 +760,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_weights_kernel(KvDev c, KvBatc
     const int g = lane >> 4, col = lane & 15;
     const int h = kv_mod(blockIdx.x, c.by_heads), chunk = kv_div(blockIdx.x, c.by_heads) % a.chunks, unit = kv_div(blockIdx.x, c.by_heads) / a.chunks;
     const int i = kv_find(b, unit);
-    const int len = b.len[i], rows = b.count[i] * a.G;
+    const int len = b.len[i], count = b.count[i], rows = count * a.G;
     const int slots0 = (unit - b.unit0[i]) * KV_WEIGHT_SLOTS;
     const int t0 = slots0 / KV_TILE + wave * KV_WT;
     const int* table = c.table + (size_t)b.seq[i] * c.W;
@@ -769,11 +769,11 @@ __global__ __launch_bounds__(256, 2) void kv_tile_weights_kernel(KvDev c, KvBatc
     int r0 = chunk * a.chunk_rows, r1 = min(r0 + a.chunk_rows, rows);
     if (a.causal) {
         // token p sees slot0 from p = slot0 on: row (slot0 - (len - count)) * G
-        const int tok = slots0 - (len - b.count[i]);
+        const int tok = slots0 - (len - count);
         if (tok > 0) r0 = max(r0, (int)min((int64_t)tok * a.G, (int64_t)rows) / 32 * 32);
     }
     if (a.window) {
-        const int64_t tok = (int64_t)min(slots0 + KV_WEIGHT_SLOTS, len) - 1 + a.window - (len - b.count[i]);
+        const int64_t tok = (int64_t)min(slots0 + KV_WEIGHT_SLOTS, len) - 1 + a.window - (len - count);
         r1 = (int)min((int64_t)r1, max(tok, (int64_t)0) * a.G);
     }
     half8 k[KV_WT][2 * S];
@@ -793,6 +793,12 @@ __global__ __launch_bounds__(256, 2) void kv_tile_weights_kernel(KvDev c, KvBatc
             k[x][2 * s + 1] = kv_half8<CODE>(r.z, r.w);
         }
     }
+    // Rows any_lo .. any_hi - 1 see some slot of the wave's tiles, all_lo .. all_hi - 1 every
+    // one: token p sees slots p - window + 1 .. p, and row (p - len + count) G is its first.
+    const auto first_row = [&](int64_t p) { return (int)min(max((p - (len - count)) * a.G, (int64_t)0), (int64_t)rows); };
+    const int64_t slot_lo = t0 * KV_TILE, slot_hi = (t0 + KV_WT) * KV_TILE;
+    const int any_lo = a.causal ? first_row(slot_lo) : 0, all_lo = a.causal ? first_row(slot_hi - 1) : 0;
+    const int any_hi = a.window ? first_row(slot_hi - 1 + a.window) : rows, all_hi = a.window ? first_row(slot_lo + a.window) : rows;
     float sum[KV_WT][8] = {};
     const size_t row_base = kv_head_row(c, b, a, i, h, 0);
     const uint4* qop = a.qop + ((size_t)(b.aux[i]) * c.H + (size_t)h * ((rows + 15) / 16)) * QT;
@@ -829,10 +835,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_weights_kernel(KvDev c, KvBatc
         for (int y = 0; y < 2; y++) {
             const int row0 = r + 16 * y, row = row0 + col;
             if (row0 >= end) break;
-            int lo0, hi0, lo1, hi1;
-            kv_range(a, len, b.count[i], row0, lo0, hi0);
-            kv_range(a, len, b.count[i], min(row0 + 16, rows) - 1, lo1, hi1);
-            if (hi1 <= t0 * KV_TILE || lo0 >= (t0 + KV_WT) * KV_TILE) continue;
+            if (row0 + 16 <= any_lo || row0 >= any_hi) continue;
             const bool real = row < end;
             const float f = fs[y], lse = ls[y];
             floatx4 u[KV_WT][2];
@@ -849,7 +852,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_weights_kernel(KvDev c, KvBatc
                         for (int j = 0; j < 2; j++)
                             u[x][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[x][j * S + s], q, u[x][j], 0, 0, 0);
                 }
-            const bool inside = !a.mask && lo1 <= t0 * KV_TILE && hi0 >= (t0 + KV_WT) * KV_TILE;
+            const bool inside = !a.mask && row0 >= all_lo && min(row0 + 16, rows) <= all_hi;
             if (inside) {
 #pragma unroll
                 for (int x = 0; x < KV_WT; x++)
@@ -858,7 +861,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_weights_kernel(KvDev c, KvBatc
                         sum[x][j] += __builtin_amdgcn_exp2f(__builtin_fmaf(u[x][j >> 2][j & 3], f * ks[x], -lse));
             } else {
                 int lo = 0, hi = 0;
-                if (real) kv_range(a, len, b.count[i], row, lo, hi);
+                if (real) kv_range(a, len, count, row, lo, hi);
 #pragma unroll
                 for (int x = 0; x < KV_WT; x++)
 #pragma unroll
