@@ -599,7 +599,7 @@ int vgpu_kv_evict(vgpu_kv* h, const int32_t* seqs, const int32_t* into, size_t n
 int vgpu_kv_read(vgpu_kv* h, const int32_t* seqs, const int64_t* first, const int64_t* counts, size_t n, int dtype,
                  void* k, void* v, int32_t* positions, float* weights, void* stream) {
     return guard([&] {
-        need(h && (n == 0 || (seqs && first && counts)), VGPU_ERR_INVALID_PARAMETER, "null argument");
+        need(h && (n == 0 || (seqs && first)), VGPU_ERR_INVALID_PARAMETER, "null argument");
         std::lock_guard<std::mutex> lk(h->kv->mu);
         h->kv->read(seqs, first, counts, n, dtype, k, v, positions, weights, (hipStream_t)stream);
     });

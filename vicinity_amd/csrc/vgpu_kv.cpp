@@ -10,9 +10,13 @@ namespace vgpu {
 
 namespace {
 
-void need(bool ok, const std::string& msg, int code = VGPU_ERR_INVALID_PARAMETER) {
-    if (!ok) throw Error(code, msg);
-}
+// The message is put together only when the check fails.
+#define need(ok, msg, ...)                                      \
+    do {                                                        \
+        if (!(ok)) refuse(msg, ##__VA_ARGS__);                  \
+    } while (0)
+
+[[noreturn]] void refuse(const std::string& msg, int code = VGPU_ERR_INVALID_PARAMETER) { throw Error(code, msg); }
 
 size_t item_size(int type) { return type == KV_F32 ? 4 : 2; }
 
@@ -235,10 +239,12 @@ void KvCache::read(const int32_t* ids, const int64_t* first, const int64_t* coun
     check_ids(*this, seen, ids, n);
     need(dtype == VGPU_F32 || dtype == VGPU_F16 || dtype == VGPU_BF16, "dtype must be float32, float16 or bfloat16");
     int64_t tok = 0;
+    const auto count_of = [&](size_t i) { return counts ? counts[i] : seqs[ids[i]].len - first[i]; };
     for (size_t i = 0; i < n; i++) {
-        need(first[i] >= 0 && counts[i] >= 0 && first[i] <= seqs[ids[i]].len && counts[i] <= seqs[ids[i]].len - first[i],
+        const int64_t count = count_of(i);
+        need(first[i] >= 0 && count >= 0 && first[i] <= seqs[ids[i]].len && count <= seqs[ids[i]].len - first[i],
              "slots outside sequence " + std::to_string(ids[i]) + " of length " + std::to_string(seqs[ids[i]].len));
-        tok += counts[i];
+        tok += count;
         need(tok <= INT_MAX / 2, "more than 2^30 tokens in one call");
     }
     KvReadOut o;
@@ -254,12 +260,12 @@ void KvCache::read(const int32_t* ids, const int64_t* first, const int64_t* coun
             b.seq[j] = ids[i];
             b.len[j] = (int)seqs[ids[i]].len;
             b.tok0[j] = (int)tok;
-            b.count[j] = (int)counts[i];
+            const int64_t count = count_of(i), last = first[i] + count;
+            b.count[j] = (int)count;
             b.aux[j] = (int)first[i];
-            const int64_t last = first[i] + counts[i];
-            b.unit0[j + 1] = b.unit0[j] + (counts[i] ? (int)((last + KV_READ - 1) / KV_READ - first[i] / KV_READ) : 0);
+            b.unit0[j + 1] = b.unit0[j] + (count ? (int)((last + KV_READ - 1) / KV_READ - first[i] / KV_READ) : 0);
             b.n++;
-            tok += counts[i];
+            tok += count;
         }
         if (k || v || pos || wts) launch_kv_read(dev, b, o, s);
     }

@@ -105,6 +105,7 @@ __device__ inline int kv_value_byte(int r, int d) {
 }
 // The batch entry of a workgroup: how many unit0 are not above it, less one.
 __device__ inline int kv_find(const KvBatch& b, int unit) {
+    if (b.n == 1) return 0;
     const int lane = threadIdx.x & 63;
     const int e0 = lane < b.n && b.unit0[lane] <= unit;
     const int e1 = lane + 64 < b.n && b.unit0[lane + 64] <= unit;
