@@ -393,9 +393,9 @@ __device__ __forceinline__ void kv_finish(const KvDev& c, const KvBatch& b, cons
     if (a.lse2) a.lse2[kv_head_row(c, b, a, i, h, row)] = lse2;
 }
 
-// What a workgroup does: its sequence, split and first row (first splits before second
-// ones, and the last rows, which see most, before the first ones: long work starts
-// early), and the tiles t0 .. t1 - 1 that its rows see in its split.
+// What a workgroup does: its sequence, split and first row (last splits first, they are
+// the shorter ones of their rows, and last rows, which see most, before the first: the
+// short work comes at the end), and the tiles t0 .. t1 - 1 that its rows see in its split.
 struct KvJob {
     int i, h, split, row0, row1;
     int t0, t1;
@@ -409,7 +409,7 @@ __device__ __forceinline__ KvJob kv_job(const KvDev& c, const KvBatch& b, const 
     j.i = kv_find(b, unit);
     const int u = unit - b.unit0[j.i], rows = b.count[j.i] * a.G, row_tiles = (rows + wg_rows - 1) / wg_rows;
     const int tile = row_tiles - 1 - u % row_tiles;
-    j.split = u / row_tiles;
+    j.split = b.splits[j.i] - 1 - u / row_tiles;
     j.row0 = tile * wg_rows, j.row1 = min(j.row0 + wg_rows, rows);
     int lo0, hi0, lo1, hi1;
     kv_range(a, b.len[j.i], b.count[j.i], j.row0, lo0, hi0);
@@ -671,8 +671,9 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvDev c, KvBatch b, KvAtte
     const int splits = (tiles + b.per[i] - 1) / b.per[i];
     if (splits <= 1) return;  // the one workgroup has written the rows
     if (WIDE ? row >= rows : (grp >= groups || r >= wg_rows || row >= rows)) return;
-    const size_t stride = (size_t)(b.unit0[i + 1] - b.unit0[i]) * c.H * wg_rows;
-    const size_t base = ((size_t)(b.aux[i] + u) * c.H + h) * wg_rows + r;
+    const int row_tiles = b.unit0[i + 1] - b.unit0[i];
+    const int64_t stride = -(int64_t)row_tiles * c.H * wg_rows;  // the first split's parts lie last
+    const int64_t base = ((int64_t)(b.aux[i] + u + (b.splits[i] - 1) * row_tiles) * c.H + h) * wg_rows + r;
     float mx = KV_NEG;
     if (WIDE) {
         for (int s = tid & 63; s < splits; s += 64) mx = fmaxf(mx, a.part_ml[base + s * stride].x);

@@ -14,6 +14,8 @@ namespace vgpu {
 
 namespace {
 
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+
 // Scales are 0 below this largest magnitude, so 1 / s stays finite.
 constexpr float KV_TINY = 0x1p-100f;
 
@@ -281,9 +283,10 @@ template <int T, int N>
 __device__ __forceinline__ void store_row(void* p, size_t row, int d, int D, bool vec, const float* v) {
     if (vec && d + N <= D) {
         if (T == KV_F32) {
-            float4* at = (float4*)((float*)p + row + d);
+            floatx4* at = (floatx4*)((float*)p + row + d);
 #pragma unroll
-            for (int j = 0; j < N / 4; j++) at[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            for (int j = 0; j < N / 4; j++)
+                __builtin_nontemporal_store(floatx4{v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]}, at + j);
         } else {
             uint32_t w[N / 2];
 #pragma unroll
@@ -313,54 +316,56 @@ __device__ __forceinline__ void read_tile(const KvDev& c, const uint8_t* tile, f
     const int lane = threadIdx.x & 63, g = lane >> 4, x = lane & 15;
     const int S = c.Dp / 32;
     const uint4* at = (const uint4*)tile + lane;
+    // A lane's two pieces of 4 dims, of the lower and the upper 16 of 32 dims of its slot, go
+    // out in two stores: of the even lanes' slots, then of the odd ones'.  Eight lanes hold a
+    // slot's 32 dims, so that a float32 store is of whole 128-byte lines.
+    const bool odd = lane & 1;
+    const auto emit = [&](void* out, uint32_t lower, uint32_t upper, float s, const size_t* r, int d) {
+        const uint32_t other = (uint32_t)__builtin_amdgcn_mov_dpp((int)(odd ? lower : upper), 0xb1, 0xf, 0xf, true);
+        const uint32_t two[2] = {odd ? other : lower, odd ? upper : other};
+#pragma unroll
+        for (int y = 0; y < 2; y++) {
+            float e[4];
+            decode4(two[y], c.code, e);
+#pragma unroll
+            for (int i = 0; i < 4; i++) e[i] *= s;
+            if (r[y] != ~(size_t)0) store_row<T, 4>(out, r[y], d + (odd ? 16 : 0), c.D, vec, e);
+        }
+    };
     if (ko) {
-        const size_t rows[2] = {row(x), row(16 + x)};
+        size_t rows[2][2];
+#pragma unroll
+        for (int y = 0; y < 2; y++) rows[0][y] = row((x & ~1) + y), rows[1][y] = row(16 + (x & ~1) + y);
         for (int p = 0; p < S; p++) {
             const uint4 w = at[p * 64];
 #pragma unroll
             for (int o = 0; o < 2; o++) {
                 const int j = (2 * p + o) / S, s = (2 * p + o) % S;
-                const size_t r = j ? rows[1] : rows[0];
-                // dims 8 g .. + 3 and + 4 .. + 7 of lane group g become 4 g .. and 16 + 4 g ..,
-                // so that a store of the four groups is contiguous
+                // dims 8 g .. + 3 and + 4 .. + 7 of lane group g become 4 g .. and 16 + 4 g ..
                 const auto half = __builtin_amdgcn_permlane16_swap(o ? w.z : w.x, o ? w.w : w.y, false, false);
                 const auto two = __builtin_amdgcn_permlane32_swap(half[0], half[1], false, false);
-#pragma unroll
-                for (int y = 0; y < 2; y++) {
-                    float e[4];
-                    decode4(two[y], c.code, e);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) e[i] *= ks;
-                    if (r != ~(size_t)0) store_row<T, 4>(ko, r, 32 * s + 16 * y + 4 * g, c.D, vec, e);
-                }
+                emit(ko, two[0], two[1], ks, j ? rows[1] : rows[0], 32 * s + 4 * g);
             }
         }
     }
     if (vo) {
         // a quad of lanes exchanges bytes, so that a lane has 4 dims of slots 4 g + (x & 3)
         // and 16 above
-        const int r = 4 * g + (x & 3);
-        const size_t rows[2] = {row(r), row(16 + r)};
+        const int r = 4 * g + (x & 2);
+        const size_t rows[2][2] = {{row(r), row(r + 1)}, {row(16 + r), row(17 + r)}};
         for (int p = 0; p < S; p++) {
             const uint4 w = at[(S + p) * 64];
-#pragma unroll
-            for (int o = 0; o < 2; o++) {
-                const int d = (2 * p + o) * 16 + (x & ~3);
-#pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    float e[4];
-                    decode4(quad_transpose(half ? (o ? w.w : w.y) : (o ? w.z : w.x)), c.code, e);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) e[i] *= vs;
-                    if (rows[half] != ~(size_t)0) store_row<T, 4>(vo, rows[half], d, c.D, vec, e);
-                }
-            }
+            const int d = 32 * p + (x & ~3);
+            emit(vo, quad_transpose(w.x), quad_transpose(w.z), vs, rows[0], d);
+            emit(vo, quad_transpose(w.y), quad_transpose(w.w), vs, rows[1], d);
         }
     }
 }
 
 // One workgroup: 128 slots of one head, a tile to a wave.  Bound by the bytes written:
-// no element passes through LDS, and four lanes store 64 contiguous bytes.
+// no element passes through LDS, and stores of whole lines leave the caches to the pool
+// (nontemporal: 31 sequences moved in 41 us for 64 before them; 64-byte halves of lines
+// stored so took 68 us of reading for 58).
 template <int T>
 __global__ __launch_bounds__(256) void kv_read_kernel(KvDev c, KvBatch b, KvReadOut o) {
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);

@@ -449,23 +449,30 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
         }
     }
     const int rows = kv_attend_rows(a, dev.Dp);
+    // Where a workgroup's work depends on its sequence, the short sequences come first: the
+    // light rows of the longest end the launch.
+    std::vector<size_t> order(n);
+    std::vector<int64_t> tok0(n);
     int64_t tok = 0;
+    for (size_t i = 0; i < n; i++) order[i] = i, tok0[i] = tok, tok += counts[i];
+    if (a.by_rows)
+        std::stable_sort(order.begin(), order.end(), [&](size_t x, size_t y) { return seqs[ids[x]].len < seqs[ids[y]].len; });
     for (size_t i0 = 0; i0 < n; i0 += KV_BATCH) {
         KvBatch b;
         b.n = 0;
         b.unit0[0] = 0;
         int64_t work = 0, units = 0, score_tiles = 0, row_tiles = 0;
         int64_t tiles[KV_BATCH], row_units[KV_BATCH];  // that a row tile can see; row tiles
-        for (size_t i = i0; i < std::min(n, i0 + KV_BATCH); i++) {
+        for (size_t x = i0; x < std::min(n, i0 + KV_BATCH); x++) {
+            const size_t i = order[x];
             const int64_t len = seqs[ids[i]].len;
             const int j = b.n++;
             b.seq[j] = ids[i];
             b.len[j] = (int)len;
-            b.tok0[j] = (int)tok;
+            b.tok0[j] = (int)tok0[i];
             b.count[j] = (int)counts[i];
             row_units[j] = (counts[i] * a.G + rows - 1) / rows;
             units += row_units[j] * dev.H;
-            tok += counts[i];
             tiles[j] = (len + KV_TILE - 1) / KV_TILE;
             need(score_tiles <= INT_MAX / 2, "too many scores in one call");
             b.aux[j] = (int)(keep_scores ? score_tiles : row_tiles);
