@@ -363,12 +363,13 @@ __device__ __forceinline__ void kv_add_values(KvWave<S, CODE, PARTS, 1>& w, cons
     }
 }
 
-// A half of a tile, 16 contiguous bytes of a lane at a time.
-template <int S>
+// A half of a tile, 16 contiguous bytes of a lane at a time.  ONCE: no other workgroup reads
+// it, so it passes the caches by.
+template <int S, bool ONCE>
 __device__ __forceinline__ void kv_fetch(uint4 (&k)[S], const uint8_t* half) {
-    const uint4* p = (const uint4*)half + (threadIdx.x & 63);
+    const u32x4* p = (const u32x4*)half + (threadIdx.x & 63);
 #pragma unroll
-    for (int s = 0; s < S; s++) k[s] = p[s * 64];
+    for (int s = 0; s < S; s++) k[s] = __builtin_bit_cast(uint4, ONCE ? __builtin_nontemporal_load(p + s * 64) : p[s * 64]);
 }
 
 // What a part with reference m and sum l is multiplied with under reference mx.  A part
@@ -425,7 +426,9 @@ __device__ __forceinline__ KvJob kv_job(const KvDev& c, const KvBatch& b, const 
 // joined at the end.  The next tile's keys are loaded when this one's are used up, under
 // its softmax and values, and its values under the next one's keys: one tile of registers.  Bound by the cache's bytes: a tile's 64 Dp bytes against 4 Dp / 16
 // matrix instructions of 16 cycles.
-template <int S, int CODE, int PARTS>
+// ONCE: no row tile but this one reads the tiles (64 sequences of 4096, 8 x 128, one row tile:
+// 86 us, by the caches 97; two row tiles 145 and 129).
+template <int S, int CODE, int PARTS, bool ONCE>
 __global__ __launch_bounds__(256, S <= 4 ? 3 : 2) void kv_step_kernel(KvDev c, KvBatch b, KvAttend a) {
     extern __shared__ __align__(16) float lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -447,7 +450,7 @@ __global__ __launch_bounds__(256, S <= 4 ? 3 : 2) void kv_step_kernel(KvDev c, K
     KvTiles info = kv_tile_infos(c, table, h, tw, 4, sp.t1);
     const auto tile = [&](const KvTiles& f, int x) { return kv_tile_of(c, f, x & 63); };
     uint4 kc[S], vc[S];
-    if (n > 0) kv_fetch<S>(kc, tile(info, 0)), kv_fetch<S>(vc, tile(info, 0) + kv_half(32 * S));
+    if (n > 0) kv_fetch<S, ONCE>(kc, tile(info, 0)), kv_fetch<S, ONCE>(vc, tile(info, 0) + kv_half(32 * S));
     KvWave<S, CODE, PARTS, 1> w;
     kv_load_rows(w, c, b, a, i, h, row0);
     for (int x = 0; x < n; x++) {
@@ -458,14 +461,14 @@ __global__ __launch_bounds__(256, S <= 4 ? 3 : 2) void kv_step_kernel(KvDev c, K
         const uint8_t* next = tile(info, x + 1 < n ? x + 1 : x);
         floatx4 u[1][2];
         kv_scores(w, kc, u);
-        if (x + 1 < n) kv_fetch<S>(kc, next);
+        if (x + 1 < n) kv_fetch<S, ONCE>(kc, next);
         half8 p0[1], p1[1];
         const bool inside = t * KV_TILE >= all_lo && (t + 1) * KV_TILE <= all_hi && !a.mask;
         float z[1][8];
         kv_reference(w, u, ks, lv, bad, t * KV_TILE, inside, a, b.tok0[i], scores, score_row, z);
         kv_exponents(w, z, rv, p0, p1);
         kv_add_values(w, vc, p0[0], p1[0]);
-        if (x + 1 < n) kv_fetch<S>(vc, next + kv_half(32 * S));
+        if (x + 1 < n) kv_fetch<S, ONCE>(vc, next + kv_half(32 * S));
     }
     w.l[0] = kv_sum4(w.l[0]), w.bad[0] = kv_sum4(w.bad[0]);
 
@@ -910,7 +913,9 @@ void attend_s(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s
         return;
     }
     const size_t lds = (size_t)4 * 16 * (32 * S + 4 + 2) * 4;
-    const auto kernel = kv_step_kernel<S, CODE, PARTS>;
+    int most = 0;
+    for (int i = 0; i < b.n; i++) most = b.count[i] * a.G > most ? b.count[i] * a.G : most;
+    const auto kernel = most <= 16 ? kv_step_kernel<S, CODE, PARTS, true> : kv_step_kernel<S, CODE, PARTS, false>;
     if (lds > 65536) ensure_dyn_lds((const void*)kernel, lds);
     hipLaunchKernelGGL(kernel, grid, dim3(256), lds, s, c, b, a);
 }
