@@ -616,6 +616,10 @@ __global__ __launch_bounds__(256, S == 8 ? 1 : 2) void kv_chunk_kernel(KvDev c, 
         for (int o = 0; o < 2 * S; o++) vop[o] = tiles[b0][2 * S + o][lane];
         // the loads first: their use waits behind the keys' products (two halves: no registers for it)
         if (PARTS == 1) __builtin_amdgcn_sched_barrier(0);
+        // a wave among its products yields to one that prepares its own, so that the two waves of a
+        // SIMD part company (2048 tokens over 32768 slots: 1248 us without, 1147 the other way round,
+        // 1120 so; eight waves to a workgroup instead: 1168)
+        __builtin_amdgcn_s_setprio(0);
         products(kop, u);
         kv_exponents(w, z, rv, p0, p1);
 #pragma unroll
@@ -627,6 +631,7 @@ __global__ __launch_bounds__(256, S == 8 ? 1 : 2) void kv_chunk_kernel(KvDev c, 
             }
         }
         stage(b2, next);
+        __builtin_amdgcn_s_setprio(1);
         if (xt + 3 < n_tiles) fetch(next, y + 3 < 64 ? kv_tile_of(c, info, y + 3) : kv_tile_of(c, ahead, y + 3 - 64));
         __syncthreads();
         const int tmp = b0;
