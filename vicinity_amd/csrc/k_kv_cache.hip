@@ -278,32 +278,23 @@ __device__ __forceinline__ void store1(void* p, size_t i, float v, int type) {
         ((__hip_bfloat16*)p)[i] = __float2bfloat16(v);
 }
 
-// N values of a row from dim d on (those below D), rounded once.
-template <int T, int N>
+// Four values of a row from dim d on (those below D), rounded once.
+template <int T>
 __device__ __forceinline__ void store_row(void* p, size_t row, int d, int D, bool vec, const float* v) {
-    if (vec && d + N <= D) {
+    if (vec && d + 4 <= D) {
         if (T == KV_F32) {
-            floatx4* at = (floatx4*)((float*)p + row + d);
-#pragma unroll
-            for (int j = 0; j < N / 4; j++)
-                __builtin_nontemporal_store(floatx4{v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]}, at + j);
+            __builtin_nontemporal_store(floatx4{v[0], v[1], v[2], v[3]}, (floatx4*)((float*)p + row + d));
         } else {
-            uint32_t w[N / 2];
+            uint16_t e[4];
 #pragma unroll
-            for (int j = 0; j < N / 2; j++) {
-                uint16_t h[2];
-                store1(h, 0, v[2 * j], T), store1(h, 1, v[2 * j + 1], T);
-                w[j] = (uint32_t)h[0] | (uint32_t)h[1] << 16;
-            }
-            if (N == 4)
-                *(uint2*)((uint16_t*)p + row + d) = make_uint2(w[0], w[1]);
-            else
-                *(uint4*)((uint16_t*)p + row + d) = make_uint4(w[0], w[1], w[N / 2 - 2], w[N / 2 - 1]);
+            for (int j = 0; j < 4; j++) store1(e, j, v[j], T);
+            *(uint2*)((uint16_t*)p + row + d) =
+                make_uint2((uint32_t)e[0] | (uint32_t)e[1] << 16, (uint32_t)e[2] | (uint32_t)e[3] << 16);
         }
         return;
     }
 #pragma unroll
-    for (int j = 0; j < N; j++)
+    for (int j = 0; j < 4; j++)
         if (d + j < D) store1(p, row + d + j, v[j], T);
 }
 
@@ -329,7 +320,7 @@ __device__ __forceinline__ void read_tile(const KvDev& c, const uint8_t* tile, f
             decode4(two[y], c.code, e);
 #pragma unroll
             for (int i = 0; i < 4; i++) e[i] *= s;
-            if (r[y] != ~(size_t)0) store_row<T, 4>(out, r[y], d + (odd ? 16 : 0), c.D, vec, e);
+            if (r[y] != ~(size_t)0) store_row<T>(out, r[y], d + (odd ? 16 : 0), c.D, vec, e);
         }
     };
     if (ko) {

@@ -99,7 +99,7 @@ size_t KvCache::device_bytes() const {
            w_ml.bytes() + w_hist.bytes() + w_counts.bytes() + w_qop.bytes() + w_qs.bytes() + w_wpart.bytes();
 }
 
-void KvCache::check_call(const int32_t* ids, size_t n, hipStream_t s) {
+void KvCache::check_call(hipStream_t s) {
     int cur = -1;
     VGPU_HIP(hipGetDevice(&cur));
     need(cur == device, "the cache's device (" + std::to_string(device) + ") must be current, not device " +
@@ -107,7 +107,6 @@ void KvCache::check_call(const int32_t* ids, size_t n, hipStream_t s) {
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
     VGPU_HIP(hipStreamIsCapturing(s, &st));
     need(st == hipStreamCaptureStatusNone, "the cache's lengths cannot follow a captured stream", VGPU_ERR_UNSUPPORTED);
-    (void)ids, (void)n;
 }
 
 static void check_ids(const KvCache& c, std::vector<uint8_t>& seen, const int32_t* ids, size_t n) {
@@ -170,7 +169,7 @@ void KvCache::release_blocks(std::vector<int>& blocks, size_t keep) {
 
 void KvCache::append(const int32_t* ids, const int64_t* counts, size_t n, const vgpu_tensor3& k, const vgpu_tensor3& v,
                      const int32_t* pos, const float* wts, hipStream_t s) {
-    check_call(ids, n, s);
+    check_call(s);
     check_ids(*this, seen, ids, n);
     need(k.dtype == v.dtype, "k and v must have the same dtype");
     const KvTensor kt = tensor(k, "k"), vt = tensor(v, "v");
@@ -235,7 +234,7 @@ void KvCache::append(const int32_t* ids, const int64_t* counts, size_t n, const 
 
 void KvCache::read(const int32_t* ids, const int64_t* first, const int64_t* counts, size_t n, int dtype, void* k,
                    void* v, int32_t* pos, float* wts, hipStream_t s) {
-    check_call(ids, n, s);
+    check_call(s);
     check_ids(*this, seen, ids, n);
     need(dtype == VGPU_F32 || dtype == VGPU_F16 || dtype == VGPU_BF16, "dtype must be float32, float16 or bfloat16");
     int64_t tok = 0;
@@ -288,7 +287,7 @@ void KvCache::truncate(const int32_t* ids, const int64_t* lengths, size_t n) {
 
 void KvCache::evict(const int32_t* ids, const int32_t* into, size_t n, size_t budget, size_t recent,
                     size_t num_dropped, int32_t* dpos, float* dk, float* dv, hipStream_t s) {
-    check_call(ids, n, s);
+    check_call(s);
     check_ids(*this, seen, ids, n);
     need(budget <= (size_t)INT_MAX / 2, "budget must not exceed 2^30");
     need(recent <= budget, "recent must not exceed budget");
@@ -401,7 +400,7 @@ void KvCache::evict(const int32_t* ids, const int32_t* into, size_t n, size_t bu
 }
 
 void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const vgpu_kv_query& q, hipStream_t s) {
-    check_call(ids, n, s);
+    check_call(s);
     check_ids(*this, seen, ids, n);
     need(q.num_q_heads > 0 && q.num_q_heads % (size_t)dev.H == 0 && q.num_q_heads <= 65536,
          "num_q_heads must be a multiple of the cache's heads (" + std::to_string(dev.H) + ")");

@@ -376,7 +376,7 @@ struct KvCache {
 
   private:
     size_t blocks_of(int64_t slots) const { return (size_t)((slots + dev.B - 1) >> dev.shift); }
-    void check_call(const int32_t* ids, size_t n, hipStream_t s);
+    void check_call(hipStream_t s);
     KvTensor tensor(const vgpu_tensor3& t, const char* name) const;
     // Blocks from the pool for `count` more of a sequence, written to `tab`'s row.
     void take_blocks(std::vector<int>& out, size_t count, size_t row, int* tab, KvRuns& runs, hipStream_t s);
