@@ -521,6 +521,22 @@ def test_evict_long_sequence_and_in_place_without_spare_blocks():
     assert pair.cache.info()["free_blocks"] == 9
 
 
+def test_evict_to_a_budget_far_above_the_lengths():
+    """What the call holds follows the sequences, not the budget: 17 of 2^30 would take 1.1 TB."""
+    torch = _torch()
+    _case("evict with a budget of 2^30")
+    pair = Pair(34, 8, 64, 32, "int8", blocks=64)
+    lens = [2 + i for i in range(17)]
+    k = _rand((sum(lens), 8, 64), "bfloat16", 112)
+    pair.append(k, k.flip(0), list(range(17)), lens)
+    want = pair.cache.read(seqs=list(range(17)))
+    budget = 2 ** 30 - 1
+    pair.cache.evict(budget, recent=budget, seqs=list(range(17)), into=list(range(17, 34)))
+    got = pair.cache.read(seqs=list(range(17, 34)))
+    for name in ("k", "v", "positions", "weights"):
+        assert torch.equal(got[name], want[name]), name
+
+
 def test_evict_keeps_poisoned_slots_poisoned():
     torch = _torch()
     _case("evict with NaN scales")
@@ -686,6 +702,27 @@ def test_refusals_leave_the_cache_as_it_was():
     one = va.KVCache(1, 2, 64, 6, block_tokens=32)
     one.append(x, x)
     assert all(torch.equal(a, b) for a, b in zip(got.values(), one.read().values()))
+
+
+def test_calls_of_more_workgroups_than_a_launch_can_have():
+    """4096 heads: 40960 tokens enter 10.5 M parts of the pool, two such sequences take two launches."""
+    torch = _torch()
+    _case("4096 heads, 2 x 40960 tokens")
+    import vicinity_amd as va
+
+    heads, n = 4096, 40960
+    cache = va.KVCache(2, heads, 1, 2 * n // 32 + 2, block_tokens=32, max_blocks=2560)
+    k = (torch.arange(2 * n, device="cuda:0") % 128).to(torch.float16)[:, None, None]
+    k = torch.where(k == 0, 127, k)  # and every block's scale is 1
+    k[::32] = 127
+    k = k.expand(2 * n, heads, 1)
+    with pytest.raises(ValueError, match="one sequence in one call"):
+        cache.append(k[:65600], k[:65600], seqs=[0])
+    assert cache.lengths.tolist() == [0, 0]
+    cache.append(k, k, seqs=[0, 1], counts=[n, n])
+    for field in ("k", "v"):
+        got = cache.read(seqs=[0, 1], fields=(field,), dtype=torch.float16)[field]
+        assert torch.equal(got, k), field
 
 
 def test_capture_is_refused():

@@ -27,6 +27,8 @@ constexpr int64_t kStepWorkgroups = 768;
 // split too, which costs a partial result for every row and split.
 constexpr int64_t kChunkWorkgroups = 512;
 constexpr int64_t kWeightWorkgroups = 3072;
+// Workgroups of one launch: its threads, 256 to a workgroup, are counted in 32 bits.
+constexpr int64_t kMaxWorkgroups = (1 << 24) - 1;
 // Bytes of partial results of one launch.
 constexpr int64_t kPartBytes = (int64_t)256 << 20;
 // Calls of at most this many rows per head keep their scores for the weights; with more a
@@ -184,6 +186,8 @@ void KvCache::append(const int32_t* ids, const int64_t* counts, size_t n, const 
         need(total <= (size_t)dev.W, "sequence " + std::to_string(ids[i]) + " would need " + std::to_string(total) +
                                          " blocks, more than max_blocks (" + std::to_string(dev.W) + ")");
         need(pos || q.next + counts[i] <= INT_MAX, "positions must stay below 2^31");
+        need((int64_t)(total - (q.len >> dev.shift)) * dev.H * 2 <= kMaxWorkgroups,
+             "too many tokens of one sequence in one call");
         want += total - q.blocks.size();
     }
     need(!tokens || (k.data && v.data), "null argument");
@@ -205,21 +209,22 @@ void KvCache::append(const int32_t* ids, const int64_t* counts, size_t n, const 
     }
     launch_kv_table(table.p, runs, s);
     int64_t tok = 0;
-    for (size_t i0 = 0; i0 < n; i0 += KV_BATCH) {
+    for (size_t i = 0; i < n;) {
         KvBatch b;
         b.n = 0;
         b.unit0[0] = 0;
-        for (size_t i = i0; i < std::min(n, i0 + KV_BATCH); i++) {
+        for (; i < n && b.n < KV_BATCH; i++) {
             Seq& q = seqs[ids[i]];
             const int j = b.n;
+            // blocks that the new tokens enter
+            const int64_t first = q.len >> dev.shift;
+            const int64_t touched = counts[i] ? (int64_t)blocks_of(q.len + counts[i]) - first : 0;
+            if ((b.unit0[j] + touched) * dev.H * 2 > kMaxWorkgroups) break;
             b.seq[j] = ids[i];
             b.len[j] = (int)q.len;
             b.tok0[j] = (int)tok;
             b.count[j] = (int)counts[i];
             b.aux[j] = (int)q.next;
-            // blocks that the new tokens enter
-            const int64_t first = q.len >> dev.shift;
-            const int64_t touched = counts[i] ? (int64_t)blocks_of(q.len + counts[i]) - first : 0;
             b.splits[j] = touched == 1 ? q.blocks[first] : -1;
             b.unit0[j + 1] = b.unit0[j] + (int)touched;
             b.n++;
@@ -245,24 +250,27 @@ void KvCache::read(const int32_t* ids, const int64_t* first, const int64_t* coun
              "slots outside sequence " + std::to_string(ids[i]) + " of length " + std::to_string(seqs[ids[i]].len));
         tok += count;
         need(tok <= INT_MAX / 2, "more than 2^30 tokens in one call");
+        need((count / KV_READ + 2) * dev.H <= kMaxWorkgroups, "too many slots of one sequence in one call");
     }
     KvReadOut o;
     o.k = k, o.v = v, o.positions = pos, o.weights = wts, o.type = dtype;
     o.vec = dev.D % 8 == 0 && ((uintptr_t)k | (uintptr_t)v) % 16 == 0;
     tok = 0;
-    for (size_t i0 = 0; i0 < n; i0 += KV_BATCH) {
+    for (size_t i = 0; i < n;) {
         KvBatch b;
         b.n = 0;
         b.unit0[0] = 0;
-        for (size_t i = i0; i < std::min(n, i0 + KV_BATCH); i++) {
+        for (; i < n && b.n < KV_BATCH; i++) {
             const int j = b.n;
+            const int64_t count = count_of(i), last = first[i] + count;
+            const int64_t groups = count ? (last + KV_READ - 1) / KV_READ - first[i] / KV_READ : 0;
+            if ((b.unit0[j] + groups) * dev.H > kMaxWorkgroups) break;
             b.seq[j] = ids[i];
             b.len[j] = (int)seqs[ids[i]].len;
             b.tok0[j] = (int)tok;
-            const int64_t count = count_of(i), last = first[i] + count;
             b.count[j] = (int)count;
             b.aux[j] = (int)first[i];
-            b.unit0[j + 1] = b.unit0[j] + (count ? (int)((last + KV_READ - 1) / KV_READ - first[i] / KV_READ) : 0);
+            b.unit0[j + 1] = b.unit0[j] + (int)groups;
             b.n++;
             tok += count;
         }
@@ -309,6 +317,7 @@ void KvCache::evict(const int32_t* ids, const int32_t* into, size_t n, size_t bu
              "num_dropped is below what leaves sequence " + std::to_string(ids[i]));
         if (!into && q.len <= (int64_t)budget) continue;
         const size_t take = blocks_of(stays(i));
+        need((int64_t)take * dev.H * 2 <= kMaxWorkgroups, "too many slots of one sequence in one call");
         need(take <= have, "the cut sequences need " + std::to_string(take) + " free blocks and find " +
                                std::to_string(have), VGPU_ERR_OUT_OF_MEMORY);
         have -= take;
@@ -317,11 +326,15 @@ void KvCache::evict(const int32_t* ids, const int32_t* into, size_t n, size_t bu
     const int drop = drops ? (int)num_dropped : 0;
     need((int64_t)dev.H * drop <= INT_MAX / KV_BATCH && (int64_t)n * drop <= INT_MAX,
          "too many dropped slots in one call");
-    const size_t group = std::min<size_t>(n, KV_BATCH);
-    if (!into) table2.reserve(table.n);
-    grow(w_kept, group * dev.H * std::max<size_t>(budget, 1));
     int64_t longest = 0;
     for (size_t i = 0; i < n; i++) longest = std::max(longest, seqs[ids[i]].len);
+    // sequences of one launch, which has a grid for the longest of them
+    const int64_t grid = (longest / KV_READ + 1) * dev.H;
+    need(grid <= kMaxWorkgroups, "too many slots of one sequence in one call");
+    const size_t group = std::min<size_t>({n, (size_t)KV_BATCH, (size_t)(kMaxWorkgroups / grid)});
+    if (!into) table2.reserve(table.n);
+    const size_t most = std::max<size_t>(std::min<size_t>(budget, (size_t)longest), 1);  // slots that stay
+    grow(w_kept, group * dev.H * most);
     if (drop) grow(w_gone, group * dev.H * (size_t)longest);
     const KvSelectSpace space = kv_select_space(dev, (int)group, (int)longest);
     grow(w_hist, space.hist);
@@ -334,7 +347,7 @@ void KvCache::evict(const int32_t* ids, const int32_t* into, size_t n, size_t bu
         free_blocks.reserve(params.num_blocks);
 
     KvEvict e;
-    e.budget = (int)std::max<size_t>(budget, 1), e.recent = (int)recent, e.drop = drop;
+    e.budget = (int)most, e.recent = (int)std::min(recent, most), e.drop = drop;
     e.kept = w_kept.p, e.gone = drop ? w_gone.p : nullptr;
     e.dst = into ? table.p : table2.p;
     e.dpos = dpos, e.dk = dk, e.dv = dv;
@@ -347,12 +360,13 @@ void KvCache::evict(const int32_t* ids, const int32_t* into, size_t n, size_t bu
         b.n = 0;
         b.unit0[0] = 0;
         size_t i = i0;
-        for (; i < n && b.n < KV_BATCH; i++) {
+        for (; i < n && b.n < (int)group; i++) {
             Seq& q = seqs[ids[i]];
             const int64_t stay = stays(i);
             const bool cut = into || q.len > stay;
             const size_t take = cut ? blocks_of(stay) : 0;
             if (take > free_blocks.size()) break;  // the blocks of those before come back first
+            if ((int64_t)(b.unit0[b.n] + take) * dev.H * 2 > kMaxWorkgroups) break;
             const int j = b.n++;
             b.seq[j] = ids[i];
             b.len[j] = (int)q.len;
@@ -483,7 +497,7 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
             const int64_t seen = a.causal && !a.window ? std::max<int64_t>(2 * len - counts[i], 0) : 2 * KV_TILE * tiles[j];
             work += row_units[j] * dev.H * ((seen + 2 * KV_TILE - 1) / (2 * KV_TILE));
         }
-        need(units <= INT_MAX / 64, "too many query rows in one call");
+        need(units <= kMaxWorkgroups, "too many query rows in one call");
         if (units) {
             // Tiles of one workgroup: as few as keep all workgroups on the card at once
             const int64_t target = a.by_rows ? kChunkWorkgroups : kStepWorkgroups;
