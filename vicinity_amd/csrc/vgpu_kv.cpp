@@ -26,6 +26,8 @@ constexpr int64_t kStepWorkgroups = 768;
 // Workgroups of a call with many rows, two to a compute unit: with fewer, the tiles are
 // split too, which costs a partial result for every row and split.
 constexpr int64_t kChunkWorkgroups = 512;
+// Workgroups of the second pass that makes weights: twelve to a compute unit, for its rows
+// differ in length (8192: no faster).
 constexpr int64_t kWeightWorkgroups = 3072;
 // Workgroups of one launch: its threads, 256 to a workgroup, are counted in 32 bits.
 constexpr int64_t kMaxWorkgroups = (1 << 24) - 1;
@@ -540,7 +542,7 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
             const int per = keep_scores ? KV_SCORE_SLOTS : KV_WEIGHT_SLOTS;
             for (int j = 0; j < b.n; j++) b.unit0[j + 1] = b.unit0[j] + (b.len[j] + per - 1) / per;
             if (!keep_scores) {
-                // chunks of at least 256 rows, until there are four workgroups to a compute unit
+                // chunks of at least 256 rows, until there are workgroups enough
                 const int64_t groups = std::max<int64_t>((int64_t)b.unit0[b.n] * dev.H, 1);
                 const int64_t chunks = std::min((most + 255) / 256, (kWeightWorkgroups + groups - 1) / groups);
                 a.chunk_rows = (int)(((most + chunks - 1) / chunks + 31) / 32 * 32);

@@ -183,8 +183,9 @@ struct KvAttend {
     int by_rows = 0;           // waves of a workgroup take different rows (else different tiles)
 };
 // 16-row tiles of a wave of the many-row kernel, by what its registers hold: Dp / 4
-// accumulators and Dp * parts / 8 query operands for each.  (256 dims: one workgroup to a
-// compute unit, by its LDS, with all the registers.)
+// accumulators and Dp * parts / 8 query operands for each (128 dims: 1431 us with two, 2311
+// with four; in float32 924 with two, 1029 with one; 192 dims: 1087 with one, 2603 with two).
+// 256 dims: one workgroup to a compute unit, by its LDS, with all the registers.
 constexpr int kv_chunk_nc(int Dp, int parts) { return Dp * parts <= 64 ? 4 : Dp <= 128 || Dp * parts == 256 ? 2 : 1; }
 // Rows that one workgroup takes.
 inline int kv_attend_rows(const KvAttend& a, int Dp) {
