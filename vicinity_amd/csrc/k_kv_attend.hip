@@ -818,7 +818,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_weights_kernel(KvDev c, KvBatc
     const auto fetch = [&](int r, uint4* to) {
         for (int x = wave; x < 2 * PARTS * S; x += 4)
             __builtin_amdgcn_global_load_lds(
-                (const __attribute__((address_space(1))) void*)(qop + min(r / 16 * PARTS * S + x, last_kib) * 64 + lane),
+                (const __attribute__((address_space(1))) void*)(qop + (size_t)min(r / 16 * PARTS * S + x, last_kib) * 64 + lane),
                 (__attribute__((address_space(3))) void*)(to + x * 64), 16, 0, 0);
 #pragma unroll
         for (int y = 0; y < 2; y++) {

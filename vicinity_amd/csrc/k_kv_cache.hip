@@ -1,8 +1,11 @@
 // The attention memory: quantising append, reading back, the block table.
 //
-// append  s = amax * (1 / Z) per (block, head), codes round(x / s): two passes over the
-//         new elements, the second from L2.  Bound by the bytes in and out.
+// append  s = amax * (1 / Z) per (block, head), codes round(x * (1 / s)): the elements are
+//         read once and stay in registers until s is known (long float32 rows: read twice).
 // read    code * s.
+// evict   the weight of the last slot that stays by a radix selection, the kept codes
+//         gathered into new blocks under their largest scale.
+// Each is bound by the bytes in and out; what the kernels reach stands at each.
 // Rounding: codes are the cache's format; every value before them is float32.
 #include "vgpu_kv.h"
 
