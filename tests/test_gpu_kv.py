@@ -339,6 +339,23 @@ def test_scores_far_apart_and_value_scales_far_apart():
         _check_attend(pair, q, [0], [3], decay=0.0)
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("size", [-30, -20, 0, 20])
+@pytest.mark.parametrize("n,counts", [(320, 3), (320, 150), (1 << 13, 600)])
+def test_blocks_of_zeros_beside_values_of_any_size(dtype, size, n, counts):
+    """The zeros, first and in the middle, are the slots that the rows see best."""
+    _case(f"zeros beside 2^{size} {dtype} {n} {counts}")
+    pair = Pair(1, 1, 64, 32, "int8", blocks=n // 32)
+    k = _rand((n, 1, 64), "float32", 83, 0.3)
+    v = _rand((n, 1, 64), "float32", 84) * 2.0 ** size
+    q = _rand((counts, 8, 64), dtype, 89)
+    for at in (0, 160):
+        v[at:at + 32] = 0
+        k[at:at + 32] *= 4
+    pair.append(k, v, [0], [n])
+    _check_attend(pair, q, [0], [counts], decay=0.0)
+
+
 @pytest.mark.parametrize("code", ["int8", "fp8"])
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
 @pytest.mark.parametrize("group", [1, 40, 130])

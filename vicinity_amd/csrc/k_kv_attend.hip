@@ -30,6 +30,11 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float KV_TOP = 6.f;    // p of the reference is 2^KV_TOP
 constexpr float KV_SLACK = 8.f;  // and may grow to 2^(KV_TOP + KV_SLACK)
+// A value scale of 0 stands for codes of 0, so any number does in its place: a small one,
+// for the reference must not follow slots that add nothing (with 1 the halves of p lost
+// values below 2^-20 beside them), but one whose p, 2^-40 of that beside values near 1,
+// still counts in the denominators.
+constexpr float KV_ZERO = 0x1p-40f;
 #define KV_NEG (-__builtin_huge_valf())
 
 // Two halves of 8 codes.
@@ -216,7 +221,7 @@ __device__ __forceinline__ KvTiles kv_tile_infos(const KvDev& c, const int* tabl
     r.ks = in ? c.kscale[part] : 0.f;
     const float vs = in ? c.vscale[part] : 1.f;
     r.bad = __ballot(vs != vs);
-    const float sv = vs > 0.f ? vs : 1.f;  // a scale of 0 stands for codes of 0: any number does
+    const float sv = vs > 0.f ? vs : KV_ZERO;
     r.lv = log2f(sv);
     r.rv = 1.f / sv;
     return r;
