@@ -357,6 +357,17 @@ def test_blocks_of_zeros_beside_values_of_any_size(dtype, size, n, counts):
 
 
 @pytest.mark.parametrize("code", ["int8", "fp8"])
+@pytest.mark.parametrize("size,n,counts", [(-102, 100_000, 2), (-101, 9000, 300), (120, 3000, 2), (120, 3000, 300)])
+def test_smallest_and_largest_value_scales(code, size, n, counts):
+    _case(f"values of 2^{size} {code} {n} {counts}")
+    pair = Pair(1, 1, 64, 64, code, blocks=n // 64 + 1)
+    k = _rand((n, 1, 64), "float32", 90, 0.02)
+    v = _rand((n, 1, 64), "float32", 91) * 2.0 ** size
+    pair.append(k, v, [0], [n])
+    _check_attend(pair, _rand((counts, 2, 64), "float32", 92), [0], [counts], decay=0.0)
+
+
+@pytest.mark.parametrize("code", ["int8", "fp8"])
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
 @pytest.mark.parametrize("group", [1, 40, 130])
 def test_logarithms_and_weights_keep_float32_whatever_the_query_type(code, dtype, group):

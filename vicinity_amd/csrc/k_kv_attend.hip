@@ -4,7 +4,7 @@
 // o = sum 2^(u_j) v_j / sum 2^(u_j).  One pass over the tiles with a running
 // reference m: the value scale s_b of a block goes into the exponent,
 // p_j = 2^(u_j + log2 s_b - m), so o's accumulators add p_j * code directly in the
-// matrix instruction and the denominator adds p_j / s_b.
+// matrix instruction and the denominator adds 2^-8 p_j / s_b.
 //
 // Products: codes are integers up to 127 or e4m3 numbers, both exact in half
 // precision.  A query row is scaled by a power of two to a largest element of 2^14
@@ -30,6 +30,10 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float KV_TOP = 6.f;    // p of the reference is 2^KV_TOP
 constexpr float KV_SLACK = 8.f;  // and may grow to 2^(KV_TOP + KV_SLACK)
+// The denominators hold 2^-KV_DOWN of their sums: scales lie between 2^-109 and 2^121, and of
+// the smallest 10^4 slots' sum passed the largest float.
+constexpr float KV_DOWN = 8.f;
+constexpr float KV_DOWN_F = 0x1p-8f;
 // A value scale of 0 stands for codes of 0, so any number does in its place: a small one,
 // for the reference must not follow slots that add nothing (with 1 the halves of p lost
 // values below 2^-20 beside them), but one whose p, 2^-40 of that beside values near 1,
@@ -205,7 +209,7 @@ __device__ __forceinline__ void kv_load_rows(KvWave<S, CODE, PARTS, NC>& w, cons
 // step waits for the block table or a scale.
 struct KvTiles {
     uint32_t lo, hi;   // its offset in the pool
-    float ks, lv, rv;  // key scale, log2 and inverse of the value scale
+    float ks, lv, rv;  // key scale, log2 of the value scale and KV_DOWN_F by it
     uint64_t bad;      // tiles whose value scale is NaN
 };
 
@@ -223,7 +227,7 @@ __device__ __forceinline__ KvTiles kv_tile_infos(const KvDev& c, const int* tabl
     r.bad = __ballot(vs != vs);
     const float sv = vs > 0.f ? vs : KV_ZERO;
     r.lv = log2f(sv);
-    r.rv = 1.f / sv;
+    r.rv = KV_DOWN_F / sv;
     return r;
 }
 __device__ __forceinline__ const uint8_t* kv_tile_of(const KvDev& c, const KvTiles& f, int lane) {
@@ -394,7 +398,7 @@ __device__ __forceinline__ size_t kv_head_row(const KvDev& c, const KvBatch& b, 
 // A finished row's logarithm.
 __device__ __forceinline__ void kv_finish(const KvDev& c, const KvBatch& b, const KvAttend& a, int i, int h, int row,
                                           float m, float l) {
-    const float lse2 = l == 0.f ? KV_NEG : m - KV_TOP + log2f(l);
+    const float lse2 = l == 0.f ? KV_NEG : m + (KV_DOWN - KV_TOP) + log2f(l);
     if (a.lse) a.lse[kv_row(c, b, a, i, h, row)] = lse2 * 0.69314718055994531f;
     if (a.lse2) a.lse2[kv_head_row(c, b, a, i, h, row)] = lse2;
 }
@@ -505,7 +509,7 @@ __global__ __launch_bounds__(256, S <= 4 ? 3 : 2) void kv_step_kernel(KvDev c, K
             const size_t at = kv_row(c, b, a, i, h, row);
             if (d == 0) kv_finish(c, b, a, i, h, row, mx, l);
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            kv_store4<PARTS>(a, at * c.D, d, c.D, o * inv);
+            kv_store4<PARTS>(a, at * c.D, d, c.D, o * KV_DOWN_F * inv);
         } else {
             const size_t at = (size_t)blockIdx.x * 16 + r;
             if (d == 0) a.part_ml[at] = make_float2(mx, l);
@@ -651,7 +655,7 @@ __global__ __launch_bounds__(256, S == 8 ? 1 : 2) void kv_chunk_kernel(KvDev c, 
             if (g == 0) kv_finish(c, b, a, i, h, w.row[n], w.m[n], w.l[n]);
             const float inv = w.l[n] == 0.f ? 0.f : 1.f / w.l[n];
 #pragma unroll
-            for (int j = 0; j < 2 * S; j++) kv_store4<PARTS>(a, at * c.D, 16 * j + 4 * g, c.D, w.o[n][j] * inv + w.bad[n]);
+            for (int j = 0; j < 2 * S; j++) kv_store4<PARTS>(a, at * c.D, 16 * j + 4 * g, c.D, w.o[n][j] * KV_DOWN_F * inv + w.bad[n]);
         } else {
             const size_t at = (size_t)blockIdx.x * WG_ROWS + (w.row[n] - wg_row0);
             if (g == 0) a.part_ml[at] = make_float2(w.m[n], w.l[n]);
@@ -719,7 +723,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvDev c, KvBatch b, KvAtte
     }
     if (d4 == 0) kv_finish(c, b, a, i, h, row, mx, l);
     const size_t at = kv_row(c, b, a, i, h, row) * c.D;
-    o = o * (l == 0.f ? 0.f : 1.f / l);
+    o = o * KV_DOWN_F * (l == 0.f ? 0.f : 1.f / l);
     if (a.q.type == KV_F32)
         kv_store4<2>(a, at, 4 * d4, c.D, o);
     else
