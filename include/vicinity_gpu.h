@@ -403,7 +403,7 @@ int vgpu_kv_append(vgpu_kv *h, const int32_t *seqs, const int64_t *counts, size_
  * nothing gets 0, and -inf in lse (the natural logarithm of the softmax
  * denominator).  track: weight[slot, head] = decay * weight + the sum of the
  * probabilities that the slot got from the call's tokens and the heads that share
- * it (decay 0: that sum alone). */
+ * it (decay 0: that sum alone).  A call that returns an error has changed no weight. */
 int vgpu_kv_attend(vgpu_kv *h, const int32_t *seqs, const int64_t *counts, size_t n,
                    const vgpu_kv_query *query, void *stream);
 

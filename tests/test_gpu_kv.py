@@ -802,3 +802,33 @@ def test_allocation_failure_reports_and_recovers():
         _lib.check(lib.vgpu_test_fail_device_allocations(0, 0))
     assert not cache.read(fields=("weights",))["weights"].any()
     assert torch.isfinite(cache.attend(q, decay=1.0)).all()
+
+
+def test_a_later_launch_without_memory_leaves_the_weights():
+    """130 sequences take two launches; only the second needs more workspace than there is."""
+    torch = _torch()
+    _case("allocation failure, second launch")
+    import vicinity_amd as va
+    from vicinity_amd import _lib
+
+    cache = va.KVCache(130, 2, 64, 129 + 300)
+    x = _rand((130, 2, 64), "bfloat16", 172)
+    cache.append(x, x)
+    q = _rand((130, 2, 64), "bfloat16", 173)
+    cache.attend(q, decay=1.0)
+    more = _rand((9000, 2, 64), "bfloat16", 174)
+    cache.append(more, more, seqs=[129])
+    before = cache.read(fields=("weights",))["weights"]
+    lib = _lib.load()
+    _lib.check(lib.vgpu_test_fail_device_allocations(0, 1))
+    try:
+        with pytest.raises(_lib.VicinityGpuError) as e:
+            cache.attend(q, decay=1.0)
+        assert e.value.code == _lib.ERR_OUT_OF_MEMORY
+    finally:
+        _lib.check(lib.vgpu_test_fail_device_allocations(0, 0))
+    assert torch.equal(cache.read(fields=("weights",))["weights"], before)
+    cache.attend(q, decay=1.0)
+    # every row gives its head a weight of 1 in all
+    gave = (cache.read(fields=("weights",))["weights"] - before).sum(0)
+    assert torch.allclose(gave, torch.full_like(gave, 130.0), rtol=1e-4)

@@ -472,6 +472,9 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
     for (size_t i = 0; i < n; i++) order[i] = i, tok0[i] = tok, tok += counts[i];
     if (a.by_rows)
         std::stable_sort(order.begin(), order.end(), [&](size_t x, size_t y) { return seqs[ids[x]].len < seqs[ids[y]].len; });
+    // Where several launches add weights, all of them are checked and their workspaces grown
+    // before the first, so that a call that fails has added none.
+    for (int dry = a.track && n > KV_BATCH; dry >= 0; dry--)
     for (size_t i0 = 0; i0 < n; i0 += KV_BATCH) {
         KvBatch b;
         b.n = 0;
@@ -536,7 +539,7 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
                 grow(w_qop, (size_t)row_tiles * dev.H * parts * (dev.Dp / 32) * 64);
                 a.qop = w_qop.p;
             }
-            launch_kv_attend(dev, b, a, s);
+            if (!dry) launch_kv_attend(dev, b, a, s);
         }
         if (a.track) {
             const int per = keep_scores ? KV_SCORE_SLOTS : KV_WEIGHT_SLOTS;
@@ -550,7 +553,7 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
                 grow(w_wpart, (size_t)(groups * a.chunks * KV_WEIGHT_SLOTS));
                 a.wpart = w_wpart.p;
             }
-            launch_kv_weights(dev, b, a, s);
+            if (!dry) launch_kv_weights(dev, b, a, s);
         }
     }
     VGPU_HIP(hipGetLastError());
