@@ -662,6 +662,30 @@ def test_repeated_calls_give_the_same_bits():
             assert torch.equal(pair.cache.read(fields=("weights",))["weights"], w)
 
 
+@pytest.mark.parametrize("rows", [0, 1, 70])
+def test_sequences_without_query_tokens_only_decay(rows):
+    """No token at all, one of an empty sequence, 70 of the first (a second pass over the keys,
+    and a second launch without rows)."""
+    torch = _torch()
+    _case(f"weights without tokens, {rows} rows")
+    import vicinity_amd as va
+
+    n, lens = 130, [0] + [40 + i for i in range(129)]
+    if rows > 1:
+        lens[0] = 100
+    cache = va.KVCache(n, 2, 64, 6 * n, block_tokens=32)
+    x = _rand((sum(lens), 2, 64), "bfloat16", 180)
+    w = torch.rand((sum(lens), 2), device="cuda:0")
+    cache.append(x, x, counts=lens, weights=w)
+    q = _rand((rows, 2, 64), "bfloat16", 181)
+    out = cache.attend(q, counts=[rows] + [0] * (n - 1), decay=0.5)
+    assert out.shape == q.shape and torch.isfinite(out).all()
+    got = cache.read(fields=("weights",))["weights"]
+    assert torch.equal(got[lens[0]:], 0.5 * w[lens[0]:])
+    gave = (got - 0.5 * w)[:lens[0]].sum(0)
+    assert torch.allclose(gave, torch.full_like(gave, float(rows if lens[0] else 0)), rtol=1e-4)
+
+
 # ---- refusals --------------------------------------------------------------------------
 
 

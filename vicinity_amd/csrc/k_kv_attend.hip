@@ -999,7 +999,7 @@ void launch_kv_attend(const KvDev& c, const KvBatch& b, const KvAttend& a, hipSt
 void launch_kv_weights(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s) {
     if (!b.unit0[b.n]) return;
     const dim3 grid((unsigned)b.unit0[b.n] * c.H);
-    if (a.scores) {
+    if (!a.by_rows) {  // (a.scores is null where no row has a slot: none is read then)
         hipLaunchKernelGGL(kv_score_weights_kernel, grid, dim3(256), 0, s, c, b, a);
         return;
     }
