@@ -433,8 +433,9 @@ __device__ __forceinline__ KvJob kv_job(const KvDev& c, const KvBatch& b, const 
 
 // Few rows: the four waves of a workgroup take the same 16 rows and every fourth tile,
 // joined at the end.  The next tile's keys are loaded when this one's are used up, under
-// its softmax and values, and its values under the next one's keys: one tile of registers.  Bound by the cache's bytes: a tile's 64 Dp bytes against 4 Dp / 16
-// matrix instructions of 16 cycles.
+// its softmax and values, and its values under the next one's keys: one tile of registers.
+// Bound by the cache's bytes: a tile's 64 Dp bytes against 4 Dp / 16 matrix instructions of
+// 16 cycles (61 sequences up to 8191 slots, 8 x 128: 349 MB in 69 us, 5.1 TB/s).
 // ONCE: no row tile but this one reads the tiles (64 sequences of 4096, 8 x 128, one row tile:
 // 86 us, by the caches 97; two row tiles 145 and 129).
 template <int S, int CODE, int PARTS, bool ONCE>
