@@ -427,7 +427,8 @@ int vgpu_kv_evict(vgpu_kv *h, const int32_t *seqs, const int32_t *into, size_t n
 /* The slots first[i] .. first[i]+counts[i]-1 of each sequence: k, v [tokens,
  * num_heads, head_dim] in dtype (code * scale, rounded once), positions i32 and
  * weights f32 [tokens, num_heads]; device memory, each may be NULL.  counts NULL: to
- * the end of each sequence. */
+ * the end of each sequence, for a caller whose threads do not change the lengths between
+ * the outputs' allocation and the call. */
 int vgpu_kv_read(vgpu_kv *h, const int32_t *seqs, const int64_t *first, const int64_t *counts,
                  size_t n, int dtype, void *k, void *v, int32_t *positions, float *weights,
                  void *stream);

@@ -1,0 +1,88 @@
+"""KVCache calls of several threads on one handle, against a library that keeps lengths and
+notes what it is asked to do: no GPU."""
+
+import ctypes
+import threading
+import types
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+
+class Library:
+    """Lengths, and the calls in the order in which they arrive."""
+
+    def __init__(self, lengths):
+        self.lengths = list(lengths)
+        self.calls = []
+        self.after_lengths = None  # what another thread does next
+
+    def vgpu_kv_new(self, params, out):
+        return 0
+
+    def vgpu_kv_lengths(self, h, out):
+        for i, n in enumerate(self.lengths):
+            ctypes.c_int64.from_address(out + 8 * i).value = n
+        if self.after_lengths:
+            self.after_lengths()
+        return 0
+
+    def vgpu_kv_read(self, h, ids, first, counts, n, dtype, k, v, pos, wts, stream):
+        ids = np.ctypeslib.as_array(ctypes.cast(ids, ctypes.POINTER(ctypes.c_int32)), (n,))
+        first = np.ctypeslib.as_array(ctypes.cast(first, ctypes.POINTER(ctypes.c_int64)), (n,))
+        if counts is None:  # to the end, as the library counts it
+            rows = sum(self.lengths[i] - f for i, f in zip(ids, first))
+        else:
+            rows = np.ctypeslib.as_array(ctypes.cast(counts, ctypes.POINTER(ctypes.c_int64)), (n,)).sum()
+        self.calls.append(("read", int(rows)))
+        return 0
+
+    def vgpu_kv_append(self, h, ids, counts, n, k, v, pos, wts, stream):
+        self.calls.append(("append", stream))
+        return 0
+
+
+@pytest.fixture
+def cache(monkeypatch):
+    import vicinity_amd as va
+    from vicinity_amd import _lib
+
+    lib = Library([5, 0, 7])
+    monkeypatch.setattr(_lib, "load", lambda: lib)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 0, raising=False)
+    monkeypatch.setattr(torch.cuda, "current_stream",
+                        lambda device=None: types.SimpleNamespace(cuda_stream=0, wait_stream=lambda other: None))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+
+    class On:
+        def __init__(self, stream):
+            pass
+
+        def __enter__(self):
+            return self
+
+        def __exit__(self, *exc):
+            return False
+
+    monkeypatch.setattr(torch.cuda, "stream", On)
+    c = va.KVCache(3, 2, 4, 16)
+    c.device = torch.device("cpu")
+    return c, lib
+
+
+@pytest.mark.parametrize("seqs,first", [(None, None), ([2, 0], [3, 1]), ([0], 2)])
+@pytest.mark.parametrize("change", [+3, -2])
+def test_read_to_the_end_writes_as_many_rows_as_it_allocated(cache, seqs, first, change):
+    """Another thread appends to, or truncates, sequence 0 once the tensors' size is known."""
+    c, lib = cache
+
+    def other():
+        lib.after_lengths = None
+        lib.lengths[0] += change
+
+    lib.after_lengths = other
+    got = c.read(seqs=seqs, first=first)
+    assert lib.calls == [("read", got["k"].shape[0])]

@@ -223,13 +223,12 @@ class KVCache:
                 raise ValueError(f"fields must be among {FIELDS}")
         ids = self._seqs(seqs)
         at = self._ints(0 if first is None else first, len(ids), "first")
-        if counts is None:  # to the end; the library refuses a first beyond it
-            lens, n = self._lengths(), None
-            tokens = sum(lens) if ids is self._all else sum([lens[i] for i in ids])
-            tokens = max(tokens - sum(at), 0)
+        if counts is None:  # to the end as it is now; the library checks what the tensors were sized by
+            lens = self._lengths()
+            n = array("q", [lens[i] - max(f, 0) for i, f in zip(ids, at)])
         else:
             n = self._ints(counts, len(ids), "counts")
-            tokens = max(sum(n), 0)
+        tokens = max(sum(n), 0)
         s, ctx = self._stream(stream, ())
         types = {"positions": torch.int32, "weights": torch.float32}
         res = {}
@@ -238,8 +237,8 @@ class KVCache:
                 shape = (tokens, self.num_heads) + ((self.head_dim,) if f in "kv" else ())
                 res[f] = torch.empty(shape, dtype=types.get(f, dtype), device=self.device)
         ptr = [res[f].data_ptr() if f in res else None for f in FIELDS]
-        _lib.check(self._L.vgpu_kv_read(self._h, _ptr(ids), _ptr(at), None if n is None else _ptr(n),
-                                        len(ids), self._types[dtype], *ptr, s))
+        _lib.check(self._L.vgpu_kv_read(self._h, _ptr(ids), _ptr(at), _ptr(n), len(ids),
+                                        self._types[dtype], *ptr, s))
         return res
 
     # ---- arguments ------------------------------------------------------------
