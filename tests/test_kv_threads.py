@@ -17,6 +17,7 @@ class Library:
     def __init__(self, lengths):
         self.lengths = list(lengths)
         self.calls = []
+        self.streams = []  # ("call", stream) and ("wait", stream, for that one)
         self.after_lengths = None  # what another thread does next
 
     def vgpu_kv_new(self, params, out):
@@ -37,10 +38,7 @@ class Library:
         else:
             rows = np.ctypeslib.as_array(ctypes.cast(counts, ctypes.POINTER(ctypes.c_int64)), (n,)).sum()
         self.calls.append(("read", int(rows)))
-        return 0
-
-    def vgpu_kv_append(self, h, ids, counts, n, k, v, pos, wts, stream):
-        self.calls.append(("append", stream))
+        self.streams.append(("call", stream or 0))
         return 0
 
 
@@ -86,3 +84,32 @@ def test_read_to_the_end_writes_as_many_rows_as_it_allocated(cache, seqs, first,
     lib.after_lengths = other
     got = c.read(seqs=seqs, first=first)
     assert lib.calls == [("read", got["k"].shape[0])]
+
+
+class Stream:
+    def __init__(self, lib, number, hold=None):
+        self.lib, self.cuda_stream, self.hold = lib, number, hold
+
+    def wait_stream(self, other):
+        if self.hold:
+            self.hold()
+        self.lib.streams.append(("wait", self.cuda_stream, other.cuda_stream))
+
+
+def test_calls_of_two_threads_on_two_streams_follow_one_another(cache):
+    """While the first thread's stream is put behind the last call, a second thread calls: what
+    each thread queues must lie behind what the library was given before it."""
+    c, lib = cache
+    c.read()
+    second = threading.Thread(target=lambda: c.read(stream=Stream(lib, 2)))
+
+    def hold():
+        second.start()
+        second.join(0.5)  # time enough to get past the first thread, if nothing keeps it
+
+    c.read(stream=Stream(lib, 1, hold))
+    second.join()
+    calls = [i for i, e in enumerate(lib.streams) if e[0] == "call"]
+    assert sorted(lib.streams[i][1] for i in calls) == [0, 1, 2]
+    for a, b in zip(calls, calls[1:]):
+        assert ("wait", lib.streams[b][1], lib.streams[a][1]) in lib.streams[a:b], lib.streams

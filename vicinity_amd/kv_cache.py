@@ -15,6 +15,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import math
+import threading
 from array import array
 
 import numpy as np
@@ -72,6 +73,9 @@ class KVCache:
         self.device = torch.device("cuda", torch.cuda.current_device())
         self._types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
         self._all = array("i", range(num_seqs))
+        # Held while a call reads the lengths, goes behind the last one's stream and queues its
+        # work, so that two threads' calls reach the GPU in the order of their waits.
+        self._turn = threading.Lock()
         self._last = None      # the stream of the last call, and its handle
         self._last_raw = None
 
@@ -97,7 +101,8 @@ class KVCache:
         """Forget each sequence's slots from lengths[i] on; 0 empties it."""
         ids = self._seqs(seqs)
         lens = self._ints(lengths, len(ids), "lengths")
-        _lib.check(self._L.vgpu_kv_truncate(self._h, _ptr(ids), _ptr(lens), len(ids)))
+        with self._turn:
+            _lib.check(self._L.vgpu_kv_truncate(self._h, _ptr(ids), _ptr(lens), len(ids)))
 
     # ---- operators ----------------------------------------------------------
     def append(self, k, v, seqs=None, counts=None, positions=None, weights=None,
@@ -117,9 +122,10 @@ class KVCache:
         n = self._counts(counts, len(ids), k.shape[0])
         pos = self._side(positions, "positions", k.shape[0], "int32")
         wts = self._side(weights, "weights", k.shape[0], "float32")
-        s, _ = self._stream(stream, (k, v, positions, weights))
-        _lib.check(self._L.vgpu_kv_append(self._h, _ptr(ids), _ptr(n), len(ids),
-                                          ctypes.byref(kt), ctypes.byref(vt), pos, wts, s))
+        with self._turn:
+            s, _ = self._stream(stream, (k, v, positions, weights))
+            _lib.check(self._L.vgpu_kv_append(self._h, _ptr(ids), _ptr(n), len(ids),
+                                              ctypes.byref(kt), ctypes.byref(vt), pos, wts, s))
 
     def attend(self, q, seqs=None, counts=None, scale: float | None = None, causal: bool = True,
                window: int = 0, mask=None, decay: float | None = None, out=None,
@@ -154,21 +160,22 @@ class KVCache:
                     or mask.shape[0] != tokens or mask.device != self.device:
                 raise ValueError("mask must be a bool or uint8 tensor [tokens, slots] on the "
                                  "cache's GPU")
-        s, ctx = self._stream(stream, (q, mask, out))
-        with ctx:
-            if out is None:
-                out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) \
-                if return_lse else None
-        query = _lib.KvQuery(
-            qt, heads, 1.0 / math.sqrt(self.head_dim) if scale is None else scale, int(causal),
-            int(window), mask.data_ptr() if mask is not None else None,
-            mask.stride(0) if mask is not None else 0, mask.stride(1) if mask is not None else 0,
-            mask.shape[1] if mask is not None else 0, int(decay is not None),
-            0.0 if decay is None else decay, out.data_ptr(),
-            lse.data_ptr() if lse is not None else None)
-        _lib.check(self._L.vgpu_kv_attend(self._h, _ptr(ids), _ptr(n), len(ids),
-                                          ctypes.byref(query), s))
+        with self._turn:
+            s, ctx = self._stream(stream, (q, mask, out))
+            with ctx:
+                if out is None:
+                    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+                lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) \
+                    if return_lse else None
+            query = _lib.KvQuery(
+                qt, heads, 1.0 / math.sqrt(self.head_dim) if scale is None else scale, int(causal),
+                int(window), mask.data_ptr() if mask is not None else None,
+                mask.stride(0) if mask is not None else 0, mask.stride(1) if mask is not None else 0,
+                mask.shape[1] if mask is not None else 0, int(decay is not None),
+                0.0 if decay is None else decay, out.data_ptr(),
+                lse.data_ptr() if lse is not None else None)
+            _lib.check(self._L.vgpu_kv_attend(self._h, _ptr(ids), _ptr(n), len(ids),
+                                              ctypes.byref(query), s))
         return (out, lse) if return_lse else out
 
     def evict(self, budget: int, recent: int = 0, seqs=None, into=None, dropped: bool = False,
@@ -190,21 +197,22 @@ class KVCache:
         for name, value in (("budget", budget), ("recent", recent)):
             if not isinstance(value, (int, np.integer)) or value < 0:
                 raise ValueError(f"{name} must be an int, 0 or more")
-        s, ctx = self._stream(stream, ())
-        gone, most = None, 0
-        if dropped:
-            lens = self._lengths()
-            most = max(max((lens[i] for i in ids), default=0) - int(budget), 0)
-            shape = (len(ids), most, self.num_heads)
-            with ctx:
-                gone = {"positions": torch.empty(shape, dtype=torch.int32, device=self.device),
-                        "k": torch.empty(shape + (self.head_dim,), device=self.device,
-                                         dtype=torch.float32)}
-                gone["v"] = torch.empty_like(gone["k"])
-        ptr = [gone[f].data_ptr() if gone and most else None for f in ("positions", "k", "v")]
-        _lib.check(self._L.vgpu_kv_evict(self._h, _ptr(ids),
-                                         None if to is None else _ptr(to), len(ids), budget,
-                                         recent, most, *ptr, s))
+        with self._turn:
+            s, ctx = self._stream(stream, ())
+            gone, most = None, 0
+            if dropped:
+                lens = self._lengths()
+                most = max(max((lens[i] for i in ids), default=0) - int(budget), 0)
+                shape = (len(ids), most, self.num_heads)
+                with ctx:
+                    gone = {"positions": torch.empty(shape, dtype=torch.int32, device=self.device),
+                            "k": torch.empty(shape + (self.head_dim,), device=self.device,
+                                             dtype=torch.float32)}
+                    gone["v"] = torch.empty_like(gone["k"])
+            ptr = [gone[f].data_ptr() if gone and most else None for f in ("positions", "k", "v")]
+            _lib.check(self._L.vgpu_kv_evict(self._h, _ptr(ids),
+                                             None if to is None else _ptr(to), len(ids), budget,
+                                             recent, most, *ptr, s))
         return gone
 
     def read(self, seqs=None, first=None, counts=None, fields=FIELDS, dtype=None,
@@ -223,22 +231,23 @@ class KVCache:
                 raise ValueError(f"fields must be among {FIELDS}")
         ids = self._seqs(seqs)
         at = self._ints(0 if first is None else first, len(ids), "first")
-        if counts is None:  # to the end as it is now; the library checks what the tensors were sized by
-            lens = self._lengths()
-            n = array("q", [lens[i] - max(f, 0) for i, f in zip(ids, at)])
-        else:
-            n = self._ints(counts, len(ids), "counts")
-        tokens = max(sum(n), 0)
-        s, ctx = self._stream(stream, ())
-        types = {"positions": torch.int32, "weights": torch.float32}
-        res = {}
-        with ctx:
-            for f in fields:
-                shape = (tokens, self.num_heads) + ((self.head_dim,) if f in "kv" else ())
-                res[f] = torch.empty(shape, dtype=types.get(f, dtype), device=self.device)
-        ptr = [res[f].data_ptr() if f in res else None for f in FIELDS]
-        _lib.check(self._L.vgpu_kv_read(self._h, _ptr(ids), _ptr(at), _ptr(n), len(ids),
-                                        self._types[dtype], *ptr, s))
+        with self._turn:
+            if counts is None:  # to the end; the library checks what the tensors were sized by
+                lens = self._lengths()
+                n = array("q", [lens[i] - max(f, 0) for i, f in zip(ids, at)])
+            else:
+                n = self._ints(counts, len(ids), "counts")
+            tokens = max(sum(n), 0)
+            s, ctx = self._stream(stream, ())
+            types = {"positions": torch.int32, "weights": torch.float32}
+            res = {}
+            with ctx:
+                for f in fields:
+                    shape = (tokens, self.num_heads) + ((self.head_dim,) if f in "kv" else ())
+                    res[f] = torch.empty(shape, dtype=types.get(f, dtype), device=self.device)
+            ptr = [res[f].data_ptr() if f in res else None for f in FIELDS]
+            _lib.check(self._L.vgpu_kv_read(self._h, _ptr(ids), _ptr(at), _ptr(n), len(ids),
+                                            self._types[dtype], *ptr, s))
         return res
 
     # ---- arguments ------------------------------------------------------------
