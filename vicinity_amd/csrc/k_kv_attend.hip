@@ -2,9 +2,11 @@
 //
 // For a row r (a query token and head) and slot j:  u_j = scale * log2(e) * q_r.k_j,
 // o = sum 2^(u_j) v_j / sum 2^(u_j).  One pass over the tiles with a running
-// reference m: the value scale s_b of a block goes into the exponent,
-// p_j = 2^(u_j + log2 s_b - m), so o's accumulators add p_j * code directly in the
-// matrix instruction and the denominator adds 2^-8 p_j / s_b.
+// reference m: the value scale s_b = 2^E t_b of a block goes into the exponent,
+// p_j = 2^(u_j + log2 t_b - m), so o's accumulators add p_j * code directly in the
+// matrix instruction and the denominator adds p_j / t_b.  E is a power that the
+// scales of the tiles at hand lie near, so the sums stay in float32's range for
+// scales of any size; the result is 2^E o / l.
 //
 // Products: codes are integers up to 127 or e4m3 numbers, both exact in half
 // precision.  A query row is scaled by a power of two to a largest element of 2^14
@@ -30,15 +32,14 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float KV_TOP = 6.f;    // p of the reference is 2^KV_TOP
 constexpr float KV_SLACK = 8.f;  // and may grow to 2^(KV_TOP + KV_SLACK)
-// The denominators hold 2^-KV_DOWN of their sums: scales lie between 2^-109 and 2^121, and of
-// the smallest 10^4 slots' sum passed the largest float.
-constexpr float KV_DOWN = 8.f;
-constexpr float KV_DOWN_F = 0x1p-8f;
-// A value scale of 0 stands for codes of 0, so any number does in its place: a small one,
-// for the reference must not follow slots that add nothing (with 1 the halves of p lost
-// values below 2^-20 beside them), but one whose p, 2^-40 of that beside values near 1,
-// still counts in the denominators.
-constexpr float KV_ZERO = 0x1p-40f;
+// t_b of a scale far below the others, or of 0.  A scale of 0 stands for codes of 0, so any
+// number does in its place: m must not follow slots that add nothing (values down to 2^-80 of
+// the others keep their bits beside them), but their p has to count in the denominators (with
+// m from a t of 1 it is lost where u lies 2^-46 below).  Codes of a scale not 0 that is below
+// come out as if it were 2^-80 of the others.
+constexpr float KV_LEAST = 0x1p-80f;
+constexpr int KV_NEAR = 8;         // t_b stays below 2^KV_NEAR
+constexpr int KV_NONE = -(1 << 20);  // E before a scale above 0 was seen
 #define KV_NEG (-__builtin_huge_valf())
 
 // Two halves of 8 codes.
@@ -162,6 +163,7 @@ struct KvWave {
     int lo[NC], hi[NC];    // slots that the row sees
     int row[NC];
     float m[NC], l[NC], bad[NC];
+    int e = KV_NONE;       // E, the same in every lane
     floatx4 o[NC][2 * S];
 };
 
@@ -209,7 +211,8 @@ __device__ __forceinline__ void kv_load_rows(KvWave<S, CODE, PARTS, NC>& w, cons
 // step waits for the block table or a scale.
 struct KvTiles {
     uint32_t lo, hi;   // its offset in the pool
-    float ks, lv, rv;  // key scale, log2 of the value scale and KV_DOWN_F by it
+    float ks, vs;      // key and value scale
+    float lv, rv;      // log2 t and 1 / t of the value scale (kv_measure)
     uint64_t bad;      // tiles whose value scale is NaN
 };
 
@@ -223,11 +226,9 @@ __device__ __forceinline__ KvTiles kv_tile_infos(const KvDev& c, const int* tabl
     const size_t at = kv_tile_offset(c, block, h, t & (c.B / KV_TILE - 1));
     r.lo = (uint32_t)at, r.hi = (uint32_t)(at >> 32);
     r.ks = in ? c.kscale[part] : 0.f;
-    const float vs = in ? c.vscale[part] : 1.f;
-    r.bad = __ballot(vs != vs);
-    const float sv = vs > 0.f ? vs : KV_ZERO;
-    r.lv = log2f(sv);
-    r.rv = KV_DOWN_F / sv;
+    r.vs = in ? c.vscale[part] : 0.f;
+    r.lv = r.rv = 0.f;
+    r.bad = __ballot(r.vs != r.vs);
     return r;
 }
 __device__ __forceinline__ const uint8_t* kv_tile_of(const KvDev& c, const KvTiles& f, int lane) {
@@ -238,6 +239,37 @@ __device__ __forceinline__ const uint8_t* kv_tile_of(const KvDev& c, const KvTil
 __device__ __forceinline__ float kv_lane(float v, int lane) {
     return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), lane));
 }
+
+// lv and rv of 64 tiles, before the first of them.  E is the first scale's power, and moves up
+// to the largest's where one passes it by 2^KV_NEAR: then m and l take the difference, as far
+// as l stays below 2^90, and o's accumulators the rest.
+template <int S, int CODE, int PARTS, int NC>
+__device__ __forceinline__ void kv_measure(KvWave<S, CODE, PARTS, NC>& w, KvTiles& f) {
+    const bool some = f.vs > 0.f;
+    int e = some ? __builtin_amdgcn_frexp_expf(f.vs) : KV_NONE;
+    const uint64_t any = __ballot(some);
+    if (w.e == KV_NONE && any) w.e = __builtin_amdgcn_readlane(e, __builtin_ctzll(any));
+    if (__any(e > w.e + KV_NEAR)) {
+#pragma unroll
+        for (int o = 32; o; o >>= 1) e = max(e, __shfl_xor(e, o));
+        e = __builtin_amdgcn_readfirstlane(e);
+        const int up = e - w.e;
+        w.e = e;
+#pragma unroll
+        for (int n = 0; n < NC; n++) {
+            const int by = max(min(up, 90 - __builtin_amdgcn_frexp_expf(kv_max4(w.l[n]))), 0);
+            w.m[n] -= (float)by;
+            w.l[n] = ldexpf(w.l[n], by);
+            const float f1 = ldexpf(1.f, by - up);
+#pragma unroll
+            for (int j = 0; j < 2 * S; j++) w.o[n][j] *= f1;
+        }
+    }
+    const float t = some ? fmaxf(ldexpf(f.vs, -w.e), KV_LEAST) : KV_LEAST;
+    f.lv = __builtin_amdgcn_logf(t);  // (one unit in the last place each; t is a normal number)
+    f.rv = __builtin_amdgcn_rcpf(t);
+}
+__device__ __forceinline__ int kv_power(int e) { return e == KV_NONE ? 0 : e; }
 
 // Largest of 8, a NaN only if all are (fmaxf would quiet each operand first).
 __device__ __forceinline__ float kv_max8(const float (&x)[8]) {
@@ -381,8 +413,9 @@ __device__ __forceinline__ void kv_fetch(uint4 (&k)[S], const uint8_t* half) {
     for (int s = 0; s < S; s++) k[s] = __builtin_bit_cast(uint4, ONCE ? __builtin_nontemporal_load(p + s * 64) : p[s * 64]);
 }
 
-// What a part with reference m and sum l is multiplied with under reference mx.  A part
-// without a score has m -inf and l 0, or l NaN where its scores were NaN.
+// What a part's sum l is multiplied with under reference mx, m being its own; its o goes by
+// 2^(its E less the largest) too.  A part without a score has m -inf and l 0, or l NaN where
+// its scores were NaN.
 __device__ __forceinline__ float kv_join_factor(float m, float l, float mx) {
     return m == KV_NEG ? 0.f * l : exp2f(m - mx);
 }
@@ -398,7 +431,7 @@ __device__ __forceinline__ size_t kv_head_row(const KvDev& c, const KvBatch& b, 
 // A finished row's logarithm.
 __device__ __forceinline__ void kv_finish(const KvDev& c, const KvBatch& b, const KvAttend& a, int i, int h, int row,
                                           float m, float l) {
-    const float lse2 = l == 0.f ? KV_NEG : m + (KV_DOWN - KV_TOP) + log2f(l);
+    const float lse2 = l == 0.f ? KV_NEG : m - KV_TOP + log2f(l);
     if (a.lse) a.lse[kv_row(c, b, a, i, h, row)] = lse2 * 0.69314718055994531f;
     if (a.lse2) a.lse2[kv_head_row(c, b, a, i, h, row)] = lse2;
 }
@@ -441,6 +474,7 @@ __device__ __forceinline__ KvJob kv_job(const KvDev& c, const KvBatch& b, const 
 template <int S, int CODE, int PARTS, bool ONCE>
 __global__ __launch_bounds__(256, S <= 4 ? 3 : 2) void kv_step_kernel(KvDev c, KvBatch b, KvAttend a) {
     extern __shared__ __align__(16) float lds[];
+    __shared__ int powers[4];  // E of the waves
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
     const KvJob sp = kv_job(c, b, a, 16);
@@ -465,6 +499,7 @@ __global__ __launch_bounds__(256, S <= 4 ? 3 : 2) void kv_step_kernel(KvDev c, K
     kv_load_rows(w, c, b, a, i, h, row0);
     for (int x = 0; x < n; x++) {
         const int t = tw + 4 * x, y = x & 63;
+        if (y == 0) kv_measure(w, info);
         const float ks = kv_lane(info.ks, y), lv = kv_lane(info.lv, y), rv = kv_lane(info.rv, y);
         const bool bad = info.bad >> y & 1;
         if (y == 63 && x + 1 < n) info = kv_tile_infos(c, table, h, t + 4, 4, sp.t1);
@@ -489,7 +524,9 @@ __global__ __launch_bounds__(256, S <= 4 ? 3 : 2) void kv_step_kernel(KvDev c, K
 #pragma unroll
     for (int j = 0; j < 2 * S; j++) *(floatx4*)(lds + r4 * LDO + 16 * j + 4 * g) = w.o[0][j] + w.bad[0];
     if (g == 0) ml[2 * r4] = w.m[0], ml[2 * r4 + 1] = w.l[0];
+    if (lane == 0) powers[wave] = w.e;
     __syncthreads();
+    const int e = max(max(powers[0], powers[1]), max(powers[2], powers[3]));
     for (int u = threadIdx.x; u < 16 * 8 * S; u += 256) {
         const int r = u / (8 * S), d = u % (8 * S) * 4;
         const int row = row0 + r;
@@ -504,16 +541,17 @@ __global__ __launch_bounds__(256, S <= 4 ? 3 : 2) void kv_step_kernel(KvDev c, K
             const int rr = x * 16 + r;
             const float f = kv_join_factor(ml[2 * rr], ml[2 * rr + 1], mx);
             l += f * ml[2 * rr + 1];
-            o += *(const floatx4*)(lds + rr * LDO + d) * f;
+            o += *(const floatx4*)(lds + rr * LDO + d) * ldexpf(f, powers[x] - e);
         }
         if (sp.whole) {
             const size_t at = kv_row(c, b, a, i, h, row);
             if (d == 0) kv_finish(c, b, a, i, h, row, mx, l);
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            kv_store4<PARTS>(a, at * c.D, d, c.D, o * KV_DOWN_F * inv);
+            kv_store4<PARTS>(a, at * c.D, d, c.D, o * inv * ldexpf(1.f, kv_power(e)));
         } else {
             const size_t at = (size_t)blockIdx.x * 16 + r;
             if (d == 0) a.part_ml[at] = make_float2(mx, l);
+            if (u == 0) a.part_e[blockIdx.x] = e;
             *(floatx4*)(a.part_o + at * (32 * S) + d) = o;
         }
     }
@@ -610,7 +648,10 @@ __global__ __launch_bounds__(256, S == 8 ? 1 : 2) void kv_chunk_kernel(KvDev c, 
     int b0 = 0, b1 = 1, b2 = 2;  // buffers of tiles t, t + 1, t + 2
     for (int xt = 0; xt < n_tiles; xt++) {
         const int t = sp.t0 + xt, y = xt & 63;
-        if (y == 0 && xt > 0) info = ahead;
+        if (y == 0) {
+            if (xt > 0) info = ahead;
+            kv_measure(w, info);
+        }
         const bool inside = t * KV_TILE >= all_lo && (t + 1) * KV_TILE <= all_hi && !a.mask;
         const float rv = kv_lane(info.rv, y);
         float z[NC][8];
@@ -654,12 +695,13 @@ __global__ __launch_bounds__(256, S == 8 ? 1 : 2) void kv_chunk_kernel(KvDev c, 
         if (sp.whole) {
             const size_t at = kv_row(c, b, a, i, h, w.row[n]);
             if (g == 0) kv_finish(c, b, a, i, h, w.row[n], w.m[n], w.l[n]);
-            const float inv = w.l[n] == 0.f ? 0.f : 1.f / w.l[n];
+            const float inv = w.l[n] == 0.f ? 0.f : 1.f / w.l[n], power = ldexpf(1.f, kv_power(w.e));
 #pragma unroll
-            for (int j = 0; j < 2 * S; j++) kv_store4<PARTS>(a, at * c.D, 16 * j + 4 * g, c.D, w.o[n][j] * KV_DOWN_F * inv + w.bad[n]);
+            for (int j = 0; j < 2 * S; j++) kv_store4<PARTS>(a, at * c.D, 16 * j + 4 * g, c.D, w.o[n][j] * inv * power + w.bad[n]);
         } else {
             const size_t at = (size_t)blockIdx.x * WG_ROWS + (w.row[n] - wg_row0);
             if (g == 0) a.part_ml[at] = make_float2(w.m[n], w.l[n]);
+            if (w.row[n] == wg_row0 && g == 0) a.part_e[blockIdx.x] = w.e;  // the four waves': they have the same tiles
 #pragma unroll
             for (int j = 0; j < 2 * S; j++) *(floatx4*)(a.part_o + at * (32 * S) + 16 * j + 4 * g) = w.o[n][j] + w.bad[n];
         }
@@ -690,15 +732,19 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvDev c, KvBatch b, KvAtte
     if (splits <= 1) return;  // the one workgroup has written the rows
     if (WIDE ? row >= rows : (grp >= groups || r >= wg_rows || row >= rows)) return;
     const int row_tiles = b.unit0[i + 1] - b.unit0[i];
-    const int64_t stride = -(int64_t)row_tiles * c.H * wg_rows;  // the first split's parts lie last
-    const int64_t base = ((int64_t)(b.aux[i] + u + (b.splits[i] - 1) * row_tiles) * c.H + h) * wg_rows + r;
+    const int wg_stride = -row_tiles * c.H, wg = (b.aux[i] + u + (b.splits[i] - 1) * row_tiles) * c.H + h;
+    const int64_t stride = (int64_t)wg_stride * wg_rows;  // the first split's parts lie last
+    const int64_t base = (int64_t)wg * wg_rows + r;
     float mx = KV_NEG;
+    int e = KV_NONE;
     if (WIDE) {
-        for (int s = tid & 63; s < splits; s += 64) mx = fmaxf(mx, a.part_ml[base + s * stride].x);
+        for (int s = tid & 63; s < splits; s += 64)
+            mx = fmaxf(mx, a.part_ml[base + s * stride].x), e = max(e, a.part_e[wg + s * wg_stride]);
 #pragma unroll
-        for (int x = 32; x; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
+        for (int x = 32; x; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x)), e = max(e, __shfl_xor(e, x));
     } else {
-        for (int s = 0; s < splits; s++) mx = fmaxf(mx, a.part_ml[base + s * stride].x);
+        for (int s = 0; s < splits; s++)
+            mx = fmaxf(mx, a.part_ml[base + s * stride].x), e = max(e, a.part_e[wg + s * wg_stride]);
     }
     floatx4 o = {0.f, 0.f, 0.f, 0.f};
     float l = 0.f;
@@ -708,7 +754,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvDev c, KvBatch b, KvAtte
             const float2 ml = a.part_ml[base + s * stride];
             const float f = kv_join_factor(ml.x, ml.y, mx);
             l += f * ml.y;
-            o += *(const floatx4*)(a.part_o + (base + s * stride) * c.Dp + d4 * 4) * f;
+            o += *(const floatx4*)(a.part_o + (base + s * stride) * c.Dp + d4 * 4) * ldexpf(f, a.part_e[wg + s * wg_stride] - e);
         }
     }
     if (WIDE) {
@@ -724,7 +770,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvDev c, KvBatch b, KvAtte
     }
     if (d4 == 0) kv_finish(c, b, a, i, h, row, mx, l);
     const size_t at = kv_row(c, b, a, i, h, row) * c.D;
-    o = o * KV_DOWN_F * (l == 0.f ? 0.f : 1.f / l);
+    o = o * (l == 0.f ? 0.f : 1.f / l) * ldexpf(1.f, kv_power(e));
     if (a.q.type == KV_F32)
         kv_store4<2>(a, at, 4 * d4, c.D, o);
     else

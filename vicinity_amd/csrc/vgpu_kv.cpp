@@ -100,7 +100,7 @@ KvCache::~KvCache() {
 size_t KvCache::device_bytes() const {
     return pool.bytes() + kscale.bytes() + vscale.bytes() + weights.bytes() + positions.bytes() + table.bytes() +
            table2.bytes() + w_kept.bytes() + w_gone.bytes() + w_part.bytes() + w_scores.bytes() + w_lse2.bytes() +
-           w_ml.bytes() + w_hist.bytes() + w_counts.bytes() + w_qop.bytes() + w_qs.bytes() + w_wpart.bytes();
+           w_ml.bytes() + w_power.bytes() + w_hist.bytes() + w_counts.bytes() + w_qop.bytes() + w_qs.bytes() + w_wpart.bytes();
 }
 
 void KvCache::check_call(hipStream_t s) {
@@ -525,11 +525,12 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
                 }
                 if (one || ((a.by_rows || groups <= target + target / 8) && groups <= part_units)) break;
             }
-            a.part_o = nullptr, a.part_ml = nullptr, a.scores = nullptr;
+            a.part_o = nullptr, a.part_ml = nullptr, a.part_e = nullptr, a.scores = nullptr;
             if (split_units) {
                 grow(w_part, (size_t)(groups * rows) * dev.Dp);
                 grow(w_ml, (size_t)(groups * rows));
-                a.part_o = w_part.p, a.part_ml = w_ml.p;
+                grow(w_power, (size_t)groups);
+                a.part_o = w_part.p, a.part_ml = w_ml.p, a.part_e = w_power.p;
             }
             if (keep_scores) {
                 grow(w_scores, (size_t)score_tiles * KV_TILE * dev.H);
