@@ -448,6 +448,10 @@ int vgpu_test_host_lists(const uint32_t *assign, size_t n, size_t L, uint64_t *o
  * label >= k is VGPU_ERR_DEVICE. */
 int vgpu_test_host_centroid_update(const float *x, size_t n, size_t d, const uint32_t *assign,
                                    size_t k, float *centroids);
+/* How attention of few rows splits a batch of at most 128 sequences over workgroups (causal,
+ * no window): splits i32[n], and the 32-slot tiles of one, i32[n]. */
+int vgpu_test_host_kv_splits(const int64_t *lens, const int64_t *counts, size_t n, size_t heads,
+                             size_t group, int32_t *splits, int32_t *tiles);
 /* The OPQ polar factor U V^T of M f32[d*d] (compute_optimal_rotation,
  * opq.rs:280-294) into R f32[d*d]. */
 int vgpu_test_polar_factor(const float *m, size_t d, float *r);

@@ -180,6 +180,7 @@ SIGNATURES = {
     "vgpu_kv_evict": (_i, [_H, _vp, _vp, _sz, _sz, _sz, _sz, _vp, _vp, _vp, _vp]),
     "vgpu_kv_read": (_i, [_H, _vp, _vp, _vp, _sz, _i, _vp, _vp, _vp, _vp, _vp]),
     "vgpu_kv_truncate": (_i, [_H, _vp, _vp, _sz]),
+    "vgpu_test_host_kv_splits": (_i, [_vp, _vp, _sz, _sz, _sz, _vp, _vp]),
     "vgpu_test_host_lists": (_i, [_vp, _sz, _sz, _vp, _vp]),
     "vgpu_test_host_centroid_update": (_i, [_vp, _sz, _sz, _vp, _sz, _vp]),
     "vgpu_test_polar_factor": (_i, [_vp, _sz, _vp]),

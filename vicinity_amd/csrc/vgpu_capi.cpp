@@ -615,6 +615,16 @@ int vgpu_kv_truncate(vgpu_kv* h, const int32_t* seqs, const int64_t* lengths, si
 
 /* ---- per-kernel test entry points ---------------------------------------- */
 
+int vgpu_test_host_kv_splits(const int64_t* lens, const int64_t* counts, size_t n, size_t heads, size_t group,
+                             int32_t* splits, int32_t* tiles) {
+    return guard([&] {
+        need(lens && counts && splits && tiles, VGPU_ERR_INVALID_PARAMETER, "null argument");
+        need(n <= (size_t)vgpu::KV_BATCH && heads > 0 && heads <= 4096 && group > 0 && group <= 65536,
+             VGPU_ERR_INVALID_PARAMETER, "n, heads or group out of range");
+        vgpu::kv_plan_steps(lens, counts, (int)n, (int)heads, (int)group, splits, tiles);
+    });
+}
+
 int vgpu_test_host_lists(const uint32_t* assign, size_t n, size_t L, uint64_t* offsets, uint32_t* list_ids) {
     return guard([&] {
         need((n == 0 || (assign && list_ids)) && offsets && L, VGPU_ERR_INVALID_PARAMETER, "bad argument");

@@ -20,8 +20,8 @@ namespace {
 
 size_t item_size(int type) { return type == KV_F32 ? 4 : 2; }
 
-// Workgroups that a step is cut into: three for each of the 256 compute units, so
-// that sequences of different lengths even out.
+// Workgroups that a step is cut into where one round suffices: three for each of the 256
+// compute units.
 constexpr int64_t kStepWorkgroups = 768;
 // Workgroups of a call with many rows, two to a compute unit: with fewer, the tiles are
 // split too, which costs a partial result for every row and split.
@@ -43,6 +43,63 @@ constexpr int64_t kScoreRows = 48;
 // 256 rows: 29 and 16 us).
 constexpr int64_t kChunkTiles = 4096;
 
+// The row tiles of one launch's sequences, and the tiles that each goes over.
+struct KvPlan {
+    int n = 0, heads = 1;
+    int64_t tiles[KV_BATCH], row_units[KV_BATCH];
+    int64_t units = 0, work = 0;           // row tiles of all heads; their tiles
+    int64_t groups = 0, split_units = 0;   // workgroups; those that leave partial results
+
+    // A sequence of len slots whose last `count` tokens have G rows each, `rows` to a workgroup.
+    void add(int64_t len, int64_t count, int64_t G, int64_t rows, bool causal, int64_t window) {
+        row_units[n] = (count * G + rows - 1) / rows;
+        units += row_units[n] * heads;
+        tiles[n] = (len + KV_TILE - 1) / KV_TILE;
+        if (window && causal) tiles[n] = std::min(tiles[n], (window + rows / G + 2 * KV_TILE) / KV_TILE + 1);
+        // (the first tokens of a chunk see less than the last)
+        const int64_t seen = causal && !window ? std::max<int64_t>(2 * len - count, 0) : 2 * KV_TILE * tiles[n];
+        work += row_units[n] * heads * ((seen + 2 * KV_TILE - 1) / (2 * KV_TILE));
+        n++;
+    }
+
+    // Splits of at most `each` tiles: b's splits, per and unit0.  True if none is split.
+    bool cut(KvBatch& b, int64_t each) {
+        groups = split_units = 0;
+        bool one = true;
+        b.unit0[0] = 0;
+        for (int j = 0; j < n; j++) {
+            const int64_t splits = std::max<int64_t>((tiles[j] + each - 1) / each, 1);
+            b.splits[j] = (int)splits;
+            b.per[j] = (int)std::max<int64_t>((tiles[j] + splits - 1) / splits, 1);
+            b.unit0[j + 1] = b.unit0[j] + (int)(row_units[j] * splits);
+            groups += row_units[j] * splits * heads;
+            one = one && splits == 1;
+            if (splits > 1) split_units += row_units[j] * splits * heads;
+        }
+        return one;
+    }
+
+    // As few tiles to a workgroup as keep all of them on the card at once; at most
+    // part_units workgroups have room for partial results.
+    void split(KvBatch& b, bool by_rows, int64_t part_units) {
+        const int64_t target = by_rows ? kChunkWorkgroups : kStepWorkgroups;
+        const int64_t share = std::max<int64_t>((work + target - 1) / target, by_rows ? 16 : 8);
+        if (by_rows) {
+            // whole unless that would leave one workgroup at work alone
+            for (int64_t each = units >= 4 * target ? INT_MAX : share;; each += each / 8 + 1)
+                if (cut(b, each + each / 4) || groups <= part_units) return;
+        }
+        for (int64_t each = share; each <= 2 * share; each += each / 8 + 1)
+            if (cut(b, each) || groups <= std::min(target + target / 8, part_units)) return;
+        // Many row tiles, or a few sequences far above the others, do not go in one round: no
+        // workgroup takes more than its share of the work, in several (8 x 128; one sequence of
+        // 131072 among 127 of 100: 65 us, whole 1031; 128 sequences of 512 to 8191: 140 and
+        // 157; pieces of half a share 67 and 142).
+        for (int64_t each = share;; each += each / 8 + 1)
+            if (cut(b, each) || groups <= part_units) return;
+    }
+};
+
 // A workspace that grows in large steps.
 template <typename T>
 void grow(DevBuf<T>& b, size_t count) {
@@ -50,6 +107,15 @@ void grow(DevBuf<T>& b, size_t count) {
 }
 
 }  // namespace
+
+void kv_plan_steps(const int64_t* lens, const int64_t* counts, int n, int heads, int group, int32_t* splits, int32_t* per) {
+    KvPlan plan;
+    KvBatch b;
+    plan.heads = heads;
+    for (int i = 0; i < n; i++) plan.add(lens[i], counts[i], group, 16, true, 0);
+    plan.split(b, false, kPartBytes / (16 * (KV_MAX_DIM * 4 + 8)));
+    for (int i = 0; i < n; i++) splits[i] = b.splits[i], per[i] = b.per[i];
+}
 
 KvCache::KvCache(const vgpu_kv_params& p) : params(p) {
     const auto cfg = [](bool ok, const char* msg) { need(ok, msg, VGPU_ERR_INVALID_CONFIG); };
@@ -438,13 +504,14 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
     a.vec_out = dev.D % 4 == 0 && (uintptr_t)q.out % (4 * item_size(a.q.type)) == 0;
     const int parts = a.q.type == KV_F32 ? 2 : 1;
     const int64_t chunk_rows = 64 * kv_chunk_nc(dev.Dp, parts);
-    int64_t tokens = 0, longest = 0, most = 0, chunk_tiles = 0;
+    int64_t tokens = 0, longest = 0, most = 0, chunk_tiles = 0, step_units = 0;
     for (size_t i = 0; i < n; i++) {
         need(counts[i] >= 0, "counts must not be negative");
         tokens += counts[i];
         need(tokens * (int64_t)q.num_q_heads <= INT_MAX / 2, "more than 2^30 query rows in one call");
         longest = std::max(longest, seqs[ids[i]].len);
         most = std::max(most, counts[i] * a.G);
+        step_units += (counts[i] * a.G + 15) / 16 * dev.H;
         chunk_tiles += (counts[i] * a.G + chunk_rows - 1) / chunk_rows * dev.H * ((seqs[ids[i]].len + KV_TILE - 1) / KV_TILE);
     }
     need(!q.mask || (int64_t)q.mask_slots >= longest, "a mask row must cover the longest sequence (" +
@@ -465,13 +532,16 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
     }
     const int rows = kv_attend_rows(a, dev.Dp);
     // Where a workgroup's work depends on its sequence, the short sequences come first: the
-    // light rows of the longest end the launch.
+    // light rows of the longest end the launch.  Steps that may have more workgroups than
+    // are on the card at once begin with the longest.
     std::vector<size_t> order(n);
     std::vector<int64_t> tok0(n);
     int64_t tok = 0;
     for (size_t i = 0; i < n; i++) order[i] = i, tok0[i] = tok, tok += counts[i];
     if (a.by_rows)
         std::stable_sort(order.begin(), order.end(), [&](size_t x, size_t y) { return seqs[ids[x]].len < seqs[ids[y]].len; });
+    else if (step_units > kStepWorkgroups / 2)
+        std::stable_sort(order.begin(), order.end(), [&](size_t x, size_t y) { return seqs[ids[x]].len > seqs[ids[y]].len; });
     // Where several launches add weights, all of them are checked and their workspaces grown
     // before the first, so that a call that fails has added none.
     for (int dry = a.track && n > KV_BATCH; dry >= 0; dry--)
@@ -479,8 +549,9 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
         KvBatch b;
         b.n = 0;
         b.unit0[0] = 0;
-        int64_t work = 0, units = 0, score_tiles = 0, row_tiles = 0;
-        int64_t tiles[KV_BATCH], row_units[KV_BATCH];  // that a row tile can see; row tiles
+        KvPlan plan;
+        plan.heads = dev.H;
+        int64_t score_tiles = 0, row_tiles = 0;
         for (size_t x = i0; x < std::min(n, i0 + KV_BATCH); x++) {
             const size_t i = order[x];
             const int64_t len = seqs[ids[i]].len;
@@ -489,44 +560,18 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
             b.len[j] = (int)len;
             b.tok0[j] = (int)tok0[i];
             b.count[j] = (int)counts[i];
-            row_units[j] = (counts[i] * a.G + rows - 1) / rows;
-            units += row_units[j] * dev.H;
-            tiles[j] = (len + KV_TILE - 1) / KV_TILE;
             need(score_tiles <= INT_MAX / 2, "too many scores in one call");
             b.aux[j] = (int)(keep_scores ? score_tiles : row_tiles);
-            if (keep_scores) score_tiles += tiles[j] * counts[i] * a.G;
+            if (keep_scores) score_tiles += (len + KV_TILE - 1) / KV_TILE * counts[i] * a.G;
             row_tiles += (counts[i] * a.G + 15) / 16;
-            if (a.window && a.causal)
-                tiles[j] = std::min<int64_t>(tiles[j], (a.window + rows / a.G + 2 * KV_TILE) / KV_TILE + 1);
-            // (the first tokens of a chunk see less than the last)
-            const int64_t seen = a.causal && !a.window ? std::max<int64_t>(2 * len - counts[i], 0) : 2 * KV_TILE * tiles[j];
-            work += row_units[j] * dev.H * ((seen + 2 * KV_TILE - 1) / (2 * KV_TILE));
+            plan.add(len, counts[i], a.G, rows, a.causal, a.window);
         }
-        need(units <= kMaxWorkgroups, "too many query rows in one call");
-        if (units) {
-            // Tiles of one workgroup: as few as keep all workgroups on the card at once
-            const int64_t target = a.by_rows ? kChunkWorkgroups : kStepWorkgroups;
-            const int64_t part_units = kPartBytes / (rows * ((int64_t)dev.Dp * 4 + 8));
-            int64_t each = std::max<int64_t>((work + target - 1) / target, a.by_rows ? 16 : 8), groups, split_units;
-            for (;; each += each / 8 + 1) {
-                groups = split_units = 0;
-                bool one = true;
-                for (int j = 0; j < b.n; j++) {
-                    // many rows: whole unless that would leave one workgroup at work alone
-                    const int64_t most_tiles = a.by_rows ? each + each / 4 : each;
-                    const int64_t splits = a.by_rows && units >= 4 * target
-                                               ? 1 : std::max<int64_t>((tiles[j] + most_tiles - 1) / most_tiles, 1);
-                    b.splits[j] = (int)splits;
-                    b.per[j] = (int)std::max<int64_t>((tiles[j] + splits - 1) / splits, 1);
-                    b.unit0[j + 1] = b.unit0[j] + (int)(row_units[j] * splits);
-                    groups += row_units[j] * splits * dev.H;
-                    one = one && splits == 1;
-                    if (splits > 1) split_units += row_units[j] * splits * dev.H;
-                }
-                if (one || ((a.by_rows || groups <= target + target / 8) && groups <= part_units)) break;
-            }
+        need(plan.units <= kMaxWorkgroups, "too many query rows in one call");
+        if (plan.units) {
+            plan.split(b, a.by_rows, kPartBytes / (rows * ((int64_t)dev.Dp * 4 + 8)));
+            const int64_t groups = plan.groups;
             a.part_o = nullptr, a.part_ml = nullptr, a.part_e = nullptr, a.scores = nullptr;
-            if (split_units) {
+            if (plan.split_units) {
                 grow(w_part, (size_t)(groups * rows) * dev.Dp);
                 grow(w_ml, (size_t)(groups * rows));
                 grow(w_power, (size_t)groups);

@@ -335,6 +335,9 @@ struct FlatIndex {
                      hipStream_t s);
 };
 
+// The splits of a step's sequences (causal, no window; n at most KV_BATCH) and the tiles of each.
+void kv_plan_steps(const int64_t* lens, const int64_t* counts, int n, int heads, int group, int32_t* splits, int32_t* per);
+
 // The attention memory: a pool of blocks in HBM, each sequence's blocks and length on
 // the host.  The calls queue kernels on the caller's stream and do not wait; the host
 // state changes with them, under the lock.
