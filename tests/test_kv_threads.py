@@ -113,3 +113,10 @@ def test_calls_of_two_threads_on_two_streams_follow_one_another(cache):
     assert sorted(lib.streams[i][1] for i in calls) == [0, 1, 2]
     for a, b in zip(calls, calls[1:]):
         assert ("wait", lib.streams[b][1], lib.streams[a][1]) in lib.streams[a:b], lib.streams
+
+
+def test_read_refuses_a_negative_first_before_it_allocates(cache):
+    c, lib = cache
+    with pytest.raises(ValueError, match="first"):
+        c.read(first=[0, 0, -(1 << 62)])
+    assert not lib.calls

@@ -17,6 +17,7 @@ import ctypes
 import math
 import threading
 from array import array
+from operator import sub
 
 import numpy as np
 
@@ -231,10 +232,14 @@ class KVCache:
                 raise ValueError(f"fields must be among {FIELDS}")
         ids = self._seqs(seqs)
         at = self._ints(0 if first is None else first, len(ids), "first")
+        if at and min(at) < 0:
+            raise ValueError("first must not be negative")
         with self._turn:
             if counts is None:  # to the end; the library checks what the tensors were sized by
                 lens = self._lengths()
-                n = array("q", [lens[i] - max(f, 0) for i, f in zip(ids, at)])
+                n = lens if ids is self._all else array("q", map(lens.__getitem__, ids))
+                if first is not None:
+                    n = array("q", map(sub, n, at))
             else:
                 n = self._ints(counts, len(ids), "counts")
             tokens = max(sum(n), 0)
