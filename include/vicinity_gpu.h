@@ -324,7 +324,9 @@ int vgpu_flat_last_fallbacks(const vgpu_flat *h, uint32_t *queries);
  * All pointers marked "device" are device memory of the cache's device, which
  * must be current; host arrays (seqs, counts, ...) are read before the call
  * returns.  The calls queue their work on `stream` (a hipStream_t, NULL the
- * device's default stream) and return without waiting; calls on one cache that
+ * device's default stream) and return without waiting, but for a call that needs
+ * larger workspaces than those before it: it frees the old ones, which waits for
+ * the device.  Calls on one cache that
  * use different streams are put in order by the caller.  Lengths are host state
  * and change when the call returns.  Under stream capture the calls are
  * VGPU_ERR_UNSUPPORTED: a graph would replay with the lengths of its recording. */

@@ -100,10 +100,18 @@ struct KvPlan {
     }
 };
 
-// A workspace that grows in large steps.
+// A workspace that grows in large steps, where there is memory for them.
 template <typename T>
 void grow(DevBuf<T>& b, size_t count) {
-    if (count > b.n) b.reserve(std::max(count, b.n + b.n / 2));
+    if (count <= b.n) return;
+    const size_t step = b.n + b.n / 2;
+    if (step > count) try {
+        b.reserve(step);
+        return;
+    } catch (const Error& e) {
+        if (e.code != VGPU_ERR_OUT_OF_MEMORY) throw;
+    }
+    b.reserve(count);
 }
 
 }  // namespace
