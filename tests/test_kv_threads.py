@@ -1,5 +1,5 @@
-"""KVCache calls of several threads on one handle, against a library that keeps lengths and
-notes what it is asked to do: no GPU."""
+"""KVCache against a library that keeps lengths and notes what it is asked to do, no GPU: calls
+of several threads on one handle, and integers that the C interface cannot hold."""
 
 import ctypes
 import threading
@@ -39,6 +39,14 @@ class Library:
             rows = np.ctypeslib.as_array(ctypes.cast(counts, ctypes.POINTER(ctypes.c_int64)), (n,)).sum()
         self.calls.append(("read", int(rows)))
         self.streams.append(("call", stream or 0))
+        return 0
+
+    def vgpu_kv_evict(self, h, ids, into, n, budget, recent, dropped, dpos, dk, dv, stream):
+        self.calls.append(("evict", ctypes.c_size_t(budget).value, ctypes.c_size_t(recent).value))
+        return 0
+
+    def vgpu_kv_attend(self, h, ids, counts, n, query, stream):
+        self.calls.append(("attend", query._obj.window))
         return 0
 
 
@@ -120,3 +128,23 @@ def test_read_refuses_a_negative_first_before_it_allocates(cache):
     with pytest.raises(ValueError, match="first"):
         c.read(first=[0, 0, -(1 << 62)])
     assert not lib.calls
+
+
+@pytest.mark.parametrize("name", ["budget", "recent"])
+@pytest.mark.parametrize("value", [1 << 30, (1 << 64) + 5, (1 << 64) - 1])
+def test_budgets_beyond_the_interface_are_refused(cache, name, value):
+    """2^64 + 5 would arrive as 5, and cut every sequence to 5 slots."""
+    c, lib = cache
+    with pytest.raises(ValueError, match=name):
+        c.evict(**({"budget": 8, "recent": 0} | {name: value}))
+    assert not lib.calls
+    c.evict((1 << 30) - 1, np.int64(4))
+    assert lib.calls == [("evict", (1 << 30) - 1, 4)]
+
+
+@pytest.mark.parametrize("window,arrives", [(0, 0), (7, 7), (np.int32(9), 9), (1 << 31, 1 << 31),
+                                            ((1 << 64) + 1, 1 << 62), (1 << 64, 1 << 62)])
+def test_a_window_beyond_the_interface_is_as_good_as_none(cache, window, arrives):
+    c, lib = cache
+    c.attend(torch.zeros((3, 2, 4)), counts=[1, 1, 1], window=window)
+    assert lib.calls == [("attend", arrives)]

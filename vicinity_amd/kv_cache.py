@@ -170,7 +170,7 @@ class KVCache:
                     if return_lse else None
             query = _lib.KvQuery(
                 qt, heads, 1.0 / math.sqrt(self.head_dim) if scale is None else scale, int(causal),
-                int(window), mask.data_ptr() if mask is not None else None,
+                min(int(window), 1 << 62), mask.data_ptr() if mask is not None else None,
                 mask.stride(0) if mask is not None else 0, mask.stride(1) if mask is not None else 0,
                 mask.shape[1] if mask is not None else 0, int(decay is not None),
                 0.0 if decay is None else decay, out.data_ptr(),
@@ -196,8 +196,8 @@ class KVCache:
         if to is not None and len(to) != len(ids):
             raise ValueError(f"into names {len(to)} sequences, seqs {len(ids)}")
         for name, value in (("budget", budget), ("recent", recent)):
-            if not isinstance(value, (int, np.integer)) or value < 0:
-                raise ValueError(f"{name} must be an int, 0 or more")
+            if not isinstance(value, (int, np.integer)) or not 0 <= value < 1 << 30:
+                raise ValueError(f"{name} must be an int from 0 to 2**30 - 1")
         with self._turn:
             s, ctx = self._stream(stream, ())
             gone, most = None, 0
