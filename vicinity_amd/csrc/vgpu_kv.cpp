@@ -514,7 +514,7 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
     const int64_t chunk_rows = 64 * kv_chunk_nc(dev.Dp, parts);
     int64_t tokens = 0, longest = 0, most = 0, chunk_tiles = 0, step_units = 0;
     for (size_t i = 0; i < n; i++) {
-        need(counts[i] >= 0, "counts must not be negative");
+        need(counts[i] >= 0 && counts[i] <= INT_MAX / 2, "counts must not be negative, nor above 2^30");
         tokens += counts[i];
         need(tokens * (int64_t)q.num_q_heads <= INT_MAX / 2, "more than 2^30 query rows in one call");
         longest = std::max(longest, seqs[ids[i]].len);
