@@ -34,9 +34,9 @@ constexpr float KV_TOP = 6.f;    // p of the reference is 2^KV_TOP
 constexpr float KV_SLACK = 8.f;  // and may grow to 2^(KV_TOP + KV_SLACK)
 // t_b of a scale far below the others, or of 0.  A scale of 0 stands for codes of 0, so any
 // number does in its place: m must not follow slots that add nothing (values down to 2^-80 of
-// the others keep their bits beside them), but their p has to count in the denominators (with
-// m from a t of 1 it is lost where u lies 2^-46 below).  Codes of a scale not 0 that is below
-// come out as if it were 2^-80 of the others.
+// the others keep their bits beside them), but their p has to count in the denominators (beside
+// m from a t of 1 it is lost where u lies 52 below).  Codes of a scale not 0 that is below come
+// out as if it were 2^-80 of the others.
 constexpr float KV_LEAST = 0x1p-80f;
 constexpr int KV_NEAR = 8;         // t_b stays below 2^KV_NEAR
 constexpr int KV_NONE = -(1 << 20);  // E before a scale above 0 was seen
@@ -192,7 +192,9 @@ __device__ __forceinline__ void kv_load_rows(KvWave<S, CODE, PARTS, NC>& w, cons
         big = kv_max4(big);
         int ex = 0;
         if (big > 0.f && big < __builtin_huge_valf()) (void)frexpf(big, &ex), ex -= 15;
-        w.qs[n] = ldexpf(a.scale2, ex);
+        // An infinite element makes every score infinite or NaN, and the softmax of any of them
+        // NaN: also where all are -inf, which the sums would take for a row that sees nothing.
+        w.qs[n] = big < __builtin_huge_valf() ? ldexpf(a.scale2, ex) : __uint_as_float(0x7fc00000u);
 #pragma unroll
         for (int s = 0; s < S; s++)
 #pragma unroll
