@@ -141,7 +141,12 @@ class KVCache:
         scale None: 1 / sqrt(head_dim).  decay: the accumulated weight of a slot and head
         becomes decay * weight + what the call's tokens gave it (None: weights stay).
         return_lse: also the float32 logarithms of the softmax denominators
-        [tokens, heads]."""
+        [tokens, heads].
+
+        Sums, logarithms and weights are float32.  16-bit queries are taken exactly and
+        their probabilities multiply the values with 11 bits; float32 queries with 22 bits
+        of their row's largest element, and so the probabilities; what is below 2^-30 of
+        the largest adds nothing to the result."""
         import torch
 
         ids = self._seqs(seqs)
