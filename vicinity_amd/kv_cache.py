@@ -17,7 +17,6 @@ import ctypes
 import math
 import threading
 from array import array
-from operator import sub
 
 import numpy as np
 
@@ -243,8 +242,9 @@ class KVCache:
             if counts is None:  # to the end; the library checks what the tensors were sized by
                 lens = self._lengths()
                 n = lens if ids is self._all else array("q", map(lens.__getitem__, ids))
-                if first is not None:
-                    n = array("q", map(sub, n, at))
+                if first is not None and n:
+                    left = np.frombuffer(n, np.int64)  # n's own memory
+                    np.subtract(left, at, out=left)
             else:
                 n = self._ints(counts, len(ids), "counts")
             tokens = max(sum(n), 0)
