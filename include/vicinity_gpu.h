@@ -397,7 +397,12 @@ int vgpu_kv_append(vgpu_kv *h, const int32_t *seqs, const int64_t *counts, size_
                    const vgpu_tensor3 *k, const vgpu_tensor3 *v, const int32_t *positions,
                    const float *weights, void *stream);
 
-/* softmax(scale * q.k) v over the cached slots, accumulated in float32.  Token i
+/* softmax(scale * q.k) v over the cached slots, accumulated in float32: 16-bit
+ * queries enter the scores exactly (elements down to 2^-28 of their row's largest),
+ * float32 ones with 22 bits of that; probabilities enter the product with the values with 11 bits, 22 for
+ * float32 queries, and as 0 below 2^-30 of the largest; denominators, lse and weights
+ * come from float32 probabilities.  A value scale of the head below 2^-80 of one before
+ * it in the sequence counts as that.  There is no backward.  Token i
  * of sequence s (of counts[s], the last ones appended) stands at slot
  * p = len - counts[s] + i.  It sees the slots j <= p (causal; else all of them),
  * of them those with j > p - window (window != 0), of them those whose mask is
@@ -436,7 +441,8 @@ int vgpu_kv_read(vgpu_kv *h, const int32_t *seqs, const int64_t *first, const in
                  void *stream);
 
 /* Forget the slots from lengths[i] on (0 empties the sequence); blocks that hold
- * nothing any more return to the pool.  A block keeps its scales. */
+ * nothing any more return to the pool.  A block keeps its scales, also one that a
+ * forgotten token raised, or made NaN. */
 int vgpu_kv_truncate(vgpu_kv *h, const int32_t *seqs, const int64_t *lengths, size_t n);
 
 /* ---- per-kernel test entry points (host buffers) -------------------------- */

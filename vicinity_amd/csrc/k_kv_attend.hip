@@ -10,9 +10,10 @@
 //
 // Products: codes are integers up to 127 or e4m3 numbers, both exact in half
 // precision.  A query row is scaled by a power of two to a largest element of 2^14
-// and split into 1 (bf16, f16: exact) or 2 (f32: 22 bits) halves, so the scores are
-// float32 sums of exact products.  p is rounded to half precision (2^-12) for 16-bit
-// results and to two halves for float32 ones; p is held near 2^6 .. 2^14 at the top,
+// and split into 1 (bf16, f16: exact for elements down to 2^-28 of it) or 2 (f32: 22 bits)
+// halves, so the scores are float32 sums of exact products.  p is rounded to half precision (2^-11), the
+// matrix instruction's, for 16-bit queries, whose results are rounded to as many bits or
+// fewer, and to two halves (2^-22) for float32 ones; p is held near 2^6 .. 2^14 at the top,
 // so what is below 2^-30 of the largest rounds to zero.
 // m only moves when a score exceeds it by 2^8: a step that costs a scaling of the
 // accumulators, taken by a whole wave, nearly always in the first tile only.
@@ -469,8 +470,9 @@ __device__ __forceinline__ KvJob kv_job(const KvDev& c, const KvBatch& b, const 
 // Few rows: the four waves of a workgroup take the same 16 rows and every fourth tile,
 // joined at the end.  The next tile's keys are loaded when this one's are used up, under
 // its softmax and values, and its values under the next one's keys: one tile of registers.
-// Bound by the cache's bytes: a tile's 64 Dp bytes against 4 Dp / 16 matrix instructions of
-// 16 cycles (61 sequences up to 8191 slots, 8 x 128: 349 MB in 69 us, 5.1 TB/s).
+// Bound by the cache's bytes: a tile's 64 Dp bytes against Dp / 8 matrix instructions of
+// 16 cycles, Dp / 4 for float32 queries (61 sequences up to 8191 slots, 8 x 128: 349 MB in
+// 63 us, 5.5 TB/s; 64 to 256 dims, 61 sequences of 4096: 5.6 to 6.3).
 // ONCE: no row tile but this one reads the tiles (64 sequences of 4096, 8 x 128, one row tile:
 // 86 us, by the caches 97; two row tiles 145 and 129).
 template <int S, int CODE, int PARTS, bool ONCE>
@@ -562,6 +564,9 @@ __global__ __launch_bounds__(256, S <= 4 ? 3 : 2) void kv_step_kernel(KvDev c, K
 // Many rows: the four waves of a workgroup take 4 * NC * 16 rows and every tile.  A tile's
 // codes are converted once, a quarter by each wave, and shared as half-precision operands
 // through LDS (three buffers, one barrier to a tile); an operand read feeds NC products.
+// 2048 tokens over 32768 slots, 8 x 4 x 128: the vector unit is busy 61% of the time and
+// the matrix unit 42%; over 16384 slots 970 TFLOP/s, 760 to 630 at other widths, and 400 to
+// 560 in float32, which has two products for one.
 template <int S, int CODE, int PARTS, int NC>
 __global__ __launch_bounds__(256, S == 8 ? 1 : 2) void kv_chunk_kernel(KvDev c, KvBatch b, KvAttend a) {
     __shared__ half8 tiles[3][4 * S][64];  // operands of keys, then of values
@@ -813,9 +818,9 @@ __global__ __launch_bounds__(256) void kv_score_weights_kernel(KvDev c, KvBatch 
 // 2^(u_rj - lse_r).  The attention left its query operands (a.qop) and each row's
 // factor (a.qs) and logarithm.  A wave holds the operands of KV_WT tiles and goes over
 // the rows of its chunk, 32 at a time through LDS, which the four waves share; the
-// chunks' sums are added in their order by kv_chunk_weights_kernel.  Bound by the
-// exponentials: 16 cycles of a SIMD for 64 of them, against 16 of the matrix unit for
-// the 512 multiply-adds of 4 scores of 128 dims.
+// chunks' sums are added in their order by kv_chunk_weights_kernel.  Bound by waits, at the
+// loads and the barrier of each 32 rows: prompts of 4001, 2036 and 604 tokens, 4 x 4 x 128,
+// take 92 us, of which the vector unit is busy 42% and the matrix unit 19%.
 constexpr int KV_WT = 1;              // 32-slot tiles of a wave
 static_assert(KV_WEIGHT_SLOTS == 4 * KV_WT * KV_TILE, "four waves of KV_WT tiles");
 

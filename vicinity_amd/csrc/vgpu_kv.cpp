@@ -21,10 +21,10 @@ namespace {
 size_t item_size(int type) { return type == KV_F32 ? 4 : 2; }
 
 // Workgroups that a step is cut into where one round suffices: three for each of the 256
-// compute units.
+// compute units, which hold as many up to 128 dims; above, two fit, and the third ones follow.
 constexpr int64_t kStepWorkgroups = 768;
-// Workgroups of a call with many rows, two to a compute unit: with fewer, the tiles are
-// split too, which costs a partial result for every row and split.
+// Workgroups of a call with many rows, two to a compute unit (at 256 dims one fits): with
+// fewer, the tiles are split too, which costs a partial result for every row and split.
 constexpr int64_t kChunkWorkgroups = 512;
 // Workgroups of the second pass that makes weights: twelve to a compute unit, for its rows
 // differ in length (8192: no faster).
@@ -35,12 +35,12 @@ constexpr int64_t kMaxWorkgroups = (1 << 24) - 1;
 constexpr int64_t kPartBytes = (int64_t)256 << 20;
 // Calls of at most this many rows per head keep their scores for the weights; with more a
 // second pass over the keys is cheaper (16 sequences of 4096, 8 x 128: 32 rows 70 and 93 us,
-// 48 rows 91 and 96, 64 rows 116 and 102).
+// 48 rows 91 and 96, 64 rows 116 and 102; measured in bfloat16 there, and taken for all).
 constexpr int64_t kScoreRows = 48;
 // The kernel of many rows takes over where its workgroups are filled to three quarters and
 // have this many 32-slot tiles to do in all (16 sequences of 4096, 8 x 128, 128 rows: 65 us
 // against 77 by row tiles of 16, 96 rows 67 and 58, 256 rows 106 and 139; 4 sequences of 1024,
-// 256 rows: 29 and 16 us).
+// 256 rows: 29 and 16 us; measured in bfloat16 there, and taken for all).
 constexpr int64_t kChunkTiles = 4096;
 
 // The row tiles of one launch's sequences, and the tiles that each goes over.

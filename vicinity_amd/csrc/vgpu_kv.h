@@ -2,10 +2,12 @@
 //
 // The pool is made of blocks of B slots; a block holds every head's part one
 // after the other, and a part is B / 32 tiles of 32 slots.  A tile is 32 * Dp
-// bytes of key codes, then 32 * Dp bytes of value codes (Dp: the head dimension
-// padded to 32), in the order in which the lanes of a wave take them as operands
-// of the 16x16x32 matrix instruction, so every load of the attention is 16
-// contiguous bytes per lane and no element changes lanes between the two products:
+// bytes of key codes, then 32 * Dp bytes of value codes, in the order in which the
+// lanes of a wave take them as operands of the 16x16x32 matrix instruction, so every
+// load of the attention is 16 contiguous bytes per lane and no element changes lanes
+// between the two products.  Dp is the smallest of 64, 96, 128, 192 and 256 that holds
+// the head dimension, for which the kernels are compiled; the rest is stored and read
+// as zeros (dimension 32 takes the bytes of 64, 136 those of 192):
 //
 //   keys    operand (j, s) = slots 16 j .. 16 j + 15 x dims 32 s .. 32 s + 31;
 //           lane 16 g + r holds slot 16 j + r, dims 32 s + 8 g .. + 7.

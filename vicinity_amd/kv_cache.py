@@ -7,7 +7,9 @@ attention takes them with.
 
 Tensors are torch tensors on the cache's GPU.  Calls are queued on the current torch
 stream, or on ``stream``, and return without waiting; a call on another stream than the
-one before it waits for that one on the GPU.
+one before it waits for that one on the GPU.  Calls of several threads on one cache take
+turns, on the host and on the GPU alike.  There is no backward: what enters the cache is
+held without its gradient, and results have none.
 """
 
 from __future__ import annotations
@@ -98,7 +100,8 @@ class KVCache:
         return {"free_blocks": out.free_blocks, "device_bytes": out.device_bytes}
 
     def truncate(self, lengths, seqs=None) -> None:
-        """Forget each sequence's slots from lengths[i] on; 0 empties it."""
+        """Forget each sequence's slots from lengths[i] on; 0 empties it.  A block that keeps
+        slots keeps its scales, also one that a forgotten token raised, or made NaN."""
         ids = self._seqs(seqs)
         lens = self._ints(lengths, len(ids), "lengths")
         with self._turn:
