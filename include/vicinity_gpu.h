@@ -401,8 +401,10 @@ int vgpu_kv_append(vgpu_kv *h, const int32_t *seqs, const int64_t *counts, size_
  * queries enter the scores exactly (elements down to 2^-28 of their row's largest),
  * float32 ones with 22 bits of that; probabilities enter the product with the values with 11 bits, 22 for
  * float32 queries, and as 0 below 2^-30 of the largest; denominators, lse and weights
- * come from float32 probabilities.  A value scale of the head below 2^-80 of one before
- * it in the sequence counts as that.  There is no backward.  Token i
+ * come from float32 probabilities.  A value scale below 2^-80 of the largest that a
+ * row has seen so far counts as that for it.  Scores are float32: neighbours of more
+ * than 2^24 are not told apart, and beyond 2^27 their rounding can make results NaN
+ * and weights infinite.  There is no backward.  Token i
  * of sequence s (of counts[s], the last ones appended) stands at slot
  * p = len - counts[s] + i.  It sees the slots j <= p (causal; else all of them),
  * of them those with j > p - window (window != 0), of them those whose mask is

@@ -2,19 +2,19 @@
 //
 // For a row r (a query token and head) and slot j:  u_j = scale * log2(e) * q_r.k_j,
 // o = sum 2^(u_j) v_j / sum 2^(u_j).  One pass over the tiles with a running
-// reference m: the value scale s_b = 2^E t_b of a block goes into the exponent,
-// p_j = 2^(u_j + log2 t_b - m), so o's accumulators add p_j * code directly in the
-// matrix instruction and the denominator adds p_j / t_b.  E is a power that the
-// scales of the tiles at hand lie near, so the sums stay in float32's range for
-// scales of any size; the result is 2^E o / l.
+// reference m: the value scale s_b of a block goes into the exponent,
+// p_j = 2^(u_j + log2 s_b - m), so o's accumulators add p_j * code directly in the
+// matrix instruction, and the denominator adds p_j S / s_b.  S is a row's own power of
+// two, near the largest scale that moved its m, so that l stays in float32's range for
+// scales of any size; the result is S o / l.
 //
 // Products: codes are integers up to 127 or e4m3 numbers, both exact in half
 // precision.  A query row is scaled by a power of two to a largest element of 2^14
 // and split into 1 (bf16, f16: exact for elements down to 2^-28 of it) or 2 (f32: 22 bits)
-// halves, so the scores are float32 sums of exact products.  p is rounded to half precision (2^-11), the
-// matrix instruction's, for 16-bit queries, whose results are rounded to as many bits or
-// fewer, and to two halves (2^-22) for float32 ones; p is held near 2^6 .. 2^14 at the top,
-// so what is below 2^-30 of the largest rounds to zero.
+// halves, so the scores are float32 sums of exact products.  p is rounded to half precision
+// (2^-11), the matrix instruction's, for 16-bit queries, whose results are rounded to as many
+// bits or fewer, and to two halves (2^-22) for float32 ones; p is held near 2^6 .. 2^14 at the
+// top, so what is below 2^-30 of the largest rounds to zero.
 // m only moves when a score exceeds it by 2^8: a step that costs a scaling of the
 // accumulators, taken by a whole wave, nearly always in the first tile only.
 #include "vgpu_kv.h"
@@ -33,15 +33,16 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float KV_TOP = 6.f;    // p of the reference is 2^KV_TOP
 constexpr float KV_SLACK = 8.f;  // and may grow to 2^(KV_TOP + KV_SLACK)
-// t_b of a scale far below the others, or of 0.  A scale of 0 stands for codes of 0, so any
-// number does in its place: m must not follow slots that add nothing (values down to 2^-80 of
-// the others keep their bits beside them), but their p has to count in the denominators (beside
-// m from a t of 1 it is lost where u lies 52 below).  Codes of a scale not 0 that is below come
-// out as if it were 2^-80 of the others.
-constexpr float KV_LEAST = 0x1p-80f;
-constexpr int KV_NEAR = 8;         // t_b stays below 2^KV_NEAR
-constexpr int KV_NONE = -(1 << 20);  // E before a scale above 0 was seen
+// S / s_b at most, and log2 s_b at least log2 S less its logarithm.  So a scale of 0, which
+// stands for codes of 0, takes part in the denominators without setting m beside values down
+// to 2^-80 of those that the row has seen; codes of a smaller scale that is not 0 come out as
+// if it were 2^-80 of theirs.
+constexpr float KV_FAR = 80.f, KV_FAR_F = 0x1p80f;
+// S before a scale above 0 moved m: below all of them (2^-109 and up)
+constexpr int KV_FIRST = -125;
 #define KV_NEG (-__builtin_huge_valf())
+// m - KV_TOP of a row that has seen no slot: whatever it sees stands far above (the least float).
+constexpr float KV_START = -0x1.fffffep127f;
 
 // Two halves of 8 codes.
 template <int CODE>
@@ -163,8 +164,9 @@ struct KvWave {
     float qs[NC];          // 2^-(the row's scaling) * scale * log2(e)
     int lo[NC], hi[NC];    // slots that the row sees
     int row[NC];
-    float m[NC], l[NC], bad[NC];
-    int e = KV_NONE;       // E, the same in every lane
+    int row0, len, count;
+    float t[NC], l[NC], bad[NC];  // t: m - KV_TOP
+    float s[NC], low[NC];  // S; log2 S - KV_FAR
     floatx4 o[NC][2 * S];
 };
 
@@ -173,12 +175,14 @@ __device__ __forceinline__ void kv_load_rows(KvWave<S, CODE, PARTS, NC>& w, cons
                                              const KvAttend& a, int i, int h, int row0) {
     const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
     const int rows = b.count[i] * a.G, len = b.len[i];
+    w.row0 = row0, w.len = len, w.count = b.count[i];
 #pragma unroll
     for (int n = 0; n < NC; n++) {
         const int row = row0 + n * 16 + col;
         w.row[n] = row < rows ? row : -1;
         w.lo[n] = 0, w.hi[n] = 0;  // rows past the end see nothing
-        w.m[n] = KV_NEG, w.l[n] = 0.f, w.bad[n] = 0.f;
+        w.t[n] = KV_START, w.l[n] = 0.f, w.bad[n] = 0.f;
+        w.s[n] = __builtin_ldexpf(1.f, KV_FIRST), w.low[n] = (float)KV_FIRST - KV_FAR;
         float big = 0.f;
         // (a row past the end loads the last one's and is not used)
         const int real = min(row, rows - 1);
@@ -210,12 +214,22 @@ __device__ __forceinline__ void kv_load_rows(KvWave<S, CODE, PARTS, NC>& w, cons
     }
 }
 
+// Four column tiles have no registers for their rows' numbers and slots: here they are worked
+// out again, before they are needed (64 dims, 2048 tokens over 16384 slots: 372 us, 377 kept).
+template <int S, int CODE, int PARTS, int NC>
+__device__ __forceinline__ void kv_rows_again(KvWave<S, CODE, PARTS, NC>& w, const KvAttend& a, int n) {
+    if (NC <= 2) return;
+    const int row = w.row0 + n * 16 + (threadIdx.x & 15);
+    w.row[n] = row < w.count * a.G ? row : -1;
+    w.lo[n] = w.hi[n] = 0;
+    if (w.row[n] >= 0) kv_range(a, w.len, w.count, row, w.lo[n], w.hi[n]);
+}
+
 // What a wave needs to know of 64 tiles, one to a lane: refilled every 64 tiles, so no
 // step waits for the block table or a scale.
 struct KvTiles {
     uint32_t lo, hi;   // its offset in the pool
-    float ks, vs;      // key and value scale
-    float lv, rv;      // log2 t and 1 / t of the value scale (kv_measure)
+    float ks, lv, rv;  // key scale, log2 of the value scale and 1 by it (0 and NaN: -inf and inf)
     uint64_t bad;      // tiles whose value scale is NaN
 };
 
@@ -229,9 +243,10 @@ __device__ __forceinline__ KvTiles kv_tile_infos(const KvDev& c, const int* tabl
     const size_t at = kv_tile_offset(c, block, h, t & (c.B / KV_TILE - 1));
     r.lo = (uint32_t)at, r.hi = (uint32_t)(at >> 32);
     r.ks = in ? c.kscale[part] : 0.f;
-    r.vs = in ? c.vscale[part] : 0.f;
-    r.lv = r.rv = 0.f;
-    r.bad = __ballot(r.vs != r.vs);
+    const float vs = in ? c.vscale[part] : 0.f;
+    r.bad = __ballot(vs != vs);
+    r.lv = vs > 0.f ? log2f(vs) : KV_NEG;
+    r.rv = vs > 0.f ? 1.f / vs : -KV_NEG;
     return r;
 }
 __device__ __forceinline__ const uint8_t* kv_tile_of(const KvDev& c, const KvTiles& f, int lane) {
@@ -243,37 +258,6 @@ __device__ __forceinline__ float kv_lane(float v, int lane) {
     return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), lane));
 }
 
-// lv and rv of 64 tiles, before the first of them.  E is the first scale's power, and moves up
-// to the largest's where one passes it by 2^KV_NEAR: then m and l take the difference, as far
-// as l stays below 2^90, and o's accumulators the rest.
-template <int S, int CODE, int PARTS, int NC>
-__device__ __forceinline__ void kv_measure(KvWave<S, CODE, PARTS, NC>& w, KvTiles& f) {
-    const bool some = f.vs > 0.f;
-    int e = some ? __builtin_amdgcn_frexp_expf(f.vs) : KV_NONE;
-    const uint64_t any = __ballot(some);
-    if (w.e == KV_NONE && any) w.e = __builtin_amdgcn_readlane(e, __builtin_ctzll(any));
-    if (__any(e > w.e + KV_NEAR)) {
-#pragma unroll
-        for (int o = 32; o; o >>= 1) e = max(e, __shfl_xor(e, o));
-        e = __builtin_amdgcn_readfirstlane(e);
-        const int up = e - w.e;
-        w.e = e;
-#pragma unroll
-        for (int n = 0; n < NC; n++) {
-            const int by = max(min(up, 90 - __builtin_amdgcn_frexp_expf(kv_max4(w.l[n]))), 0);
-            w.m[n] -= (float)by;
-            w.l[n] = ldexpf(w.l[n], by);
-            const float f1 = ldexpf(1.f, by - up);
-#pragma unroll
-            for (int j = 0; j < 2 * S; j++) w.o[n][j] *= f1;
-        }
-    }
-    const float t = some ? fmaxf(ldexpf(f.vs, -w.e), KV_LEAST) : KV_LEAST;
-    f.lv = __builtin_amdgcn_logf(t);  // (one unit in the last place each; t is a normal number)
-    f.rv = __builtin_amdgcn_rcpf(t);
-}
-__device__ __forceinline__ int kv_power(int e) { return e == KV_NONE ? 0 : e; }
-
 // Largest of 8, a NaN only if all are (fmaxf would quiet each operand first).
 __device__ __forceinline__ float kv_max8(const float (&x)[8]) {
     float r;
@@ -284,9 +268,8 @@ __device__ __forceinline__ float kv_max8(const float (&x)[8]) {
     return r;
 }
 
-// A tile's base-2 scores above m - KV_TOP (above 0 while there is no m) from its products
-// u with the rows; m moves if one is too far above it.  inside: every row sees all 32
-// slots.
+// A tile's base-2 scores above m - KV_TOP from its products u with the rows; m moves if one
+// is too far above it.  inside: every row sees all 32 slots.
 template <int S, int CODE, int PARTS, int NC>
 __device__ __forceinline__ void kv_reference(KvWave<S, CODE, PARTS, NC>& w, const floatx4 (&u)[NC][2], float ks, float lv,
                                              bool bad, int slot0, bool inside, const KvAttend& a, int tok0, float* scores,
@@ -296,7 +279,7 @@ __device__ __forceinline__ void kv_reference(KvWave<S, CODE, PARTS, NC>& w, cons
     if (inside && !scores) {
 #pragma unroll
         for (int n = 0; n < NC; n++) {
-            const float f = w.qs[n] * ks, base = w.m[n] == KV_NEG ? lv : lv - (w.m[n] - KV_TOP);
+            const float f = w.qs[n] * ks, base = fmaxf(lv, w.low[n]) - w.t[n];
 #pragma unroll
             for (int j = 0; j < 8; j++) x[n][j] = __builtin_fmaf(u[n][j >> 2][j & 3], f, base);
         }
@@ -306,11 +289,12 @@ __device__ __forceinline__ void kv_reference(KvWave<S, CODE, PARTS, NC>& w, cons
     } else {
 #pragma unroll
         for (int n = 0; n < NC; n++) {
-            const float f = w.qs[n] * ks, base = w.m[n] == KV_NEG ? lv : lv - (w.m[n] - KV_TOP);
+            const float f = w.qs[n] * ks, base = fmaxf(lv, w.low[n]) - w.t[n];
             bool any = inside;
 #pragma unroll
             for (int j = 0; j < 8; j++) x[n][j] = u[n][j >> 2][j & 3] * f;
             if (!inside) {
+                kv_rows_again(w, a, n);
                 // slot0 + 4 g + off sees: lo <= slot < hi
                 const int first = w.lo[n] - slot0 - 4 * g, count = w.hi[n] - w.lo[n];
 #pragma unroll
@@ -344,18 +328,32 @@ __device__ __forceinline__ void kv_reference(KvWave<S, CODE, PARTS, NC>& w, cons
         }
     }
 #pragma unroll
-    for (int n = 0; n < NC; n++) over |= kv_max8(x[n]) > (w.m[n] == KV_NEG ? KV_NEG : KV_TOP + KV_SLACK);
+    for (int n = 0; n < NC; n++) over |= kv_max8(x[n]) > KV_TOP + KV_SLACK;
     if (__any(over)) {
 #pragma unroll
         for (int n = 0; n < NC; n++) {
-            const float was = w.m[n] == KV_NEG ? 0.f : w.m[n] - KV_TOP;
-            const float m1 = fmaxf(w.m[n], kv_max4(kv_max8(x[n])) + was);
-            const float now = m1 == KV_NEG ? 0.f : m1 - KV_TOP;
-            const float f1 = w.m[n] == KV_NEG ? 0.f : exp2f(w.m[n] - m1);
+            const bool none = w.t[n] == KV_START;
+            if (none) {
+                const float f = w.qs[n] * ks, base = fmaxf(lv, w.low[n]);
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    x[n][j] = x[n][j] == KV_NEG ? KV_NEG : __builtin_fmaf(u[n][j >> 2][j & 3], f, base);
+            }
+            const float was = none ? 0.f : w.t[n], best = kv_max4(kv_max8(x[n])) + was - KV_TOP;
+            const float now = fmaxf(w.t[n], best);
+            const float down = none ? KV_NEG : w.t[n] - now, f1 = exp2f(down);
 #pragma unroll
             for (int j = 0; j < 8; j++) x[n][j] += was - now;
-            w.m[n] = m1;
-            w.l[n] *= f1;
+            // S follows the scale that moved m, as far as l stays below 2^100
+            int up = 0;
+            if (now > w.t[n] && lv > w.low[n] + KV_FAR) {
+                up = (int)ceilf(lv - (w.low[n] + KV_FAR));
+                if (!none)
+                    up = max(min(up, 100 - max(__builtin_amdgcn_frexp_expf(kv_max4(w.l[n])), 0) - (int)down), 0);
+                w.s[n] = ldexpf(w.s[n], up), w.low[n] += (float)up;
+            }
+            w.t[n] = now;
+            w.l[n] *= exp2f(down + (float)up);
 #pragma unroll
             for (int j = 0; j < 2 * S; j++) w.o[n][j] *= f1;
         }
@@ -378,7 +376,7 @@ __device__ __forceinline__ void kv_exponents(KvWave<S, CODE, PARTS, NC>& w, cons
             if (PARTS > 1) p1[n][j] = (_Float16)(p - (float)ph);
             sum += p;  // (the rounded ones' sum, by dot products, would cost the logarithm its float32)
         }
-        w.l[n] = __builtin_fmaf(sum, rv, w.l[n]);
+        w.l[n] = __builtin_fmaf(sum, fminf(rv * w.s[n], KV_FAR_F), w.l[n]);
     }
 }
 
@@ -416,9 +414,13 @@ __device__ __forceinline__ void kv_fetch(uint4 (&k)[S], const uint8_t* half) {
     for (int s = 0; s < S; s++) k[s] = __builtin_bit_cast(uint4, ONCE ? __builtin_nontemporal_load(p + s * 64) : p[s * 64]);
 }
 
-// What a part's sum l is multiplied with under reference mx, m being its own; its o goes by
-// 2^(its E less the largest) too.  A part without a score has m -inf and l 0, or l NaN where
-// its scores were NaN.
+// m of a row, -inf if it has seen no slot.
+__device__ __forceinline__ float kv_reached(float t) { return t == KV_START ? KV_NEG : t + KV_TOP; }
+
+// A part leaves its sums o and l, its m less log2 S, and log2 S: of several, l goes by the
+// power of 2 that its m stands below the largest, mx, and o by that and by the power that its
+// S stands below the largest.  A part without a score has m -inf and l 0, or l NaN where its
+// scores were NaN.
 __device__ __forceinline__ float kv_join_factor(float m, float l, float mx) {
     return m == KV_NEG ? 0.f * l : exp2f(m - mx);
 }
@@ -478,7 +480,6 @@ __device__ __forceinline__ KvJob kv_job(const KvDev& c, const KvBatch& b, const 
 template <int S, int CODE, int PARTS, bool ONCE>
 __global__ __launch_bounds__(256, S <= 4 ? 3 : 2) void kv_step_kernel(KvDev c, KvBatch b, KvAttend a) {
     extern __shared__ __align__(16) float lds[];
-    __shared__ int powers[4];  // E of the waves
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
     const KvJob sp = kv_job(c, b, a, 16);
@@ -503,7 +504,6 @@ __global__ __launch_bounds__(256, S <= 4 ? 3 : 2) void kv_step_kernel(KvDev c, K
     kv_load_rows(w, c, b, a, i, h, row0);
     for (int x = 0; x < n; x++) {
         const int t = tw + 4 * x, y = x & 63;
-        if (y == 0) kv_measure(w, info);
         const float ks = kv_lane(info.ks, y), lv = kv_lane(info.lv, y), rv = kv_lane(info.rv, y);
         const bool bad = info.bad >> y & 1;
         if (y == 63 && x + 1 < n) info = kv_tile_infos(c, table, h, t + 4, 4, sp.t1);
@@ -521,23 +521,21 @@ __global__ __launch_bounds__(256, S <= 4 ? 3 : 2) void kv_step_kernel(KvDev c, K
     }
     w.l[0] = kv_sum4(w.l[0]), w.bad[0] = kv_sum4(w.bad[0]);
 
-    // join the four waves: rows of [wave][row][32 S + 4] floats, then (m, l)
+    // join the four waves: rows of [wave][row][32 S + 4] floats, then (m, l) and S
     constexpr int LDO = 32 * S + 4;
     float* ml = lds + 4 * 16 * LDO;
     const int r4 = wave * 16 + col;
 #pragma unroll
     for (int j = 0; j < 2 * S; j++) *(floatx4*)(lds + r4 * LDO + 16 * j + 4 * g) = w.o[0][j] + w.bad[0];
-    if (g == 0) ml[2 * r4] = w.m[0], ml[2 * r4 + 1] = w.l[0];
-    if (lane == 0) powers[wave] = w.e;
+    if (g == 0) ml[2 * r4] = kv_reached(w.t[0]) - (w.low[0] + KV_FAR), ml[2 * r4 + 1] = w.l[0], ml[128 + r4] = w.low[0] + KV_FAR;
     __syncthreads();
-    const int e = max(max(powers[0], powers[1]), max(powers[2], powers[3]));
     for (int u = threadIdx.x; u < 16 * 8 * S; u += 256) {
         const int r = u / (8 * S), d = u % (8 * S) * 4;
         const int row = row0 + r;
         if (row >= rows) break;
-        float mx = KV_NEG;
+        float mx = KV_NEG, top = KV_FIRST;
 #pragma unroll
-        for (int x = 0; x < 4; x++) mx = fmaxf(mx, ml[2 * (x * 16 + r)]);
+        for (int x = 0; x < 4; x++) mx = fmaxf(mx, ml[2 * (x * 16 + r)]), top = fmaxf(top, ml[128 + x * 16 + r]);
         floatx4 o = {0.f, 0.f, 0.f, 0.f};
         float l = 0.f;
 #pragma unroll
@@ -545,17 +543,16 @@ __global__ __launch_bounds__(256, S <= 4 ? 3 : 2) void kv_step_kernel(KvDev c, K
             const int rr = x * 16 + r;
             const float f = kv_join_factor(ml[2 * rr], ml[2 * rr + 1], mx);
             l += f * ml[2 * rr + 1];
-            o += *(const floatx4*)(lds + rr * LDO + d) * ldexpf(f, powers[x] - e);
+            o += *(const floatx4*)(lds + rr * LDO + d) * ldexpf(f, (int)(ml[128 + rr] - top));
         }
         if (sp.whole) {
             const size_t at = kv_row(c, b, a, i, h, row);
             if (d == 0) kv_finish(c, b, a, i, h, row, mx, l);
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            kv_store4<PARTS>(a, at * c.D, d, c.D, o * inv * ldexpf(1.f, kv_power(e)));
+            kv_store4<PARTS>(a, at * c.D, d, c.D, o * inv * ldexpf(1.f, (int)top));
         } else {
             const size_t at = (size_t)blockIdx.x * 16 + r;
-            if (d == 0) a.part_ml[at] = make_float2(mx, l);
-            if (u == 0) a.part_e[blockIdx.x] = e;
+            if (d == 0) a.part_ml[at] = make_float2(mx, l), a.part_s[at] = top;
             *(floatx4*)(a.part_o + at * (32 * S) + d) = o;
         }
     }
@@ -623,6 +620,7 @@ __global__ __launch_bounds__(256, S == 8 ? 1 : 2) void kv_chunk_kernel(KvDev c, 
             uint4* to = a.qop + ((size_t)b.aux[i] * c.H + (size_t)h * ((rows + 15) / 16) + tile) * (PARTS * S * 64);
 #pragma unroll
             for (int x = 0; x < PARTS * S; x++) to[x * 64 + lane] = __builtin_bit_cast(uint4, w.q[n][x / S][x % S]);
+            kv_rows_again(w, a, n);
             if (g == 0 && w.row[n] >= 0) a.qs[kv_head_row(c, b, a, i, h, w.row[n])] = w.qs[n];
         }
     }
@@ -655,10 +653,7 @@ __global__ __launch_bounds__(256, S == 8 ? 1 : 2) void kv_chunk_kernel(KvDev c, 
     int b0 = 0, b1 = 1, b2 = 2;  // buffers of tiles t, t + 1, t + 2
     for (int xt = 0; xt < n_tiles; xt++) {
         const int t = sp.t0 + xt, y = xt & 63;
-        if (y == 0) {
-            if (xt > 0) info = ahead;
-            kv_measure(w, info);
-        }
+        if (y == 0 && xt > 0) info = ahead;
         const bool inside = t * KV_TILE >= all_lo && (t + 1) * KV_TILE <= all_hi && !a.mask;
         const float rv = kv_lane(info.rv, y);
         float z[NC][8];
@@ -698,17 +693,18 @@ __global__ __launch_bounds__(256, S == 8 ? 1 : 2) void kv_chunk_kernel(KvDev c, 
 #pragma unroll
     for (int n = 0; n < NC; n++) {
         w.l[n] = kv_sum4(w.l[n]), w.bad[n] = kv_sum4(w.bad[n]);
+        kv_rows_again(w, a, n);
         if (w.row[n] < 0) continue;
+        const float power = w.low[n] + KV_FAR, m = kv_reached(w.t[n]) - power;
         if (sp.whole) {
             const size_t at = kv_row(c, b, a, i, h, w.row[n]);
-            if (g == 0) kv_finish(c, b, a, i, h, w.row[n], w.m[n], w.l[n]);
-            const float inv = w.l[n] == 0.f ? 0.f : 1.f / w.l[n], power = ldexpf(1.f, kv_power(w.e));
+            if (g == 0) kv_finish(c, b, a, i, h, w.row[n], m, w.l[n]);
+            const float inv = w.l[n] == 0.f ? 0.f : 1.f / w.l[n];
 #pragma unroll
-            for (int j = 0; j < 2 * S; j++) kv_store4<PARTS>(a, at * c.D, 16 * j + 4 * g, c.D, w.o[n][j] * inv * power + w.bad[n]);
+            for (int j = 0; j < 2 * S; j++) kv_store4<PARTS>(a, at * c.D, 16 * j + 4 * g, c.D, w.o[n][j] * inv * w.s[n] + w.bad[n]);
         } else {
             const size_t at = (size_t)blockIdx.x * WG_ROWS + (w.row[n] - wg_row0);
-            if (g == 0) a.part_ml[at] = make_float2(w.m[n], w.l[n]);
-            if (w.row[n] == wg_row0 && g == 0) a.part_e[blockIdx.x] = w.e;  // the four waves': they have the same tiles
+            if (g == 0) a.part_ml[at] = make_float2(m, w.l[n]), a.part_s[at] = power;
 #pragma unroll
             for (int j = 0; j < 2 * S; j++) *(floatx4*)(a.part_o + at * (32 * S) + 16 * j + 4 * g) = w.o[n][j] + w.bad[n];
         }
@@ -739,19 +735,17 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvDev c, KvBatch b, KvAtte
     if (splits <= 1) return;  // the one workgroup has written the rows
     if (WIDE ? row >= rows : (grp >= groups || r >= wg_rows || row >= rows)) return;
     const int row_tiles = b.unit0[i + 1] - b.unit0[i];
-    const int wg_stride = -row_tiles * c.H, wg = (b.aux[i] + u + (b.splits[i] - 1) * row_tiles) * c.H + h;
-    const int64_t stride = (int64_t)wg_stride * wg_rows;  // the first split's parts lie last
-    const int64_t base = (int64_t)wg * wg_rows + r;
-    float mx = KV_NEG;
-    int e = KV_NONE;
+    const int64_t stride = -(int64_t)row_tiles * c.H * wg_rows;  // the first split's parts lie last
+    const int64_t base = ((int64_t)(b.aux[i] + u + (b.splits[i] - 1) * row_tiles) * c.H + h) * wg_rows + r;
+    float mx = KV_NEG, top = KV_FIRST;
     if (WIDE) {
         for (int s = tid & 63; s < splits; s += 64)
-            mx = fmaxf(mx, a.part_ml[base + s * stride].x), e = max(e, a.part_e[wg + s * wg_stride]);
+            mx = fmaxf(mx, a.part_ml[base + s * stride].x), top = fmaxf(top, a.part_s[base + s * stride]);
 #pragma unroll
-        for (int x = 32; x; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x)), e = max(e, __shfl_xor(e, x));
+        for (int x = 32; x; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x)), top = fmaxf(top, __shfl_xor(top, x));
     } else {
         for (int s = 0; s < splits; s++)
-            mx = fmaxf(mx, a.part_ml[base + s * stride].x), e = max(e, a.part_e[wg + s * wg_stride]);
+            mx = fmaxf(mx, a.part_ml[base + s * stride].x), top = fmaxf(top, a.part_s[base + s * stride]);
     }
     floatx4 o = {0.f, 0.f, 0.f, 0.f};
     float l = 0.f;
@@ -761,7 +755,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvDev c, KvBatch b, KvAtte
             const float2 ml = a.part_ml[base + s * stride];
             const float f = kv_join_factor(ml.x, ml.y, mx);
             l += f * ml.y;
-            o += *(const floatx4*)(a.part_o + (base + s * stride) * c.Dp + d4 * 4) * ldexpf(f, a.part_e[wg + s * wg_stride] - e);
+            o += *(const floatx4*)(a.part_o + (base + s * stride) * c.Dp + d4 * 4) * ldexpf(f, (int)(a.part_s[base + s * stride] - top));
         }
     }
     if (WIDE) {
@@ -777,7 +771,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvDev c, KvBatch b, KvAtte
     }
     if (d4 == 0) kv_finish(c, b, a, i, h, row, mx, l);
     const size_t at = kv_row(c, b, a, i, h, row) * c.D;
-    o = o * (l == 0.f ? 0.f : 1.f / l) * ldexpf(1.f, kv_power(e));
+    o = o * (l == 0.f ? 0.f : 1.f / l) * ldexpf(1.f, (int)top);
     if (a.q.type == KV_F32)
         kv_store4<2>(a, at, 4 * d4, c.D, o);
     else
@@ -980,7 +974,7 @@ void attend_s(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s
         hipLaunchKernelGGL((kv_chunk_kernel<S, CODE, PARTS, kv_chunk_nc(S * 32, PARTS)>), grid, dim3(256), 0, s, c, b, a);
         return;
     }
-    const size_t lds = (size_t)4 * 16 * (32 * S + 4 + 2) * 4;
+    const size_t lds = (size_t)4 * 16 * (32 * S + 4 + 3) * 4;
     int most = 0;
     for (int i = 0; i < b.n; i++) most = b.count[i] * a.G > most ? b.count[i] * a.G : most;
     const auto kernel = most <= 16 ? kv_step_kernel<S, CODE, PARTS, true> : kv_step_kernel<S, CODE, PARTS, false>;

@@ -121,7 +121,7 @@ void kv_plan_steps(const int64_t* lens, const int64_t* counts, int n, int heads,
     KvBatch b;
     plan.heads = heads;
     for (int i = 0; i < n; i++) plan.add(lens[i], counts[i], group, 16, true, 0);
-    plan.split(b, false, kPartBytes / (16 * (KV_MAX_DIM * 4 + 8)));
+    plan.split(b, false, kPartBytes / (16 * (KV_MAX_DIM * 4 + 12)));
     for (int i = 0; i < n; i++) splits[i] = b.splits[i], per[i] = b.per[i];
 }
 
@@ -576,14 +576,14 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
         }
         need(plan.units <= kMaxWorkgroups, "too many query rows in one call");
         if (plan.units) {
-            plan.split(b, a.by_rows, kPartBytes / (rows * ((int64_t)dev.Dp * 4 + 8)));
+            plan.split(b, a.by_rows, kPartBytes / (rows * ((int64_t)dev.Dp * 4 + 12)));
             const int64_t groups = plan.groups;
-            a.part_o = nullptr, a.part_ml = nullptr, a.part_e = nullptr, a.scores = nullptr;
+            a.part_o = nullptr, a.part_ml = nullptr, a.part_s = nullptr, a.scores = nullptr;
             if (plan.split_units) {
                 grow(w_part, (size_t)(groups * rows) * dev.Dp);
                 grow(w_ml, (size_t)(groups * rows));
-                grow(w_power, (size_t)groups);
-                a.part_o = w_part.p, a.part_ml = w_ml.p, a.part_e = w_power.p;
+                grow(w_power, (size_t)(groups * rows));
+                a.part_o = w_part.p, a.part_ml = w_ml.p, a.part_s = w_power.p;
             }
             if (keep_scores) {
                 grow(w_scores, (size_t)score_tiles * KV_TILE * dev.H);

@@ -181,7 +181,7 @@ struct KvAttend {
     int chunks = 1, chunk_rows = 0;
     float* part_o = nullptr;   // split attention: partial rows [workgroup, rows, Dp]
     float2* part_ml = nullptr; // and their (max, sum), base 2
-    int* part_e = nullptr;     // [workgroup] the power of 2 that the value scales were divided by
+    float* part_s = nullptr;   // and the power of 2 that their sums are in
     float* scores = nullptr;   // tracked steps: base-2 scores [row, tile, 32] of each (sequence, head)
     int by_rows = 0;           // waves of a workgroup take different rows (else different tiles)
 };

@@ -355,7 +355,7 @@ struct KvCache {
     DevBuf<uint32_t> w_hist;
     DevBuf<uint2> w_counts;
     DevBuf<float2> w_ml;
-    DevBuf<int> w_power;
+    DevBuf<float> w_power;
 
     struct Seq {
         int64_t len = 0, next = 0;   // slots in use; position of the next token

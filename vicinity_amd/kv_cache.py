@@ -148,7 +148,8 @@ class KVCache:
         Sums, logarithms and weights are float32.  16-bit queries are taken exactly and
         their probabilities multiply the values with 11 bits; float32 queries with 22 bits
         of their row's largest element, and so the probabilities; what is below 2^-30 of
-        the largest adds nothing to the result."""
+        the largest adds nothing to the result.  Scores (scale * q k) are float32: they have
+        to stay below 2^24."""
         import torch
 
         ids = self._seqs(seqs)
