@@ -561,8 +561,8 @@ __global__ __launch_bounds__(256, S <= 4 ? 3 : 2) void kv_step_kernel(KvDev c, K
 // Many rows: the four waves of a workgroup take 4 * NC * 16 rows and every tile.  A tile's
 // codes are converted once, a quarter by each wave, and shared as half-precision operands
 // through LDS (three buffers, one barrier to a tile); an operand read feeds NC products.
-// 2048 tokens over 32768 slots, 8 x 4 x 128: the vector unit is busy 61% of the time and
-// the matrix unit 42%; over 16384 slots 970 TFLOP/s, 760 to 630 at other widths, and 400 to
+// 2048 tokens over 32768 slots, 8 x 4 x 128: the vector unit is busy 63% of the time and
+// the matrix unit 42%; over 16384 slots 980 TFLOP/s, 650 to 810 at other widths, and 400 to
 // 560 in float32, which has two products for one.
 template <int S, int CODE, int PARTS, int NC>
 __global__ __launch_bounds__(256, S == 8 ? 1 : 2) void kv_chunk_kernel(KvDev c, KvBatch b, KvAttend a) {

@@ -118,7 +118,9 @@ __global__ __launch_bounds__(256) void kv_table_kernel(int* table, KvRuns r) {
 // thread loads its pieces of 8 dims once and keeps them (HOLD of them; blocks with more are
 // read a second time, from L2) until the scale is known; the codes are put in order in LDS
 // and leave in 16-byte pieces.  A few tokens in a begun block that keeps its scale go to
-// their bytes directly.  Bound by the bytes in and out.
+// their bytes directly.  Bound by the bytes in and out, one workgroup's load, reduction and codes
+// after another: 16384 tokens of 8 x 128 16-bit elements 33 us, 3.0 TB/s, float32 41 us, 4.1;
+// of 8 x 256 in 256-slot blocks, read twice, 97 us, 2.1, and 115 us, 2.9.
 constexpr int KV_HOLD = 8;
 constexpr int KV_FEW = 4;
 
@@ -630,7 +632,9 @@ __global__ __launch_bounds__(256) void kv_zero_kernel(uint4* p, int n) {
 
 // One workgroup: the keys or the values of one block of one head of the result, gathered
 // from L2, 8 bytes of a key or one byte of a value at a time.  (Source tiles brought to LDS
-// whole: 72 us for 61, and 113 for 71 where one slot in six stays.)
+// whole: 72 us for 61, and 113 for 71 where one slot in six stays.)  31 sequences cut to 1024
+// slots, 8 x 128: 119 MB come in, for lines hold slots that leave as well, and 56 go out in
+// 41 us.
 __global__ __launch_bounds__(256) void kv_move_kernel(KvDev c, KvBatch b, KvEvict e) {
     __shared__ const uint8_t* from[256];  // a slot's tile half
     __shared__ int slots[256];            // and its place there
