@@ -447,6 +447,28 @@ int vgpu_kv_read(vgpu_kv *h, const int32_t *seqs, const int64_t *first, const in
  * forgotten token raised, or made NaN. */
 int vgpu_kv_truncate(vgpu_kv *h, const int32_t *seqs, const int64_t *lengths, size_t n);
 
+/* Each sequence into[i] (all different) becomes a continuation of its own of the
+ * first lengths[i] slots of seqs[i] (lengths NULL: all of them) as they stood before
+ * the call, with positions and weights; what it held is forgotten.  A sequence may
+ * be continued by several, and be among into itself.  Sequences that continue one
+ * another hold the same blocks, each with a count of its holders: a block returns
+ * to the pool when the last one lets it go (truncate, evict, fork), and is copied
+ * for a holder that writes into it while others hold it too: append into a begun
+ * block, and attend with `track`, which takes every block of its sequences.  These
+ * need the blocks for it, else VGPU_ERR_OUT_OF_MEMORY, and nothing is changed; the
+ * last holder keeps a block without a copy.  copy != 0: blocks of its own at once
+ * (free ones before the call).  Either way each sequence reads, attends and changes
+ * as if it were alone. */
+int vgpu_kv_fork(vgpu_kv *h, const int32_t *seqs, const int32_t *into, const int64_t *lengths,
+                 size_t n, int copy, void *stream);
+
+/* Move the used blocks to the front of the pool (num_blocks 0, or as many as there
+ * are), or to a pool of num_blocks blocks, not fewer than are used, that takes the
+ * old one's place: it is allocated beside the old one, which is then freed, and that
+ * waits for the device.  max_blocks stays.  *moved (or NULL): blocks that moved.
+ * Sequences keep what they hold. */
+int vgpu_kv_compact(vgpu_kv *h, size_t num_blocks, size_t *moved, void *stream);
+
 /* ---- per-kernel test entry points (host buffers) -------------------------- */
 /* Host steps of the build, no device needed.  Inverted lists from list
  * labels (search.rs:624-657): offsets u64[L+1], list_ids u32[n]; a label >= L

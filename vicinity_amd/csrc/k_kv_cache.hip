@@ -114,6 +114,58 @@ __global__ __launch_bounds__(256) void kv_table_kernel(int* table, KvRuns r) {
     for (int j = threadIdx.x; j < r.count[i]; j += blockDim.x) table[r.at[i] + j] = r.block[i] + j;
 }
 
+constexpr int KV_COLUMNS = 2048;  // of a workgroup that goes over table rows
+__global__ __launch_bounds__(256) void kv_rows_kernel(const int* from, int* to, int W, KvRows r) {
+    const int i = blockIdx.y;
+    const int end = min(r.end[i], r.first[i] + ((int)blockIdx.x + 1) * KV_COLUMNS);
+    for (int j = r.first[i] + blockIdx.x * KV_COLUMNS + threadIdx.x; j < end; j += 256)
+        to[(size_t)r.to[i] * W + j] = from[(size_t)r.from[i] * W + j];
+}
+
+__global__ __launch_bounds__(256) void kv_rename_kernel(int* table, int W, KvRows r, const int* map, int above) {
+    const int i = blockIdx.y;
+    const int end = min(r.end[i], r.first[i] + ((int)blockIdx.x + 1) * KV_COLUMNS);
+    for (int j = r.first[i] + blockIdx.x * KV_COLUMNS + threadIdx.x; j < end; j += 256) {
+        int* at = table + (size_t)r.to[i] * W + j;
+        if (*at >= above) *at = map[*at];
+    }
+}
+
+// Blocks copied whole: a workgroup takes 32 KiB of a block's codes (a block is contiguous, and
+// a multiple of 4 KiB); the first of a block also takes its scales, positions and weights.
+__global__ __launch_bounds__(256) void kv_moves_kernel(KvDev from, KvDev to, KvMoves m, int pieces, int* map) {
+    const int tid = threadIdx.x, unit = blockIdx.x / pieces, piece = blockIdx.x - unit * pieces;
+    int lo = 0, hi = m.n;  // the run: unit0[lo] <= unit < unit0[lo + 1]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (m.unit0[mid] <= unit) lo = mid;
+        else hi = mid;
+    }
+    const int src = m.src[lo] + unit - m.unit0[lo], dst = m.dst[lo] + unit - m.unit0[lo];
+    const size_t bytes = (size_t)from.H * from.B * 2 * from.Dp;
+    const uint4* in = (const uint4*)(from.pool + (size_t)src * bytes);
+    uint4* out = (uint4*)(to.pool + (size_t)dst * bytes);
+    const int at = piece * (KV_COPY * 256) + tid, end = (int)(bytes / 16);
+    uint4 x[KV_COPY];
+#pragma unroll
+    for (int j = 0; j < KV_COPY; j++)
+        if (at + j * 256 < end) x[j] = in[at + j * 256];
+#pragma unroll
+    for (int j = 0; j < KV_COPY; j++)
+        if (at + j * 256 < end) out[at + j * 256] = x[j];
+    if (piece) return;
+    if (map && tid == 0) map[src] = dst;
+    for (int h = tid; h < from.H; h += 256) {
+        to.kscale[(size_t)dst * from.H + h] = from.kscale[(size_t)src * from.H + h];
+        to.vscale[(size_t)dst * from.H + h] = from.vscale[(size_t)src * from.H + h];
+    }
+    const int slots = from.H * from.B;
+    for (int j = tid; j < slots; j += 256) {
+        to.positions[(size_t)dst * slots + j] = from.positions[(size_t)src * slots + j];
+        to.weights[(size_t)dst * slots + j] = from.weights[(size_t)src * slots + j];
+    }
+}
+
 // One workgroup: the keys or the values of one (block, head) that new tokens enter.  Each
 // thread loads its pieces of 8 dims once and keeps them (HOLD of them; blocks with more are
 // read a second time, from L2) until the scale is known; the codes are put in order in LDS
@@ -756,6 +808,28 @@ __global__ __launch_bounds__(256) void kv_dropped_rest_kernel(KvDev c, KvBatch b
 
 void launch_kv_table(int* table, const KvRuns& r, hipStream_t s) {
     if (r.n > 0) hipLaunchKernelGGL(kv_table_kernel, dim3(r.n), dim3(256), 0, s, table, r);
+}
+
+static dim3 rows_grid(const KvRows& r) {
+    int most = 0;
+    for (int i = 0; i < r.n; i++) most = r.end[i] - r.first[i] > most ? r.end[i] - r.first[i] : most;
+    return dim3((unsigned)((most + KV_COLUMNS - 1) / KV_COLUMNS), (unsigned)r.n);
+}
+
+void launch_kv_rows(const KvDev& c, const int* from, int* to, const KvRows& r, hipStream_t s) {
+    const dim3 grid = rows_grid(r);
+    if (grid.x && grid.y) hipLaunchKernelGGL(kv_rows_kernel, grid, dim3(256), 0, s, from, to, c.W, r);
+}
+
+void launch_kv_rename(const KvDev& c, const KvRows& r, const int* map, int above, hipStream_t s) {
+    const dim3 grid = rows_grid(r);
+    if (grid.x && grid.y) hipLaunchKernelGGL(kv_rename_kernel, grid, dim3(256), 0, s, c.table, c.W, r, map, above);
+}
+
+void launch_kv_moves(const KvDev& from, const KvDev& to, const KvMoves& m, int* map, hipStream_t s) {
+    if (!m.n) return;
+    const int pieces = kv_move_pieces(from);
+    hipLaunchKernelGGL(kv_moves_kernel, dim3((unsigned)(m.unit0[m.n] * pieces)), dim3(256), 0, s, from, to, m, pieces, map);
 }
 
 void launch_kv_append(const KvDev& c, const KvBatch& b, const KvTensor& k, const KvTensor& v,

@@ -613,6 +613,24 @@ int vgpu_kv_truncate(vgpu_kv* h, const int32_t* seqs, const int64_t* lengths, si
     });
 }
 
+int vgpu_kv_fork(vgpu_kv* h, const int32_t* seqs, const int32_t* into, const int64_t* lengths, size_t n, int copy,
+                 void* stream) {
+    return guard([&] {
+        need(h && (n == 0 || (seqs && into)), VGPU_ERR_INVALID_PARAMETER, "null argument");
+        std::lock_guard<std::mutex> lk(h->kv->mu);
+        h->kv->fork(seqs, into, lengths, n, copy != 0, (hipStream_t)stream);
+    });
+}
+
+int vgpu_kv_compact(vgpu_kv* h, size_t num_blocks, size_t* moved, void* stream) {
+    return guard([&] {
+        need(h, VGPU_ERR_INVALID_PARAMETER, "null argument");
+        std::lock_guard<std::mutex> lk(h->kv->mu);
+        const size_t count = h->kv->compact(num_blocks, (hipStream_t)stream);
+        if (moved) *moved = count;
+    });
+}
+
 /* ---- per-kernel test entry points ---------------------------------------- */
 
 int vgpu_test_host_kv_splits(const int64_t* lens, const int64_t* counts, size_t n, size_t heads, size_t group,

@@ -43,6 +43,9 @@ constexpr int64_t kScoreRows = 48;
 // 256 rows: 29 and 16 us; measured in bfloat16 there, and taken for all).
 constexpr int64_t kChunkTiles = 4096;
 
+// Entries of one fork's row of the table that go as kernel arguments; more are copied on the GPU.
+constexpr size_t kRowRuns = 64;
+
 // The row tiles of one launch's sequences, and the tiles that each goes over.
 struct KvPlan {
     int n = 0, heads = 1;
@@ -160,6 +163,7 @@ KvCache::KvCache(const vgpu_kv_params& p) : params(p) {
     seen.assign(p.num_seqs, 0);
     free_blocks.resize(p.num_blocks);
     for (size_t i = 0; i < p.num_blocks; i++) free_blocks[i] = (int)(p.num_blocks - 1 - i);
+    holders.assign(p.num_blocks, 0);
 }
 
 KvCache::~KvCache() {
@@ -173,7 +177,7 @@ KvCache::~KvCache() {
 
 size_t KvCache::device_bytes() const {
     return pool.bytes() + kscale.bytes() + vscale.bytes() + weights.bytes() + positions.bytes() + table.bytes() +
-           table2.bytes() + w_kept.bytes() + w_gone.bytes() + w_part.bytes() + w_scores.bytes() + w_lse2.bytes() +
+           table2.bytes() + w_map.bytes() + w_kept.bytes() + w_gone.bytes() + w_part.bytes() + w_scores.bytes() + w_lse2.bytes() +
            w_ml.bytes() + w_power.bytes() + w_hist.bytes() + w_counts.bytes() + w_qop.bytes() + w_qs.bytes() + w_wpart.bytes();
 }
 
@@ -218,31 +222,108 @@ KvTensor KvCache::tensor(const vgpu_tensor3& t, const char* name) const {
     return x;
 }
 
+// One more entry of the table.
+static void add_run(KvRuns& runs, size_t at, int block, int* tab, hipStream_t s) {
+    if (runs.n && runs.at[runs.n - 1] + runs.count[runs.n - 1] == at &&
+        runs.block[runs.n - 1] + runs.count[runs.n - 1] == block) {
+        runs.count[runs.n - 1]++;
+        return;
+    }
+    if (runs.n == KvRuns::MAX) {
+        launch_kv_table(tab, runs, s);
+        runs.n = 0;
+    }
+    runs.at[runs.n] = at, runs.block[runs.n] = block, runs.count[runs.n] = 1;
+    runs.n++;
+}
+
+// Copies of blocks, gathered into launches.
+struct KvCopies {
+    const KvDev &from, &to;
+    int* map;
+    hipStream_t s;
+    int64_t most;  // blocks of one launch
+    KvMoves m;
+    KvCopies(const KvDev& a, const KvDev& b, int* names, hipStream_t stream) : from(a), to(b), map(names), s(stream) {
+        most = kMaxWorkgroups / kv_move_pieces(a);
+        m.unit0[0] = 0;
+    }
+    void add(int src, int dst) {
+        if (m.unit0[m.n] == most) flush();
+        const int i = m.n - 1;
+        if (m.n && m.src[i] + m.unit0[i + 1] - m.unit0[i] == src && m.dst[i] + m.unit0[i + 1] - m.unit0[i] == dst) {
+            m.unit0[i + 1]++;
+        } else {
+            if (m.n == KvMoves::MAX) flush();
+            m.src[m.n] = src, m.dst[m.n] = dst, m.unit0[m.n + 1] = m.unit0[m.n] + 1;
+            m.n++;
+        }
+    }
+    void flush() {
+        launch_kv_moves(from, to, m, map, s);
+        m.n = 0;
+    }
+};
+
+int KvCache::take_block() {
+    const int block = free_blocks.back();
+    free_blocks.pop_back();
+    holders[block] = 1;
+    return block;
+}
+
+void KvCache::let_go(int block) {
+    if (--holders[block] == 0) free_blocks.push_back(block);
+}
+
 void KvCache::take_blocks(std::vector<int>& out, size_t count, size_t row, int* tab, KvRuns& runs, hipStream_t s) {
     for (size_t j = 0; j < count; j++) {
-        const int block = free_blocks.back();
-        const size_t at = row * (size_t)dev.W + out.size();
-        if (runs.n && runs.at[runs.n - 1] + runs.count[runs.n - 1] == at &&
-            runs.block[runs.n - 1] + runs.count[runs.n - 1] == block) {
-            runs.count[runs.n - 1]++;
-        } else {
-            if (runs.n == KvRuns::MAX) {
-                launch_kv_table(tab, runs, s);
-                runs.n = 0;
-            }
-            runs.at[runs.n] = at, runs.block[runs.n] = block, runs.count[runs.n] = 1;
-            runs.n++;
-        }
+        const int block = take_block();
+        add_run(runs, row * (size_t)dev.W + out.size(), block, tab, s);
         out.push_back(block);
-        free_blocks.pop_back();
     }
 }
 
 void KvCache::release_blocks(std::vector<int>& blocks, size_t keep) {
     while (blocks.size() > keep) {
-        free_blocks.push_back(blocks.back());
+        let_go(blocks.back());
         blocks.pop_back();
     }
+}
+
+size_t KvCache::shared_blocks(const int32_t* ids, const int64_t* first, size_t n) {
+    // as own_blocks will find them: of the batch's holders of a block, the last one keeps it
+    size_t count = 0;
+    for (size_t i = 0; i < n; i++) {
+        const std::vector<int>& b = seqs[ids[i]].blocks;
+        for (size_t j = (size_t)first[i]; j < b.size(); j++)
+            if (holders[b[j]] > 1) holders[b[j]]--, count++;
+            else holders[b[j]] = -holders[b[j]];  // kept
+    }
+    // and back
+    for (size_t i = n; i-- > 0;) {
+        const std::vector<int>& b = seqs[ids[i]].blocks;
+        for (size_t j = (size_t)first[i]; j < b.size(); j++)
+            if (holders[b[j]] < 0) holders[b[j]] = -holders[b[j]];
+            else holders[b[j]]++;
+    }
+    return count;
+}
+
+void KvCache::own_blocks(const int32_t* ids, const int64_t* first, size_t n, KvRuns& runs, hipStream_t s) {
+    KvCopies copies(dev, dev, nullptr, s);
+    for (size_t i = 0; i < n; i++) {
+        std::vector<int>& b = seqs[ids[i]].blocks;
+        for (size_t j = (size_t)first[i]; j < b.size(); j++) {
+            if (holders[b[j]] <= 1) continue;
+            const int block = take_block();
+            copies.add(b[j], block);
+            add_run(runs, (size_t)ids[i] * (size_t)dev.W + j, block, table.p, s);
+            let_go(b[j]);
+            b[j] = block;
+        }
+    }
+    copies.flush();
 }
 
 void KvCache::append(const int32_t* ids, const int64_t* counts, size_t n, const vgpu_tensor3& k, const vgpu_tensor3& v,
@@ -253,8 +334,10 @@ void KvCache::append(const int32_t* ids, const int64_t* counts, size_t n, const 
     const KvTensor kt = tensor(k, "k"), vt = tensor(v, "v");
     int64_t tokens = 0;
     size_t want = 0;
+    std::vector<int64_t> begun(n);  // the block that the first new token enters
     for (size_t i = 0; i < n; i++) {
         const Seq& q = seqs[ids[i]];
+        begun[i] = counts[i] ? q.len >> dev.shift : (int64_t)q.blocks.size();
         need(counts[i] >= 0 && counts[i] <= INT_MAX / 2, "counts must not be negative, nor above 2^30");
         tokens += counts[i];
         need(tokens <= INT_MAX / 2, "more than 2^30 tokens in one call");
@@ -267,18 +350,19 @@ void KvCache::append(const int32_t* ids, const int64_t* counts, size_t n, const 
         want += total - q.blocks.size();
     }
     need(!tokens || (k.data && v.data), "null argument");
+    want += shared_blocks(ids, begun.data(), n);
     need(want <= free_blocks.size(),
          "the cache needs " + std::to_string(want) + " more blocks and has " + std::to_string(free_blocks.size()),
          VGPU_ERR_OUT_OF_MEMORY);
     for (size_t i = 0; i < n; i++) seqs[ids[i]].blocks.reserve(blocks_of(seqs[ids[i]].len + counts[i]));
     KvRuns runs;
+    own_blocks(ids, begun.data(), n, runs, s);
     for (size_t i = 0; i < n; i++) {
         Seq& q = seqs[ids[i]];
         const size_t more = blocks_of(q.len + counts[i]) - q.blocks.size();
         // one block touched: the append itself writes the table
         if (more == 1 && q.len % dev.B == 0 && counts[i] <= dev.B) {
-            q.blocks.push_back(free_blocks.back());
-            free_blocks.pop_back();
+            q.blocks.push_back(take_block());
         } else {
             take_blocks(q.blocks, more, ids[i], table.p, runs, s);
         }
@@ -369,6 +453,178 @@ void KvCache::truncate(const int32_t* ids, const int64_t* lengths, size_t n) {
     }
 }
 
+void KvCache::fork(const int32_t* ids, const int32_t* into, const int64_t* lengths, size_t n, bool copy, hipStream_t s) {
+    check_call(s);
+    check_ids(*this, seen, into, n);
+    size_t want = 0;
+    const auto slots = [&](size_t i) { return lengths ? lengths[i] : seqs[ids[i]].len; };
+    for (size_t i = 0; i < n; i++) {
+        need(ids[i] >= 0 && (size_t)ids[i] < seqs.size(),
+             "sequence " + std::to_string(ids[i]) + " out of range [0, " + std::to_string(seqs.size()) + ")");
+        need(slots(i) >= 0 && slots(i) <= seqs[ids[i]].len,
+             "length " + std::to_string(slots(i)) + " outside sequence " + std::to_string(ids[i]) + " of length " +
+                 std::to_string(seqs[ids[i]].len));
+        if (copy) want += blocks_of(slots(i));
+    }
+    need(want <= free_blocks.size(),
+         "the copies need " + std::to_string(want) + " free blocks, the cache has " + std::to_string(free_blocks.size()),
+         VGPU_ERR_OUT_OF_MEMORY);
+    // The table rows to be written: by runs where few entries differ, else row by row, through
+    // the second table where one row is both read and written.
+    struct Next {
+        Seq q;
+        size_t common;  // leading blocks that the sequence holds already
+        bool row;
+    };
+    std::vector<Next> next(n);
+    bool rows = false, crossed = false;
+    for (size_t i = 0; i < n; i++) {
+        const Seq& from = seqs[ids[i]];
+        const std::vector<int>& old = seqs[into[i]].blocks;
+        Next& x = next[i];
+        x.q.len = slots(i);
+        x.q.next = x.q.len ? from.next - (from.len - x.q.len) : 0;
+        const size_t count = blocks_of(x.q.len);
+        if (copy) {
+            x.q.blocks.reserve(count);
+            continue;
+        }
+        x.q.blocks.assign(from.blocks.begin(), from.blocks.begin() + (ptrdiff_t)count);
+        // where both hold a block they hold all before it
+        size_t lo = 0, hi = std::min(count, old.size());
+        while (lo < hi) {
+            const size_t mid = (lo + hi) / 2;
+            if (old[mid] == from.blocks[mid]) lo = mid + 1;
+            else hi = mid;
+        }
+        x.common = lo;
+        x.row = count - lo > kRowRuns;
+        rows = rows || x.row;
+    }
+    if (rows) {
+        for (size_t i = 0; i < n; i++) seen[into[i]] = 1;
+        for (size_t i = 0; i < n; i++) crossed = crossed || (next[i].row && seen[ids[i]] && ids[i] != into[i]);
+        for (size_t i = 0; i < n; i++) seen[into[i]] = 0;
+        if (crossed) table2.reserve(table.n);
+    }
+    const auto copy_rows = [&](const int* from, int* to, bool back) {
+        KvRows r;
+        for (size_t i = 0; i < n; i++) {
+            if (!next[i].row) continue;
+            if (r.n == KV_BATCH) {
+                launch_kv_rows(dev, from, to, r, s);
+                r.n = 0;
+            }
+            r.from[r.n] = back ? into[i] : ids[i], r.to[r.n] = into[i];
+            r.first[r.n] = (int)next[i].common, r.end[r.n] = (int)next[i].q.blocks.size();
+            r.n++;
+        }
+        launch_kv_rows(dev, from, to, r, s);
+    };
+    if (rows) copy_rows(table.p, crossed ? table2.p : table.p, false);
+    if (crossed) copy_rows(table2.p, table.p, true);
+    KvRuns runs;
+    if (copy) {
+        KvCopies copies(dev, dev, nullptr, s);
+        for (size_t i = 0; i < n; i++) {
+            const size_t count = blocks_of(next[i].q.len);
+            take_blocks(next[i].q.blocks, count, into[i], table.p, runs, s);
+            for (size_t j = 0; j < count; j++) copies.add(seqs[ids[i]].blocks[j], next[i].q.blocks[j]);
+        }
+        copies.flush();
+    } else {
+        for (size_t i = 0; i < n; i++) {
+            const std::vector<int>& b = next[i].q.blocks;
+            for (size_t j = next[i].common; j < b.size(); j++) {
+                holders[b[j]]++;
+                if (!next[i].row) add_run(runs, (size_t)into[i] * (size_t)dev.W + j, b[j], table.p, s);
+            }
+        }
+    }
+    launch_kv_table(table.p, runs, s);
+    // what the sequences held, beyond what they keep
+    for (size_t i = 0; i < n; i++) {
+        Seq& q = seqs[into[i]];
+        release_blocks(q.blocks, copy ? 0 : next[i].common);
+        q = std::move(next[i].q);
+    }
+    VGPU_HIP(hipGetLastError());
+}
+
+size_t KvCache::compact(size_t num_blocks, hipStream_t s) {
+    check_call(s);
+    const size_t old_blocks = params.num_blocks, used = old_blocks - free_blocks.size();
+    if (!num_blocks) num_blocks = old_blocks;
+    need(num_blocks <= (size_t)1 << 30, "num_blocks must be in the range 1..=2^30");
+    need(num_blocks >= used, "the cache holds " + std::to_string(used) + " blocks, more than num_blocks (" +
+                                 std::to_string(num_blocks) + ")");
+    const bool other = num_blocks != old_blocks;
+    // old numbers of the blocks 0 .. used - 1, and the new number of each old one
+    std::vector<int> to(old_blocks, -1), from(used, -1);
+    size_t moved = 0;
+    if (other) {  // in the order of the sequences
+        for (const Seq& q : seqs)
+            for (int b : q.blocks)
+                if (to[b] < 0) to[b] = (int)moved, from[moved++] = b;
+    } else {  // those behind fill the gaps
+        size_t gap = 0;
+        for (size_t b = used; b < old_blocks; b++) {
+            if (!holders[b]) continue;
+            while (holders[gap]) gap++;
+            to[b] = (int)gap, from[gap++] = (int)b, moved++;
+        }
+        if (!moved) return 0;
+    }
+    std::vector<int> fresh_free, fresh_holders(num_blocks, 0);
+    fresh_free.reserve(num_blocks);
+    DevBuf<uint8_t> new_pool;
+    DevBuf<float> new_k, new_v, new_w;
+    DevBuf<int> new_pos;
+    KvDev now = dev;
+    if (other) {
+        const size_t parts = num_blocks * params.num_heads, count = parts * params.block_tokens;
+        new_pool.reserve(count * 2 * dev.Dp);
+        new_k.reserve(parts), new_v.reserve(parts);
+        new_pos.reserve(count), new_w.reserve(count);
+        now.pool = new_pool.p, now.kscale = new_k.p, now.vscale = new_v.p;
+        now.positions = new_pos.p, now.weights = new_w.p;
+    }
+    w_map.reserve(old_blocks);
+    const int above = other ? 0 : (int)used;  // blocks from here on have new numbers
+    KvCopies copies(dev, now, w_map.p, s);
+    for (size_t b = 0; b < used; b++)
+        if (from[b] >= 0) copies.add(from[b], (int)b);
+    copies.flush();
+    KvRows r;
+    for (size_t i = 0; i < seqs.size(); i++) {
+        std::vector<int>& b = seqs[i].blocks;
+        size_t first = b.size(), end = 0;
+        for (size_t j = 0; j < b.size(); j++)
+            if (b[j] >= above) first = std::min(first, j), end = j + 1;
+        if (first >= end) continue;
+        if (r.n == KV_BATCH) {
+            launch_kv_rename(dev, r, w_map.p, above, s);
+            r.n = 0;
+        }
+        r.to[r.n] = r.from[r.n] = (int)i, r.first[r.n] = (int)first, r.end[r.n] = (int)end;
+        r.n++;
+        for (size_t j = first; j < end; j++)
+            if (b[j] >= above) b[j] = to[b[j]];
+    }
+    launch_kv_rename(dev, r, w_map.p, above, s);
+    for (size_t b = 0; b < used; b++) fresh_holders[b] = holders[from[b] >= 0 ? (size_t)from[b] : b];
+    for (size_t b = num_blocks; b > used; b--) fresh_free.push_back((int)b - 1);
+    holders.swap(fresh_holders);
+    free_blocks.swap(fresh_free);
+    if (other) {
+        pool.swap(new_pool), kscale.swap(new_k), vscale.swap(new_v), positions.swap(new_pos), weights.swap(new_w);
+        dev = now;
+        params.num_blocks = num_blocks;
+    }
+    VGPU_HIP(hipGetLastError());
+    return moved;
+}
+
 void KvCache::evict(const int32_t* ids, const int32_t* into, size_t n, size_t budget, size_t recent,
                     size_t num_dropped, int32_t* dpos, float* dk, float* dv, hipStream_t s) {
     check_call(s);
@@ -385,20 +641,36 @@ void KvCache::evict(const int32_t* ids, const int32_t* into, size_t n, size_t bu
             need(seqs[into[i]].len == 0, "sequence " + std::to_string(into[i]) + " is not empty");
     }
     const auto stays = [&](size_t i) { return std::min<int64_t>(seqs[ids[i]].len, (int64_t)budget); };
-    // does the pool hold the new blocks, given what comes back on the way?
+    // Does the pool hold the new blocks, given what comes back on the way?
+    std::vector<int> gone;  // blocks that the sequences before have let go
+    if (!into) {
+        size_t all = 0;
+        for (size_t i = 0; i < n; i++) all += seqs[ids[i]].blocks.size();
+        gone.reserve(all);
+    }
+    std::string bad;
+    int code = VGPU_ERR_INVALID_PARAMETER;
     size_t have = free_blocks.size();
-    for (size_t i = 0; i < n; i++) {
+    for (size_t i = 0; i < n && bad.empty(); i++) {
         const Seq& q = seqs[ids[i]];
-        need(!drops || q.len - stays(i) <= (int64_t)num_dropped,
-             "num_dropped is below what leaves sequence " + std::to_string(ids[i]));
+        if (drops && q.len - stays(i) > (int64_t)num_dropped)
+            bad = "num_dropped is below what leaves sequence " + std::to_string(ids[i]);
         if (!into && q.len <= (int64_t)budget) continue;
         const size_t take = blocks_of(stays(i));
-        need((int64_t)take * dev.H * 2 <= kMaxWorkgroups, "too many slots of one sequence in one call");
-        need(take <= have, "the cut sequences need " + std::to_string(take) + " free blocks and find " +
-                               std::to_string(have), VGPU_ERR_OUT_OF_MEMORY);
+        if ((int64_t)take * dev.H * 2 > kMaxWorkgroups) bad = "too many slots of one sequence in one call";
+        if (take > have && bad.empty()) {
+            bad = "the cut sequences need " + std::to_string(take) + " free blocks and find " + std::to_string(have);
+            code = VGPU_ERR_OUT_OF_MEMORY;
+        }
         have -= take;
-        if (!into) have += q.blocks.size();
+        if (into) continue;
+        for (int block : q.blocks) {
+            if (--holders[block] == 0) have++;
+            gone.push_back(block);
+        }
     }
+    for (int block : gone) holders[block]++;
+    need(bad.empty(), bad, code);
     const int drop = drops ? (int)num_dropped : 0;
     need((int64_t)dev.H * drop <= INT_MAX / KV_BATCH && (int64_t)n * drop <= INT_MAX,
          "too many dropped slots in one call");
@@ -531,6 +803,15 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
     a.by_rows = a.track ? most > kScoreRows : most > chunk_rows * 3 / 4 && chunk_tiles >= kChunkTiles;
     const bool keep_scores = a.track && !a.by_rows;
     if (a.track) {
+        // weights are written to every slot: the blocks have to be the sequences' own
+        const std::vector<int64_t> all(n, 0);
+        const size_t want = shared_blocks(ids, all.data(), n);
+        need(want <= free_blocks.size(),
+             "weights of shared blocks need " + std::to_string(want) + " more blocks, the cache has " +
+                 std::to_string(free_blocks.size()), VGPU_ERR_OUT_OF_MEMORY);
+        KvRuns runs;
+        own_blocks(ids, all.data(), n, runs, s);
+        launch_kv_table(table.p, runs, s);
         grow(w_lse2, (size_t)tokens * q.num_q_heads);
         a.lse2 = w_lse2.p;
         if (!keep_scores) {

@@ -124,6 +124,32 @@ struct KvRuns {
 };
 void launch_kv_table(int* table, const KvRuns& r, hipStream_t s);
 
+// Rows of the table: columns first[i] .. end[i] - 1 of row from[i] of one go to row to[i] of
+// another.
+struct KvRows {
+    int n = 0;
+    int from[KV_BATCH], to[KV_BATCH], first[KV_BATCH], end[KV_BATCH];
+};
+void launch_kv_rows(const KvDev& c, const int* from, int* to, const KvRows& r, hipStream_t s);
+
+// Blocks copied whole, with scales, positions and weights: runs of count blocks from src[i]
+// on to dst[i] and after.  unit0 counts blocks.
+struct KvMoves {
+    static constexpr int MAX = 384;
+    int n = 0;
+    int src[MAX], dst[MAX], unit0[MAX + 1];
+};
+// Workgroups that a block's copy takes, 32 KiB of its codes each.
+constexpr int KV_COPY = 8;  // 16-byte pieces of a thread
+inline int kv_move_pieces(const KvDev& c) {
+    const int64_t bytes = (int64_t)c.H * c.B * 2 * c.Dp;
+    return (int)((bytes + KV_COPY * 4096 - 1) / (KV_COPY * 4096));
+}
+// map (or null): map[block] becomes the block's new number.
+void launch_kv_moves(const KvDev& from, const KvDev& to, const KvMoves& m, int* map, hipStream_t s);
+// Entries of rows to[i], columns first[i] .. end[i] - 1: those not below `above` become map[entry].
+void launch_kv_rename(const KvDev& c, const KvRows& r, const int* map, int above, hipStream_t s);
+
 void launch_kv_append(const KvDev& c, const KvBatch& b, const KvTensor& k, const KvTensor& v,
                       const int* positions, const float* weights, hipStream_t s);
 

@@ -48,6 +48,7 @@ struct DevBuf {
         n = 0;
     }
     size_t bytes() const { return p ? n * sizeof(T) : 0; }
+    void swap(DevBuf& o) { std::swap(p, o.p), std::swap(n, o.n); }
     // Grow-only allocation (contents are not preserved on growth).
     void reserve(size_t count) {
         if (count <= n && p) return;
@@ -348,7 +349,8 @@ struct KvCache {
     DevBuf<uint8_t> pool;
     DevBuf<float> kscale, vscale, weights;
     DevBuf<int> positions, table;
-    DevBuf<int> table2;              // eviction in place: the new blocks
+    DevBuf<int> table2;              // eviction in place, forks of one another: the new blocks
+    DevBuf<int> w_map;               // compaction: new numbers of blocks
     DevBuf<int> w_kept, w_gone;      // eviction: slots that stay, slots that leave
     DevBuf<float> w_part, w_scores, w_lse2, w_qs, w_wpart;
     DevBuf<uint4> w_qop;
@@ -363,6 +365,9 @@ struct KvCache {
     };
     std::vector<Seq> seqs;
     std::vector<int> free_blocks;    // taken from the back
+    // Sequences that hold a block.  Only forks share blocks, a parent's first ones: so where two
+    // sequences hold the same block, it is the same slots of both, and so are all before it.
+    std::vector<int> holders;
     std::vector<uint8_t> seen;       // batch checks
     std::mutex mu;
 
@@ -376,12 +381,20 @@ struct KvCache {
     void read(const int32_t* ids, const int64_t* first, const int64_t* counts, size_t n, int dtype, void* k, void* v,
               int32_t* pos, float* wts, hipStream_t s);
     void truncate(const int32_t* ids, const int64_t* lengths, size_t n);
+    void fork(const int32_t* ids, const int32_t* into, const int64_t* lengths, size_t n, bool copy, hipStream_t s);
+    size_t compact(size_t num_blocks, hipStream_t s);
     size_t device_bytes() const;
 
   private:
     size_t blocks_of(int64_t slots) const { return (size_t)((slots + dev.B - 1) >> dev.shift); }
     void check_call(hipStream_t s);
     KvTensor tensor(const vgpu_tensor3& t, const char* name) const;
+    int take_block();
+    void let_go(int block);
+    // Before a call writes to the blocks first[i] .. of ids[i]: how many new ones that takes, for
+    // those with other holders; and the copies, to blocks of the sequence's own.
+    size_t shared_blocks(const int32_t* ids, const int64_t* first, size_t n);
+    void own_blocks(const int32_t* ids, const int64_t* first, size_t n, KvRuns& runs, hipStream_t s);
     // Blocks from the pool for `count` more of a sequence, written to `tab`'s row.
     void take_blocks(std::vector<int>& out, size_t count, size_t row, int* tab, KvRuns& runs, hipStream_t s);
     void release_blocks(std::vector<int>& blocks, size_t keep);

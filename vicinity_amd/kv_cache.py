@@ -224,6 +224,43 @@ class KVCache:
                                              recent, most, *ptr, s))
         return gone
 
+    def fork(self, seqs, into, lengths=None, copy: bool = False, stream=None) -> None:
+        """Each sequence into[i] becomes a continuation of its own of the first lengths[i] slots
+        of seqs[i] (None: all) as they stood before the call; what it held is forgotten.
+
+        into are different sequences; one of seqs may be continued by several, and be among
+        into: a step of beam search is ``fork(parents, beams)``.  Blocks are shared, and copied
+        when a holder writes into one that others hold too (append into a begun block, attend
+        with decay); copy=True: copied at once.  Both need free blocks for the copies.  Either
+        way each sequence reads, attends and changes as if it were alone; attend reads what
+        several sequences share once for all of them."""
+        to = self._seqs(into)
+        ids = _array("i", seqs, "sequences")
+        if len(ids) != len(to):
+            raise ValueError(f"into names {len(to)} sequences, seqs {len(ids)}")
+        if ids and not 0 <= min(ids) <= max(ids) < self.num_seqs:
+            raise ValueError(f"sequence out of range [0, {self.num_seqs})")
+        lens = None if lengths is None else self._ints(lengths, len(ids), "lengths")
+        with self._turn:
+            s, _ = self._stream(stream, ())
+            _lib.check(self._L.vgpu_kv_fork(self._h, _ptr(ids), _ptr(to),
+                                            None if lens is None else _ptr(lens), len(ids),
+                                            int(bool(copy)), s))
+
+    def compact(self, num_blocks: int | None = None, stream=None) -> int:
+        """Move the used blocks to the front of the pool; returns how many moved.  num_blocks:
+        to a pool of so many blocks, not fewer than are used, in place of the old one, whose
+        memory is given back (both exist during the call, which then waits for the GPU)."""
+        if num_blocks is not None and not (isinstance(num_blocks, (int, np.integer))
+                                           and 0 < num_blocks <= 1 << 30):
+            raise ValueError("num_blocks must be an int from 1 to 2**30")
+        moved = ctypes.c_size_t()
+        with self._turn:
+            s, _ = self._stream(stream, ())
+            _lib.check(self._L.vgpu_kv_compact(self._h, num_blocks or 0, ctypes.byref(moved), s))
+            self.num_blocks = int(num_blocks or self.num_blocks)
+        return moved.value
+
     def read(self, seqs=None, first=None, counts=None, fields=FIELDS, dtype=None,
              stream=None) -> dict:
         """What the slots first[i] .. first[i] + counts[i] - 1 of seqs[i] hold (None: from
