@@ -469,6 +469,33 @@ int vgpu_kv_fork(vgpu_kv *h, const int32_t *seqs, const int32_t *into, const int
  * Sequences keep what they hold. */
 int vgpu_kv_compact(vgpu_kv *h, size_t num_blocks, size_t *moved, void *stream);
 
+/* ---- selection of beams ------------------------------------------------------
+ * rows = groups * beams rows of logits; a group's row and a token have the total
+ *   scores[row] + logits[row][token] - log(sum over t of exp(logits[row][t])).
+ * The k largest totals of each group, descending, of equal ones the lower row and
+ * then the lower token first: out_scores f32, out_parents (rows) and out_tokens i64
+ * [groups, k].  A logit of -inf is a token that cannot follow; a row of them, or one
+ * whose score is -inf, has totals of -inf alone.  A NaN or +inf among a row's logits
+ * or in its score makes all of its totals NaN, which come first.  Exponentials are
+ * float32, sums and totals float64, rounded once.
+ * All arrays are memory of the current device.  Queued on `stream`; nothing waits, and
+ * the call may be captured.  Two calls may run at once with workspaces of their own. */
+typedef struct vgpu_beams {
+    const void *logits;  /* [rows, vocab], strides in elements */
+    int dtype;           /* VGPU_F32, VGPU_F16 or VGPU_BF16 */
+    int64_t stride_row, stride_token;
+    size_t rows, vocab, beams, k; /* beams at most 1024, k 256 and beams * vocab */
+    const float *scores; /* of the rows; NULL: 0 */
+    int64_t stride_score;
+    void *workspace;     /* of vgpu_beams_workspace bytes, aligned to 16 */
+    size_t workspace_bytes;
+    float *out_scores;
+    int64_t *out_parents, *out_tokens;
+} vgpu_beams;
+int vgpu_beams_workspace(int dtype, size_t rows, size_t vocab, size_t beams, size_t k,
+                         size_t *bytes);
+int vgpu_select_beams(const vgpu_beams *q, void *stream);
+
 /* ---- per-kernel test entry points (host buffers) -------------------------- */
 /* Host steps of the build, no device needed.  Inverted lists from list
  * labels (search.rs:624-657): offsets u64[L+1], list_ids u32[n]; a label >= L

@@ -9,6 +9,7 @@ from .filtering import MetadataFilter
 from .file_searcher import IVFPQFileSearcher
 from .flat import FlatIndex
 from . import datagen
+from .beams import select_beams
 from .kv_cache import KVCache
 from .ivf_pq import MISSING_DISTANCE, MISSING_LABEL, IVFPQIndex, default_codebooks
 
@@ -23,6 +24,7 @@ __all__ = [
     "VicinityGpuError",
     "default_codebooks",
     "device_available",
+    "select_beams",
     "LIB_PATH",
     "build_library",
 ]

@@ -116,6 +116,17 @@ class KvQuery(ctypes.Structure):
                 ("decay", ctypes.c_float), ("out", ctypes.c_void_p), ("lse", ctypes.c_void_p)]
 
 
+class Beams(ctypes.Structure):
+    """vgpu_beams: one selection, strides in elements."""
+    _fields_ = [("logits", ctypes.c_void_p), ("dtype", ctypes.c_int), ("stride_row", ctypes.c_int64),
+                ("stride_token", ctypes.c_int64), ("rows", ctypes.c_size_t),
+                ("vocab", ctypes.c_size_t), ("beams", ctypes.c_size_t), ("k", ctypes.c_size_t),
+                ("scores", ctypes.c_void_p), ("stride_score", ctypes.c_int64),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+                ("out_scores", ctypes.c_void_p), ("out_parents", ctypes.c_void_p),
+                ("out_tokens", ctypes.c_void_p)]
+
+
 _sz = ctypes.c_size_t
 _vp = ctypes.c_void_p
 _H = ctypes.c_void_p
@@ -182,6 +193,8 @@ SIGNATURES = {
     "vgpu_kv_truncate": (_i, [_H, _vp, _vp, _sz]),
     "vgpu_kv_fork": (_i, [_H, _vp, _vp, _vp, _sz, _i, _vp]),
     "vgpu_kv_compact": (_i, [_H, _sz, ctypes.POINTER(_sz), _vp]),
+    "vgpu_beams_workspace": (_i, [_i, _sz, _sz, _sz, _sz, ctypes.POINTER(_sz)]),
+    "vgpu_select_beams": (_i, [ctypes.POINTER(Beams), _vp]),
     "vgpu_test_host_kv_splits": (_i, [_vp, _vp, _sz, _sz, _sz, _vp, _vp]),
     "vgpu_test_host_lists": (_i, [_vp, _sz, _sz, _vp, _vp]),
     "vgpu_test_host_centroid_update": (_i, [_vp, _sz, _sz, _vp, _sz, _vp]),

@@ -631,6 +631,20 @@ int vgpu_kv_compact(vgpu_kv* h, size_t num_blocks, size_t* moved, void* stream) 
     });
 }
 
+int vgpu_beams_workspace(int dtype, size_t rows, size_t vocab, size_t beams, size_t k, size_t* bytes) {
+    return guard([&] {
+        need(bytes, VGPU_ERR_INVALID_PARAMETER, "null argument");
+        *bytes = vgpu::beams_workspace(dtype, rows, vocab, beams, k);
+    });
+}
+
+int vgpu_select_beams(const vgpu_beams* q, void* stream) {
+    return guard([&] {
+        need(q, VGPU_ERR_INVALID_PARAMETER, "null argument");
+        vgpu::select_beams(*q, (hipStream_t)stream);
+    });
+}
+
 /* ---- per-kernel test entry points ---------------------------------------- */
 
 int vgpu_test_host_kv_splits(const int64_t* lens, const int64_t* counts, size_t n, size_t heads, size_t group,

@@ -400,6 +400,10 @@ struct KvCache {
     void release_blocks(std::vector<int>& blocks, size_t keep);
 };
 
+// Selection of beams (vgpu_select_beams) and the bytes of its workspace.
+size_t beams_workspace(int dtype, size_t rows, size_t vocab, size_t beams, size_t k);
+void select_beams(const vgpu_beams& q, hipStream_t s);
+
 // A file descriptor closed with its owner (also when a constructor throws).
 struct UniqueFd {
     int v = -1;
