@@ -46,6 +46,11 @@ constexpr int64_t kChunkTiles = 4096;
 // Entries of one fork's row of the table that go as kernel arguments; more are copied on the GPU.
 constexpr size_t kRowRuns = 64;
 
+// Sequences that share so many slots are taken over them together.
+constexpr int64_t kSharedSlots = 256;
+// Levels of branches that are looked at for the best groups.
+constexpr int kSharedDepth = 4;
+
 // The row tiles of one launch's sequences, and the tiles that each goes over.
 struct KvPlan {
     int n = 0, heads = 1;
@@ -62,6 +67,15 @@ struct KvPlan {
         // (the first tokens of a chunk see less than the last)
         const int64_t seen = causal && !window ? std::max<int64_t>(2 * len - count, 0) : 2 * KV_TILE * tiles[n];
         work += row_units[n] * heads * ((seen + 2 * KV_TILE - 1) / (2 * KV_TILE));
+        n++;
+    }
+
+    // An entry of shared slots: count rows over so many tiles.
+    void add_entry(int64_t count, int64_t over, int64_t rows) {
+        row_units[n] = (count + rows - 1) / rows;
+        units += row_units[n] * heads;
+        tiles[n] = over;
+        work += row_units[n] * heads * over;
         n++;
     }
 
@@ -761,6 +775,189 @@ void KvCache::evict(const int32_t* ids, const int32_t* into, size_t n, size_t bu
     VGPU_HIP(hipGetLastError());
 }
 
+// Of sequences members[0..m), which hold the same blocks before block `from`, those that are to
+// be taken together over the slots that they share, so that the most slots are read once for
+// several; groups is given them, with the slots.
+void KvCache::find_groups(const int32_t* ids, const int64_t* counts, const KvAttend& a, std::vector<uint32_t>& members,
+                          size_t from, int depth, std::vector<Group>& groups, int64_t& saved) const {
+    saved = 0;
+    // leading blocks that all hold, and the slots of them that some row sees
+    const std::vector<int>& one = seqs[ids[members[0]]].blocks;
+    size_t common = one.size();
+    int64_t slots = INT64_MAX, low = INT64_MAX;
+    for (uint32_t i : members) {
+        const Seq& q = seqs[ids[i]];
+        size_t lo = from, hi = std::min(common, q.blocks.size());
+        while (lo < hi) {
+            const size_t mid = (lo + hi) / 2;
+            if (q.blocks[mid] == one[mid]) lo = mid + 1;
+            else hi = mid;
+        }
+        common = std::min(common, lo);
+        slots = std::min(slots, q.len);
+        low = std::min(low, a.window ? std::max<int64_t>(q.len - counts[i] + 1 - a.window, 0) : 0);
+    }
+    slots = std::min(slots, (int64_t)common << dev.shift) / KV_TILE * KV_TILE;
+    low = low / KV_TILE * KV_TILE;
+    const int64_t together = slots - low >= kSharedSlots ? (slots - low) * (int64_t)(members.size() - 1) : 0;
+    // or apart where they part
+    std::vector<Group> apart;
+    int64_t apart_saved = 0;
+    if (depth < kSharedDepth && members.size() > 2) {
+        std::vector<uint32_t> by(members);
+        const auto next = [&](uint32_t i) { return common < seqs[ids[i]].blocks.size() ? seqs[ids[i]].blocks[common] : -1; };
+        std::stable_sort(by.begin(), by.end(), [&](uint32_t x, uint32_t y) { return next(x) < next(y); });
+        for (size_t x = 0, y; x < by.size(); x = y) {
+            for (y = x + 1; y < by.size() && next(by[y]) == next(by[x]);) y++;
+            if (y - x < 2 || next(by[x]) < 0 || y - x == by.size()) continue;
+            std::vector<uint32_t> part(by.begin() + (ptrdiff_t)x, by.begin() + (ptrdiff_t)y);
+            int64_t more = 0;
+            find_groups(ids, counts, a, part, common, depth + 1, apart, more);
+            apart_saved += more;
+        }
+    }
+    if (apart_saved > together) {
+        saved = apart_saved;
+        groups.insert(groups.end(), std::make_move_iterator(apart.begin()), std::make_move_iterator(apart.end()));
+    } else if (together) {
+        saved = together;
+        groups.push_back(Group{members, low, slots});
+    }
+}
+
+void KvCache::attend_shared(const int32_t* ids, const int64_t* counts, const std::vector<int64_t>& tok0, size_t n,
+                            KvAttend a, std::vector<size_t>& rest, hipStream_t s) {
+    // sequences whose first block others hold too, by that block
+    std::vector<std::pair<int, uint32_t>> roots;
+    if (!a.track)
+        for (size_t i = 0; i < n; i++) {
+            const std::vector<int>& b = seqs[ids[i]].blocks;
+            if (counts[i] && !b.empty() && holders[b[0]] > 1) roots.push_back({b[0], (uint32_t)i});
+        }
+    std::vector<Group> groups;
+    if (roots.size() > 1) {
+        std::sort(roots.begin(), roots.end());
+        for (size_t x = 0, y; x < roots.size(); x = y) {
+            std::vector<uint32_t> members;
+            for (y = x; y < roots.size() && roots[y].first == roots[x].first; y++) members.push_back(roots[y].second);
+            int64_t saved;
+            if (members.size() > 1) find_groups(ids, counts, a, members, 0, 0, groups, saved);
+        }
+    }
+    // Groups in pieces of as many sequences as one launch takes: each has an entry of its own and
+    // the piece one more, and every row leaves partial results of both.
+    const int parts = a.q.type == KV_F32 ? 2 : 1;
+    const int64_t chunk_rows = 64 * kv_chunk_nc(dev.Dp, parts);
+    const int64_t row_bytes = (int64_t)dev.Dp * 4 + 12, room = kPartBytes / 2 / row_bytes / dev.H;
+    const auto rows_of = [&](uint32_t i) { return (counts[i] * a.G + chunk_rows - 1) / chunk_rows * chunk_rows; };
+    struct Piece {
+        const Group* group;
+        size_t first, end;  // of its members
+        int64_t rows;
+    };
+    std::vector<Piece> pieces;
+    for (const Group& x : groups) {
+        Piece p{&x, 0, 0, 0};
+        for (size_t j = 0; j <= x.members.size(); j++) {
+            const int64_t more = j < x.members.size() ? rows_of(x.members[j]) : 0;
+            if (j < x.members.size() && j - p.first < (size_t)KV_BATCH - 1 && p.rows + more <= room) {
+                p.rows += more, p.end = j + 1;
+                continue;
+            }
+            if (p.end - p.first > 1) pieces.push_back(p);
+            p = Piece{&x, j, j, 0};
+            if (more && more <= room) p.rows = more, p.end = j + 1;
+            else p.first = p.end = j + 1;  // too many rows for any launch
+        }
+    }
+    std::vector<uint8_t> done(n, 0);
+    for (size_t x = 0; x < pieces.size();) {
+        struct Entry {
+            int seq, first, rows, members;
+            int64_t t0, end;
+        };
+        std::vector<Entry> entries[2];  // shared slots, own slots
+        KvMembers mem;
+        KvShares shares;
+        int64_t used = 0;
+        mem.row0[0] = 0;
+        for (; x < pieces.size(); x++) {
+            const Piece& p = pieces[x];
+            const size_t many = p.end - p.first;
+            if (mem.n && (mem.n + many + entries[0].size() + 1 > (size_t)KV_BATCH || used + p.rows > room)) break;
+            used += p.rows;
+            const int first = mem.n;
+            for (size_t j = p.first; j < p.end; j++) {
+                const uint32_t i = p.group->members[j];
+                const Seq& q = seqs[ids[i]];
+                const int m = mem.n++, count = (int)(counts[i] * a.G);
+                mem.tok0[m] = (int)tok0[i], mem.len[m] = (int)q.len, mem.count[m] = (int)counts[i];
+                mem.row0[m + 1] = mem.row0[m] + count;
+                shares.row0[m] = mem.row0[m] - mem.row0[first];
+                shares.unit[1][m] = shares.tiles[1][m] = shares.splits[1][m] = 0;
+                const int64_t low = a.window ? std::max<int64_t>(q.len - counts[i] + 1 - a.window, 0) : 0;
+                const int64_t t0 = std::max(p.group->slots, low) / KV_TILE;
+                if (t0 * KV_TILE < q.len) entries[1].push_back({ids[i], m, count, 1, t0, q.len});
+                done[i] = 1;
+            }
+            entries[0].push_back({ids[p.group->members[p.first]], first, mem.row0[mem.n] - mem.row0[first], (int)many,
+                                  p.group->low / KV_TILE, p.group->slots});
+        }
+        // the kernel that suits the rows, for each kind of slots; one launch where it is the same
+        bool by_rows[2];
+        for (int y = 0; y < 2; y++) {
+            int64_t most = 0, tiles = 0;
+            for (const Entry& e : entries[y]) {
+                most = std::max<int64_t>(most, e.rows);
+                tiles += (e.rows + chunk_rows - 1) / chunk_rows * dev.H * ((e.end + KV_TILE - 1) / KV_TILE - e.t0);
+            }
+            by_rows[y] = most > chunk_rows * 3 / 4 && tiles >= kChunkTiles;
+        }
+        const int launches = by_rows[0] == by_rows[1] ? 1 : 2;
+        KvBatch b[2];
+        int64_t base[2] = {0, 0}, all_rows = 0;
+        for (int y = 0; y < launches; y++) {
+            const int wg = by_rows[y] ? (int)chunk_rows : 16, z1 = launches == 1 ? 2 : y + 1;
+            KvPlan plan;
+            plan.heads = dev.H;
+            b[y].n = 0, b[y].unit0[0] = 0;
+            for (int z = y; z < z1; z++)
+                for (const Entry& e : entries[z]) {
+                    const int j = b[y].n++;
+                    b[y].seq[j] = e.seq, b[y].aux[j] = e.first, b[y].count[j] = e.rows;
+                    b[y].tok0[j] = (int)e.t0, b[y].len[j] = (int)e.end;
+                    plan.add_entry(e.rows, (e.end + KV_TILE - 1) / KV_TILE - e.t0, wg);
+                }
+            plan.split(b[y], by_rows[y], kPartBytes / 2 / (wg * row_bytes));
+            base[y] = all_rows;
+            all_rows += plan.groups * wg;
+            int j = 0;
+            for (int z = y; z < z1; z++) {
+                shares.rows[z] = wg, shares.base[z] = (size_t)base[y];
+                for (const Entry& e : entries[z]) {
+                    for (int m = e.first; m < e.first + e.members; m++) {
+                        shares.unit[z][m] = b[y].unit0[j], shares.splits[z][m] = b[y].splits[j];
+                        shares.tiles[z][m] = (e.rows + wg - 1) / wg;
+                    }
+                    j++;
+                }
+            }
+        }
+        grow(w_part, (size_t)all_rows * dev.Dp);
+        grow(w_ml, (size_t)all_rows);
+        grow(w_power, (size_t)all_rows);
+        for (int y = 0; y < launches; y++) {
+            a.by_rows = by_rows[y];
+            a.part_o = w_part.p + base[y] * dev.Dp, a.part_ml = w_ml.p + base[y], a.part_s = w_power.p + base[y];
+            launch_kv_shared(dev, b[y], a, mem, s);
+        }
+        a.part_o = w_part.p, a.part_ml = w_ml.p, a.part_s = w_power.p;
+        launch_kv_shared_join(dev, a, mem, shares, s);
+    }
+    for (size_t i = 0; i < n; i++)
+        if (!done[i]) rest.push_back(i);
+}
+
 void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const vgpu_kv_query& q, hipStream_t s) {
     check_call(s);
     check_ids(*this, seen, ids, n);
@@ -784,21 +981,33 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
     a.vec_out = dev.D % 4 == 0 && (uintptr_t)q.out % (4 * item_size(a.q.type)) == 0;
     const int parts = a.q.type == KV_F32 ? 2 : 1;
     const int64_t chunk_rows = 64 * kv_chunk_nc(dev.Dp, parts);
-    int64_t tokens = 0, longest = 0, most = 0, chunk_tiles = 0, step_units = 0;
+    int64_t tokens = 0, longest = 0;
+    std::vector<int64_t> tok0(n);
     for (size_t i = 0; i < n; i++) {
         need(counts[i] >= 0 && counts[i] <= INT_MAX / 2, "counts must not be negative, nor above 2^30");
+        tok0[i] = tokens;
         tokens += counts[i];
         need(tokens * (int64_t)q.num_q_heads <= INT_MAX / 2, "more than 2^30 query rows in one call");
         longest = std::max(longest, seqs[ids[i]].len);
-        most = std::max(most, counts[i] * a.G);
-        step_units += (counts[i] * a.G + 15) / 16 * dev.H;
-        chunk_tiles += (counts[i] * a.G + chunk_rows - 1) / chunk_rows * dev.H * ((seqs[ids[i]].len + KV_TILE - 1) / KV_TILE);
     }
     need(!q.mask || (int64_t)q.mask_slots >= longest, "a mask row must cover the longest sequence (" +
                                                           std::to_string(longest) + " slots)");
     need(!tokens || (q.q.data && q.out), "null argument");
     need((uintptr_t)q.out % item_size(a.q.type) == 0 && (uintptr_t)q.lse % 4 == 0, "outputs must be aligned to their dtype");
 
+    // The sequences that share their first blocks with others of the call, and the rest.
+    std::vector<size_t> order;
+    attend_shared(ids, counts, tok0, n, a, order, s);
+    if (order.empty() && n) {
+        VGPU_HIP(hipGetLastError());
+        return;
+    }
+    int64_t most = 0, chunk_tiles = 0, step_units = 0;
+    for (size_t i : order) {
+        most = std::max(most, counts[i] * a.G);
+        step_units += (counts[i] * a.G + 15) / 16 * dev.H;
+        chunk_tiles += (counts[i] * a.G + chunk_rows - 1) / chunk_rows * dev.H * ((seqs[ids[i]].len + KV_TILE - 1) / KV_TILE);
+    }
     // Many rows: each wave has its own; few: the waves share them and split the tiles.
     a.by_rows = a.track ? most > kScoreRows : most > chunk_rows * 3 / 4 && chunk_tiles >= kChunkTiles;
     const bool keep_scores = a.track && !a.by_rows;
@@ -823,25 +1032,22 @@ void KvCache::attend(const int32_t* ids, const int64_t* counts, size_t n, const 
     // Where a workgroup's work depends on its sequence, the short sequences come first: the
     // light rows of the longest end the launch.  Steps that may have more workgroups than
     // are on the card at once begin with the longest.
-    std::vector<size_t> order(n);
-    std::vector<int64_t> tok0(n);
-    int64_t tok = 0;
-    for (size_t i = 0; i < n; i++) order[i] = i, tok0[i] = tok, tok += counts[i];
     if (a.by_rows)
         std::stable_sort(order.begin(), order.end(), [&](size_t x, size_t y) { return seqs[ids[x]].len < seqs[ids[y]].len; });
     else if (step_units > kStepWorkgroups / 2)
         std::stable_sort(order.begin(), order.end(), [&](size_t x, size_t y) { return seqs[ids[x]].len > seqs[ids[y]].len; });
     // Where several launches add weights, all of them are checked and their workspaces grown
     // before the first, so that a call that fails has added none.
-    for (int dry = a.track && n > KV_BATCH; dry >= 0; dry--)
-    for (size_t i0 = 0; i0 < n; i0 += KV_BATCH) {
+    const size_t rest = order.size();
+    for (int dry = a.track && rest > KV_BATCH; dry >= 0; dry--)
+    for (size_t i0 = 0; i0 < rest; i0 += KV_BATCH) {
         KvBatch b;
         b.n = 0;
         b.unit0[0] = 0;
         KvPlan plan;
         plan.heads = dev.H;
         int64_t score_tiles = 0, row_tiles = 0;
-        for (size_t x = i0; x < std::min(n, i0 + KV_BATCH); x++) {
+        for (size_t x = i0; x < std::min(rest, i0 + KV_BATCH); x++) {
             const size_t i = order[x];
             const int64_t len = seqs[ids[i]].len;
             const int j = b.n++;

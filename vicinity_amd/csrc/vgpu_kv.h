@@ -222,6 +222,38 @@ inline int kv_attend_rows(const KvAttend& a, int Dp) {
 }
 // unit0 counts row tiles times splits of the sequences (of one head).
 void launch_kv_attend(const KvDev& c, const KvBatch& b, const KvAttend& a, hipStream_t s);
+// Attention of sequences that hold the same first blocks.  The sequences of one launch, in an
+// order in which those that share lie together; sequence m's rows (token after token, the G
+// heads of each) are rows row0[m] .. row0[m + 1] - 1.  A launch's entries (KvBatch) are ranges
+// of slots: count rows, from the first of sequence aux on, over the tiles from tok0 on of the
+// slots up to len that sequence seq holds.
+struct KvMembers {
+    int n = 0;
+    int tok0[KV_BATCH], len[KV_BATCH], count[KV_BATCH];
+    int row0[KV_BATCH + 1];
+};
+struct KvAlone {};
+template <bool SH>
+struct KvMemOf {
+    typedef KvAlone type;
+};
+template <>
+struct KvMemOf<true> {
+    typedef KvMembers type;
+};
+template <bool SH>
+using KvMem = typename KvMemOf<SH>::type;
+void launch_kv_shared(const KvDev& c, const KvBatch& b, const KvAttend& a, const KvMembers& mem, hipStream_t s);
+
+// Where a sequence's partial results lie: entry units unit .. + tiles * splits - 1 of the shared
+// slots' launch [0] and of its own slots' [1] (splits 0: none); row0: its first row in the entry.
+struct KvShares {
+    int unit[2][KV_BATCH], tiles[2][KV_BATCH], splits[2][KV_BATCH];
+    int row0[KV_BATCH];
+    int rows[2];      // of a workgroup
+    size_t base[2];   // first partial row of the launch
+};
+void launch_kv_shared_join(const KvDev& c, const KvAttend& a, const KvMembers& mem, const KvShares& j, hipStream_t s);
 // Slots of a workgroup that makes weights of kept scores, and of one that goes over the keys.
 constexpr int KV_SCORE_SLOTS = 1024, KV_WEIGHT_SLOTS = 128;
 // unit0 counts these.  aux: with scores the tiles of the score rows of the sequences
