@@ -5,8 +5,8 @@
 // the slice's largest logit and sum of exponentials, and its k best tokens.  Within a row the
 // order is the logits' own, so no slice needs the row's sum for it.  A second kernel adds the
 // slices' sums and takes the k best of a group's lists.
-// The k-th largest of the threads' largest logits bounds the slice's k-th best from below,
-// and few others reach it: those are put in order by counting.
+// The largest logits of threads bound the slice's k-th best from below, and few others reach
+// that: those are put in order by counting.
 // Differences and exponentials are float32, sums and totals float64: candidates of different
 // beams lie close together, and their order is what the kernel answers.
 #include <hip/hip_bf16.h>
@@ -51,13 +51,15 @@ __device__ __forceinline__ float element(const uint4& r, int e) {
 
 constexpr int BEAM_LIST = 1024;  // tokens that one slice puts in order
 
-// One workgroup: one slice of one row.
+// One workgroup: one slice of one row, loaded at once.  Bound by the vector unit where rows are
+// many: a conversion, a comparison, a difference, a product, an exponential (four times as
+// long) and a sum for each logit.
 template <int T, int N>
 __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs a) {
-    constexpr int W = T == KV_F32 ? 4 : 8, SLICE = 256 * N * W;
-    __shared__ __align__(16) uint32_t tops[256];
+    constexpr int W = T == KV_F32 ? 4 : 8, SLICE = 256 * N * W, HALF = (N + 1) / 2;
     __shared__ uint64_t list[BEAM_LIST];  // (key, ~token)
-    __shared__ uint32_t count, shared_key, scan[4];
+    __shared__ uint32_t count, scan[4], bounds[4];
+    __shared__ float tops[4];
     __shared__ double sums[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int row = blockIdx.x / a.slices, slice = blockIdx.x - row * a.slices;
@@ -68,62 +70,86 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs a) {
     const int skew = a.st_token == 1 ? (int)((uintptr_t)base & 15) / (int)item : 0;
     const int first = slice * SLICE + tid * W - skew;  // token of the thread's first element
     const auto token = [&](int p, int e) { return first + p * (256 * W) + e; };
+    const auto load = [&](int p) {
+        const int t0 = token(p, 0);
+        if (a.st_token == 1 && t0 >= 0 && t0 + W <= a.vocab) return *(const uint4*)(base + (int64_t)t0 * (int64_t)item);
+        // ends of the row, or elements apart: one by one, -inf outside
+        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < W; e++) {
+            const bool in = t0 + e >= 0 && t0 + e < a.vocab;
+            const int64_t at = (int64_t)(t0 + e) * a.st_token;
+            if (T == KV_F32)
+                w[e] = in ? ((const uint32_t*)base)[at] : 0xff800000u;
+            else
+                w[e >> 1] |= (in ? (uint32_t)((const uint16_t*)base)[at] : T == KV_F16 ? 0xfc00u : 0xff80u) << (16 * (e & 1));
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    };
+    // (the elements stay as they lie in memory: 148 registers and more, kept as floats)
+    const auto keep = [](uint4(&r)[N]) {
+#pragma unroll
+        for (int p = 0; p < N; p++) asm volatile("" : "+v"(r[p].x), "+v"(r[p].y), "+v"(r[p].z), "+v"(r[p].w));
+    };
     uint4 x[N];
 #pragma unroll
-    for (int p = 0; p < N; p++) {
-        const int t0 = token(p, 0);
-        if (a.st_token == 1 && t0 >= 0 && t0 + W <= a.vocab) {
-            x[p] = *(const uint4*)(base + (int64_t)t0 * (int64_t)item);
-        } else {  // ends of the row, or elements apart: one by one, -inf outside
-            uint32_t w[4] = {0, 0, 0, 0};
+    for (int p = 0; p < N; p++) x[p] = load(p);
+    if (tid == 0) count = 0;
+    // the largest of each piece, and of each half of the pieces (NaN are passed over)
+    float tp[N], th[2] = {BEAM_NEG, BEAM_NEG};
 #pragma unroll
-            for (int e = 0; e < W; e++) {
-                const bool in = t0 + e >= 0 && t0 + e < a.vocab;
-                const int64_t at = (int64_t)(t0 + e) * a.st_token;
-                if (T == KV_F32)
-                    w[e] = in ? ((const uint32_t*)base)[at] : 0xff800000u;
-                else
-                    w[e >> 1] |= (in ? (uint32_t)((const uint16_t*)base)[at] : T == KV_F16 ? 0xfc00u : 0xff80u) << (16 * (e & 1));
+    for (int p = 0; p < N; p++) {
+        tp[p] = element<T>(x[p], 0);
+#pragma unroll
+        for (int e = 1; e < W; e++) tp[p] = fmaxf(tp[p], element<T>(x[p], e));
+        th[p / HALF] = fmaxf(th[p / HALF], tp[p]);
+    }
+    keep(x);
+    float top = fmaxf(th[0], th[1]);
+    // A lower bound of the slice's k-th best: each wave finds the largest number (the first BITS
+    // bits of its key) that a quarter of k halves' largest reach, and the least of the four is
+    // reached by k.  In a short slice the waves that have tokens take more.  0: no such number.
+    {
+        constexpr int BITS = T == KV_BF16 ? 16 : T == KV_F16 ? 19 : 18, SHIFT = 32 - BITS;
+        const uint32_t k0 = token(0, 0) < a.vocab ? size_key(th[0]) >> SHIFT : 0;
+        const uint32_t k1 = token(HALF, 0) < a.vocab ? size_key(th[1]) >> SHIFT : 0;
+        const int used = min(max((a.vocab + skew - slice * SLICE + W - 1) / W, 0), 256);  // threads that have a token
+        const auto most_of = [&](int r) {  // halves, with at most r of each wave
+            return min(r, min(used, 64)) + min(r, min(max(used - 64, 0), 64)) + min(r, min(max(used - 128, 0), 64)) +
+                   min(r, max(used - 192, 0));
+        };
+        int need = (a.k + 3) / 4;
+        while (most_of(need) < a.k && need < 64) need++;
+        const bool enough = most_of(need) >= a.k;
+        need = min(need, min(max(used - 64 * wave, 0), 64));
+        uint32_t key = 0;
+#pragma unroll
+        for (int bit = BITS - 1; bit >= 0; bit--) {
+            const uint32_t more = key | 1u << bit;
+            if (__popcll(__ballot(k0 >= more)) + __popcll(__ballot(k1 >= more)) >= need) key = more;
+        }
+#pragma unroll
+        for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+        if (lane == 0) bounds[wave] = enough ? key << SHIFT : 0, tops[wave] = top;
+    }
+    __syncthreads();
+    const uint32_t bound = min(min(bounds[0], bounds[1]), min(bounds[2], bounds[3]));
+    const float least = bound < size_key(BEAM_NEG) ? BEAM_NEG : of_key(bound);
+    const float most = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+#pragma unroll
+    for (int p = 0; p < N; p++) {
+        if (!(tp[p] >= least)) continue;
+#pragma unroll
+        for (int e = 0; e < W; e++) {
+            const float v = element<T>(x[p], e);
+            const int t = token(p, e);
+            if (v >= least && t >= 0 && t < a.vocab) {
+                const uint32_t at = atomicAdd(&count, 1u);
+                if (at < BEAM_LIST) list[at] = (uint64_t)size_key(v) << 32 | (uint32_t)~t;
             }
-            x[p] = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
-    float top = BEAM_NEG;
-#pragma unroll
-    for (int p = 0; p < N; p++)
-#pragma unroll
-        for (int e = 0; e < W; e++) top = fmaxf(top, element<T>(x[p], e));
-    const bool any = token(0, W - 1) >= 0 && token(0, 0) < a.vocab;  // has the thread a token?
-    const uint32_t my = any ? size_key(top) : 0;
-    tops[tid] = my;
-    if (tid == 0) count = 0;
-    __syncthreads();
-    // the k-th largest of the threads' largest, and the slice's largest
-    uint32_t rank = 0, big = 0;
-#pragma unroll 4
-    for (int j = 0; j < 256; j += 4) {
-        const uint4 o = *(const uint4*)(tops + j);
-        rank += (o.x > my || (o.x == my && j < tid)) + (o.y > my || (o.y == my && j + 1 < tid)) +
-                (o.z > my || (o.z == my && j + 2 < tid)) + (o.w > my || (o.w == my && j + 3 < tid));
-        big = max(max(big, max(o.x, o.y)), max(o.z, o.w));
-    }
-    if ((int)rank == a.k - 1) shared_key = my;
-    __syncthreads();
-    const uint32_t bound = shared_key;
-    const float most = big ? of_key(big) : BEAM_NEG;
-    if (my >= bound) {
-#pragma unroll
-        for (int p = 0; p < N; p++)
-#pragma unroll
-            for (int e = 0; e < W; e++) {
-                const uint32_t key = size_key(element<T>(x[p], e));
-                const int t = token(p, e);
-                if (key >= bound && t >= 0 && t < a.vocab) {
-                    const uint32_t at = atomicAdd(&count, 1u);
-                    if (at < BEAM_LIST) list[at] = (uint64_t)key << 32 | (uint32_t)~t;
-                }
-            }
-    }
+    keep(x);
     // (a row of -inf alone: exp(-inf - 0) = 0; NaN and +inf make the sum NaN)
     const float off = most == BEAM_NEG ? 0.f : most;
     float sum = 0.f;
@@ -143,15 +169,18 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs a) {
     if (n > BEAM_LIST) {
         // Many reach the bound: the k-th best key itself, then the tokens above it and the first
         // of those that have it.  Every wave of the workgroup comes here.
+        // (the logits come from memory again: this is rare, and needs their registers)
         const auto reach = [&](uint32_t key) {  // how many of the slice's tokens are not below key
             uint32_t c = 0;
-#pragma unroll
-            for (int p = 0; p < N; p++)
+#pragma unroll 1
+            for (int p = 0; p < N; p++) {
+                const uint4 r = load(p);
 #pragma unroll
                 for (int e = 0; e < W; e++) {
                     const int t = token(p, e);
-                    c += size_key(element<T>(x[p], e)) >= key && t >= 0 && t < a.vocab;
+                    c += size_key(element<T>(r, e)) >= key && t >= 0 && t < a.vocab;
                 }
+            }
 #pragma unroll
             for (int o = 32; o; o >>= 1) c += (uint32_t)__shfl_xor((int)c, o);
             __syncthreads();
@@ -160,7 +189,8 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs a) {
             return scan[0] + scan[1] + scan[2] + scan[3];
         };
         uint32_t lo = bound, hi = ~0u;  // reach(lo) >= k (NaN lie above every number)
-        if (lo < hi && reach(lo + 1) < (uint32_t)a.k) hi = lo;
+        if (reach(size_key(most)) >= (uint32_t)a.k)
+            lo = max(lo, size_key(most));  // (one value, -inf for example)
         while (lo < hi) {
             const uint32_t mid = lo + (hi - lo) / 2 + 1;
             if (reach(mid) >= (uint32_t)a.k) lo = mid;
@@ -169,24 +199,27 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs a) {
         __syncthreads();
         if (tid == 0) count = 0;
         __syncthreads();
-#pragma unroll
-        for (int p = 0; p < N; p++)
+#pragma unroll 1
+        for (int p = 0; p < N; p++) {
+            const uint4 r = load(p);
 #pragma unroll
             for (int e = 0; e < W; e++) {
-                const uint32_t key = size_key(element<T>(x[p], e));
+                const uint32_t key = size_key(element<T>(r, e));
                 const int t = token(p, e);
                 if (key > lo && t >= 0 && t < a.vocab) list[atomicAdd(&count, 1u)] = (uint64_t)key << 32 | (uint32_t)~t;
             }
+        }
         __syncthreads();
         n = count;  // below k
-#pragma unroll
+#pragma unroll 1
         for (int p = 0; p < N; p++) {
             if (n >= (uint32_t)a.k) break;
+            const uint4 r = load(p);
             uint32_t c = 0;
 #pragma unroll
             for (int e = 0; e < W; e++) {
                 const int t = token(p, e);
-                c += size_key(element<T>(x[p], e)) == lo && t >= 0 && t < a.vocab;
+                c += size_key(element<T>(r, e)) == lo && t >= 0 && t < a.vocab;
             }
             uint32_t before = c;
 #pragma unroll
@@ -202,7 +235,7 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs a) {
 #pragma unroll
             for (int e = 0; e < W; e++) {
                 const int t = token(p, e);
-                if (size_key(element<T>(x[p], e)) == lo && t >= 0 && t < a.vocab) {
+                if (size_key(element<T>(r, e)) == lo && t >= 0 && t < a.vocab) {
                     if (n + before < (uint32_t)a.k) list[n + before] = (uint64_t)lo << 32 | (uint32_t)~t;
                     before++;
                 }
@@ -221,68 +254,73 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs a) {
     for (int i = (int)n + tid; i < a.k; i += 256) best[i] = make_uint2(0, ~0u);
 }
 
-constexpr int BEAM_POOL = 2048;  // candidates that a group puts in order at once
+constexpr int BEAM_POOL = 2048;     // candidates that a group puts in order at once
+constexpr int BEAM_SAMPLES = 4096;  // keys of samples that are kept
+constexpr int BEAM_BINS = 2048;
 
-// One workgroup: one group.  Threads go down the lists of the group's slices, L of them, from
-// the top, several threads to a list (every 1024 / L-th entry each) or several lists to a thread.
+// One workgroup: one group, of L lists (one of each row and slice), k places each.
+//
+// Places 0, 1, 3, 7, ... of every list are its samples; a sample stands for the places from the
+// one before it to its own.  Of the totals rounded to float32 (which keeps the order) the
+// largest that samples for k places reach, found by two digits of 11 bits, bounds the k-th best
+// from below; and as a list's places beyond its last sample that reaches it are fewer than
+// those up to there, about 2 k candidates pass.
 __global__ __launch_bounds__(1024) void beam_group_kernel(BeamArgs a) {
     // total = (logit - largest) + lift, lift = score - log sum exp(logit - largest)
     __shared__ double lift[BEAM_MAX_BEAMS];
     __shared__ float largest[BEAM_MAX_BEAMS];
     __shared__ uint8_t kinds[BEAM_MAX_BEAMS];
-    __shared__ __align__(16) uint32_t tops[256];
     __shared__ uint64_t key[BEAM_POOL];  // the total's order
     __shared__ uint64_t who[BEAM_POOL];  // beam << 32 | token
-    __shared__ uint32_t count, bound32;
+    __shared__ uint32_t sample[BEAM_SAMPLES];
+    __shared__ uint32_t hist[BEAM_BINS];
+    __shared__ uint32_t place[BEAM_POOL];
+    __shared__ uint32_t scan[18], count;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int row0 = blockIdx.x * a.beams;
-    for (int b = wave; b < a.beams; b += 16) {
-        const int row = row0 + b;
+    // 16 lanes to a row
+    for (int b0 = 0; b0 < a.beams; b0 += 64) {
+        const int b = min(b0 + (tid >> 4), a.beams - 1), row = row0 + b;
         int kind = score_kind(score_of(a, row));
         double total = 0.0;
         float most = BEAM_NEG;
-        if (!kind) {
-            const float* top = a.top + (size_t)row * a.slices;
-            const double* sum = a.sum + (size_t)row * a.slices;
-            // (slices of -inf alone have top 0 and sum 0)
-            for (int j = lane; j < a.slices; j += 64) most = fmaxf(most, sum[j] == 0.0 ? BEAM_NEG : top[j]);
+        const float* top = a.top + (size_t)row * a.slices;
+        const double* sum = a.sum + (size_t)row * a.slices;
+        // (slices of -inf alone have top 0 and sum 0; rows of another kind have neither)
+        if (!kind)
+            for (int j = lane & 15; j < a.slices; j += 16) most = fmaxf(most, sum[j] == 0.0 ? BEAM_NEG : top[j]);
 #pragma unroll
-            for (int o = 32; o; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
-            for (int j = lane; j < a.slices; j += 64)
+        for (int o = 8; o; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
+        if (!kind)
+            for (int j = lane & 15; j < a.slices; j += 16)
                 if (sum[j] != 0.0) total += sum[j] * exp2((double)(top[j] - most) * 1.4426950408889634);
 #pragma unroll
-            for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o);
-            kind = total == 0.0 ? 1 : total > 0.0 ? 0 : 2;
-        }
-        if (lane == 0) {
+        for (int o = 8; o; o >>= 1) total += __shfl_xor(total, o);
+        if (!kind) kind = total == 0.0 ? 1 : total > 0.0 ? 0 : 2;
+        if ((lane & 15) == 0 && b0 + (tid >> 4) < a.beams) {
             lift[b] = kind ? 0.0 : (double)score_of(a, row) - log(total);
             largest[b] = most, kinds[b] = (uint8_t)kind;
         }
     }
     if (tid == 0) count = 0;
+    for (int i = tid; i < BEAM_BINS; i += 1024) hist[i] = 0;
     __syncthreads();
 
-    const int64_t L = (int64_t)a.beams * a.slices;
-    const int per = L < 1024 ? 1024 / (int)L : 1;  // threads of a list
-    const bool used = L >= 1024 || tid < per * (int)L;
-    const int64_t list0 = L < 1024 ? tid % (int)L : tid;
-    const int place0 = L < 1024 ? tid / (int)L : 0;
     struct Entry {
         uint64_t key, who;
         uint32_t key32;
     };
-    // Entry `place` of a list: false where it ends.
-    const auto entry = [&](int64_t l, int place, Entry& r) {
-        const int b = (int)(l / a.slices), slice = (int)(l - (int64_t)b * a.slices);
-        if (place >= a.k) return false;
+    // Entry `at` of a list: false where it has none.
+    const auto entry = [&](uint32_t l, int at, Entry& r) {
+        const uint32_t b = l / (uint32_t)a.slices, slice = l - b * (uint32_t)a.slices;
         double total;
         uint32_t token;
         if (kinds[b]) {  // all totals alike: the first tokens, as one list
-            if (slice || place >= a.vocab) return false;
-            token = (uint32_t)place;
+            if (slice || at >= a.vocab) return false;
+            token = (uint32_t)at;
             total = kinds[b] == 1 ? -__builtin_huge_val() : __builtin_nan("");
         } else {
-            const uint2 c = a.best[((size_t)(row0 + b) * a.slices + slice) * a.k + place];
+            const uint2 c = a.best[((size_t)row0 * a.slices + l) * a.k + at];
             if (c.y == ~0u) return false;
             token = c.y;
             total = ((double)__uint_as_float(c.x) - (double)largest[b]) + lift[b];
@@ -292,91 +330,130 @@ __global__ __launch_bounds__(1024) void beam_group_kernel(BeamArgs a) {
         r.who = (uint64_t)b << 32 | token;
         return true;
     };
-    // The k-th largest of 256 quads of threads' first entries, rounded to float32 (which keeps
-    // the order), bounds the k-th best from below; 0 where there are not so many.
-    uint32_t my = 0;
-    Entry e;
-    if (used)
-        for (int64_t l = list0; l < L; l += 1024)
-            if (entry(l, place0, e)) my = max(my, e.key32);
-    my = max(my, (uint32_t)__shfl_xor((int)my, 1));
-    my = max(my, (uint32_t)__shfl_xor((int)my, 2));
-    if ((tid & 3) == 0) tops[tid >> 2] = my;
-    __syncthreads();
-    if (tid < 256) {
-        const uint32_t mine = tops[tid];
-        uint32_t rank = 0;
-#pragma unroll 4
-        for (int j = 0; j < 256; j += 4) {
-            const uint4 o = *(const uint4*)(tops + j);
-            rank += (o.x > mine || (o.x == mine && j < tid)) + (o.y > mine || (o.y == mine && j + 1 < tid)) +
-                    (o.z > mine || (o.z == mine && j + 2 < tid)) + (o.w > mine || (o.w == mine && j + 3 < tid));
+    // The digit in which the samples' weights, from the top, reach `need`.
+    const auto digit = [&](uint32_t& need) {
+        const int hi = BEAM_BINS - 1 - 2 * tid;  // this thread's two bins, from the top
+        const uint32_t c0 = hist[hi], c1 = hist[hi - 1];
+        uint32_t sum = c0 + c1;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t up = (uint32_t)__shfl_up((int)sum, o);
+            if (lane >= o) sum += up;
         }
-        if ((int)rank == a.k - 1) bound32 = mine;
-    }
+        if (lane == 63) scan[wave] = sum;
+        if (tid == 0) scan[16] = ~0u;
+        __syncthreads();
+        for (int w = 0; w < wave; w++) sum += scan[w];
+        const uint32_t before = sum - c0 - c1;
+        if (before < need && sum >= need) {  // one thread at most
+            const bool one = before + c0 >= need;
+            scan[16] = (uint32_t)(one ? hi : hi - 1);
+            scan[17] = need - before - (one ? 0 : c0);
+        }
+        hist[hi] = hist[hi - 1] = 0;
+        __syncthreads();
+        const uint32_t d = scan[16];
+        need = scan[17];
+        return d;
+    };
+    const uint32_t L = (uint32_t)a.beams * a.slices, places = L * (uint32_t)a.k;
+    const int steps = 32 - __clz(a.k);  // samples of a list
+    const auto each_sample = [&](auto&& f) {
+        for (uint32_t i = tid; i < L * steps; i += 1024) {
+            const int step = (int)(i / L);
+            const int at = (1 << step) - 1;
+            if (at < a.k) f(i, i - step * L, at, step ? 1u << (step - 1) : 1u);
+        }
+    };
+    Entry e;
+    const bool keep = L * steps <= BEAM_SAMPLES;
+    each_sample([&](uint32_t i, uint32_t l, int at, uint32_t weight) {
+        const uint32_t k32 = entry(l, at, e) ? e.key32 : 0;
+        if (keep) sample[i] = k32;
+        if (k32) atomicAdd(&hist[k32 >> 21], weight);
+    });
     __syncthreads();
-    const uint32_t least = bound32;
-    uint64_t kth_key = 0, kth_who = ~0ull;  // of the pool, once it held k: what is behind cannot win
+    uint32_t need = (uint32_t)a.k, least = 0;
+    const uint32_t d0 = digit(need);
+    if (d0 != ~0u) {
+        each_sample([&](uint32_t i, uint32_t l, int at, uint32_t weight) {
+            const uint32_t k32 = keep ? sample[i] : entry(l, at, e) ? e.key32 : 0;
+            if (k32 && k32 >> 21 == d0) atomicAdd(&hist[k32 >> 10 & 2047u], weight);
+        });
+        __syncthreads();
+        least = d0 << 21 | digit(need) << 10;
+    }
 
-    // Put the pool's candidates in order: the k best stay, or go out.
+    // Put the pool's n candidates in order: the k best stay, or go out.
     const auto order = [&](uint32_t n, bool out) {
+        // as many threads to a candidate as there are
+        int wide = 64;
+        while (wide < (int)n && wide < 1024) wide <<= 1;
+        for (uint32_t i = tid; i < n; i += 1024) place[i] = 0;
+        __syncthreads();
+        for (uint32_t i = tid & (wide - 1); i < n; i += wide) {
+            const uint64_t k0 = key[i], w0 = who[i];
+            uint32_t c = 0;
+#pragma unroll 4
+            for (uint32_t j = tid / wide; j < n; j += 1024 / wide) c += key[j] > k0 || (key[j] == k0 && who[j] < w0);
+            if (c) atomicAdd(&place[i], c);
+        }
+        __syncthreads();
         uint64_t k0[2], w0[2];
-        uint32_t place[2] = {~0u, ~0u};
+        uint32_t to[2] = {~0u, ~0u};
 #pragma unroll
         for (int y = 0; y < 2; y++) {
             const uint32_t i = tid + 1024 * y;
-            if (i >= n) continue;
-            k0[y] = key[i], w0[y] = who[i];
-            uint32_t c = 0;
-#pragma unroll 4
-            for (uint32_t j = 0; j < n; j++) c += key[j] > k0[y] || (key[j] == k0[y] && who[j] < w0[y]);
-            place[y] = c;
+            if (i < n) k0[y] = key[i], w0[y] = who[i], to[y] = place[i];
         }
         __syncthreads();
 #pragma unroll
         for (int y = 0; y < 2; y++) {
-            if (place[y] >= (uint32_t)a.k) continue;
+            if (to[y] >= (uint32_t)a.k) continue;
             if (out) {
-                const size_t at = (size_t)blockIdx.x * a.k + place[y];
-                const int64_t parent = row0 + (int64_t)(w0[y] >> 32);
+                const size_t at = (size_t)blockIdx.x * a.k + to[y];
                 const uint64_t u = k0[y] >> 63 ? k0[y] & ~(1ull << 63) : ~k0[y];
                 a.out_scores[at] = (float)__longlong_as_double((long long)u);
-                a.out_parents[at] = parent;
+                a.out_parents[at] = row0 + (int64_t)(w0[y] >> 32);
                 a.out_tokens[at] = (int64_t)(uint32_t)w0[y];
             } else {
-                key[place[y]] = k0[y], who[place[y]] = w0[y];
+                key[to[y]] = k0[y], who[to[y]] = w0[y];
             }
         }
         __syncthreads();
     };
-    // Down the lists: each thread adds one candidate to the pool at a time.
-    int64_t l = list0;
-    int place = place0;
-    bool more = used && l < L;
-    while (true) {
-        bool add = false;
-        while (more && !add) {
-            add = entry(l, place, e) && e.key32 >= least && !(e.key < kth_key || (e.key == kth_key && e.who > kth_who));
-            if (add) {
-                place += per;
-            } else {  // the rest of the list is behind
-                l += 1024, place = place0;
-                more = per == 1 && l < L;
-            }
-        }
-        if (add) {
+#pragma unroll 4
+    for (uint32_t i = tid; i < places; i += 1024) {
+        const uint32_t l = i / (uint32_t)a.k;
+        if (entry(l, (int)(i - l * a.k), e) && e.key32 >= least) {
             const uint32_t at = atomicAdd(&count, 1u);
-            key[at] = e.key, who[at] = e.who;
+            if (at < BEAM_POOL) key[at] = e.key, who[at] = e.who;
         }
-        if (!__syncthreads_or(add)) break;
-        const uint32_t n = count;
+    }
+    __syncthreads();
+    if (count > BEAM_POOL) {
+        // Many equal totals: 1024 entries at a time, beside the k best of those before.
+        uint64_t kth_key = 0, kth_who = ~0ull;
         __syncthreads();
-        if (n > BEAM_POOL - 1024) {
-            order(n, false);
-            const uint32_t kept = min(n, (uint32_t)a.k);
-            if (kept == (uint32_t)a.k) kth_key = key[kept - 1], kth_who = who[kept - 1];
-            if (tid == 0) count = kept;
+        if (tid == 0) count = 0;
+        __syncthreads();
+        for (uint32_t i0 = 0; i0 < places; i0 += 1024) {
+            const uint32_t i = i0 + tid, l = i / (uint32_t)a.k;
+            if (i < places && entry(l, (int)(i - l * a.k), e) && e.key32 >= least &&
+                (e.key > kth_key || (e.key == kth_key && e.who < kth_who))) {
+                const uint32_t at = atomicAdd(&count, 1u);
+                key[at] = e.key, who[at] = e.who;
+            }
             __syncthreads();
+            const uint32_t n = count;
+            __syncthreads();
+            if (n > BEAM_POOL - 1024) {
+                order(n, false);
+                const uint32_t kept = min(n, (uint32_t)a.k);
+                if (kept == (uint32_t)a.k) kth_key = key[kept - 1], kth_who = who[kept - 1];
+                if (tid == 0) count = kept;
+                __syncthreads();
+            }
         }
     }
     order(count, true);
