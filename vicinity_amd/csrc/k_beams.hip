@@ -49,16 +49,36 @@ __device__ __forceinline__ float element(const uint4& r, int e) {
     return T == KV_F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)h) : __uint_as_float(h << 16);
 }
 
-constexpr int BEAM_LIST = 1024;  // tokens that one slice puts in order
+// Largest element of a piece, a NaN only if all are (fmaxf would quiet each operand first).
+template <int T>
+__device__ __forceinline__ float piece_top(const uint4& r) {
+    float x[T == KV_F32 ? 4 : 8], m;
+#pragma unroll
+    for (int e = 0; e < (T == KV_F32 ? 4 : 8); e++) x[e] = element<T>(r, e);
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(x[0]), "v"(x[1]), "v"(x[2]));
+    if (T == KV_F32) {
+        asm("v_max_f32 %0, %1, %2" : "=v"(m) : "v"(m), "v"(x[3]));
+    } else {
+        asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(m), "v"(x[3]), "v"(x[4 % (T == KV_F32 ? 4 : 8)]));
+        asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(m), "v"(x[5 % (T == KV_F32 ? 4 : 8)]), "v"(x[6 % (T == KV_F32 ? 4 : 8)]));
+        asm("v_max_f32 %0, %1, %2" : "=v"(m) : "v"(m), "v"(x[7 % (T == KV_F32 ? 4 : 8)]));
+    }
+    return m;
+}
+
+constexpr int BEAM_LIST = 1024;   // tokens that one slice puts in order
+constexpr int BEAM_PIECES = 512;  // pieces that are looked through for them
 
 // One workgroup: one slice of one row, loaded at once.  Bound by the vector unit where rows are
 // many: a conversion, a comparison, a difference, a product, an exponential (four times as
 // long) and a sum for each logit.
 template <int T, int N>
 __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs a) {
-    constexpr int W = T == KV_F32 ? 4 : 8, SLICE = 256 * N * W, HALF = (N + 1) / 2;
+    constexpr int W = T == KV_F32 ? 4 : 8, HALF = (N + 1) / 2;
     __shared__ uint64_t list[BEAM_LIST];  // (key, ~token)
-    __shared__ uint32_t count, scan[4], bounds[4];
+    __shared__ uint4 found[BEAM_PIECES];  // pieces with an element that reaches the bound
+    __shared__ int found_at[BEAM_PIECES];
+    __shared__ uint32_t count, pieces, scan[4], bounds[4];
     __shared__ float tops[4];
     __shared__ double sums[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -68,21 +88,24 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs a) {
     const uint8_t* base = (const uint8_t*)a.logits + (int64_t)row * a.st_row * (int64_t)item;
     // Places of a row count from the 16-byte boundary before it.
     const int skew = a.st_token == 1 ? (int)((uintptr_t)base & 15) / (int)item : 0;
-    const int first = slice * SLICE + tid * W - skew;  // token of the thread's first element
+    const int begin = slice * a.pieces * (256 * W) - skew, first = begin + tid * W;  // tokens at the slice's and the thread's first place
+    const int np = min(a.pieces, (a.vocab - begin + 256 * W - 1) / (256 * W));  // pieces of a thread, 0 or less: none
     const auto token = [&](int p, int e) { return first + p * (256 * W) + e; };
     const auto load = [&](int p) {
         const int t0 = token(p, 0);
         if (a.st_token == 1 && t0 >= 0 && t0 + W <= a.vocab) return *(const uint4*)(base + (int64_t)t0 * (int64_t)item);
-        // ends of the row, or elements apart: one by one, -inf outside
+        constexpr uint32_t none = T == KV_F32 ? 0xff800000u : T == KV_F16 ? 0xfc00fc00u : 0xff80ff80u;  // -inf
+        if (t0 >= a.vocab) return make_uint4(none, none, none, none);
+        // ends of the row, or elements apart: one by one
         uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int e = 0; e < W; e++) {
             const bool in = t0 + e >= 0 && t0 + e < a.vocab;
             const int64_t at = (int64_t)(t0 + e) * a.st_token;
             if (T == KV_F32)
-                w[e] = in ? ((const uint32_t*)base)[at] : 0xff800000u;
+                w[e] = in ? ((const uint32_t*)base)[at] : none;
             else
-                w[e >> 1] |= (in ? (uint32_t)((const uint16_t*)base)[at] : T == KV_F16 ? 0xfc00u : 0xff80u) << (16 * (e & 1));
+                w[e >> 1] |= (in ? (uint32_t)((const uint16_t*)base)[at] : none >> 16) << (16 * (e & 1));
         }
         return make_uint4(w[0], w[1], w[2], w[3]);
     };
@@ -93,15 +116,14 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs a) {
     };
     uint4 x[N];
 #pragma unroll
-    for (int p = 0; p < N; p++) x[p] = load(p);
-    if (tid == 0) count = 0;
+    for (int p = 0; p < N; p++)
+        if (p < np) x[p] = load(p);
+    if (tid == 0) count = 0, pieces = 0;
     // the largest of each piece, and of each half of the pieces (NaN are passed over)
     float tp[N], th[2] = {BEAM_NEG, BEAM_NEG};
 #pragma unroll
     for (int p = 0; p < N; p++) {
-        tp[p] = element<T>(x[p], 0);
-#pragma unroll
-        for (int e = 1; e < W; e++) tp[p] = fmaxf(tp[p], element<T>(x[p], e));
+        tp[p] = p < np ? piece_top<T>(x[p]) : __builtin_nanf("");
         th[p / HALF] = fmaxf(th[p / HALF], tp[p]);
     }
     keep(x);
@@ -112,8 +134,8 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs a) {
     {
         constexpr int BITS = T == KV_BF16 ? 16 : T == KV_F16 ? 19 : 18, SHIFT = 32 - BITS;
         const uint32_t k0 = token(0, 0) < a.vocab ? size_key(th[0]) >> SHIFT : 0;
-        const uint32_t k1 = token(HALF, 0) < a.vocab ? size_key(th[1]) >> SHIFT : 0;
-        const int used = min(max((a.vocab + skew - slice * SLICE + W - 1) / W, 0), 256);  // threads that have a token
+        const uint32_t k1 = HALF < np && token(HALF, 0) < a.vocab ? size_key(th[1]) >> SHIFT : 0;
+        const int used = min(max((a.vocab - begin + W - 1) / W, 0), 256);  // threads that have a token
         const auto most_of = [&](int r) {  // halves, with at most r of each wave
             return min(r, min(used, 64)) + min(r, min(max(used - 64, 0), 64)) + min(r, min(max(used - 128, 0), 64)) +
                    min(r, max(used - 192, 0));
@@ -126,7 +148,7 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs a) {
 #pragma unroll
         for (int bit = BITS - 1; bit >= 0; bit--) {
             const uint32_t more = key | 1u << bit;
-            if (__popcll(__ballot(k0 >= more)) + __popcll(__ballot(k1 >= more)) >= need) key = more;
+            if (__popcll(__builtin_amdgcn_ballot_w64(k0 >= more)) + __popcll(__builtin_amdgcn_ballot_w64(k1 >= more)) >= need) key = more;
         }
 #pragma unroll
         for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
@@ -136,36 +158,70 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs a) {
     const uint32_t bound = min(min(bounds[0], bounds[1]), min(bounds[2], bounds[3]));
     const float least = bound < size_key(BEAM_NEG) ? BEAM_NEG : of_key(bound);
     const float most = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    // Pieces that reach the bound go to LDS, where their elements are looked at side by side.
+    if (least == BEAM_NEG)  // (what lies outside of the row does too)
 #pragma unroll
-    for (int p = 0; p < N; p++) {
-        if (!(tp[p] >= least)) continue;
+        for (int p = 0; p < N; p++) tp[p] = token(p, 0) < a.vocab ? tp[p] : __builtin_nanf("");
+    uint32_t hits = 0;
 #pragma unroll
-        for (int e = 0; e < W; e++) {
-            const float v = element<T>(x[p], e);
-            const int t = token(p, e);
-            if (v >= least && t >= 0 && t < a.vocab) {
-                const uint32_t at = atomicAdd(&count, 1u);
-                if (at < BEAM_LIST) list[at] = (uint64_t)size_key(v) << 32 | (uint32_t)~t;
+    for (int p = 0; p < N; p++) hits += tp[p] >= least;
+    if (hits) {
+        uint32_t at = atomicAdd(&pieces, hits);
+#pragma unroll
+        for (int p = 0; p < N; p++)
+            if (tp[p] >= least) {
+                if (at < BEAM_PIECES) found[at] = x[p], found_at[at] = token(p, 0);
+                at++;
             }
-        }
     }
     keep(x);
-    // (a row of -inf alone: exp(-inf - 0) = 0; NaN and +inf make the sum NaN)
+    // exp(x - off) as 2^(x log2 e - c), c = off log2 e rounded, and what that rounding did taken
+    // back from the sum.  (A row of -inf alone: off 0, every term 0; NaN makes the sum NaN.)
     const float off = most == BEAM_NEG ? 0.f : most;
+    const float c = off * BEAM_LOG2E, rest = __builtin_fmaf(off, BEAM_LOG2E, -c);
+    const bool plain = fabsf(off) < 0x1p100f;
     float sum = 0.f;
+    if (plain) {
 #pragma unroll
-    for (int p = 0; p < N; p++)
+        for (int p = 0; p < N; p++)
+            if (p < np)
 #pragma unroll
-        for (int e = 0; e < W; e++) sum += __builtin_amdgcn_exp2f((element<T>(x[p], e) - off) * BEAM_LOG2E);
+            for (int e = 0; e < W; e++) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(element<T>(x[p], e), BEAM_LOG2E, -c));
+    } else {  // c may not be finite; +inf makes the sum NaN
+#pragma unroll 1
+        for (int p = 0; p < np; p++) {
+            const uint4 r = load(p);
+#pragma unroll
+            for (int e = 0; e < W; e++) sum += __builtin_amdgcn_exp2f((element<T>(r, e) - off) * BEAM_LOG2E);
+        }
+    }
     double total = sum;
 #pragma unroll
     for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o);
     if (lane == 0) sums[wave] = total;
     __syncthreads();
     const size_t part = (size_t)row * a.slices + slice;
-    if (tid == 0) a.top[part] = off, a.sum[part] = sums[0] + sums[1] + sums[2] + sums[3];
+    if (tid == 0)
+        a.top[part] = off, a.sum[part] = (sums[0] + sums[1] + sums[2] + sums[3]) * exp2(plain ? -(double)rest : 0.0);
     uint2* best = a.best + part * a.k;
-    uint32_t n = count;
+    uint32_t n = pieces;
+    if (n <= BEAM_PIECES) {
+        for (uint32_t i = tid; i < n * W; i += 256) {
+            const int t = found_at[i / W] + (int)(i & (W - 1));
+            float v;
+            if (T == KV_F32) v = ((const float*)found)[i];
+            else if (T == KV_F16) v = (float)((const _Float16*)found)[i];
+            else v = __uint_as_float((uint32_t)((const uint16_t*)found)[i] << 16);
+            if (v >= least && t >= 0 && t < a.vocab) {
+                const uint32_t at = atomicAdd(&count, 1u);
+                if (at < BEAM_LIST) list[at] = (uint64_t)size_key(v) << 32 | (uint32_t)~t;
+            }
+        }
+        __syncthreads();
+        n = count;
+    } else {
+        n = BEAM_LIST + 1;
+    }
     if (n > BEAM_LIST) {
         // Many reach the bound: the k-th best key itself, then the tokens above it and the first
         // of those that have it.  Every wave of the workgroup comes here.
@@ -173,7 +229,7 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs a) {
         const auto reach = [&](uint32_t key) {  // how many of the slice's tokens are not below key
             uint32_t c = 0;
 #pragma unroll 1
-            for (int p = 0; p < N; p++) {
+            for (int p = 0; p < np; p++) {
                 const uint4 r = load(p);
 #pragma unroll
                 for (int e = 0; e < W; e++) {
@@ -200,7 +256,7 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs a) {
         if (tid == 0) count = 0;
         __syncthreads();
 #pragma unroll 1
-        for (int p = 0; p < N; p++) {
+        for (int p = 0; p < np; p++) {
             const uint4 r = load(p);
 #pragma unroll
             for (int e = 0; e < W; e++) {
@@ -212,7 +268,7 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs a) {
         __syncthreads();
         n = count;  // below k
 #pragma unroll 1
-        for (int p = 0; p < N; p++) {
+        for (int p = 0; p < np; p++) {
             if (n >= (uint32_t)a.k) break;
             const uint4 r = load(p);
             uint32_t c = 0;
@@ -422,13 +478,22 @@ __global__ __launch_bounds__(1024) void beam_group_kernel(BeamArgs a) {
         }
         __syncthreads();
     };
-#pragma unroll 4
-    for (uint32_t i = tid; i < places; i += 1024) {
-        const uint32_t l = i / (uint32_t)a.k;
-        if (entry(l, (int)(i - l * a.k), e) && e.key32 >= least) {
-            const uint32_t at = atomicAdd(&count, 1u);
-            if (at < BEAM_POOL) key[at] = e.key, who[at] = e.who;
+    // 16 lanes to a list, as far as the sample that does not reach the bound
+    for (uint32_t l0 = 0; l0 < L; l0 += 64) {
+        const uint32_t l = l0 + (tid >> 4);
+        const int step = lane & 15;
+        bool reaches = false;
+        if (l < L && step < steps) {
+            const int at = (1 << step) - 1;
+            reaches = keep ? sample[step * L + l] >= max(least, 1u) : entry(l, at, e) && e.key32 >= least;
         }
+        const int reached = __popc((uint32_t)(__ballot(reaches) >> (lane & 48)) & 0xffffu);
+        const int end = reached == steps ? a.k : (1 << reached) - 1;
+        for (int at = step; at < end; at += 16)
+            if (entry(l, at, e) && e.key32 >= least) {
+                const uint32_t to = atomicAdd(&count, 1u);
+                if (to < BEAM_POOL) key[to] = e.key, who[to] = e.who;
+            }
     }
     __syncthreads();
     if (count > BEAM_POOL) {
@@ -462,7 +527,7 @@ __global__ __launch_bounds__(1024) void beam_group_kernel(BeamArgs a) {
 template <int T>
 void slices_of(const BeamArgs& a, hipStream_t s) {
     const dim3 grid((unsigned)(a.rows * a.slices));
-    if (a.pieces == 8)
+    if (a.pieces > 2)
         hipLaunchKernelGGL((beam_slice_kernel<T, 8>), grid, dim3(256), 0, s, a);
     else
         hipLaunchKernelGGL((beam_slice_kernel<T, 2>), grid, dim3(256), 0, s, a);
@@ -472,10 +537,11 @@ void slices_of(const BeamArgs& a, hipStream_t s) {
 
 void beam_plan(BeamArgs& a) {
     const int skew = a.type == KV_F32 ? 3 : 7;  // places before a row, at most
-    for (int pieces : {8, 2}) {
-        a.pieces = pieces;
-        const int64_t slice = beam_slice(a);
-        a.slices = (int)((a.vocab + skew + slice - 1) / slice);
+    const int64_t piece = 256 * (a.type == KV_F32 ? 4 : 8), all = (a.vocab + skew + piece - 1) / piece;
+    // Slices of at most 8 pieces, alike; of 2 where that leaves the card's workgroups idle.
+    for (int most : {8, 2}) {
+        a.slices = (int)((all + most - 1) / most);
+        a.pieces = (int)((all + a.slices - 1) / a.slices);
         if ((int64_t)a.rows * a.slices >= 512) break;
     }
 }

@@ -16,7 +16,7 @@ struct BeamArgs {
     const float* scores = nullptr;     // of the rows, or null: 0
     int64_t st_score = 0;
     int rows = 0, vocab = 0, beams = 0, k = 0;
-    int pieces = 0;                    // 16-byte pieces of a thread in a slice of a row
+    int pieces = 0;                    // of 16 bytes, of each of 256 threads, in a slice of a row
     int slices = 0;                    // of a row
     // of each row and slice: largest logit, sum of exp(logit - it), and its k best tokens
     float* top = nullptr;
@@ -26,8 +26,6 @@ struct BeamArgs {
     int64_t *out_parents = nullptr, *out_tokens = nullptr;
 };
 
-// Elements of a slice: 256 threads of `pieces` 16-byte pieces.
-inline int beam_slice(const BeamArgs& a) { return 256 * a.pieces * (a.type == 0 ? 4 : 8); }
 // Sets pieces and slices.
 void beam_plan(BeamArgs& a);
 void launch_beams(const BeamArgs& a, hipStream_t s);
