@@ -19,6 +19,8 @@ namespace vgpu {
 
 namespace {
 
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
 #define BEAM_NEG (-__builtin_huge_valf())
 constexpr float BEAM_LOG2E = 1.44269504088896341f;
 
@@ -82,30 +84,38 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs a) {
     __shared__ float tops[4];
     __shared__ double sums[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int row = blockIdx.x / a.slices, slice = blockIdx.x - row * a.slices;
+    const int row = __builtin_amdgcn_readfirstlane(blockIdx.x / a.slices), slice = blockIdx.x - row * a.slices;
     if (score_kind(score_of(a, row))) return;  // its logits do not matter
     const size_t item = T == KV_F32 ? 4 : 2;
-    const uint8_t* base = (const uint8_t*)a.logits + (int64_t)row * a.st_row * (int64_t)item;
+    typedef const __attribute__((address_space(1))) uint8_t* Bytes;
+    const Bytes base = (Bytes)a.logits + (int64_t)row * a.st_row * (int64_t)item;
     // Places of a row count from the 16-byte boundary before it.
     const int skew = a.st_token == 1 ? (int)((uintptr_t)base & 15) / (int)item : 0;
     const int begin = slice * a.pieces * (256 * W) - skew, first = begin + tid * W;  // tokens at the slice's and the thread's first place
     const int np = min(a.pieces, (a.vocab - begin + 256 * W - 1) / (256 * W));  // pieces of a thread, 0 or less: none
     const auto token = [&](int p, int e) { return first + p * (256 * W) + e; };
+    const bool apart = a.st_token != 1;
+    const auto piece = [&](int t0) {
+        return __builtin_bit_cast(uint4, *(const __attribute__((address_space(1))) u32x4*)(base + (int64_t)t0 * (int64_t)item));
+    };
     const auto load = [&](int p) {
         const int t0 = token(p, 0);
-        if (a.st_token == 1 && t0 >= 0 && t0 + W <= a.vocab) return *(const uint4*)(base + (int64_t)t0 * (int64_t)item);
+        if (!apart && t0 >= 0 && t0 + W <= a.vocab) return piece(t0);
         constexpr uint32_t none = T == KV_F32 ? 0xff800000u : T == KV_F16 ? 0xfc00fc00u : 0xff80ff80u;  // -inf
         if (t0 >= a.vocab) return make_uint4(none, none, none, none);
-        // ends of the row, or elements apart: one by one
-        uint32_t w[4] = {0, 0, 0, 0};
+        // ends of the row, or elements apart: one by one, those outside from an end
+        uint32_t r[W], w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < W; e++) {
+            const Bytes at = base + (int64_t)min(max(t0 + e, 0), a.vocab - 1) * a.st_token * (int64_t)item;
+            r[e] = T == KV_F32 ? *(const __attribute__((address_space(1))) uint32_t*)at
+                               : (uint32_t) * (const __attribute__((address_space(1))) uint16_t*)at;
+        }
 #pragma unroll
         for (int e = 0; e < W; e++) {
             const bool in = t0 + e >= 0 && t0 + e < a.vocab;
-            const int64_t at = (int64_t)(t0 + e) * a.st_token;
-            if (T == KV_F32)
-                w[e] = in ? ((const uint32_t*)base)[at] : none;
-            else
-                w[e >> 1] |= (in ? (uint32_t)((const uint16_t*)base)[at] : none >> 16) << (16 * (e & 1));
+            if (T == KV_F32) w[e] = in ? r[e] : none;
+            else w[e >> 1] |= (in ? r[e] : none >> 16) << (16 * (e & 1));
         }
         return make_uint4(w[0], w[1], w[2], w[3]);
     };
@@ -115,9 +125,15 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs a) {
         for (int p = 0; p < N; p++) asm volatile("" : "+v"(r[p].x), "+v"(r[p].y), "+v"(r[p].z), "+v"(r[p].w));
     };
     uint4 x[N];
+    if (!apart && begin >= 0 && begin + np * (256 * W) <= a.vocab) {
 #pragma unroll
-    for (int p = 0; p < N; p++)
-        if (p < np) x[p] = load(p);
+        for (int p = 0; p < N; p++)
+            if (p < np) x[p] = piece(token(p, 0));
+    } else {
+#pragma unroll
+        for (int p = 0; p < N; p++)
+            if (p < np) x[p] = load(p);
+    }
     if (tid == 0) count = 0, pieces = 0;
     // the largest of each piece, and of each half of the pieces (NaN are passed over)
     float tp[N], th[2] = {BEAM_NEG, BEAM_NEG};
@@ -179,7 +195,7 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs a) {
     // back from the sum.  (A row of -inf alone: off 0, every term 0; NaN makes the sum NaN.)
     const float off = most == BEAM_NEG ? 0.f : most;
     const float c = off * BEAM_LOG2E, rest = __builtin_fmaf(off, BEAM_LOG2E, -c);
-    const bool plain = fabsf(off) < 0x1p100f;
+    const bool plain = fabsf(off) < 0x1p12f;  // then rest is below 2^-11
     float sum = 0.f;
     if (plain) {
 #pragma unroll
@@ -187,7 +203,7 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs a) {
             if (p < np)
 #pragma unroll
             for (int e = 0; e < W; e++) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(element<T>(x[p], e), BEAM_LOG2E, -c));
-    } else {  // c may not be finite; +inf makes the sum NaN
+    } else {  // (c may not be finite; +inf makes the sum NaN)
 #pragma unroll 1
         for (int p = 0; p < np; p++) {
             const uint4 r = load(p);
@@ -201,8 +217,10 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs a) {
     if (lane == 0) sums[wave] = total;
     __syncthreads();
     const size_t part = (size_t)row * a.slices + slice;
-    if (tid == 0)
-        a.top[part] = off, a.sum[part] = (sums[0] + sums[1] + sums[2] + sums[3]) * exp2(plain ? -(double)rest : 0.0);
+    if (tid == 0) {
+        const double y = plain ? (double)rest * -0.6931471805599453 : 0.0;  // 2^-rest by its series
+        a.top[part] = off, a.sum[part] = (sums[0] + sums[1] + sums[2] + sums[3]) * (1.0 + y + y * y * 0.5);
+    }
     uint2* best = a.best + part * a.k;
     uint32_t n = pieces;
     if (n <= BEAM_PIECES) {
