@@ -5,12 +5,19 @@ It stands beside KVCache: the rows that it returns are what ``KVCache.fork`` con
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import functools
 
 import numpy as np
 
 from . import _lib
+
+
+@functools.lru_cache(maxsize=64)
+def _workspace(*sizes) -> int:
+    size = ctypes.c_size_t()
+    _lib.check(_lib.load().vgpu_beams_workspace(*sizes, ctypes.byref(size)))
+    return size.value
 
 
 def select_beams(logits, scores, beams: int, k: int | None = None, stream=None):
@@ -33,39 +40,44 @@ def select_beams(logits, scores, beams: int, k: int | None = None, stream=None):
     graph.  There is no backward."""
     import torch
 
-    types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-    if not isinstance(logits, torch.Tensor) or logits.dtype not in types:
+    if not isinstance(logits, torch.Tensor) or logits.dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise TypeError("logits must be a float32, float16 or bfloat16 tensor")
     if logits.dim() != 2 or not logits.is_cuda:
         raise ValueError("logits must have the shape [rows, vocab], on a GPU")
     rows, vocab = logits.shape
-    if scores is not None and (not isinstance(scores, torch.Tensor) or scores.dtype != torch.float32):
-        raise TypeError("scores must be a float32 tensor")
-    if scores is not None and (scores.shape != (rows,) or scores.device != logits.device):
-        raise ValueError(f"scores must have the shape [{rows}], on the logits' GPU")
+    if scores is not None:
+        if not isinstance(scores, torch.Tensor) or scores.dtype != torch.float32:
+            raise TypeError("scores must be a float32 tensor")
+        if scores.shape != (rows,) or scores.device != logits.device:
+            raise ValueError(f"scores must have the shape [{rows}], on the logits' GPU")
     k = beams if k is None else k
     for name, value in (("beams", beams), ("k", k)):
         if not isinstance(value, (int, np.integer)) or not 0 < value < 1 << 31:
             raise ValueError(f"{name} must be an int above 0")
-    lib = _lib.load()
-    size = ctypes.c_size_t()
-    _lib.check(lib.vgpu_beams_workspace(types[logits.dtype], rows, vocab, beams, k, ctypes.byref(size)))
-    use = torch.cuda.current_stream(logits.device) if stream is None else stream
-    with contextlib.ExitStack() as ctx:
-        ctx.enter_context(torch.cuda.device(logits.device))
-        if stream is not None:
-            ctx.enter_context(torch.cuda.stream(stream))
-            for t in (logits, scores):
-                if t is not None:
-                    t.record_stream(stream)
-        shape = (rows // beams, k)
-        totals = torch.empty(shape, dtype=torch.float32, device=logits.device)
-        parents = torch.empty(shape, dtype=torch.int64, device=logits.device)
-        tokens = torch.empty(shape, dtype=torch.int64, device=logits.device)
-        work = torch.empty(size.value, dtype=torch.uint8, device=logits.device)
-        call = _lib.Beams(logits.data_ptr(), types[logits.dtype], *logits.stride(), rows, vocab, beams, k,
-                          scores.data_ptr() if scores is not None else None,
-                          scores.stride(0) if scores is not None else 0, work.data_ptr(), size.value,
-                          totals.data_ptr(), parents.data_ptr(), tokens.data_ptr())
-        _lib.check(lib.vgpu_select_beams(ctypes.byref(call), use.cuda_stream or None))
+    dtype = 0 if logits.dtype == torch.float32 else 1 if logits.dtype == torch.float16 else 2
+    size = _workspace(dtype, rows, vocab, int(beams), int(k))
+    device = logits.device
+    if stream is None and device.index == torch.cuda.current_device():
+        return _select(torch, logits, scores, dtype, beams, k, size,
+                       torch._C._cuda_getCurrentRawStream(device.index))
+    use = torch.cuda.current_stream(device) if stream is None else stream
+    with torch.cuda.device(device), torch.cuda.stream(use):
+        for t in (logits, scores):
+            if t is not None:
+                t.record_stream(use)
+        return _select(torch, logits, scores, dtype, beams, k, size, use.cuda_stream)
+
+
+def _select(torch, logits, scores, dtype, beams, k, size, stream):
+    device, (rows, vocab) = logits.device, logits.shape
+    shape = (rows // beams, k)
+    totals = torch.empty(shape, dtype=torch.float32, device=device)
+    parents = torch.empty(shape, dtype=torch.int64, device=device)
+    tokens = torch.empty(shape, dtype=torch.int64, device=device)
+    work = torch.empty(size, dtype=torch.uint8, device=device)
+    call = _lib.Beams(logits.data_ptr(), dtype, *logits.stride(), rows, vocab, beams, k,
+                      None if scores is None else scores.data_ptr(),
+                      0 if scores is None else scores.stride(0), work.data_ptr(), size,
+                      totals.data_ptr(), parents.data_ptr(), tokens.data_ptr())
+    _lib.check(_lib.load().vgpu_select_beams(ctypes.byref(call), stream or None))
     return totals, parents, tokens

@@ -75,7 +75,7 @@ constexpr int BEAM_PIECES = 512;  // pieces that are looked through for them
 // many: a conversion, a comparison, a difference, a product, an exponential (four times as
 // long) and a sum for each logit.
 template <int T, int N>
-__global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs a) {
+__global__ __launch_bounds__(256, T == KV_F32 ? 6 : 7) void beam_slice_kernel(BeamArgs a) {
     constexpr int W = T == KV_F32 ? 4 : 8, HALF = (N + 1) / 2;
     __shared__ uint64_t list[BEAM_LIST];  // (key, ~token)
     __shared__ uint4 found[BEAM_PIECES];  // pieces with an element that reaches the bound
@@ -344,11 +344,10 @@ __global__ __launch_bounds__(1024) void beam_group_kernel(BeamArgs a) {
     __shared__ double lift[BEAM_MAX_BEAMS];
     __shared__ float largest[BEAM_MAX_BEAMS];
     __shared__ uint8_t kinds[BEAM_MAX_BEAMS];
-    __shared__ uint64_t key[BEAM_POOL];  // the total's order
-    __shared__ uint64_t who[BEAM_POOL];  // beam << 32 | token
+    __shared__ ulonglong2 pool[BEAM_POOL];  // the total's order; beam << 32 | token
     __shared__ uint32_t sample[BEAM_SAMPLES];
     __shared__ uint32_t hist[BEAM_BINS];
-    __shared__ uint32_t place[BEAM_POOL];
+    __shared__ uint32_t place[256];
     __shared__ uint32_t scan[18], count;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int row0 = blockIdx.x * a.beams;
@@ -431,6 +430,7 @@ __global__ __launch_bounds__(1024) void beam_group_kernel(BeamArgs a) {
         return d;
     };
     const uint32_t L = (uint32_t)a.beams * a.slices, places = L * (uint32_t)a.k;
+    const bool few = places <= 256;  // put in order without a bound
     const int steps = 32 - __clz(a.k);  // samples of a list
     const auto each_sample = [&](auto&& f) {
         for (uint32_t i = tid; i < L * steps; i += 1024) {
@@ -441,57 +441,75 @@ __global__ __launch_bounds__(1024) void beam_group_kernel(BeamArgs a) {
     };
     Entry e;
     const bool keep = L * steps <= BEAM_SAMPLES;
-    each_sample([&](uint32_t i, uint32_t l, int at, uint32_t weight) {
-        const uint32_t k32 = entry(l, at, e) ? e.key32 : 0;
-        if (keep) sample[i] = k32;
-        if (k32) atomicAdd(&hist[k32 >> 21], weight);
-    });
-    __syncthreads();
     uint32_t need = (uint32_t)a.k, least = 0;
-    const uint32_t d0 = digit(need);
-    if (d0 != ~0u) {
+    if (!few) {
         each_sample([&](uint32_t i, uint32_t l, int at, uint32_t weight) {
-            const uint32_t k32 = keep ? sample[i] : entry(l, at, e) ? e.key32 : 0;
-            if (k32 && k32 >> 21 == d0) atomicAdd(&hist[k32 >> 10 & 2047u], weight);
+            const uint32_t k32 = entry(l, at, e) ? e.key32 : 0;
+            if (keep) sample[i] = k32;
+            if (k32) atomicAdd(&hist[k32 >> 21], weight);
         });
         __syncthreads();
-        least = d0 << 21 | digit(need) << 10;
+        const uint32_t d0 = digit(need);
+        if (d0 != ~0u) {
+            each_sample([&](uint32_t i, uint32_t l, int at, uint32_t weight) {
+                const uint32_t k32 = keep ? sample[i] : entry(l, at, e) ? e.key32 : 0;
+                if (k32 && k32 >> 21 == d0) atomicAdd(&hist[k32 >> 10 & 2047u], weight);
+            });
+            __syncthreads();
+            least = d0 << 21 | digit(need) << 10;
+        }
     }
 
-    // Put the pool's n candidates in order: the k best stay, or go out.
+    // Put the pool's n candidates in order: the k best stay in front, or go out.
+    const auto before = [](const ulonglong2& x, const ulonglong2& y) { return (x.x > y.x) | ((x.x == y.x) & (x.y < y.y)); };
     const auto order = [&](uint32_t n, bool out) {
-        // as many threads to a candidate as there are
-        int wide = 64;
-        while (wide < (int)n && wide < 1024) wide <<= 1;
-        for (uint32_t i = tid; i < n; i += 1024) place[i] = 0;
-        __syncthreads();
-        for (uint32_t i = tid & (wide - 1); i < n; i += wide) {
-            const uint64_t k0 = key[i], w0 = who[i];
-            uint32_t c = 0;
-#pragma unroll 4
-            for (uint32_t j = tid / wide; j < n; j += 1024 / wide) c += key[j] > k0 || (key[j] == k0 && who[j] < w0);
-            if (c) atomicAdd(&place[i], c);
+        ulonglong2 mine;
+        uint32_t to = ~0u;
+        if (n <= 256) {
+            // by counting, 4 threads to a candidate: first by the upper halves of the orders, and
+            // in full where those are equal
+            const uint32_t* upper = (const uint32_t*)pool + 1;
+            const uint32_t i = tid & 255;
+            if (tid < 256) place[tid] = 0;
+            __syncthreads();
+            if (i < n) {
+                mine = pool[i];
+                const uint32_t top = (uint32_t)(mine.x >> 32);
+                uint32_t above = 0, equal = 0;
+#pragma unroll 8
+                for (uint32_t j = tid >> 8; j < n; j += 4) above += upper[4 * j] > top, equal += upper[4 * j] == top;
+                if (equal > (i % 4 == tid >> 8 ? 1u : 0u))
+                    for (uint32_t j = tid >> 8; j < n; j += 4) above += upper[4 * j] == top && before(pool[j], mine);
+                if (above) atomicAdd(&place[i], above);
+            }
+            __syncthreads();
+            if (tid < (int)n) to = place[tid];
+        } else {
+            uint32_t size = 512;
+            while (size < n) size <<= 1;
+            for (uint32_t i = n + tid; i < size; i += 1024) pool[i] = make_ulonglong2(0, ~0ull);
+            for (uint32_t run = 2; run <= size; run <<= 1)
+                for (uint32_t step = run >> 1; step; step >>= 1) {
+                    __syncthreads();
+                    for (uint32_t x = tid; x < size / 2; x += 1024) {
+                        const uint32_t i = 2 * x - (x & (step - 1)), j = i + step;
+                        const ulonglong2 p = pool[i], q = pool[j];
+                        if (before(q, p) == !(i & run)) pool[i] = q, pool[j] = p;
+                    }
+                }
+            __syncthreads();
+            if (tid < a.k && tid < (int)n) mine = pool[tid], to = tid;
         }
         __syncthreads();
-        uint64_t k0[2], w0[2];
-        uint32_t to[2] = {~0u, ~0u};
-#pragma unroll
-        for (int y = 0; y < 2; y++) {
-            const uint32_t i = tid + 1024 * y;
-            if (i < n) k0[y] = key[i], w0[y] = who[i], to[y] = place[i];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int y = 0; y < 2; y++) {
-            if (to[y] >= (uint32_t)a.k) continue;
+        if (to < (uint32_t)a.k) {
             if (out) {
-                const size_t at = (size_t)blockIdx.x * a.k + to[y];
-                const uint64_t u = k0[y] >> 63 ? k0[y] & ~(1ull << 63) : ~k0[y];
+                const size_t at = (size_t)blockIdx.x * a.k + to;
+                const uint64_t u = mine.x >> 63 ? mine.x & ~(1ull << 63) : ~mine.x;
                 a.out_scores[at] = (float)__longlong_as_double((long long)u);
-                a.out_parents[at] = row0 + (int64_t)(w0[y] >> 32);
-                a.out_tokens[at] = (int64_t)(uint32_t)w0[y];
+                a.out_parents[at] = row0 + (int64_t)(mine.y >> 32);
+                a.out_tokens[at] = (int64_t)(uint32_t)mine.y;
             } else {
-                key[to[y]] = k0[y], who[to[y]] = w0[y];
+                pool[to] = mine;
             }
         }
         __syncthreads();
@@ -503,14 +521,14 @@ __global__ __launch_bounds__(1024) void beam_group_kernel(BeamArgs a) {
         bool reaches = false;
         if (l < L && step < steps) {
             const int at = (1 << step) - 1;
-            reaches = keep ? sample[step * L + l] >= max(least, 1u) : entry(l, at, e) && e.key32 >= least;
+            reaches = few || (keep ? sample[step * L + l] >= max(least, 1u) : entry(l, at, e) && e.key32 >= least);
         }
         const int reached = __popc((uint32_t)(__ballot(reaches) >> (lane & 48)) & 0xffffu);
         const int end = reached == steps ? a.k : (1 << reached) - 1;
         for (int at = step; at < end; at += 16)
             if (entry(l, at, e) && e.key32 >= least) {
                 const uint32_t to = atomicAdd(&count, 1u);
-                if (to < BEAM_POOL) key[to] = e.key, who[to] = e.who;
+                if (to < BEAM_POOL) pool[to] = make_ulonglong2(e.key, e.who);
             }
     }
     __syncthreads();
@@ -525,7 +543,7 @@ __global__ __launch_bounds__(1024) void beam_group_kernel(BeamArgs a) {
             if (i < places && entry(l, (int)(i - l * a.k), e) && e.key32 >= least &&
                 (e.key > kth_key || (e.key == kth_key && e.who < kth_who))) {
                 const uint32_t at = atomicAdd(&count, 1u);
-                key[at] = e.key, who[at] = e.who;
+                pool[at] = make_ulonglong2(e.key, e.who);
             }
             __syncthreads();
             const uint32_t n = count;
@@ -533,7 +551,7 @@ __global__ __launch_bounds__(1024) void beam_group_kernel(BeamArgs a) {
             if (n > BEAM_POOL - 1024) {
                 order(n, false);
                 const uint32_t kept = min(n, (uint32_t)a.k);
-                if (kept == (uint32_t)a.k) kth_key = key[kept - 1], kth_who = who[kept - 1];
+                if (kept == (uint32_t)a.k) kth_key = pool[kept - 1].x, kth_who = pool[kept - 1].y;
                 if (tid == 0) count = kept;
                 __syncthreads();
             }
