@@ -18,6 +18,7 @@ namespace vgpu {
 namespace {
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
 // Scales are 0 below this largest magnitude, so 1 / s stays finite.
 constexpr float KV_TINY = 0x1p-100f;
@@ -131,8 +132,10 @@ __global__ __launch_bounds__(256) void kv_rename_kernel(int* table, int W, KvRow
     }
 }
 
-// Blocks copied whole: a workgroup takes 32 KiB of a block's codes (a block is contiguous, and
+// Blocks copied whole: a workgroup takes 16 KiB of a block's codes (a block is contiguous, and
 // a multiple of 4 KiB); the first of a block also takes its scales, positions and weights.
+// Stores pass the caches by, which leaves them to what is read (206 MB by themselves: 52 us,
+// cached stores 78, 32 KiB to a workgroup 63).
 __global__ __launch_bounds__(256) void kv_moves_kernel(KvDev from, KvDev to, KvMoves m, int pieces, int* map) {
     const int tid = threadIdx.x, unit = blockIdx.x / pieces, piece = blockIdx.x - unit * pieces;
     int lo = 0, hi = m.n;  // the run: unit0[lo] <= unit < unit0[lo + 1]
@@ -143,16 +146,16 @@ __global__ __launch_bounds__(256) void kv_moves_kernel(KvDev from, KvDev to, KvM
     }
     const int src = m.src[lo] + unit - m.unit0[lo], dst = m.dst[lo] + unit - m.unit0[lo];
     const size_t bytes = (size_t)from.H * from.B * 2 * from.Dp;
-    const uint4* in = (const uint4*)(from.pool + (size_t)src * bytes);
-    uint4* out = (uint4*)(to.pool + (size_t)dst * bytes);
+    const u32x4* in = (const u32x4*)(from.pool + (size_t)src * bytes);
+    u32x4* out = (u32x4*)(to.pool + (size_t)dst * bytes);
     const int at = piece * (KV_COPY * 256) + tid, end = (int)(bytes / 16);
-    uint4 x[KV_COPY];
+    u32x4 x[KV_COPY];
 #pragma unroll
     for (int j = 0; j < KV_COPY; j++)
         if (at + j * 256 < end) x[j] = in[at + j * 256];
 #pragma unroll
     for (int j = 0; j < KV_COPY; j++)
-        if (at + j * 256 < end) out[at + j * 256] = x[j];
+        if (at + j * 256 < end) __builtin_nontemporal_store(x[j], out + at + j * 256);
     if (piece) return;
     if (map && tid == 0) map[src] = dst;
     for (int h = tid; h < from.H; h += 256) {

@@ -139,8 +139,8 @@ struct KvMoves {
     int n = 0;
     int src[MAX], dst[MAX], unit0[MAX + 1];
 };
-// Workgroups that a block's copy takes, 32 KiB of its codes each.
-constexpr int KV_COPY = 8;  // 16-byte pieces of a thread
+// Workgroups that a block's copy takes, 16 KiB of its codes each.
+constexpr int KV_COPY = 4;  // 16-byte pieces of a thread
 inline int kv_move_pieces(const KvDev& c) {
     const int64_t bytes = (int64_t)c.H * c.B * 2 * c.Dp;
     return (int)((bytes + KV_COPY * 4096 - 1) / (KV_COPY * 4096));
