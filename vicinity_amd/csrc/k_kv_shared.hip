@@ -6,76 +6,84 @@ namespace vgpu {
 
 namespace {
 
-// Up to so many rows have a workgroup each in the join.
-constexpr int64_t KV_WIDE_JOIN = 16384;
-
-// A row's parts, of the shared slots and of its own, by Dp / 4 threads each: the sums o and l
-// go by the power of 2 that a part's m stands below the largest.  WIDE: a workgroup per row,
-// its thread groups take parts in turn; else a thread group per row.
-template <bool WIDE>
-__global__ __launch_bounds__(256) void kv_shared_join_kernel(KvDev c, KvAttend a, KvMembers mem, KvShares j) {
+// A row's parts, of the shared slots and of its own, by `share` groups of Dp / 4 threads, each of
+// which takes parts in turn, four at a time: the sums o and l go by the power of 2 that a part's
+// m stands below the largest, o also by the power of 2 that its S does.
+__global__ __launch_bounds__(256) void kv_shared_join_kernel(KvDev c, KvAttend a, KvMembers mem, KvShares j, int share) {
     __shared__ floatx4 sh_o[256];
-    __shared__ float sh_l[64];
+    __shared__ float sh_m[64], sh_l[64], sh_top[64];
+    __shared__ int row0[KV_BATCH + 1];
     const int tid = threadIdx.x;
-    const int width = c.Dp / 4, groups = 256 / width, grp = tid / width, d4 = tid % width;
-    const int h = kv_mod(blockIdx.x, c.by_heads), unit = kv_div(blockIdx.x, c.by_heads);
-    const int row = WIDE ? unit : unit * groups + grp;
-    if (!WIDE && (grp >= groups || row >= mem.row0[mem.n])) return;
+    const int width = c.Dp / 4, per_wg = 256 / width / share, grp = tid / width, d4 = tid % width;
+    if (tid <= mem.n) row0[tid] = mem.row0[tid];
+    __syncthreads();
+    const int h = kv_mod(blockIdx.x, c.by_heads);
+    const int row = kv_div(blockIdx.x, c.by_heads) * per_wg + grp / share, mine = grp % share;
+    const bool used = grp < per_wg * share && row < row0[mem.n];
     int m = 0, end = mem.n;
     while (end - m > 1) {
         const int mid = (m + end) / 2;
-        if (mem.row0[mid] <= row) m = mid;
+        if (row0[mid] <= row) m = mid;
         else end = mid;
     }
-    const int mine = row - mem.row0[m], s0 = j.splits[0][m], splits = s0 + j.splits[1][m];
-    size_t first[2], step[2];
-#pragma unroll
-    for (int y = 0; y < 2; y++) {
-        const int r = mine + (y ? 0 : j.row0[m]), tile = r / j.rows[y];
-        first[y] = j.base[y] + ((size_t)(j.unit[y][m] + tile) * c.H + h) * j.rows[y] + (r - tile * j.rows[y]);
-        step[y] = (size_t)j.tiles[y][m] * c.H * j.rows[y];
-    }
-    const auto part = [&](int s) { return s < s0 ? first[0] + s * step[0] : first[1] + (s - s0) * step[1]; };
-    float mx = KV_NEG, top = KV_FIRST;
-    if (WIDE) {
-        for (int s = tid & 63; s < splits; s += 64) {
-            const size_t at = part(s);
-            mx = fmaxf(mx, a.part_ml[at].x), top = fmaxf(top, a.part_s[at]);
-        }
-#pragma unroll
-        for (int x = 32; x; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x)), top = fmaxf(top, __shfl_xor(top, x));
-    } else {
-        for (int s = 0; s < splits; s++) {
-            const size_t at = part(s);
-            mx = fmaxf(mx, a.part_ml[at].x), top = fmaxf(top, a.part_s[at]);
-        }
-    }
+    const int r0 = row - row0[m];  // its row among the sequence's
+    float mx = KV_NEG, top = KV_FIRST, l = 0.f;
     floatx4 o = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.f;
-    if (grp < groups) {
-#pragma unroll 4
-        for (int s = WIDE ? grp : 0; s < splits; s += WIDE ? groups : 1) {
-            const size_t at = part(s);
-            const float2 ml = a.part_ml[at];
-            if (ml.x == KV_NEG && ml.y == 0.f) continue;  // has seen nothing (and left no o)
-            const float f = kv_join_factor(ml.x, ml.y, mx);
-            l += f * ml.y;
-            o += *(const floatx4*)(a.part_o + at * c.Dp + d4 * 4) * ldexpf(f, (int)(a.part_s[at] - top));
+    if (used) {
+        const int s0 = j.splits[0][m], splits = s0 + j.splits[1][m];
+        size_t first[2], step[2];
+#pragma unroll
+        for (int y = 0; y < 2; y++) {
+            const int r = r0 + (y ? 0 : j.row0[m]), tile = r / j.rows[y];
+            first[y] = j.base[y] + ((size_t)(j.unit[y][m] + tile) * c.H + h) * j.rows[y] + (r - tile * j.rows[y]);
+            step[y] = (size_t)j.tiles[y][m] * c.H * j.rows[y];
+        }
+        for (int s = mine; s < splits; s += 4 * share) {
+            float2 ml[4];
+            float st[4];
+            floatx4 po[4];
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const int t = min(s + x * share, splits - 1);
+                const size_t at = t < s0 ? first[0] + t * step[0] : first[1] + (t - s0) * step[1];
+                ml[x] = a.part_ml[at], st[x] = a.part_s[at];
+                po[x] = *(const floatx4*)(a.part_o + at * c.Dp + d4 * 4);
+            }
+            float now = mx, high = top;
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                // past the end, or without a slot (and then without an o)
+                if (s + x * share >= splits || (ml[x].x == KV_NEG && ml[x].y == 0.f))
+                    ml[x] = make_float2(KV_NEG, 0.f), st[x] = KV_FIRST, po[x] = floatx4{0.f, 0.f, 0.f, 0.f};
+                now = fmaxf(now, ml[x].x), high = fmaxf(high, st[x]);
+            }
+            const float down = kv_join_factor(mx, l, now);
+            l *= down, o *= ldexpf(down, (int)(top - high));
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const float f = kv_join_factor(ml[x].x, ml[x].y, now);
+                l += f * ml[x].y;
+                o += po[x] * ldexpf(f, (int)(st[x] - high));
+            }
+            mx = now, top = high;
         }
     }
-    if (WIDE) {
-        if (grp < groups) {
-            sh_o[tid] = o;
-            if (d4 == 0) sh_l[grp] = l;
-        }
+    if (share > 1) {
+        sh_o[tid] = o;
+        if (d4 == 0) sh_m[grp] = mx, sh_l[grp] = l, sh_top[grp] = top;
         __syncthreads();
-        if (tid >= width) return;
-        for (int x = 1; x < groups; x++) o += sh_o[x * width + tid];
-        l = sh_l[0];
-        for (int x = 1; x < groups; x++) l += sh_l[x];
+        if (mine) return;
+        for (int x = 1; x < share; x++) mx = fmaxf(mx, sh_m[grp + x]), top = fmaxf(top, sh_top[grp + x]);
+        o = floatx4{0.f, 0.f, 0.f, 0.f}, l = 0.f;
+        for (int x = 0; x < share; x++) {
+            const float f = kv_join_factor(sh_m[grp + x], sh_l[grp + x], mx);
+            l += f * sh_l[grp + x];
+            o += sh_o[tid + x * width] * ldexpf(f, (int)(sh_top[grp + x] - top));
+        }
     }
-    const int tok = kv_div(mine, a.by_group);
-    const size_t out = (size_t)(mem.tok0[m] + tok) * c.H * a.G + (size_t)h * a.G + (mine - tok * a.G);
+    if (!used) return;
+    const int tok = kv_div(r0, a.by_group);
+    const size_t out = (size_t)(mem.tok0[m] + tok) * c.H * a.G + (size_t)h * a.G + (r0 - tok * a.G);
     if (d4 == 0 && a.lse) a.lse[out] = (l == 0.f ? KV_NEG : mx - KV_TOP + log2f(l)) * 0.69314718055994531f;
     o = o * (l == 0.f ? 0.f : 1.f / l) * ldexpf(1.f, (int)top);
     if (a.q.type == KV_F32)
@@ -122,11 +130,12 @@ void launch_kv_shared(const KvDev& c, const KvBatch& b, const KvAttend& a, const
 }
 
 void launch_kv_shared_join(const KvDev& c, const KvAttend& a, const KvMembers& mem, const KvShares& j, hipStream_t s) {
+    int most = 0;
+    for (int m = 0; m < mem.n; m++) most = j.splits[0][m] + j.splits[1][m] > most ? j.splits[0][m] + j.splits[1][m] : most;
+    // a group of threads for every four parts, as many as there are
     const int rows = mem.row0[mem.n], groups = 256 / (c.Dp / 4);
-    if ((int64_t)rows * c.H <= KV_WIDE_JOIN)
-        hipLaunchKernelGGL(kv_shared_join_kernel<true>, dim3((unsigned)(rows * c.H)), dim3(256), 0, s, c, a, mem, j);
-    else
-        hipLaunchKernelGGL(kv_shared_join_kernel<false>, dim3((unsigned)((rows + groups - 1) / groups * c.H)), dim3(256), 0, s, c, a, mem, j);
+    const int share = (most + 3) / 4 < groups ? (most + 3) / 4 : groups, per_wg = groups / share;
+    hipLaunchKernelGGL(kv_shared_join_kernel, dim3((unsigned)((rows + per_wg - 1) / per_wg * c.H)), dim3(256), 0, s, c, a, mem, j, share);
 }
 
 }  // namespace vgpu

@@ -48,6 +48,8 @@ constexpr size_t kRowRuns = 64;
 
 // Sequences that share so many slots are taken over them together.
 constexpr int64_t kSharedSlots = 256;
+// Tiles of a workgroup over shared slots, at least.
+constexpr int64_t kLeastTiles = 8;
 // Levels of branches that are looked at for the best groups.
 constexpr int kSharedDepth = 4;
 
@@ -94,6 +96,20 @@ struct KvPlan {
             if (splits > 1) split_units += row_units[j] * splits * heads;
         }
         return one;
+    }
+
+    // The same for entries of shared slots, which are whole rectangles: the least share that
+    // keeps all workgroups on the card at once.
+    void split_entries(KvBatch& b, bool by_rows, int64_t part_units) {
+        const int64_t most = std::min(by_rows ? kChunkWorkgroups : kStepWorkgroups, part_units);
+        int64_t lo = kLeastTiles, hi = lo;
+        for (int j = 0; j < n; j++) hi = std::max(hi, tiles[j]);
+        while (lo < hi) {
+            const int64_t mid = (lo + hi) / 2;
+            if (cut(b, mid), groups <= most) hi = mid;
+            else lo = mid + 1;
+        }
+        cut(b, lo);
     }
 
     // As few tiles to a workgroup as keep all of them on the card at once; at most
@@ -928,7 +944,7 @@ void KvCache::attend_shared(const int32_t* ids, const int64_t* counts, const std
                     b[y].tok0[j] = (int)e.t0, b[y].len[j] = (int)e.end;
                     plan.add_entry(e.rows, (e.end + KV_TILE - 1) / KV_TILE - e.t0, wg);
                 }
-            plan.split(b[y], by_rows[y], kPartBytes / 2 / (wg * row_bytes));
+            plan.split_entries(b[y], by_rows[y], kPartBytes / 2 / (wg * row_bytes));
             base[y] = all_rows;
             all_rows += plan.groups * wg;
             int j = 0;
