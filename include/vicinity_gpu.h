@@ -511,6 +511,9 @@ int vgpu_test_host_centroid_update(const float *x, size_t n, size_t d, const uin
  * no window): splits i32[n], and the 32-slot tiles of one, i32[n]. */
 int vgpu_test_host_kv_splits(const int64_t *lens, const int64_t *counts, size_t n, size_t heads,
                              size_t group, int32_t *splits, int32_t *tiles);
+/* Attention reads slots that several sequences of a call share once for all of them where that
+ * saves so many bytes (0: wherever they share 256 slots). */
+int vgpu_test_set_kv_shared_bytes(vgpu_kv *h, size_t bytes);
 /* The OPQ polar factor U V^T of M f32[d*d] (compute_optimal_rotation,
  * opq.rs:280-294) into R f32[d*d]. */
 int vgpu_test_polar_factor(const float *m, size_t d, float *r);

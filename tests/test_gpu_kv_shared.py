@@ -22,7 +22,19 @@ def _torch():
     return torch
 
 
+def share(cache):
+    """Shared slots are read once also where that saves little."""
+    from vicinity_amd import _lib
+
+    _lib.check(_lib.load().vgpu_test_set_kv_shared_bytes(cache._h, 0))
+    return cache
+
+
 class Forks(Pair):
+    def __init__(self, *args, **kw):
+        super().__init__(*args, **kw)
+        share(self.cache)
+
     def fork(self, seqs, into, lengths=None):
         self.cache.fork(seqs, into, lengths)
         was = [(copy.deepcopy(self.k[s]), copy.deepcopy(self.v[s])) for s in seqs]
@@ -96,8 +108,8 @@ def _large(prefix, own, heads, dim, block, code, dtype):
     import vicinity_amd as va
 
     n = len(own)
-    cache = va.KVCache(n + 1, heads, dim, -(-prefix // block) + sum(-(-o // block) + 1 for o in own),
-                       block_tokens=block, code=code)
+    cache = share(va.KVCache(n + 1, heads, dim, -(-prefix // block) + sum(-(-o // block) + 1 for o in own),
+                             block_tokens=block, code=code))
     for seqs, counts, seed in (([0], [prefix], 1), (list(range(1, n + 1)), own, 3)):
         if seed > 1:
             cache.fork([0] * n, seqs)
@@ -169,13 +181,13 @@ def test_many_rows_over_a_long_prefix(dtype, dim, group):
     """Rows enough for the kernel of many rows over the shared slots."""
     _case(f"{dtype} dim {dim} group {group}")
     torch = _torch()
-    heads = 16
-    cache = _large(9000, [1, 70, 33, 5, 200, 64, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 40], heads, dim, 128, "int8", "bfloat16")
+    heads = 16 if dim < 128 else 32  # 98304 tiles of 16 rows
+    cache = _large(12000, [1, 70, 33, 5, 200, 64, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 40], heads, dim, 128, "int8", "bfloat16")
     seqs = list(range(1, 18))
     q = _rand((17, heads * group, dim), dtype, 7)
     _check_large(cache, q, seqs, [1] * 17)
     _check_large(cache, q, seqs, [1] * 17, window=5000)
-    mask = (torch.rand((17, 9200), generator=torch.Generator().manual_seed(1)) < 0.9).to("cuda:0")
+    mask = (torch.rand((17, 12200), generator=torch.Generator().manual_seed(1)) < 0.9).to("cuda:0")
     _check_large(cache, q, seqs, [1] * 17, mask=mask)
 
 

@@ -195,6 +195,7 @@ SIGNATURES = {
     "vgpu_kv_compact": (_i, [_H, _sz, ctypes.POINTER(_sz), _vp]),
     "vgpu_beams_workspace": (_i, [_i, _sz, _sz, _sz, _sz, ctypes.POINTER(_sz)]),
     "vgpu_select_beams": (_i, [ctypes.POINTER(Beams), _vp]),
+    "vgpu_test_set_kv_shared_bytes": (_i, [_H, _sz]),
     "vgpu_test_host_kv_splits": (_i, [_vp, _vp, _sz, _sz, _sz, _vp, _vp]),
     "vgpu_test_host_lists": (_i, [_vp, _sz, _sz, _vp, _vp]),
     "vgpu_test_host_centroid_update": (_i, [_vp, _sz, _sz, _vp, _sz, _vp]),

@@ -647,6 +647,15 @@ int vgpu_select_beams(const vgpu_beams* q, void* stream) {
 
 /* ---- per-kernel test entry points ---------------------------------------- */
 
+int vgpu_test_set_kv_shared_bytes(vgpu_kv* h, size_t bytes) {
+    return guard([&] {
+        need(h, VGPU_ERR_INVALID_PARAMETER, "null argument");
+        need(bytes < (size_t)1 << 62, VGPU_ERR_INVALID_PARAMETER, "bytes out of range");
+        std::lock_guard<std::mutex> lk(h->kv->mu);
+        h->kv->shared_bytes = (int64_t)bytes;
+    });
+}
+
 int vgpu_test_host_kv_splits(const int64_t* lens, const int64_t* counts, size_t n, size_t heads, size_t group,
                              int32_t* splits, int32_t* tiles) {
     return guard([&] {

@@ -48,6 +48,16 @@ constexpr size_t kRowRuns = 64;
 
 // Sequences that share so many slots are taken over them together.
 constexpr int64_t kSharedSlots = 256;
+// ... where that leaves so many bytes of a call unread, which the join of the parts costs (32
+// query heads on 8 of 128: 8 pairs of 512 slots, 8.4 MB, 16 us against 17; 4 sequences of 512,
+// 3.1 MB, 15 and 13; 8 x 8 of 512, 59 MB, 17 and 19).
+constexpr int64_t kSharedBytes = (int64_t)8 << 20;
+// The kernel of many rows takes over shared slots from so many tiles of 16 rows on, which are a
+// launch apart from the own slots then, with partial rows four times as many (8 x 128: 244 rows
+// over 8192 slots 70 us and 49 by 16 rows, over 16384 61 and 72; 384 over 65536 156, by 16 rows
+// 480; 128 rows of 192 over 16384 55 and 44; at 256 dims 108 and 53, where it has a compute
+// unit for one workgroup; measured in bfloat16 and taken for all).
+constexpr int64_t kSharedTiles = 98304;
 // Tiles of a workgroup over shared slots, at least.
 constexpr int64_t kLeastTiles = 8;
 // Levels of branches that are looked at for the best groups.
@@ -189,6 +199,7 @@ KvCache::KvCache(const vgpu_kv_params& p) : params(p) {
     table.reserve(p.num_seqs * params.max_blocks);
     dev.pool = pool.p, dev.kscale = kscale.p, dev.vscale = vscale.p;
     dev.positions = positions.p, dev.weights = weights.p, dev.table = table.p;
+    shared_bytes = kSharedBytes;
     seqs.resize(p.num_seqs);
     seen.assign(p.num_seqs, 0);
     free_blocks.resize(p.num_blocks);
@@ -851,15 +862,17 @@ void KvCache::attend_shared(const int32_t* ids, const int64_t* counts, const std
             if (counts[i] && !b.empty() && holders[b[0]] > 1) roots.push_back({b[0], (uint32_t)i});
         }
     std::vector<Group> groups;
+    int64_t saved_slots = 0;
     if (roots.size() > 1) {
         std::sort(roots.begin(), roots.end());
         for (size_t x = 0, y; x < roots.size(); x = y) {
             std::vector<uint32_t> members;
             for (y = x; y < roots.size() && roots[y].first == roots[x].first; y++) members.push_back(roots[y].second);
             int64_t saved;
-            if (members.size() > 1) find_groups(ids, counts, a, members, 0, 0, groups, saved);
+            if (members.size() > 1) find_groups(ids, counts, a, members, 0, 0, groups, saved), saved_slots += saved;
         }
     }
+    if (saved_slots * dev.H * 2 * dev.Dp < shared_bytes) groups.clear();
     // Groups in pieces of as many sequences as one launch takes: each has an entry of its own and
     // the piece one more, and every row leaves partial results of both.
     const int parts = a.q.type == KV_F32 ? 2 : 1;
@@ -925,9 +938,9 @@ void KvCache::attend_shared(const int32_t* ids, const int64_t* counts, const std
             int64_t most = 0, tiles = 0;
             for (const Entry& e : entries[y]) {
                 most = std::max<int64_t>(most, e.rows);
-                tiles += (e.rows + chunk_rows - 1) / chunk_rows * dev.H * ((e.end + KV_TILE - 1) / KV_TILE - e.t0);
+                tiles += (e.rows + 15) / 16 * dev.H * ((e.end + KV_TILE - 1) / KV_TILE - e.t0);
             }
-            by_rows[y] = most > chunk_rows * 3 / 4 && tiles >= kChunkTiles;
+            by_rows[y] = dev.Dp < 256 && most > chunk_rows * 3 / 4 && tiles >= kSharedTiles;
         }
         const int launches = by_rows[0] == by_rows[1] ? 1 : 2;
         KvBatch b[2];
