@@ -196,8 +196,11 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvDev c, KvBatch b, KvTe
     // a sequence that touches one block brings its number, and the table learns a new one here
     int* entry = c.table + (size_t)b.seq[i] * c.W + blk;
     const int block = b.splits[i] >= 0 ? b.splits[i] : *entry;
-    if (b.splits[i] >= 0 && !held && h == 0 && !vals && tid == 0) *entry = block;
-    const size_t part = (size_t)block * c.H + h;
+    // a begun block that others hold too is copied on the way: what it held comes from there
+    const int source = blk == len0 >> c.shift && b.per[i] >= 0 ? b.per[i] : block;
+    const bool copied = source != block;
+    if (b.splits[i] >= 0 && (!held || copied) && h == 0 && !vals && tid == 0) *entry = block;
+    const size_t part = (size_t)block * c.H + h, part0 = (size_t)source * c.H + h;
     const KvTensor& x = vals ? v : k;
     const int64_t tok0 = (int64_t)b.tok0[i] + slot0 - len0;  // token of slot 0 of the block
     // piece u: 8 dims m of the new slot r.  Values go by quads of slots, aligned in the block
@@ -221,8 +224,9 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvDev c, KvBatch b, KvTe
         return piece(u, r, m) ? load8<T>(x, (tok0 + r) * x.st + (int64_t)h * x.sh, m, c.D) : Eight<T>{};
     };
     float* scale = (vals ? c.vscale : c.kscale) + part;
-    const float s_old = held ? *scale : 0.f;
+    const float s_old = held ? (vals ? c.vscale : c.kscale)[part0] : 0.f;
     uint8_t* base = c.pool + kv_tile_offset(c, block, h, 0) + (vals ? kv_half(c.Dp) : 0);
+    const uint8_t* base0 = c.pool + kv_tile_offset(c, source, h, 0) + (vals ? kv_half(c.Dp) : 0);
     const int half = kv_half(c.Dp);
 
     // largest magnitude, as bits: infinities and NaN are above every number
@@ -260,8 +264,13 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvDev c, KvBatch b, KvTe
     const float inv = s > 0.f ? 1.f / s : 0.f;
     const float ratio = s > 0.f ? s_old / s : 0.f;
     const bool grown = held && s > s_old;  // (false for NaN: the old codes stay as they are)
-    if (tid == 0 && !(s == s_old && held)) *scale = s;
+    if (tid == 0 && !(s == s_old && held && !copied)) *scale = s;
     if (!vals) {
+        if (copied)
+            for (int r = tid; r < held; r += 256) {
+                c.positions[part * c.B + r] = c.positions[part0 * c.B + r];
+                c.weights[part * c.B + r] = c.weights[part0 * c.B + r];
+            }
         for (int r = held + tid; r < end; r += 256) {
             const int64_t at = (tok0 + r) * c.H + h;
             c.positions[part * c.B + r] = positions ? positions[at] : b.aux[i] + slot0 + r - len0;
@@ -269,14 +278,14 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvDev c, KvBatch b, KvTe
         }
     }
 
-    const bool direct = held % KV_TILE && !grown && end - held <= KV_FEW && held / KV_TILE == (end - 1) / KV_TILE;
-    const int first = grown ? 0 : held / KV_TILE, last = (end + KV_TILE - 1) / KV_TILE;  // tiles that change
+    const bool direct = held % KV_TILE && !grown && !copied && end - held <= KV_FEW && held / KV_TILE == (end - 1) / KV_TILE;
+    const int first = grown || copied ? 0 : held / KV_TILE, last = (end + KV_TILE - 1) / KV_TILE;  // tiles that change
     if (!direct) {
         for (int t = first; t < last; t++)
             for (int o = tid; o < half / 16; o += 256) {
                 uint4 w = {zero_codes(c.code), zero_codes(c.code), zero_codes(c.code), zero_codes(c.code)};
                 if (t * KV_TILE < held) {
-                    w = ((const uint4*)(base + (size_t)t * 2 * half))[o];
+                    w = ((const uint4*)(base0 + (size_t)t * 2 * half))[o];
                     if (grown) {
                         w.x = rescale4(w.x, ratio, c.code), w.y = rescale4(w.y, ratio, c.code);
                         w.z = rescale4(w.z, ratio, c.code), w.w = rescale4(w.w, ratio, c.code);

@@ -391,13 +391,46 @@ void KvCache::append(const int32_t* ids, const int64_t* counts, size_t n, const 
         want += total - q.blocks.size();
     }
     need(!tokens || (k.data && v.data), "null argument");
-    want += shared_blocks(ids, begun.data(), n);
+    const size_t shared = shared_blocks(ids, begun.data(), n);
+    want += shared;
     need(want <= free_blocks.size(),
          "the cache needs " + std::to_string(want) + " more blocks and has " + std::to_string(free_blocks.size()),
          VGPU_ERR_OUT_OF_MEMORY);
     for (size_t i = 0; i < n; i++) seqs[ids[i]].blocks.reserve(blocks_of(seqs[ids[i]].len + counts[i]));
     KvRuns runs;
-    own_blocks(ids, begun.data(), n, runs, s);
+    // Begun blocks that others hold too: the append itself copies them, but those that another
+    // sequence of the call goes on in.
+    std::vector<int> source(n, -1), kept;
+    if (shared) {
+        for (size_t i = 0; i < n; i++) {
+            Seq& q = seqs[ids[i]];
+            if ((size_t)begun[i] >= q.blocks.size()) continue;
+            int& block = q.blocks[(size_t)begun[i]];
+            if (holders[block] > 1) {
+                source[i] = block;
+                block = take_block();
+                let_go(source[i]);
+            } else {
+                kept.push_back(block);
+            }
+        }
+        std::sort(kept.begin(), kept.end());
+        KvCopies copies(dev, dev, nullptr, s);
+        for (size_t i = 0; i < n; i++) {
+            if (source[i] < 0) continue;
+            const Seq& q = seqs[ids[i]];
+            const int block = q.blocks[(size_t)begun[i]];
+            const bool one = q.len % dev.B + counts[i] <= dev.B;  // the append writes the table too
+            if (std::binary_search(kept.begin(), kept.end(), source[i])) {
+                copies.add(source[i], block);
+                add_run(runs, (size_t)ids[i] * (size_t)dev.W + (size_t)begun[i], block, table.p, s);
+                source[i] = -1;
+            } else if (!one) {
+                add_run(runs, (size_t)ids[i] * (size_t)dev.W + (size_t)begun[i], block, table.p, s);
+            }
+        }
+        copies.flush();
+    }
     for (size_t i = 0; i < n; i++) {
         Seq& q = seqs[ids[i]];
         const size_t more = blocks_of(q.len + counts[i]) - q.blocks.size();
@@ -427,6 +460,7 @@ void KvCache::append(const int32_t* ids, const int64_t* counts, size_t n, const 
             b.count[j] = (int)counts[i];
             b.aux[j] = (int)q.next;
             b.splits[j] = touched == 1 ? q.blocks[first] : -1;
+            b.per[j] = source[i];
             b.unit0[j + 1] = b.unit0[j] + (int)touched;
             b.n++;
             tok += counts[i];

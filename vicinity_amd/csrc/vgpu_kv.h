@@ -73,7 +73,7 @@ struct KvBatch {
                           // evict: sequence that receives the result; attend: see there
     int splits[KV_BATCH]; // attend: parts that the tiles of its rows go to, of per[i] tiles;
                           // append: the one block it touches, or -1 (see the table)
-    int per[KV_BATCH];
+    int per[KV_BATCH];    // append: the block that its first one continues a copy of, or -1
     int unit0[KV_BATCH + 1];
 };
 

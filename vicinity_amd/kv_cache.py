@@ -234,12 +234,9 @@ class KVCache:
         with decay); copy=True: copied at once.  Both need free blocks for the copies.  Either
         way each sequence reads, attends and changes as if it were alone; attend reads what
         several sequences share once for all of them."""
-        to = self._seqs(into)
-        ids = _array("i", seqs, "sequences")
+        to, ids = self._seqs(into), _array("i", seqs, "sequences")  # (the library checks their range)
         if len(ids) != len(to):
             raise ValueError(f"into names {len(to)} sequences, seqs {len(ids)}")
-        if ids and not 0 <= min(ids) <= max(ids) < self.num_seqs:
-            raise ValueError(f"sequence out of range [0, {self.num_seqs})")
         lens = None if lengths is None else self._ints(lengths, len(ids), "lengths")
         with self._turn:
             s, _ = self._stream(stream, ())
@@ -310,6 +307,9 @@ class KVCache:
     def _seqs(self, seqs) -> array:
         if seqs is None:
             return self._all
+        if type(seqs) is range and seqs and 0 <= min(seqs[0], seqs[-1]) \
+                and max(seqs[0], seqs[-1]) < self.num_seqs:
+            return array("i", seqs)
         a = _array("i", seqs, "sequences")
         if a and not 0 <= min(a) <= max(a) < self.num_seqs:
             raise ValueError(f"sequence out of range [0, {self.num_seqs})")
