@@ -54,8 +54,9 @@ def select_beams(logits, scores, beams: int, k: int | None = None, stream=None):
     for name, value in (("beams", beams), ("k", k)):
         if not isinstance(value, (int, np.integer)) or not 0 < value < 1 << 31:
             raise ValueError(f"{name} must be an int above 0")
+    beams, k = int(beams), int(k)
     dtype = 0 if logits.dtype == torch.float32 else 1 if logits.dtype == torch.float16 else 2
-    size = _workspace(dtype, rows, vocab, int(beams), int(k))
+    size = _workspace(dtype, rows, vocab, beams, k)
     device = logits.device
     if stream is None and device.index == torch.cuda.current_device():
         return _select(torch, logits, scores, dtype, beams, k, size,

@@ -23,7 +23,8 @@ BeamArgs sizes(int dtype, size_t rows, size_t vocab, size_t beams, size_t k) {
     a.rows = (int)rows, a.vocab = (int)vocab, a.beams = (int)beams, a.k = (int)k;
     beam_plan(a);
     // a launch's threads, 256 to a workgroup, are counted in 32 bits
-    need((int64_t)a.rows * a.slices < 1 << 24, "too many logits in one call");
+    need((int64_t)a.rows * a.slices < 1 << 24 && (int64_t)a.beams * a.slices * a.k < (int64_t)1 << 31,
+         "too many logits in one call");
     return a;
 }
 
