@@ -235,7 +235,8 @@ def _logits(case, seed):
     likely = torch.randint(0, vocab, (case["prompts"], some), generator=g, device=DEV)
     likely = likely.repeat_interleave(case["beams"], dim=0)
     lift = 8.0 + 4.0 * torch.rand((rows, some), generator=g, device=DEV)
-    logits.scatter_(1, likely, lift)
+    # (the same token drawn twice: the larger lift, whatever order the GPU writes them in)
+    logits.scatter_reduce_(1, likely, lift, "amax", include_self=False)
     if case["masked"]:
         logits[torch.rand((rows, vocab), generator=g, device=DEV) < 0.9] = -math.inf
         logits[:, 0] = 0.0  # the end is always allowed
