@@ -17,7 +17,8 @@ HEADER = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))
     (dict(rows=(1 << 24) + 2), "rows"), (dict(vocab=0), "vocab"), (dict(vocab=(1 << 30) + 1), "vocab"),
     (dict(beams=0), "beams"), (dict(beams=1025, rows=1025), "beams"), (dict(k=0), "k must"),
     (dict(k=257), "k must"), (dict(k=9, vocab=4), "k must"), (dict(rows=1 << 20, vocab=1 << 30), "too many"),
-    (dict(rows=1024, beams=1024, vocab=1 << 27, k=256), "too many")])
+    (dict(rows=1024, beams=1024, vocab=1 << 27, k=256), "too many"),
+    (dict(rows=1 << 22, beams=1, vocab=100), "groups")])
 def test_sizes_that_are_refused(change, match):
     from vicinity_amd import _lib
 

@@ -93,10 +93,8 @@ class Both:
         self.cache.fork(seqs, into, lengths, **kw)
         was = [copy.deepcopy(self.seqs[s]) for s in seqs]
         for i, (s, to) in enumerate(zip(was, into)):
-            if lengths is not None:
+            if lengths is not None and lengths[i] < len(s):
                 s.cut(lengths[i])
-            elif not len(s):
-                s.next = 0
             self.seqs[to] = s
 
     def truncate(self, lengths, seqs):
@@ -231,6 +229,17 @@ def test_eviction_counts_what_comes_back():
     b.truncate([0], [1])
     b.evict(32, 0, [3])
     b.check()
+
+
+def test_positions_go_on_as_the_parents():
+    b = Both(4, blocks=30)
+    b.append([0, 1], [50, 40])
+    b.evict(0, 0, [0])  # nothing is left, and the next token has position 50
+    b.evict(10, 2, [1])
+    b.fork([0, 1, 1], [2, 3, 1], [0, 10, 7])
+    b.append([0, 1, 2, 3], [2, 2, 2, 2])
+    b.check()
+    assert b.seqs[2].positions[0, 0] == 50 and b.seqs[3].positions[-1, 0] == 41
 
 
 @pytest.mark.parametrize("num_blocks", [None, 24, 40, 64])
@@ -434,3 +443,55 @@ def test_blocks_past_32_bits():
     assert cache.compact(8) == 2
     got = cache.read(seqs=[1], fields=("k", "v", "positions"))
     assert all(torch.equal(got[f], want[f]) for f in want)
+
+
+def test_two_threads_fork_one_cache():
+    """Threads on streams of their own, each with its own sequences of one cache."""
+    import threading
+
+    torch = _torch()
+    b = Both(10, heads=2, dim=64, blocks=300)
+    b.append([0, 5], [333, 402])
+    torch.cuda.synchronize()
+    plan = {first: [([first + i for i in order], [1 + (i * 7 + first) % 40 for i in range(5)])
+                    for order in ([0, 0, 0, 0, 0], [3, 1, 4, 1, 0], [2, 2, 0, 4, 3], [1, 0, 3, 2, 4])]
+            for first in (0, 5)}
+    tokens = {}
+    for first, steps in plan.items():
+        for s, (_, counts) in enumerate(steps):
+            g = torch.Generator().manual_seed(100 * first + s)
+            t = sum(counts)
+            tokens[first, s] = (torch.randn((t, 2, 64), generator=g), torch.randn((t, 2, 64), generator=g),
+                                torch.rand((t, 2), generator=g))
+    dev = {key: [x.to("cuda:0") for x in v] for key, v in tokens.items()}
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(first):
+        try:
+            stream = torch.cuda.Stream()
+            own = list(range(first, first + 5))
+            for s, (parents, counts) in enumerate(plan[first]):
+                k, v, w = dev[first, s]
+                b.cache.fork(parents, own, stream=stream)
+                b.cache.append(k, v, seqs=own, counts=counts, weights=w, stream=stream)
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(first,)) for first in plan]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    torch.cuda.synchronize()
+    for first, steps in plan.items():
+        for s, (parents, counts) in enumerate(steps):
+            was = [copy.deepcopy(b.seqs[p]) for p in parents]
+            at = 0
+            for i, n in enumerate(counts):
+                k, v, w = (x[at:at + n].numpy() for x in tokens[first, s])
+                was[i].append(k, v, w)
+                b.seqs[first + i] = was[i]
+                at += n
+    b.check()

@@ -17,12 +17,14 @@ BeamArgs sizes(int dtype, size_t rows, size_t vocab, size_t beams, size_t k) {
     need(beams > 0 && beams <= (size_t)BEAM_MAX_BEAMS, "beams must be in the range 1..=1024");
     need(vocab > 0 && vocab <= (size_t)1 << 30, "vocab must be in the range 1..=2^30");
     need(rows % beams == 0 && rows <= (size_t)1 << 24, "rows must be a multiple of beams, at most 2^24");
+    // a launch's threads, 1024 to a group, are counted in 32 bits
+    need(rows / beams < (size_t)1 << 22, "more than 2^22 - 1 groups in one call");
     need(k > 0 && k <= (size_t)BEAM_MAX_K && k <= beams * vocab, "k must be in the range 1..=256 and at most beams * vocab");
     BeamArgs a;
     a.type = dtype;
     a.rows = (int)rows, a.vocab = (int)vocab, a.beams = (int)beams, a.k = (int)k;
     beam_plan(a);
-    // a launch's threads, 256 to a workgroup, are counted in 32 bits
+    // (and 256 to a slice)
     need((int64_t)a.rows * a.slices < 1 << 24 && (int64_t)a.beams * a.slices * a.k < (int64_t)1 << 31,
          "too many logits in one call");
     return a;

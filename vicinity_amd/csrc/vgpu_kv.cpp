@@ -402,6 +402,7 @@ void KvCache::append(const int32_t* ids, const int64_t* counts, size_t n, const 
     // sequence of the call goes on in.
     std::vector<int> source(n, -1), kept;
     if (shared) {
+        kept.reserve(n);
         for (size_t i = 0; i < n; i++) {
             Seq& q = seqs[ids[i]];
             if ((size_t)begun[i] >= q.blocks.size()) continue;
@@ -558,7 +559,8 @@ void KvCache::fork(const int32_t* ids, const int32_t* into, const int64_t* lengt
         const std::vector<int>& old = seqs[into[i]].blocks;
         Next& x = next[i];
         x.q.len = slots(i);
-        x.q.next = x.q.len ? from.next - (from.len - x.q.len) : 0;
+        // (as truncate leaves it; whole, also where nothing is left of it, it goes on counting)
+        x.q.next = x.q.len == from.len ? from.next : x.q.len ? from.next - (from.len - x.q.len) : 0;
         const size_t count = blocks_of(x.q.len);
         if (copy) {
             x.q.blocks.reserve(count);
