@@ -1,5 +1,14 @@
 // Softmax attention of sequences that hold the same first blocks: the rows of all of them
 // over the shared slots, read once, each over its own, and the join of the parts.
+//
+// Few rows (kv_step_kernel): 61 sequences of 32 query heads on 8 of 128 under 8192 shared slots
+// 43 us (135 MB in; the vector unit 44% busy: 16 workgroups convert the same tiles for 16 rows
+// each, three to a compute unit), 64 beams of 8 prompts of 3000 slots 18 us (48 MB; latency:
+// some eight tiles to a workgroup).  Many (kv_chunk_kernel): 48 sequences of 64 query heads on 8 of 128
+// over 65536 shared slots 137 us, 750 TFLOP/s (matrix unit 34% busy, vector unit 49%; 33 MB of
+// partial rows).  One launch of both kernels' code for shared and own slots was slower (the
+// first 60 us for 56 with the join, the last 159 to 205 for 145), as were two tiles of 16 rows
+// to a workgroup of few (64 beams 32 us for 18).
 #include "kv_attend.h"
 
 namespace vgpu {
@@ -8,7 +17,8 @@ namespace {
 
 // A row's parts, of the shared slots and of its own, by `share` groups of Dp / 4 threads, each of
 // which takes parts in turn, four at a time: the sums o and l go by the power of 2 that a part's
-// m stands below the largest, o also by the power of 2 that its S does.
+// m stands below the largest, o also by the power of 2 that its S does.  Bound by latency: the
+// parts of a row lie one launch's tiles apart (33 MB, 10.5 us; 3 MB 4.9).
 __global__ __launch_bounds__(256) void kv_shared_join_kernel(KvDev c, KvAttend a, KvMembers mem, KvShares j, int share) {
     __shared__ floatx4 sh_o[256];
     __shared__ float sh_m[64], sh_l[64], sh_top[64];
@@ -72,7 +82,7 @@ __global__ __launch_bounds__(256) void kv_shared_join_kernel(KvDev c, KvAttend a
         sh_o[tid] = o;
         if (d4 == 0) sh_m[grp] = mx, sh_l[grp] = l, sh_top[grp] = top;
         __syncthreads();
-        if (mine) return;
+        if (mine || !used) return;
         for (int x = 1; x < share; x++) mx = fmaxf(mx, sh_m[grp + x]), top = fmaxf(top, sh_top[grp + x]);
         o = floatx4{0.f, 0.f, 0.f, 0.f}, l = 0.f;
         for (int x = 0; x < share; x++) {
@@ -132,8 +142,8 @@ void launch_kv_shared(const KvDev& c, const KvBatch& b, const KvAttend& a, const
 void launch_kv_shared_join(const KvDev& c, const KvAttend& a, const KvMembers& mem, const KvShares& j, hipStream_t s) {
     int most = 0;
     for (int m = 0; m < mem.n; m++) most = j.splits[0][m] + j.splits[1][m] > most ? j.splits[0][m] + j.splits[1][m] : most;
-    // A group of threads for every four parts, up to 768 workgroups (3072 rows of 22 parts: 10 us
-    // with two, 14 with six; 512 rows of 25 parts: 8.5 and 6.4).
+    // A group of threads for every four parts, up to 768 workgroups (48 tokens of 64 query
+    // heads, 22 parts each: 10 us with two, 14 with six; 512 rows in all of 25 parts: 8.5 and 6.4).
     const int rows = mem.row0[mem.n], groups = 256 / (c.Dp / 4);
     const int64_t room = 768ll * groups / ((int64_t)rows * c.H);
     int share = (most + 3) / 4 < groups ? (most + 3) / 4 : groups;

@@ -315,6 +315,7 @@ int KvCache::take_block() {
 
 void KvCache::let_go(int block) {
     if (--holders[block] == 0) free_blocks.push_back(block);
+    else shared_holds--;
 }
 
 void KvCache::take_blocks(std::vector<int>& out, size_t count, size_t row, int* tab, KvRuns& runs, hipStream_t s) {
@@ -333,6 +334,7 @@ void KvCache::release_blocks(std::vector<int>& blocks, size_t keep) {
 }
 
 size_t KvCache::shared_blocks(const int32_t* ids, const int64_t* first, size_t n) {
+    if (!shared_holds) return 0;
     // as own_blocks will find them: of the batch's holders of a block, the last one keeps it
     size_t count = 0;
     for (size_t i = 0; i < n; i++) {
@@ -352,6 +354,7 @@ size_t KvCache::shared_blocks(const int32_t* ids, const int64_t* first, size_t n
 }
 
 void KvCache::own_blocks(const int32_t* ids, const int64_t* first, size_t n, KvRuns& runs, hipStream_t s) {
+    if (!shared_holds) return;
     KvCopies copies(dev, dev, nullptr, s);
     for (size_t i = 0; i < n; i++) {
         std::vector<int>& b = seqs[ids[i]].blocks;
@@ -613,7 +616,7 @@ void KvCache::fork(const int32_t* ids, const int32_t* into, const int64_t* lengt
         for (size_t i = 0; i < n; i++) {
             const std::vector<int>& b = next[i].q.blocks;
             for (size_t j = next[i].common; j < b.size(); j++) {
-                holders[b[j]]++;
+                holders[b[j]]++, shared_holds++;
                 if (!next[i].row) add_run(runs, (size_t)into[i] * (size_t)dev.W + j, b[j], table.p, s);
             }
         }
@@ -892,7 +895,7 @@ void KvCache::attend_shared(const int32_t* ids, const int64_t* counts, const std
                             KvAttend a, std::vector<size_t>& rest, hipStream_t s) {
     // sequences whose first block others hold too, by that block
     std::vector<std::pair<int, uint32_t>> roots;
-    if (!a.track)
+    if (!a.track && shared_holds)
         for (size_t i = 0; i < n; i++) {
             const std::vector<int>& b = seqs[ids[i]].blocks;
             if (counts[i] && !b.empty() && holders[b[0]] > 1) roots.push_back({b[0], (uint32_t)i});

@@ -368,6 +368,7 @@ struct KvCache {
     // Sequences that hold a block.  Only forks share blocks, a parent's first ones: so where two
     // sequences hold the same block, it is the same slots of both, and so are all before it.
     std::vector<int> holders;
+    int64_t shared_holds = 0;        // holders beyond the first, of all blocks
     int64_t shared_bytes;            // shared slots are read once where that saves so many
     std::vector<uint8_t> seen;       // batch checks
     std::mutex mu;
