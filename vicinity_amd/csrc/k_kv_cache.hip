@@ -196,7 +196,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvDev c, KvBatch b, KvTe
     const int held = max(len0 - slot0, 0), end = min(len1 - slot0, c.B);  // new slots held .. end - 1
     // a sequence that touches one block brings its number, and the table learns a new one here
     int* entry = c.table + (size_t)b.seq[i] * c.W + blk;
-    const int block = b.splits[i] >= 0 ? b.splits[i] : *entry;
+    const int block = __builtin_amdgcn_readfirstlane(b.splits[i] >= 0 ? b.splits[i] : *entry);
     // a begun block that others hold too is copied on the way: what it held comes from there
     const int source = blk == len0 >> c.shift && b.per[i] >= 0 ? b.per[i] : block;
     const bool copied = source != block;
@@ -349,23 +349,38 @@ __device__ __forceinline__ void store1(void* p, size_t i, float v, int type) {
 }
 
 // Four values of a row from dim d on (those below D), rounded once.
-template <int T>
-__device__ __forceinline__ void store_row(void* p, size_t row, int d, int D, bool vec, const float* v) {
+__device__ __forceinline__ void store_row(float* p, size_t row, int d, int D, bool vec, const float* v) {
     if (vec && d + 4 <= D) {
-        if (T == KV_F32) {
-            __builtin_nontemporal_store(floatx4{v[0], v[1], v[2], v[3]}, (floatx4*)((float*)p + row + d));
-        } else {
-            uint16_t e[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) store1(e, j, v[j], T);
-            *(uint2*)((uint16_t*)p + row + d) =
-                make_uint2((uint32_t)e[0] | (uint32_t)e[1] << 16, (uint32_t)e[2] | (uint32_t)e[3] << 16);
-        }
+        __builtin_nontemporal_store(floatx4{v[0], v[1], v[2], v[3]}, (floatx4*)(p + row + d));
         return;
     }
 #pragma unroll
     for (int j = 0; j < 4; j++)
-        if (d + j < D) store1(p, row + d + j, v[j], T);
+        if (d + j < D) p[row + d + j] = v[j];
+}
+
+// Eight codes of a row from dim d on, in 16 bits.
+template <int T>
+__device__ __forceinline__ void store_row8(void* p, size_t row, int d, int D, bool vec, uint32_t c0, uint32_t c1, int code, float s) {
+    float v[8];
+    decode4(c0, code, v);
+    decode4(c1, code, v + 4);
+    uint16_t e[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) store1(e, j, v[j] * s, T);
+    if (vec && d + 8 <= D) {
+        u32x4 w;
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[j] = (uint32_t)e[2 * j] | (uint32_t)e[2 * j + 1] << 16;
+        u32x4* to = (u32x4*)((uint16_t*)p + row + d);
+        // (rows of whole 128-byte lines leave past the caches)
+        if (D % 64 == 0) __builtin_nontemporal_store(w, to);
+        else *to = w;
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+        if (d + j < D) ((uint16_t*)p)[row + d + j] = e[j];
 }
 
 // The values of a tile, by one wave: a lane takes its 16 bytes of each piece, which are
@@ -377,10 +392,67 @@ __device__ __forceinline__ void read_tile(const KvDev& c, const uint8_t* tile, f
     const int lane = threadIdx.x & 63, g = lane >> 4, x = lane & 15;
     const int S = c.Dp / 32;
     const uint4* at = (const uint4*)tile + lane;
+    const bool odd = lane & 1;
+    if constexpr (T != KV_F32) {
+        // A lane's two pieces of 8 dims, of 32 dims each of its slot, go out in two stores: of
+        // the even lanes' slots, then of the odd ones'.  Eight lanes hold a slot's 64 dims: whole
+        // 128-byte lines, but where the pieces are odd in number.
+        const auto swap = [&](uint32_t first, uint32_t second, uint32_t (&to)[2]) {
+            const uint32_t other = (uint32_t)__builtin_amdgcn_mov_dpp((int)(odd ? first : second), 0xb1, 0xf, 0xf, true);
+            to[0] = odd ? other : first, to[1] = odd ? second : other;
+        };
+        if (ko) {
+            const int r = x & ~1;
+            const size_t rows[2][2] = {{row(r), row(r + 1)}, {row(16 + r), row(17 + r)}};
+            for (int p = 0; p < S; p++) {
+                const uint4 w = at[p * 64];
+                uint32_t a[2], b[2];
+                swap(w.x, w.z, a), swap(w.y, w.w, b);
+                const int o = 2 * p + odd, j = o >= S, d = 32 * (o - (j ? S : 0)) + 8 * g;
+#pragma unroll
+                for (int y = 0; y < 2; y++) {
+                    const size_t to = j ? rows[1][y] : rows[0][y];
+                    if (to != ~(size_t)0) store_row8<T>(ko, to, d, c.D, vec, a[y], b[y], c.code, ks);
+                }
+            }
+        }
+        if (vo) {
+            const int r = 4 * g + (x & 2);
+            const size_t rows[2][2] = {{row(r), row(r + 1)}, {row(16 + r), row(17 + r)}};
+            for (int p = 0; p < S; p += 2) {
+                // as below, then a quad and the next exchange 4 dims, so that a lane has 8
+                const bool far = lane & 4;
+                uint32_t e[2][2][2];  // [piece][lower or upper slots][4 dims]
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+                    const uint4 w = at[(S + min(p + q, S - 1)) * 64];
+                    const uint32_t t[4] = {quad_transpose(w.x), quad_transpose(w.y), quad_transpose(w.z), quad_transpose(w.w)};
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        const int mine = (int)(far ? t[u] : t[2 + u]);
+                        // (from 4 lanes on for quads 0 and 2, from 4 lanes before for 1 and 3)
+                        const int up = __builtin_amdgcn_update_dpp(0, mine, 0x104, 0xf, 0x5, false);
+                        const uint32_t other = (uint32_t)__builtin_amdgcn_update_dpp(up, mine, 0x114, 0xf, 0xa, false);
+                        e[q][u][0] = far ? other : t[u], e[q][u][1] = far ? t[2 + u] : other;
+                    }
+                }
+                const int piece = p + odd, d = 32 * piece + 4 * (x >> 2 & 2) + (far ? 16 : 0);
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    uint32_t a[2], b[2];
+                    swap(e[0][u][0], e[1][u][0], a), swap(e[0][u][1], e[1][u][1], b);
+#pragma unroll
+                    for (int y = 0; y < 2; y++)
+                        if (rows[u][y] != ~(size_t)0 && piece < S)
+                            store_row8<T>(vo, rows[u][y], d, c.D, vec, a[y], b[y], c.code, vs);
+                }
+            }
+        }
+        return;
+    }
     // A lane's two pieces of 4 dims, of the lower and the upper 16 of 32 dims of its slot, go
     // out in two stores: of the even lanes' slots, then of the odd ones'.  Eight lanes hold a
-    // slot's 32 dims, so that a float32 store is of whole 128-byte lines.
-    const bool odd = lane & 1;
+    // slot's 32 dims, so that a store is of whole 128-byte lines.
     const auto emit = [&](void* out, uint32_t lower, uint32_t upper, float s, const size_t* r, int d) {
         const uint32_t other = (uint32_t)__builtin_amdgcn_mov_dpp((int)(odd ? lower : upper), 0xb1, 0xf, 0xf, true);
         const uint32_t two[2] = {odd ? other : lower, odd ? upper : other};
@@ -390,7 +462,7 @@ __device__ __forceinline__ void read_tile(const KvDev& c, const uint8_t* tile, f
             decode4(two[y], c.code, e);
 #pragma unroll
             for (int i = 0; i < 4; i++) e[i] *= s;
-            if (r[y] != ~(size_t)0) store_row<T>(out, r[y], d + (odd ? 16 : 0), c.D, vec, e);
+            if (r[y] != ~(size_t)0) store_row((float*)out, r[y], d + (odd ? 16 : 0), c.D, vec, e);
         }
     };
     if (ko) {
@@ -426,7 +498,8 @@ __device__ __forceinline__ void read_tile(const KvDev& c, const uint8_t* tile, f
 // One workgroup: 128 slots of one head, a tile to a wave.  Bound by the bytes written:
 // no element passes through LDS, and stores of whole lines leave the caches to the pool
 // (nontemporal: 31 sequences moved in 41 us for 64 before them; 64-byte halves of lines
-// stored so took 68 us of reading for 58).
+// stored so took 68 us of reading for 58).  110000 slots of 8 x 128 in bfloat16: 690 MB in
+// 124 us, 5.5 TB/s; by 8 bytes to a lane, which left as halves of lines (810 MB), 173.
 template <int T>
 __global__ __launch_bounds__(256) void kv_read_kernel(KvDev c, KvBatch b, KvReadOut o) {
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
