@@ -234,7 +234,9 @@ class KVCache:
         with decay); copy=True: copied at once.  Both need free blocks for the copies.  Either
         way each sequence reads, attends and changes as if it were alone; attend reads what
         several sequences share once for all of them."""
-        to, ids = self._seqs(into), _array("i", seqs, "sequences")  # (the library checks their range)
+        to, part = self._seqs(into), self._slice(seqs)
+        # (the library checks their range)
+        ids = _array("i", seqs, "sequences") if part is None else self._all[part]
         if len(ids) != len(to):
             raise ValueError(f"into names {len(to)} sequences, seqs {len(ids)}")
         lens = None if lengths is None else self._ints(lengths, len(ids), "lengths")
@@ -274,12 +276,14 @@ class KVCache:
                 raise ValueError(f"fields must be among {FIELDS}")
         ids = self._seqs(seqs)
         at = self._ints(0 if first is None else first, len(ids), "first")
-        if at and min(at) < 0:
+        if first is not None and at and min(at) < 0:
             raise ValueError("first must not be negative")
         with self._turn:
             if counts is None:  # to the end; the library checks what the tensors were sized by
                 lens = self._lengths()
-                n = lens if ids is self._all else array("q", map(lens.__getitem__, ids))
+                part = self._slice(seqs)
+                n = lens if ids is self._all else lens[part] if part is not None else \
+                    array("q", map(lens.__getitem__, ids))
                 if first is not None and n:
                     left = np.frombuffer(n, np.int64)  # n's own memory
                     np.subtract(left, at, out=left)
@@ -292,7 +296,8 @@ class KVCache:
             with ctx:
                 for f in fields:
                     shape = (tokens, self.num_heads) + ((self.head_dim,) if f in "kv" else ())
-                    res[f] = torch.empty(shape, dtype=types.get(f, dtype), device=self.device)
+                    res[f] = torch.empty_like(res["k"]) if f == "v" and "k" in res else \
+                        torch.empty(shape, dtype=types.get(f, dtype), device=self.device)
             ptr = [res[f].data_ptr() if f in res else None for f in FIELDS]
             _lib.check(self._L.vgpu_kv_read(self._h, _ptr(ids), _ptr(at), _ptr(n), len(ids),
                                             self._types[dtype], *ptr, s))
@@ -304,12 +309,18 @@ class KVCache:
         _lib.check(self._L.vgpu_kv_lengths(self._h, _ptr(out)))
         return out
 
+    def _slice(self, seqs) -> slice | None:
+        """An ascending range of the cache's sequences as a slice of all; anything else None."""
+        if type(seqs) is range and seqs.step > 0 and 0 <= seqs.start <= seqs.stop <= self.num_seqs:
+            return slice(seqs.start, seqs.stop, seqs.step)
+        return None
+
     def _seqs(self, seqs) -> array:
         if seqs is None:
             return self._all
-        if type(seqs) is range and seqs and 0 <= min(seqs[0], seqs[-1]) \
-                and max(seqs[0], seqs[-1]) < self.num_seqs:
-            return array("i", seqs)
+        part = self._slice(seqs)
+        if part is not None:
+            return self._all[part]
         a = _array("i", seqs, "sequences")
         if a and not 0 <= min(a) <= max(a) < self.num_seqs:
             raise ValueError(f"sequence out of range [0, {self.num_seqs})")
@@ -318,7 +329,7 @@ class KVCache:
     @staticmethod
     def _ints(values, n: int, name: str) -> array:
         if isinstance(values, (int, np.integer)):
-            return _array("q", [int(values)] * n, name)
+            return _array("q", (int(values),), name) * n
         a = _array("q", values, name)
         if len(a) != n:
             raise ValueError(f"{name} must have one entry for each of the {n} sequences")
