@@ -367,7 +367,13 @@ __device__ __forceinline__ void store_row8(void* p, size_t row, int d, int D, bo
     decode4(c1, code, v + 4);
     uint16_t e[8];
 #pragma unroll
-    for (int j = 0; j < 8; j++) store1(e, j, v[j] * s, T);
+    for (int j = 0; j < 8; j++) {
+        // (the float32 product, and its rounding: one instruction for both would round once and
+        // lose the sign of a zero)
+        float x = v[j] * s;
+        asm("" : "+v"(x));
+        store1(e, j, x, T);
+    }
     if (vec && d + 8 <= D) {
         u32x4 w;
 #pragma unroll
