@@ -501,13 +501,14 @@ __device__ __forceinline__ void read_tile(const KvDev& c, const uint8_t* tile, f
     }
 }
 
-// One workgroup: 128 slots of one head, a tile to a wave.  Bound by the bytes written:
+// One workgroup: 128 slots of one head, a tile's keys or values to a wave (both to one: 777
+// slots of 5 x 80 11.1 us for 7.4, a few code lines after another by a wave alone).  Bound by the bytes written:
 // no element passes through LDS, and stores of whole lines leave the caches to the pool
 // (nontemporal: 31 sequences moved in 41 us for 64 before them; 64-byte halves of lines
 // stored so took 68 us of reading for 58).  110000 slots of 8 x 128 in bfloat16: 690 MB in
 // 124 us, 5.5 TB/s; by 8 bytes to a lane, which left as halves of lines (810 MB), 173.
 template <int T>
-__global__ __launch_bounds__(256) void kv_read_kernel(KvDev c, KvBatch b, KvReadOut o) {
+__global__ __launch_bounds__(512) void kv_read_kernel(KvDev c, KvBatch b, KvReadOut o) {
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = kv_mod(blockIdx.x, c.by_heads), unit = kv_div(blockIdx.x, c.by_heads);
     const int i = kv_find(b, unit);
@@ -516,17 +517,18 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvDev c, KvBatch b, KvRead
     const int* table = c.table + (size_t)b.seq[i] * c.W;
     const int64_t tok = (int64_t)b.tok0[i] - first;  // row of slot 0
     const int slot0 = group + wave * KV_TILE;
-    if ((o.k || o.v) && slot0 < last && slot0 + KV_TILE > first) {
+    const bool vals = threadIdx.y;
+    if ((vals ? o.v : o.k) && slot0 < last && slot0 + KV_TILE > first) {
         const int block = __builtin_amdgcn_readfirstlane(table[slot0 >> c.shift]);
         const size_t part = (size_t)block * c.H + h;
         const uint8_t* tile = c.pool + kv_tile_offset(c, block, h, (slot0 & (c.B - 1)) / KV_TILE);
-        read_tile<T>(c, tile, c.kscale[part], c.vscale[part], o.k, o.v, o.vec, [&](int r) -> size_t {
+        read_tile<T>(c, tile, c.kscale[part], c.vscale[part], vals ? nullptr : o.k, vals ? o.v : nullptr, o.vec, [&](int r) -> size_t {
             const int slot = slot0 + r;
             return slot >= first && slot < last ? ((size_t)(tok + slot) * c.H + h) * c.D : ~(size_t)0;
         });
     }
     const int slot = group + tid;
-    if (tid < KV_READ && slot >= first && slot < last && (o.positions || o.weights)) {
+    if (!vals && tid < KV_READ && slot >= first && slot < last && (o.positions || o.weights)) {
         const size_t at = (size_t)(tok + slot) * c.H + h;
         const size_t from = ((size_t)table[slot >> c.shift] * c.H + h) * c.B + (slot & (c.B - 1));
         if (o.positions) o.positions[at] = c.positions[from];
@@ -943,11 +945,11 @@ void launch_kv_read(const KvDev& c, const KvBatch& b, const KvReadOut& o, hipStr
     if (!o.k && !o.v)
         hipLaunchKernelGGL(kv_read_side_kernel, dim3((unsigned)b.unit0[b.n]), dim3(256), 0, s, c, b, o);
     else if (o.type == KV_F32)
-        hipLaunchKernelGGL(kv_read_kernel<KV_F32>, grid, dim3(256), 0, s, c, b, o);
+        hipLaunchKernelGGL(kv_read_kernel<KV_F32>, grid, dim3(256, 2), 0, s, c, b, o);
     else if (o.type == KV_F16)
-        hipLaunchKernelGGL(kv_read_kernel<KV_F16>, grid, dim3(256), 0, s, c, b, o);
+        hipLaunchKernelGGL(kv_read_kernel<KV_F16>, grid, dim3(256, 2), 0, s, c, b, o);
     else
-        hipLaunchKernelGGL(kv_read_kernel<KV_BF16>, grid, dim3(256), 0, s, c, b, o);
+        hipLaunchKernelGGL(kv_read_kernel<KV_BF16>, grid, dim3(256, 2), 0, s, c, b, o);
 }
 
 void launch_kv_evict(const KvDev& c, const KvBatch& b, const KvEvict& e, hipStream_t s) {
