@@ -502,10 +502,10 @@ __device__ __forceinline__ void read_tile(const KvDev& c, const uint8_t* tile, f
 }
 
 // One workgroup: 128 slots of one head, a tile's keys or values to a wave (both to one: 777
-// slots of 5 x 80 11.1 us for 7.4, a few code lines after another by a wave alone).  Bound by the bytes written:
-// no element passes through LDS, and stores of whole lines leave the caches to the pool
-// (nontemporal: 31 sequences moved in 41 us for 64 before them; 64-byte halves of lines
-// stored so took 68 us of reading for 58).  110000 slots of 8 x 128 in bfloat16: 690 MB in
+// slots of 5 x 80 11.1 us for 7.4: a wave alone on its SIMD waits for each result).  Bound by
+// the bytes written: no element passes through LDS, and stores of whole lines leave the caches
+// to the pool (nontemporal: 31 sequences moved in 41 us for 64 before them; 64-byte halves of
+// lines stored so took 68 us of reading for 58).  110000 slots of 8 x 128 in bfloat16: 690 MB in
 // 124 us, 5.5 TB/s; by 8 bytes to a lane, which left as halves of lines (810 MB), 173.
 template <int T>
 __global__ __launch_bounds__(512) void kv_read_kernel(KvDev c, KvBatch b, KvReadOut o) {
