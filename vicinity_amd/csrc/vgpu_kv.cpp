@@ -550,22 +550,20 @@ void KvCache::fork(const int32_t* ids, const int32_t* into, const int64_t* lengt
          VGPU_ERR_OUT_OF_MEMORY);
     // The table rows to be written: by runs where few entries differ, else row by row, through
     // the second table where one row is both read and written.
-    struct Next {
-        Seq q;
-        size_t common;  // leading blocks that the sequence holds already
-        bool row;
-    };
-    std::vector<Next> next(n);
+    std::vector<Fork>& next = forks;
+    if (next.size() < n) next.resize(n);
     bool rows = false, crossed = false;
     for (size_t i = 0; i < n; i++) {
         const Seq& from = seqs[ids[i]];
         const std::vector<int>& old = seqs[into[i]].blocks;
-        Next& x = next[i];
+        Fork& x = next[i];
+        x.common = 0, x.row = false;
         x.q.len = slots(i);
         // (as truncate leaves it; whole, also where nothing is left of it, it goes on counting)
         x.q.next = x.q.len == from.len ? from.next : x.q.len ? from.next - (from.len - x.q.len) : 0;
         const size_t count = blocks_of(x.q.len);
         if (copy) {
+            x.q.blocks.clear();
             x.q.blocks.reserve(count);
             continue;
         }
@@ -625,8 +623,8 @@ void KvCache::fork(const int32_t* ids, const int32_t* into, const int64_t* lengt
     // what the sequences held, beyond what they keep
     for (size_t i = 0; i < n; i++) {
         Seq& q = seqs[into[i]];
-        release_blocks(q.blocks, copy ? 0 : next[i].common);
-        q = std::move(next[i].q);
+        release_blocks(q.blocks, next[i].common);
+        std::swap(q, next[i].q);
     }
     VGPU_HIP(hipGetLastError());
 }

@@ -364,6 +364,12 @@ struct KvCache {
         std::vector<int> blocks;
     };
     std::vector<Seq> seqs;
+    struct Fork {
+        Seq q;          // what the sequence becomes
+        size_t common;  // leading blocks that it holds already
+        bool row;       // its row of the table is copied from its parent's
+    };
+    std::vector<Fork> forks;         // of a call; they keep their memory for the next
     std::vector<int> free_blocks;    // taken from the back
     // Sequences that hold a block.  Only forks share blocks, a parent's first ones: so where two
     // sequences hold the same block, it is the same slots of both, and so are all before it.

@@ -173,9 +173,8 @@ class KVCache:
             s, ctx = self._stream(stream, (q, mask, out))
             with ctx:
                 if out is None:
-                    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-                lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) \
-                    if return_lse else None
+                    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+                lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
             query = _lib.KvQuery(
                 qt, heads, 1.0 / math.sqrt(self.head_dim) if scale is None else scale, int(causal),
                 min(int(window), 1 << 62), mask.data_ptr() if mask is not None else None,
