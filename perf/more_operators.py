@@ -197,9 +197,6 @@ def _inputs(case, seed):
         # some of the new keys are larger than what their block held
         x["new_k"], x["new_v"] = nk * 1.25, nv
         x["parents"] = _parents(case)
-        # the first slot of the block that a child's new tokens enter
-        at = _totals(case)
-        x["first"] = [at[i] // case["block"] * case["block"] for i in x["parents"]]
         return x
     n, m, heads_q = len(x["own"]), case["queries"], h * case["group"]
     g = _gen(seed, 3)
@@ -222,8 +219,8 @@ def _inputs(case, seed):
 
 
 def _totals(case):
-    w, prefixes = case["width"], _prefixes(case)
-    return [prefixes[i // w] + t for i, t in enumerate(_own(case))]
+    w = case["width"]
+    return [_prefixes(case)[i // w] + t for i, t in enumerate(_own(case))]
 
 
 def _logits(case, seed):
@@ -235,8 +232,7 @@ def _logits(case, seed):
     likely = torch.randint(0, vocab, (case["prompts"], some), generator=g, device=DEV)
     likely = likely.repeat_interleave(case["beams"], dim=0)
     lift = 8.0 + 4.0 * torch.rand((rows, some), generator=g, device=DEV)
-    # (the same token drawn twice: the larger lift, whatever order the GPU writes them in)
-    logits.scatter_reduce_(1, likely, lift, "amax", include_self=False)
+    logits.scatter_(1, likely, lift)
     if case["masked"]:
         logits[torch.rand((rows, vocab), generator=g, device=DEV) < 0.9] = -math.inf
         logits[:, 0] = 0.0  # the end is always allowed
@@ -464,7 +460,9 @@ def run(state):
         children = range(n, 2 * n)
         cache.fork(x["parents"], children)
         cache.append(x["new_k"], x["new_v"], seqs=children, counts=x["new"])
-        res = cache.read(seqs=children, first=x["first"], fields=("k", "v", "positions"))
+        at = _totals(case)
+        first = [at[p] // case["block"] * case["block"] for p in x["parents"]]
+        res = cache.read(seqs=children, first=first, fields=("k", "v", "positions"))
         cache.truncate([0] * n, seqs=children)  # the beams stay, as if the step were refused
         return res
     if kind == "copy":
