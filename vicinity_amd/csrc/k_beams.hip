@@ -24,6 +24,7 @@ namespace {
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
 #define BEAM_NEG (-__builtin_huge_valf())
+constexpr float BEAM_LOWEST = -0x1.fffffep127f;  // of all numbers
 constexpr float BEAM_LOG2E = 1.44269504088896341f;
 
 // Floats by size as unsigned numbers, 0 and -0 alike (NaN: anywhere; its row is taken apart).
@@ -176,12 +177,14 @@ __global__ __launch_bounds__(256, T == KV_F32 ? 6 : 7) void beam_slice_kernel(Be
     }
     __syncthreads();
     const uint32_t bound = min(min(bounds[0], bounds[1]), min(bounds[2], bounds[3]));
-    const float least = bound < size_key(BEAM_NEG) ? BEAM_NEG : of_key(bound);
+    // No such number, or -inf (a grammar that leaves few tokens): all numbers are looked at, and the
+    // first tokens of -inf fill up (40 tokens of 100003, 512 rows: 43 us for both kernels; the search
+    // below, which took these slices before, 617).
+    const uint32_t lowest = size_key(BEAM_LOWEST);
+    const bool open = bound < lowest;
+    const float least = open ? BEAM_LOWEST : of_key(bound);
     const float most = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
     // Pieces that reach the bound go to LDS, where their elements are looked at side by side.
-    if (least == BEAM_NEG)  // (what lies outside of the row does too)
-#pragma unroll
-        for (int p = 0; p < N; p++) tp[p] = token(p, 0) < a.vocab ? tp[p] : __builtin_nanf("");
     uint32_t hits = 0;
 #pragma unroll
     for (int p = 0; p < N; p++) hits += tp[p] >= least;
@@ -243,10 +246,12 @@ __global__ __launch_bounds__(256, T == KV_F32 ? 6 : 7) void beam_slice_kernel(Be
     } else {
         n = BEAM_LIST + 1;
     }
+    uint32_t tie = size_key(BEAM_NEG);  // tokens of this key go behind the list, the first ones, up to k
     if (n > BEAM_LIST) {
         // Many reach the bound: the k-th best key itself, then the tokens above it and the first
         // of those that have it.  Every wave of the workgroup comes here.
         // (the logits come from memory again: this is rare, and needs their registers)
+        const uint32_t high = size_key(most);  // (keys above it are NaN, whose rows are taken apart)
         const auto reach = [&](uint32_t key) {  // how many of the slice's tokens are not below key
             uint32_t c = 0;
 #pragma unroll 1
@@ -255,7 +260,8 @@ __global__ __launch_bounds__(256, T == KV_F32 ? 6 : 7) void beam_slice_kernel(Be
 #pragma unroll
                 for (int e = 0; e < W; e++) {
                     const int t = token(p, e);
-                    c += size_key(element<T>(r, e)) >= key && t >= 0 && t < a.vocab;
+                    const uint32_t x = size_key(element<T>(r, e));
+                    c += x >= key && x <= high && t >= 0 && t < a.vocab;
                 }
             }
 #pragma unroll
@@ -265,9 +271,9 @@ __global__ __launch_bounds__(256, T == KV_F32 ? 6 : 7) void beam_slice_kernel(Be
             __syncthreads();
             return scan[0] + scan[1] + scan[2] + scan[3];
         };
-        uint32_t lo = bound, hi = ~0u;  // reach(lo) >= k (NaN lie above every number)
-        if (reach(size_key(most)) >= (uint32_t)a.k)
-            lo = max(lo, size_key(most));  // (one value, -inf for example)
+        // (more than BEAM_LIST tokens or BEAM_PIECES pieces reach lo)
+        uint32_t lo = max(bound, lowest), hi = high;
+        if (reach(hi) >= (uint32_t)a.k) lo = hi;  // (one value, for example)
         while (lo < hi) {
             const uint32_t mid = lo + (hi - lo) / 2 + 1;
             if (reach(mid) >= (uint32_t)a.k) lo = mid;
@@ -283,11 +289,14 @@ __global__ __launch_bounds__(256, T == KV_F32 ? 6 : 7) void beam_slice_kernel(Be
             for (int e = 0; e < W; e++) {
                 const uint32_t key = size_key(element<T>(r, e));
                 const int t = token(p, e);
-                if (key > lo && t >= 0 && t < a.vocab) list[atomicAdd(&count, 1u)] = (uint64_t)key << 32 | (uint32_t)~t;
+                if (key > lo && key <= high && t >= 0 && t < a.vocab) list[atomicAdd(&count, 1u)] = (uint64_t)key << 32 | (uint32_t)~t;
             }
         }
         __syncthreads();
         n = count;  // below k
+        tie = lo;
+    }
+    if (n < (uint32_t)a.k) {
 #pragma unroll 1
         for (int p = 0; p < np; p++) {
             if (n >= (uint32_t)a.k) break;
@@ -296,7 +305,7 @@ __global__ __launch_bounds__(256, T == KV_F32 ? 6 : 7) void beam_slice_kernel(Be
 #pragma unroll
             for (int e = 0; e < W; e++) {
                 const int t = token(p, e);
-                c += size_key(element<T>(r, e)) == lo && t >= 0 && t < a.vocab;
+                c += size_key(element<T>(r, e)) == tie && t >= 0 && t < a.vocab;
             }
             uint32_t before = c;
 #pragma unroll
@@ -312,8 +321,8 @@ __global__ __launch_bounds__(256, T == KV_F32 ? 6 : 7) void beam_slice_kernel(Be
 #pragma unroll
             for (int e = 0; e < W; e++) {
                 const int t = token(p, e);
-                if (size_key(element<T>(r, e)) == lo && t >= 0 && t < a.vocab) {
-                    if (n + before < (uint32_t)a.k) list[n + before] = (uint64_t)lo << 32 | (uint32_t)~t;
+                if (size_key(element<T>(r, e)) == tie && t >= 0 && t < a.vocab) {
+                    if (n + before < (uint32_t)a.k) list[n + before] = (uint64_t)tie << 32 | (uint32_t)~t;
                     before++;
                 }
             }
