@@ -473,8 +473,9 @@ int vgpu_kv_compact(vgpu_kv *h, size_t num_blocks, size_t *moved, void *stream);
  * rows = groups * beams rows of logits; a group's row and a token have the total
  *   scores[row] + logits[row][token] - log(sum over t of exp(logits[row][t])).
  * The k largest totals of each group, descending, of equal ones the lower row and
- * then the lower token first: out_scores f32, out_parents (rows) and out_tokens i64
- * [groups, k].  A logit of -inf is a token that cannot follow; a row of them, or one
+ * then the lower token first (a row's larger logit, where float64 holds the totals as
+ * equal: a score of -1e30 leaves no difference): out_scores f32, out_parents (rows)
+ * and out_tokens i64 [groups, k].  A logit of -inf is a token that cannot follow; a row of them, or one
  * whose score is -inf, has totals of -inf alone.  A NaN or +inf among a row's logits
  * or in its score makes all of its totals NaN, which come first.  Exponentials are
  * float32, sums and totals float64, rounded once.

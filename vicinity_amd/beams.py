@@ -27,7 +27,8 @@ def select_beams(logits, scores, beams: int, k: int | None = None, stream=None):
     [groups * beams], the rows' log-probabilities so far (None: 0).  A continuation's total is
     scores[row] + logits[row, token] - log(sum(exp(logits[row]))).  Returns (totals, rows,
     tokens), float32, int64 and int64 [groups, k], totals descending, of equal ones the lower
-    row and then the lower token first; k None: beams.  With a cache that holds row i's tokens
+    row and then the lower token first (a row's larger logit, where float64 holds the totals as
+    equal: a score of -1e30 leaves no difference); k None: beams.  With a cache that holds row i's tokens
     in sequence i, a step of beam search is ``cache.fork(rows.view(-1).tolist(), range(n))``
     with k = beams.
 

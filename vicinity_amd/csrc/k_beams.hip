@@ -360,13 +360,17 @@ __global__ __launch_bounds__(1024) void beam_group_kernel(BeamArgs a) {
     __shared__ double lift[BEAM_MAX_BEAMS];
     __shared__ float largest[BEAM_MAX_BEAMS];
     __shared__ uint8_t kinds[BEAM_MAX_BEAMS];
-    __shared__ ulonglong2 pool[BEAM_POOL];  // the total's order; beam << 32 | token
+    __shared__ ulonglong2 pool[BEAM_POOL];  // the total's order; who: beam, logit's order, place
     __shared__ uint32_t sample[BEAM_SAMPLES];
     __shared__ uint32_t hist[BEAM_BINS];
     __shared__ uint32_t place[256];
     __shared__ uint32_t scan[18], count;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int row0 = blockIdx.x * a.beams;
+    // Equal totals go by beam, then by logit (float64 may hold the totals of different ones as
+    // equal), then by the place in the row's lists, where equal logits lie in their tokens' order.
+    // A beam and a place have 32 bits together, for a group has fewer than 2^31 places.
+    const int row_places = a.slices * a.k, place_bits = row_places > 1 ? 32 - __clz(row_places - 1) : 0;
     // 16 lanes to a row
     for (int b0 = 0; b0 < a.beams; b0 += 64) {
         const int b = min(b0 + (tid >> 4), a.beams - 1), row = row0 + b;
@@ -403,20 +407,19 @@ __global__ __launch_bounds__(1024) void beam_group_kernel(BeamArgs a) {
     const auto entry = [&](uint32_t l, int at, Entry& r) {
         const uint32_t b = l / (uint32_t)a.slices, slice = l - b * (uint32_t)a.slices;
         double total;
-        uint32_t token;
+        uint32_t logit = 0;
         if (kinds[b]) {  // all totals alike: the first tokens, as one list
             if (slice || at >= a.vocab) return false;
-            token = (uint32_t)at;
             total = kinds[b] == 1 ? -__builtin_huge_val() : __builtin_nan("");
         } else {
             const uint2 c = a.best[((size_t)row0 * a.slices + l) * a.k + at];
             if (c.y == ~0u) return false;
-            token = c.y;
+            logit = ~size_key(__uint_as_float(c.x));
             total = ((double)__uint_as_float(c.x) - (double)largest[b]) + lift[b];
         }
         r.key = total != total ? ~0ull : size_key(total);
         r.key32 = total != total ? ~0u : size_key((float)total);
-        r.who = (uint64_t)b << 32 | token;
+        r.who = ((uint64_t)b << 32 | logit) << place_bits | (slice * (uint32_t)a.k + (uint32_t)at);
         return true;
     };
     // The digit in which the samples' weights, from the top, reach `need`.
@@ -522,8 +525,10 @@ __global__ __launch_bounds__(1024) void beam_group_kernel(BeamArgs a) {
                 const size_t at = (size_t)blockIdx.x * a.k + to;
                 const uint64_t u = mine.x >> 63 ? mine.x & ~(1ull << 63) : ~mine.x;
                 a.out_scores[at] = (float)__longlong_as_double((long long)u);
-                a.out_parents[at] = row0 + (int64_t)(mine.y >> 32);
-                a.out_tokens[at] = (int64_t)(uint32_t)mine.y;
+                const int b = (int)(mine.y >> place_bits >> 32);
+                const uint32_t spot = (uint32_t)mine.y & (uint32_t)((1ull << place_bits) - 1);
+                a.out_parents[at] = row0 + b;
+                a.out_tokens[at] = kinds[b] ? spot : a.best[(size_t)(row0 + b) * row_places + spot].y;
             } else {
                 pool[to] = mine;
             }
