@@ -105,10 +105,11 @@ __global__ __launch_bounds__(256) void kv_shared_join_kernel(KvDev c, KvAttend a
 template <int S, int CODE, int PARTS>
 void shared_s(const KvDev& c, const KvBatch& b, const KvAttend& a, const KvMembers& mem, hipStream_t s) {
     const dim3 grid((unsigned)b.unit0[b.n] * c.H);
-    if (a.by_rows) {
-        hipLaunchKernelGGL((kv_chunk_kernel<S, CODE, PARTS, kv_chunk_nc(S * 32, PARTS), true>), grid, dim3(256), 0, s, c, b, a, mem);
-        return;
-    }
+    if constexpr (kv_shared_many(S * 32, PARTS))
+        if (a.by_rows) {
+            hipLaunchKernelGGL((kv_chunk_kernel<S, CODE, PARTS, kv_chunk_nc(S * 32, PARTS), true>), grid, dim3(256), 0, s, c, b, a, mem);
+            return;
+        }
     const size_t lds = (size_t)4 * 16 * (32 * S + 4 + 3) * 4;
     int most = 0;
     for (int i = 0; i < b.n; i++) most = b.count[i] > most ? b.count[i] : most;

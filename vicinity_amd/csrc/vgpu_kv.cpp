@@ -52,16 +52,30 @@ constexpr int64_t kSharedSlots = 256;
 // query heads on 8 of 128: 8 pairs of 512 slots, 8.4 MB, 16 us against 17; 4 sequences of 512,
 // 3.1 MB, 15 and 13; 8 x 8 of 512, 59 MB, 17 and 19).
 constexpr int64_t kSharedBytes = (int64_t)8 << 20;
-// The kernel of many rows takes over shared slots from so many tiles of 16 rows on, which are a
-// launch apart from the own slots then, with partial rows four times as many (8 x 128: 244 rows
-// over 8192 slots 70 us and 49 by 16 rows, over 16384 61 and 72; 384 over 65536 156, by 16 rows
-// 480; 128 rows of 192 over 16384 55 and 44; at 256 dims 108 and 53, where it has a compute
-// unit for one workgroup; measured in bfloat16 and taken for all).
-constexpr int64_t kSharedTiles = 98304;
-// Tiles of a workgroup over shared slots, at least.
+// The kernel of many rows takes over shared slots from so many tiles of 16 rows on, from twice as
+// many where its workgroups have 256 rows; they are a launch apart from the own slots then, with
+// partial rows four times as many (8 heads, a token each, own slots 300; by 16 rows and by many:
+// 128 dims in bfloat16, 32768 tiles 36 us and 50, 65536 67 and 59, 98304 82 and 67, 262144 216 and
+// 109; 192 dims, 32768 47 and 57, 65536 81 and 77, 262144 287 and 176; 64 dims in float32, 24576 27
+// and 40, 65536 56 and 51; 64 dims in bfloat16, 256 rows, 65536 51 and 54, 98304 59 and 64, 262144
+// 163 and 91).
+constexpr int64_t kSharedTiles = 65536;
+// Tiles of a workgroup over shared slots, at least (32 beams of 8 prompts of 1000 slots, 8 x 4 x
+// 128: with 2, 4, 8, 16 and 24 tiles 31, 30, 29, 30 and 31 us; 5 x 8 rows over 20000 slots of two
+// heads 23, 23, 21, 19 and 20; more rows or slots: no difference).
 constexpr int64_t kLeastTiles = 8;
 // Levels of branches that are looked at for the best groups.
 constexpr int kSharedDepth = 4;
+
+// Rows that share slots: does the kernel of many rows suit them?  Not at 256 dims, nor at 128 in
+// float32 (244 rows over 16384 slots of 8 heads: 95 us by 16 rows and 141 by many, 76 and 132; over
+// 65536 slots the second 246 and 385): two operands' tiles and where each row's sequence lies are
+// more than the registers hold.
+bool many_shared(const KvDev& dev, int type, int64_t rows, int64_t tiles) {
+    const int parts = type == KV_F32 ? 2 : 1;
+    const int64_t wg = 64 * kv_chunk_nc(dev.Dp, parts);
+    return kv_shared_many(dev.Dp, parts) && rows > wg * 3 / 4 && tiles >= (wg > 128 ? 2 : 1) * kSharedTiles;
+}
 
 // The row tiles of one launch's sequences, and the tiles that each goes over.
 struct KvPlan {
@@ -977,7 +991,7 @@ void KvCache::attend_shared(const int32_t* ids, const int64_t* counts, const std
                 most = std::max<int64_t>(most, e.rows);
                 tiles += (e.rows + 15) / 16 * dev.H * ((e.end + KV_TILE - 1) / KV_TILE - e.t0);
             }
-            by_rows[y] = dev.Dp < 256 && most > chunk_rows * 3 / 4 && tiles >= kSharedTiles;
+            by_rows[y] = many_shared(dev, a.q.type, most, tiles);
         }
         const int launches = by_rows[0] == by_rows[1] ? 1 : 2;
         KvBatch b[2];

@@ -216,6 +216,8 @@ struct KvAttend {
 // with four; in float32 924 with two, 1029 with one; 192 dims: 1087 with one, 2603 with two).
 // 256 dims: one workgroup to a compute unit, by its LDS, with all the registers.
 constexpr int kv_chunk_nc(int Dp, int parts) { return Dp * parts <= 64 ? 4 : Dp <= 128 || Dp * parts == 256 ? 2 : 1; }
+// Whether it takes the rows of several sequences (many_shared says where).
+constexpr bool kv_shared_many(int Dp, int parts) { return Dp < 256 && Dp * parts != 256; }
 // Rows that one workgroup takes.
 inline int kv_attend_rows(const KvAttend& a, int Dp) {
     return a.by_rows ? 64 * kv_chunk_nc(Dp, a.q.type == KV_F32 ? 2 : 1) : 16;
