@@ -513,7 +513,7 @@ int vgpu_test_host_centroid_update(const float *x, size_t n, size_t d, const uin
 int vgpu_test_host_kv_splits(const int64_t *lens, const int64_t *counts, size_t n, size_t heads,
                              size_t group, int32_t *splits, int32_t *tiles);
 /* Attention reads slots that several sequences of a call share once for all of them where that
- * saves so many bytes (0: wherever they share 256 slots). */
+ * saves so many bytes and their rows are few (0: wherever they share 256 slots). */
 int vgpu_test_set_kv_shared_bytes(vgpu_kv *h, size_t bytes);
 /* The OPQ polar factor U V^T of M f32[d*d] (compute_optimal_rotation,
  * opq.rs:280-294) into R f32[d*d]. */

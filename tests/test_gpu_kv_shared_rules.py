@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 from test_gpu_kv import _rand
-from test_gpu_kv_shared import _check_large, _large
+from test_gpu_kv_shared import _check_large, _large, share
 
 pytestmark = pytest.mark.gpu
 
@@ -23,3 +23,77 @@ def test_around_the_tiles_of_the_kernel_of_many_rows(dim, dtype, forks, group, s
     cache = _large(slots, [5 + i % 3 for i in range(forks)], 8, dim, 64, "int8", dtype)
     q = _rand((forks, 8 * group, dim), dtype, 7)
     _check_large(cache, q, list(range(1, forks + 1)), [1] * forks)
+
+
+def usual(cache):
+    """Shared slots are read once where a program's calls do so."""
+    from vicinity_amd import _lib
+
+    _lib.check(_lib.load().vgpu_test_set_kv_shared_bytes(cache._h, 8 << 20))
+    return cache
+
+
+# Calls that take each sequence by itself, so forks come out bit for bit as copies do: sequences
+# whose rows fill tiles by themselves, and those that the kernel of many rows takes alone.
+@pytest.mark.parametrize("forks,tokens,group,prefix,heads,dim,dtype", [
+    (32, 5, 4, 2048, 8, 128, "bfloat16"),    # 20 rows each, 512 workgroups of 16 rows
+    (32, 20, 4, 2048, 8, 64, "float16"),     # 80 rows
+    (61, 4, 4, 4096, 8, 256, "bfloat16"),    # 16 rows, a dimension that has no kernel for many
+    (8, 64, 4, 4096, 8, 128, "bfloat16"),    # 256 rows: two workgroups of many rows, full
+    (2, 512, 4, 8192, 8, 128, "float32"),
+    (2, 2048, 4, 2048, 8, 192, "bfloat16")])
+def test_forks_with_rows_of_their_own_are_taken_as_copies_are(forks, tokens, group, prefix, heads, dim, dtype):
+    import torch
+
+    import vicinity_amd as va
+
+    _case(f"{forks} forks x {tokens} tokens x {group}, {prefix} slots of {heads} x {dim}, {dtype}")
+    blocks = forks * (-(-(prefix + tokens) // 64) + 1) + prefix // 64
+    cache = va.KVCache(forks + 1, heads, dim, blocks, code="int8")
+    k, v = (_rand((prefix, heads, dim), dtype, i) for i in (1, 2))
+    nk, nv = (_rand((forks * tokens, heads, dim), dtype, i) for i in (3, 4))
+    q = _rand((forks * tokens, heads * group, dim), dtype, 5)
+    got = []
+    for copy in (False, True):
+        cache.truncate(0)
+        cache.append(k, v, seqs=[forks])
+        cache.fork([forks] * forks, range(forks), copy=copy)
+        cache.append(nk, nv, seqs=range(forks))
+        got.append(cache.attend(q, seqs=range(forks), return_lse=True))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, "bfloat16"), (80, "float32"), (128, "float16"), (256, "bfloat16")])
+def test_many_tokens_and_single_ones_of_the_same_prefix(dim, dtype):
+    """A prompt that comes in beside answers that go on: only the answers share tiles."""
+    cache = usual(_large(4100, [700, 3, 40, 9, 1, 64, 65, 300], 8, dim, 64, "fp8", dtype))
+    counts = [700, 1, 1, 5, 1, 1, 30, 257]
+    _case(f"{dim} {dtype}")
+    q = _rand((sum(counts), 8 * 4, dim), dtype, 7)
+    for window in (0, 3000):
+        _check_large(cache, q, list(range(1, 9)), counts, window=window)
+    # all of them alike, and none of them
+    share(cache)
+    _check_large(cache, q, list(range(1, 9)), counts)
+    _check_large(usual(cache), q[:8], list(range(1, 9)), [1] * 8)
+
+
+def test_groups_of_which_one_or_none_is_left():
+    """Of each prompt's answers all but one, or all, are taken by themselves."""
+    import torch
+
+    import vicinity_amd as va
+
+    cache = va.KVCache(12, 8, 128, 2000, code="int8")
+    k, v = (_rand((8192, 8, 128), "bfloat16", i) for i in (1, 2))
+    cache.append(k, v, seqs=[10, 11], counts=[4096, 4096])
+    cache.fork([10] * 5 + [11] * 5, range(10))
+    counts = [1, 150, 200, 170, 260, 99, 180, 140, 300, 210]
+    k, v = (_rand((sum(counts), 8, 128), "bfloat16", i) for i in (3, 4))
+    cache.append(k, v, seqs=range(10), counts=counts)
+    q = _rand((sum(counts), 32, 128), "bfloat16", 5)
+    _check_large(cache, q, list(range(10)), counts)
+    alone = torch.cat([cache.attend(q[sum(counts[:i]):sum(counts[:i + 1])], seqs=[i]) for i in range(10)])
+    whole = cache.attend(q, seqs=range(10), counts=counts)
+    assert (alone - whole).abs().max() <= 2.0 ** -6 * whole.abs().max()

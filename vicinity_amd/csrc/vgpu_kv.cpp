@@ -64,6 +64,21 @@ constexpr int64_t kSharedTiles = 65536;
 // 128: with 2, 4, 8, 16 and 24 tiles 31, 30, 29, 30 and 31 us; 5 x 8 rows over 20000 slots of two
 // heads 23, 23, 21, 19 and 20; more rows or slots: no difference).
 constexpr int64_t kLeastTiles = 8;
+// A sequence of more rows than this shares no tile of 16 rows with two others.  Where the tiles of
+// all such sequences are workgroups enough, they are taken apart, as if nothing were shared: the
+// caches hold what they read in common, and nobody joins their parts (8 x 128 in bfloat16: 32
+// sequences of 20 rows over 2048 shared slots 27 us apart, 32 together; 8 of 56 rows, 256
+// workgroups, 30 and 24)...
+constexpr int64_t kTileRows = 8;
+constexpr int64_t kApartWorkgroups = kStepWorkgroups / 2;
+// ... but where the kernel of many rows takes them together: for rows that it would not take one
+// sequence at a time (32 of 40 rows over 8192 slots 101 us apart, 79 together), and for others
+// where that fills its workgroups with a quarter fewer (12 sequences of 266 rows over 16224 slots of
+// 2 x 128 137 and 91; 8 of 512 rows over 8192 of 8 x 128 164 and 244).  At the widths where it
+// cannot, it is slow for single sequences as well, and four times as many workgroups stay together
+// (9 sequences of 560 rows over 3360 slots of 4 x 256 247 us apart, 181 by 16 rows together; 10 of
+// 688 over 1696 of 8 x 256 a third faster apart).
+//
 // Levels of branches that are looked at for the best groups.
 constexpr int kSharedDepth = 4;
 
@@ -923,11 +938,37 @@ void KvCache::attend_shared(const int32_t* ids, const int64_t* counts, const std
             if (members.size() > 1) find_groups(ids, counts, a, members, 0, 0, groups, saved), saved_slots += saved;
         }
     }
+    const int parts = a.q.type == KV_F32 ? 2 : 1;
+    const int64_t chunk_rows = 64 * kv_chunk_nc(dev.Dp, parts);
+    if (!groups.empty() && shared_bytes) {  // (0: tests of shared slots, for any rows)
+        const auto tiles_of = [](int64_t rows, int64_t wg) { return (rows + wg - 1) / wg; };
+        int64_t most = 0, chunk_tiles = 0, wide = 0;
+        for (size_t i = 0; i < n; i++) {
+            const int64_t rows = counts[i] * a.G;
+            most = std::max(most, rows);
+            chunk_tiles += tiles_of(rows, chunk_rows) * dev.H * tiles_of(seqs[ids[i]].len, KV_TILE);
+            if (rows > kTileRows) wide += tiles_of(rows, 16) * dev.H;
+        }
+        const bool chunks = most > chunk_rows * 3 / 4 && chunk_tiles >= kChunkTiles;  // (as for the rest)
+        saved_slots = 0;
+        for (Group& x : groups) {
+            int64_t rows = 0, alone = 0;  // of the group; workgroups of many rows of its sequences
+            for (uint32_t i : x.members) rows += counts[i] * a.G, alone += tiles_of(counts[i] * a.G, chunk_rows);
+            const bool many = many_shared(dev, a.q.type, rows, tiles_of(rows, 16) * dev.H * ((x.slots - x.low) / KV_TILE));
+            const bool fuller = 3 * alone >= 4 * tiles_of(rows, chunk_rows);
+            const auto apart = [&](uint32_t i) {
+                const int64_t own = counts[i] * a.G;
+                const bool chunk = chunks && own > chunk_rows * 3 / 4;
+                if (own <= kTileRows || (many && (!chunk || fuller))) return false;
+                return wide > (chunk && !kv_shared_many(dev.Dp, parts) ? 4 : 1) * kApartWorkgroups;
+            };
+            x.members.erase(std::remove_if(x.members.begin(), x.members.end(), apart), x.members.end());
+            if (x.members.size() > 1) saved_slots += (x.slots - x.low) * (int64_t)(x.members.size() - 1);
+        }
+    }
     if (saved_slots * dev.H * 2 * dev.Dp < shared_bytes) groups.clear();
     // Groups in pieces of as many sequences as one launch takes: each has an entry of its own and
     // the piece one more, and every row leaves partial results of both.
-    const int parts = a.q.type == KV_F32 ? 2 : 1;
-    const int64_t chunk_rows = 64 * kv_chunk_nc(dev.Dp, parts);
     const int64_t row_bytes = (int64_t)dev.Dp * 4 + 12, room = kPartBytes / 2 / row_bytes / dev.H;
     const auto rows_of = [&](uint32_t i) { return (counts[i] * a.G + chunk_rows - 1) / chunk_rows * chunk_rows; };
     struct Piece {

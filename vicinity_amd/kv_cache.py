@@ -231,8 +231,8 @@ class KVCache:
         into: a step of beam search is ``fork(parents, beams)``.  Blocks are shared, and copied
         when a holder writes into one that others hold too (append into a begun block, attend
         with decay); copy=True: copied at once.  Both need free blocks for the copies.  Either
-        way each sequence reads, attends and changes as if it were alone; attend reads what
-        several sequences share once for all of them."""
+        way each sequence reads, attends and changes as if it were alone; attend
+        without decay reads what several sequences share once for all, where that is faster."""
         to, part = self._seqs(into), self._slice(seqs)
         # (the library checks their range)
         ids = _array("i", seqs, "sequences") if part is None else self._all[part]
