@@ -29,7 +29,7 @@ def usual(cache):
     """Shared slots are read once where a program's calls do so."""
     from vicinity_amd import _lib
 
-    _lib.check(_lib.load().vgpu_test_set_kv_shared_bytes(cache._h, 8 << 20))
+    _lib.check(_lib.load().vgpu_test_set_kv_shared_bytes(cache._h, 12 << 20))
     return cache
 
 
@@ -39,6 +39,9 @@ def usual(cache):
     (32, 5, 4, 2048, 8, 128, "bfloat16"),    # 20 rows each, 512 workgroups of 16 rows
     (32, 20, 4, 2048, 8, 64, "float16"),     # 80 rows
     (61, 4, 4, 4096, 8, 256, "bfloat16"),    # 16 rows, a dimension that has no kernel for many
+    (64, 1, 4, 960, 8, 128, "bfloat16"),     # 512 workgroups that need no split, few slots shared
+    (128, 1, 1, 1900, 4, 64, "float32"),     # the same in two launches
+    (5, 1, 8, 1312, 8, 128, "bfloat16"),     # 10.7 MB that would be left unread
     (8, 64, 4, 4096, 8, 128, "bfloat16"),    # 256 rows: two workgroups of many rows, full
     (2, 512, 4, 8192, 8, 128, "float32"),
     (2, 2048, 4, 2048, 8, 192, "bfloat16")])

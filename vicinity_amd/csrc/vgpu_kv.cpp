@@ -49,9 +49,15 @@ constexpr size_t kRowRuns = 64;
 // Sequences that share so many slots are taken over them together.
 constexpr int64_t kSharedSlots = 256;
 // ... where that leaves so many bytes of a call unread, which the join of the parts costs (32
-// query heads on 8 of 128: 8 pairs of 512 slots, 8.4 MB, 16 us against 17; 4 sequences of 512,
-// 3.1 MB, 15 and 13; 8 x 8 of 512, 59 MB, 17 and 19).
-constexpr int64_t kSharedBytes = (int64_t)8 << 20;
+// query heads on 8 of 128: 4 sequences of 512 slots, 3.1 MB, 15 us against 13; 8 query heads to one,
+// 5 of 1312, 10.7 MB, 14.8 and 13.4; 8 or 4 of them, 8 of 1000 or 4 of 2048, 14 and 12.6 MB, alike;
+// 4 x 4 of 1000, 25 MB, 15.8 and 17.2).
+constexpr int64_t kSharedBytes = (int64_t)12 << 20;
+// Where the call's row tiles are workgroups enough without splits, taken apart they need no join: then
+// so many slots have to be shared for each launch of some 96 sequences (8 x 8 sequences of 32 query
+// heads on 8 of 128: 512 slots 16.6 us together and 13.7 apart, 800 17.5 and 16.6, 1000 17.8 and
+// 18.9, 1500 20.5 and 23.9; 32 x 4: 512 40 and 26, 1000 44 and 35, 2000 54 and 58).
+constexpr int64_t kCrowdedSlots = 1024, kLaunchSeqs = 96;
 // The kernel of many rows takes over shared slots from so many tiles of 16 rows on, from twice as
 // many where its workgroups have 256 rows; they are a launch apart from the own slots then, with
 // partial rows four times as many (8 heads, a token each, own slots 300; by 16 rows and by many:
@@ -70,10 +76,12 @@ constexpr int64_t kLeastTiles = 8;
 // sequences of 20 rows over 2048 shared slots 27 us apart, 32 together; 8 of 56 rows, 256
 // workgroups, 30 and 24)...
 constexpr int64_t kTileRows = 8;
+constexpr int64_t kLongSlots = 6144;
 constexpr int64_t kApartWorkgroups = kStepWorkgroups / 2;
-// ... but where the kernel of many rows takes them together: for rows that it would not take one
-// sequence at a time (32 of 40 rows over 8192 slots 101 us apart, 79 together), and for others
-// where that fills its workgroups with a quarter fewer (12 sequences of 266 rows over 16224 slots of
+// ... but where the kernel of many rows takes them together: rows that it would not take one
+// sequence at a time over so many shared slots, which pay for their parts (8 x 128: 32 of 40 rows over
+// 8192 slots 101 us apart, 79 together, 32 of 32 over 6560 a fifth faster together; 52 of 48 over
+// 1792 49 and 69; 64 dims, 63 of 16 over 3328 86 and 112), and others where that fills its workgroups with a quarter fewer (12 sequences of 266 rows over 16224 slots of
 // 2 x 128 137 and 91; 8 of 512 rows over 8192 of 8 x 128 164 and 244).  At the widths where it
 // cannot, it is slow for single sequences as well, and four times as many workgroups stay together
 // (9 sequences of 560 rows over 3360 slots of 4 x 256 247 us apart, 181 by 16 rows together; 10 of
@@ -942,24 +950,30 @@ void KvCache::attend_shared(const int32_t* ids, const int64_t* counts, const std
     const int64_t chunk_rows = 64 * kv_chunk_nc(dev.Dp, parts);
     if (!groups.empty() && shared_bytes) {  // (0: tests of shared slots, for any rows)
         const auto tiles_of = [](int64_t rows, int64_t wg) { return (rows + wg - 1) / wg; };
-        int64_t most = 0, chunk_tiles = 0, wide = 0;
+        int64_t most = 0, chunk_tiles = 0, units = 0, wide = 0;
         for (size_t i = 0; i < n; i++) {
             const int64_t rows = counts[i] * a.G;
             most = std::max(most, rows);
             chunk_tiles += tiles_of(rows, chunk_rows) * dev.H * tiles_of(seqs[ids[i]].len, KV_TILE);
+            units += tiles_of(rows, 16) * dev.H;
             if (rows > kTileRows) wide += tiles_of(rows, 16) * dev.H;
         }
         const bool chunks = most > chunk_rows * 3 / 4 && chunk_tiles >= kChunkTiles;  // (as for the rest)
+        // (as KvPlan::split would leave them whole)
+        const bool crowded = !chunks && 2 * units > kStepWorkgroups + kStepWorkgroups / 8;
+        const int64_t least = crowded ? kCrowdedSlots * tiles_of((int64_t)n, kLaunchSeqs) : 0;
         saved_slots = 0;
         for (Group& x : groups) {
             int64_t rows = 0, alone = 0;  // of the group; workgroups of many rows of its sequences
             for (uint32_t i : x.members) rows += counts[i] * a.G, alone += tiles_of(counts[i] * a.G, chunk_rows);
             const bool many = many_shared(dev, a.q.type, rows, tiles_of(rows, 16) * dev.H * ((x.slots - x.low) / KV_TILE));
+            const bool far = x.slots - x.low >= kLongSlots;
             const bool fuller = 3 * alone >= 4 * tiles_of(rows, chunk_rows);
             const auto apart = [&](uint32_t i) {
                 const int64_t own = counts[i] * a.G;
                 const bool chunk = chunks && own > chunk_rows * 3 / 4;
-                if (own <= kTileRows || (many && (!chunk || fuller))) return false;
+                if (own <= kTileRows) return x.slots - x.low < least;
+                if (many && (chunk ? fuller : far)) return false;
                 return wide > (chunk && !kv_shared_many(dev.Dp, parts) ? 4 : 1) * kApartWorkgroups;
             };
             x.members.erase(std::remove_if(x.members.begin(), x.members.end(), apart), x.members.end());
