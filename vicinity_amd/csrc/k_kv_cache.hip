@@ -133,7 +133,8 @@ __global__ __launch_bounds__(256) void kv_rename_kernel(int* table, int W, KvRow
 }
 
 // Blocks copied whole: a workgroup takes 16 KiB of a block's codes (a block is contiguous, and
-// a multiple of 4 KiB); the first of a block also takes its scales, positions and weights.
+// a multiple of 4 KiB) and its share of the positions and weights; the first of a block also takes
+// the scales (10 blocks of 64 heads x 256 slots: all of these by the first workgroup 28 us, so 10).
 // Stores pass the caches by, which leaves them to what is read (206 MB by themselves: 52 us,
 // cached stores 78, 32 KiB to a workgroup 63).
 __global__ __launch_bounds__(256) void kv_moves_kernel(KvDev from, KvDev to, KvMoves m, int pieces, int* map) {
@@ -156,16 +157,18 @@ __global__ __launch_bounds__(256) void kv_moves_kernel(KvDev from, KvDev to, KvM
 #pragma unroll
     for (int j = 0; j < KV_COPY; j++)
         if (at + j * 256 < end) __builtin_nontemporal_store(x[j], out + at + j * 256);
+    // (a head has a multiple of 32 slots)
+    const int quads = from.H * from.B / 4, q1 = (int)((int64_t)quads * (piece + 1) / pieces);
+    const uint4* pos_in = (const uint4*)from.positions + (size_t)src * quads;
+    const uint4* wts_in = (const uint4*)from.weights + (size_t)src * quads;
+    uint4* pos_out = (uint4*)to.positions + (size_t)dst * quads;
+    uint4* wts_out = (uint4*)to.weights + (size_t)dst * quads;
+    for (int j = (int)((int64_t)quads * piece / pieces) + tid; j < q1; j += 256) pos_out[j] = pos_in[j], wts_out[j] = wts_in[j];
     if (piece) return;
     if (map && tid == 0) map[src] = dst;
     for (int h = tid; h < from.H; h += 256) {
         to.kscale[(size_t)dst * from.H + h] = from.kscale[(size_t)src * from.H + h];
         to.vscale[(size_t)dst * from.H + h] = from.vscale[(size_t)src * from.H + h];
-    }
-    const int slots = from.H * from.B;
-    for (int j = tid; j < slots; j += 256) {
-        to.positions[(size_t)dst * slots + j] = from.positions[(size_t)src * slots + j];
-        to.weights[(size_t)dst * slots + j] = from.weights[(size_t)src * slots + j];
     }
 }
 
