@@ -100,3 +100,20 @@ def test_groups_of_which_one_or_none_is_left():
     alone = torch.cat([cache.attend(q[sum(counts[:i]):sum(counts[:i + 1])], seqs=[i]) for i in range(10)])
     whole = cache.attend(q, seqs=range(10), counts=counts)
     assert (alone - whole).abs().max() <= 2.0 ** -6 * whole.abs().max()
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, "float32"), (128, "bfloat16"), (192, "float16")])
+def test_prefixes_of_very_different_lengths(dim, dtype):
+    """Groups whose longest has many times the slots of the others, taken in several rounds."""
+    import vicinity_amd as va
+
+    _case(f"{dim} {dtype}")
+    prefixes = [299, 4922, 1845, 4029, 391, 4586, 9339, 329]
+    cache = share(va.KVCache(80, 8, dim, 1000, code="fp8"))
+    k, v = (_rand((sum(prefixes), 8, dim), dtype, i) for i in (1, 2))
+    cache.append(k, v, seqs=range(72, 80), counts=prefixes)
+    cache.fork([72 + i // 9 for i in range(72)], range(72))
+    k, v = (_rand((72 * 19, 8, dim), dtype, i) for i in (3, 4))
+    cache.append(k, v, seqs=range(72))
+    q = _rand((72, 32, dim), dtype, 5)
+    _check_large(cache, q, list(range(72)), [1] * 72)
