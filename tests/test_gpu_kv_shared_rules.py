@@ -29,7 +29,7 @@ def usual(cache):
     """Shared slots are read once where a program's calls do so."""
     from vicinity_amd import _lib
 
-    _lib.check(_lib.load().vgpu_test_set_kv_shared_bytes(cache._h, 12 << 20))
+    _lib.check(_lib.load().vgpu_test_set_kv_shared_bytes(cache._h, 8 << 20))
     return cache
 
 
@@ -100,6 +100,35 @@ def test_groups_of_which_one_or_none_is_left():
     alone = torch.cat([cache.attend(q[sum(counts[:i]):sum(counts[:i + 1])], seqs=[i]) for i in range(10)])
     whole = cache.attend(q, seqs=range(10), counts=counts)
     assert (alone - whole).abs().max() <= 2.0 ** -6 * whole.abs().max()
+
+
+@pytest.mark.parametrize("dim,dtype,window", [(64, "bfloat16", 0), (128, "float32", 0), (96, "float16", 700), (256, "bfloat16", 0)])
+def test_sequences_that_share_nothing_beside_those_that_do(dim, dtype, window):
+    """Sequences in no group, an empty one and one without tokens among them, in a call of forks."""
+    import torch
+
+    import vicinity_amd as va
+
+    _case(f"{dim} {dtype} window {window}")
+    heads, group = 8, 4
+    cache = va.KVCache(24, heads, dim, 800, code="int8")
+    k, v = (_rand((9000, heads, dim), dtype, i) for i in (1, 2))
+    cache.append(k, v, seqs=[20, 21], counts=[8800, 200])
+    cache.fork([20] * 9 + [21] * 3, range(12))
+    own = [5, 1, 64, 7, 33, 2, 90, 1, 12, 3, 4, 5]
+    alone = [1, 100, 300, 32]
+    k, v = (_rand((sum(own + alone), heads, dim), dtype, i) for i in (3, 4))
+    cache.append(k, v, seqs=list(range(12)) + [12, 13, 14, 15], counts=own + alone)
+    seqs, counts = [12, 3, 16, 0, 1, 9, 17, 2, 4, 10, 5, 13, 6, 7, 8, 11, 14, 15], [1] * 18
+    counts[4], counts[6] = 4, 0  # (17: empty, and without tokens; 16: empty)
+    q = _rand((sum(counts), heads * group, dim), dtype, 5)
+    for shared in (share, usual):
+        shared(cache)
+        out, lse = cache.attend(q, seqs=seqs, counts=counts, window=window, return_lse=True)
+        assert (out[2] == 0).all() and torch.isneginf(lse[2]).all()
+        live = [i for i, s in enumerate(seqs) if s not in (16, 17)]
+        rows = torch.cat([torch.arange(sum(counts[:i]), sum(counts[:i + 1])) for i in live]).to("cuda:0")
+        _check_large(cache, q[rows], [seqs[i] for i in live], [counts[i] for i in live], window=window)
 
 
 @pytest.mark.parametrize("dim,dtype", [(64, "float32"), (128, "bfloat16"), (192, "float16")])

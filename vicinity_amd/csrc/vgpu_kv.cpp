@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <functional>
 
 #include "vgpu_runtime.h"
 
@@ -48,16 +49,19 @@ constexpr size_t kRowRuns = 64;
 
 // Sequences that share so many slots are taken over them together.
 constexpr int64_t kSharedSlots = 256;
-// ... where that leaves so many bytes of a call unread, which the join of the parts costs (32
-// query heads on 8 of 128: 4 sequences of 512 slots, 3.1 MB, 15 us against 13; 8 query heads to one,
-// 5 of 1312, 10.7 MB, 14.8 and 13.4; 8 or 4 of them, 8 of 1000 or 4 of 2048, 14 and 12.6 MB, alike;
-// 4 x 4 of 1000, 25 MB, 15.8 and 17.2).
-constexpr int64_t kSharedBytes = (int64_t)12 << 20;
-// Where the call's row tiles are workgroups enough without splits, taken apart they need no join: then
-// so many slots have to be shared for each launch of some 96 sequences (8 x 8 sequences of 32 query
-// heads on 8 of 128: 512 slots 16.6 us together and 13.7 apart, 800 17.5 and 16.6, 1000 17.8 and
-// 18.9, 1500 20.5 and 23.9; 32 x 4: 512 40 and 26, 1000 44 and 35, 2000 54 and 58).
-constexpr int64_t kCrowdedSlots = 1024, kLaunchSeqs = 96;
+// ... where that leaves so many bytes of a call unread, which the join of the parts costs: with
+// sequences of more than 8 rows, and without (32 query heads on 8 of 128: 4 sequences of 512 slots,
+// 3.1 MB, 15 us against 13; 8 query heads to one, 5 of 1312, 10.7 MB, 14.8 and 13.4; 8 or 4 of them,
+// 8 of 1000 or 4 of 2048, 14 and 12.6 MB, alike; 4 x 4 of 1000, 25 MB, 15.8 and 17.2; 128 rows each:
+// 4 sequences of 1376, 8.5 MB, 21.9 and 27.7).
+constexpr int64_t kSharedBytes = (int64_t)8 << 20, kFewBytes = (int64_t)12 << 20;
+// Sequences of at most 8 rows that need no splits when each is taken by itself, and then no join,
+// have to share so many slots on average for each launch of some 96 of them (8 x 8 sequences of 32
+// query heads on 8 of 128: 512 slots 16.6 us together and 13.7 apart, 800 17.5 and 16.6, 1000 17.8
+// and 18.9, 1500 20.5 and 23.9; 32 x 4: 512 40 and 26, 1000 44 and 35, 2000 54 and 58); fewer where
+// their workgroups are more than 512, and have more than one round to do (64 of 32 heads of 64 in
+// float32: 512 slots 25 and 24, 1000 28 and 35; 65 of 32 of 192: 896 slots 44 and 81).
+constexpr int64_t kCrowdedSlots = 1024, kCrowdedUnits = 512, kLaunchSeqs = 96;
 // The kernel of many rows takes over shared slots from so many tiles of 16 rows on, from twice as
 // many where its workgroups have 256 rows; they are a launch apart from the own slots then, with
 // partial rows four times as many (8 heads, a token each, own slots 300; by 16 rows and by many:
@@ -71,22 +75,20 @@ constexpr int64_t kSharedTiles = 65536;
 // heads 23, 23, 21, 19 and 20; more rows or slots: no difference).
 constexpr int64_t kLeastTiles = 8;
 // A sequence of more rows than this shares no tile of 16 rows with two others.  Where the tiles of
-// all such sequences are workgroups enough, they are taken apart, as if nothing were shared: the
-// caches hold what they read in common, and nobody joins their parts (8 x 128 in bfloat16: 32
-// sequences of 20 rows over 2048 shared slots 27 us apart, 32 together; 8 of 56 rows, 256
-// workgroups, 30 and 24)...
+// such sequences are this many workgroups, taken apart, as if nothing were shared, they find in the
+// caches what they read in common, and nobody joins their parts (8 x 128 in bfloat16: 32 sequences of
+// 20 rows over 2048 shared slots 27 us apart, 32 together; 8 of 56 rows, 256 workgroups, 30 and 24).
 constexpr int64_t kTileRows = 8;
-constexpr int64_t kLongSlots = 6144;
 constexpr int64_t kApartWorkgroups = kStepWorkgroups / 2;
-// ... but where the kernel of many rows takes them together: rows that it would not take one
-// sequence at a time over so many shared slots, which pay for their parts (8 x 128: 32 of 40 rows over
-// 8192 slots 101 us apart, 79 together, 32 of 32 over 6560 a fifth faster together; 52 of 48 over
-// 1792 49 and 69; 64 dims, 63 of 16 over 3328 86 and 112), and others where that fills its workgroups with a quarter fewer (12 sequences of 266 rows over 16224 slots of
-// 2 x 128 137 and 91; 8 of 512 rows over 8192 of 8 x 128 164 and 244).  At the widths where it
-// cannot, it is slow for single sequences as well, and four times as many workgroups stay together
-// (9 sequences of 560 rows over 3360 slots of 4 x 256 247 us apart, 181 by 16 rows together; 10 of
-// 688 over 1696 of 8 x 256 a third faster apart).
-//
+// Rows that the kernel of many would not take one sequence at a time it takes together over so many
+// shared slots, which pay for their parts (8 x 128: 32 of 40 rows over 8192 slots 101 us apart, 79
+// together, 32 of 32 over 6560 a fifth faster together; 52 of 48 over 1792 49 and 69; 64 dims, 63 of
+// 16 over 3328 86 and 112).
+constexpr int64_t kLongSlots = 6144;
+// Rows of the kernel of many have so many tiles of 16 to do where they leave sequences of fewer rows,
+// which takes a launch more (28 sequences of which one has 684 rows over 1954 slots of 8 x 96, 34000
+// tiles: 28 us together, 49 not; five of up to 2560 over 417 of 32 x 128, 92000: 151 and 60).
+constexpr int64_t kManyTiles = 65536, kManySlots = 512;
 // Levels of branches that are looked at for the best groups.
 constexpr int kSharedDepth = 4;
 
@@ -935,6 +937,128 @@ void KvCache::find_groups(const int32_t* ids, const int64_t* counts, const KvAtt
     }
 }
 
+// Takes sequences out of the groups that are faster each by itself; true if there are such in the call.
+bool KvCache::part_groups(const int32_t* ids, const int64_t* counts, size_t n, const KvAttend& a, std::vector<Group>& groups) const {
+    const auto tiles_of = [](int64_t rows, int64_t wg) { return (rows + wg - 1) / wg; };
+    const bool can_many = kv_shared_many(dev.Dp, a.q.type == KV_F32 ? 2 : 1);
+    const int64_t chunk_rows = 64 * kv_chunk_nc(dev.Dp, a.q.type == KV_F32 ? 2 : 1);
+    // The rows of a sequence: few, more, or those that the kernel of many takes (as for the rest).
+    enum { FEW, MORE, MANY };
+    int64_t chunk_tiles = 0, other_tiles = 0;  // of its workgroups
+    for (size_t i = 0; i < n; i++)
+        (counts[i] * a.G > chunk_rows * 3 / 4 ? chunk_tiles : other_tiles) +=
+            tiles_of(counts[i] * a.G, chunk_rows) * dev.H * tiles_of(seqs[ids[i]].len, KV_TILE);
+    const bool chunks = chunk_tiles >= kChunkTiles;
+    // (taken apart beside one with many rows, those of few would go by the kernel of many as well)
+    const bool steps = !chunk_tiles || chunk_tiles + other_tiles < kChunkTiles;
+    const auto kind_of = [&](uint32_t i) {
+        const int64_t rows = counts[i] * a.G;
+        return rows <= kTileRows ? FEW : chunks && rows > chunk_rows * 3 / 4 ? MANY : MORE;
+    };
+    int64_t units[3] = {0, 0, 0}, many_tiles = 0, by_many = 0;  // workgroups of 16 rows; those of MANY: tiles, sequences
+    for (size_t i = 0; i < n; i++) {
+        const int64_t own = tiles_of(counts[i] * a.G, 16) * dev.H;
+        units[kind_of((uint32_t)i)] += own;
+        if (kind_of((uint32_t)i) == MANY) by_many++, many_tiles += own * tiles_of(seqs[ids[i]].len, KV_TILE);
+    }
+    const bool has_many = by_many > 0;
+    int64_t few = 0, few_slots = 0, others = 0, saved = 0, most = 0, most_slots = 0, tiles = 0;  // of the groups
+    for (const Group& x : groups) {
+        int64_t rows = 0;
+        for (uint32_t i : x.members) rows += counts[i] * a.G;
+        most = std::max(most, rows), most_slots = std::max(most_slots, x.slots - x.low), tiles += tiles_of(rows, 16) * dev.H * ((x.slots - x.low) / KV_TILE);
+        saved += (x.slots - x.low) * (int64_t)(x.members.size() - 1);
+        for (uint32_t i : x.members)
+            if (kind_of(i) == FEW) few++, few_slots += x.slots - x.low;
+            else others++, by_many -= kind_of(i) == MANY;
+    }
+    bool some = by_many > 0;  // not in any group
+    // Beside rows of the kernel of many, where those are nearly all, less than 512 slots are not worth the
+    // parts (39 sequences of 8 x 192 over 296 slots, a third with up to 1472 rows: 44 us apart, 116;
+    // 39 of 32 x 128 in float32 over 475, a third with up to 147 rows: 162 and 50).
+    if (!steps && most_slots < kManySlots && units[MANY] >= 8 * units[FEW]) {
+        groups.clear();
+        return true;
+    }
+    const bool whole = steps && whole_steps(ids, counts, n, a);
+    // Those of few rows go one way, and those of more with them where they are the more, for each way
+    // has launches of its own (32 sequences of 5 tokens and 32 of one, 4 x 8 x 128 over 2048 shared
+    // slots: 32 us either way, 43 one each).
+    const bool more_apart = whole && units[MORE] > kApartWorkgroups && units[MORE] >= 2 * units[FEW];
+    const int64_t launches = tiles_of((int64_t)n, kLaunchSeqs), all_units = units[FEW] + units[MORE] + units[MANY];
+    const int64_t least = kCrowdedSlots * launches * std::min(all_units, kCrowdedUnits * launches) / std::max<int64_t>(all_units, 1);
+    const bool few_apart = (whole && few_slots < few * least) ||
+                           (steps && !others && saved * dev.H * 2 * dev.Dp < kFewBytes);
+    // Rows of the kernel of many stay together where that saves a third of its time, or a quarter over slots
+    // that pay for the parts, by how full its workgroups and their last round are (11 sequences of 136
+    // rows over 2394 slots of 32 x 96 188 us apart and 127; 12 of 266 over 16224 of 2 x 128 137 and 91, 38
+    // of 204 over 8768 of 4 x 128 359 and 203, 80 of 268 over 960 of 8 x 128 204 and 315; 8 of 512
+    // over 8192 164 and 244).  At the widths where it takes one sequence only it is slow, and four
+    // times as many workgroups stay (9 of 560 rows over 3360 slots of 4 x 256 247 us, 181 by 16 rows
+    // together; 10 of 688 over 1696 of 8 x 256 a third faster apart).
+    double rounds = 1.;
+    if (has_many) {
+        KvPlan plan;
+        KvBatch b;
+        plan.heads = dev.H;
+        for (size_t i = 0; i < n && plan.n < KV_BATCH; i++)
+            if (kind_of((uint32_t)i) == MANY) plan.add(seqs[ids[i]].len, counts[i], a.G, chunk_rows, a.causal, a.window);
+        plan.split(b, true, kPartBytes / (chunk_rows * ((int64_t)dev.Dp * 4 + 12)));
+        rounds = (double)(tiles_of(plan.groups, kChunkWorkgroups) * kChunkWorkgroups) / (double)std::max<int64_t>(plan.groups, 1);
+    }
+    const bool many_apart = units[MORE] + units[MANY] > (can_many ? 1 : 4) * kApartWorkgroups &&
+                            (units[FEW] + units[MORE] == 0 || many_tiles >= kManyTiles);
+    const bool many = many_shared(dev, a.q.type, most, tiles);
+    for (Group& x : groups) {
+        int64_t rows = 0, alone = 0;  // of the group; workgroups of many rows of its sequences
+        for (uint32_t i : x.members) rows += counts[i] * a.G, alone += tiles_of(counts[i] * a.G, chunk_rows);
+        const bool far = many && x.slots - x.low >= kLongSlots;
+        const double gain = (double)alone * rounds / (double)tiles_of(rows, chunk_rows);
+        const bool fuller = (many || !can_many) && gain >= (x.slots - x.low >= kLongSlots / 2 ? 4. / 3 : 1.5);
+        const auto apart = [&](uint32_t i) {
+            const auto kind = kind_of(i);
+            return kind == MANY ? many_apart && !fuller : (more_apart && !far) || (kind == FEW && few_apart);
+        };
+        const auto end = std::remove_if(x.members.begin(), x.members.end(), apart);
+        some = some || end != x.members.end();
+        x.members.erase(end, x.members.end());
+    }
+    return some;
+}
+
+// Makes groups of one of the sequences that are in none, where they are the fewer: a launch of both
+// takes less than one after the other (8 x 11 beams of prompts of 211 to 6393 slots, of which
+// two are too short to share, 4 x 8 x 128: 72 us by two ways, 49 each by itself).
+void KvCache::add_singles(const int32_t* ids, const int64_t* counts, size_t n, const KvAttend& a, std::vector<Group>& groups) const {
+    const auto units_of = [&](size_t i) { return (counts[i] * a.G + 15) / 16; };
+    std::vector<uint8_t> in(n, 0);
+    int64_t together = 0, alone = 0;
+    for (const Group& x : groups)
+        for (uint32_t i : x.members)
+            if (x.members.size() > 1) in[i] = 1, together += units_of(i);
+    for (size_t i = 0; i < n; i++)
+        if (!in[i]) alone += units_of(i);
+    if (alone > together) return;
+    for (size_t i = 0; i < n; i++)
+        if (!in[i] && counts[i]) groups.push_back(Group{{(uint32_t)i}, 0, 0});
+}
+
+// Whether steps of 16 rows, each sequence by itself, need no splits.
+bool KvCache::whole_steps(const int32_t* ids, const int64_t* counts, size_t n, const KvAttend& a) const {
+    std::vector<std::pair<int64_t, int64_t>> order(n);  // length, tokens
+    for (size_t i = 0; i < n; i++) order[i] = {seqs[ids[i]].len, counts[i]};
+    std::sort(order.begin(), order.end(), std::greater<>());
+    for (size_t i = 0; i < n;) {
+        KvPlan plan;
+        KvBatch b;
+        plan.heads = dev.H;
+        for (; i < n && plan.n < KV_BATCH; i++) plan.add(order[i].first, order[i].second, a.G, 16, a.causal, a.window);
+        plan.split(b, false, kPartBytes / (16 * ((int64_t)dev.Dp * 4 + 12)));
+        if (plan.split_units) return false;
+    }
+    return true;
+}
+
 void KvCache::attend_shared(const int32_t* ids, const int64_t* counts, const std::vector<int64_t>& tok0, size_t n,
                             KvAttend a, std::vector<size_t>& rest, hipStream_t s) {
     // sequences whose first block others hold too, by that block
@@ -957,39 +1081,16 @@ void KvCache::attend_shared(const int32_t* ids, const int64_t* counts, const std
     }
     const int parts = a.q.type == KV_F32 ? 2 : 1;
     const int64_t chunk_rows = 64 * kv_chunk_nc(dev.Dp, parts);
+    bool some = false;
     if (!groups.empty() && shared_bytes) {  // (0: tests of shared slots, for any rows)
-        const auto tiles_of = [](int64_t rows, int64_t wg) { return (rows + wg - 1) / wg; };
-        int64_t most = 0, chunk_tiles = 0, units = 0, wide = 0;
-        for (size_t i = 0; i < n; i++) {
-            const int64_t rows = counts[i] * a.G;
-            most = std::max(most, rows);
-            chunk_tiles += tiles_of(rows, chunk_rows) * dev.H * tiles_of(seqs[ids[i]].len, KV_TILE);
-            units += tiles_of(rows, 16) * dev.H;
-            if (rows > kTileRows) wide += tiles_of(rows, 16) * dev.H;
-        }
-        const bool chunks = most > chunk_rows * 3 / 4 && chunk_tiles >= kChunkTiles;  // (as for the rest)
-        // (as KvPlan::split would leave them whole)
-        const bool crowded = !chunks && 2 * units > kStepWorkgroups + kStepWorkgroups / 8;
-        const int64_t least = crowded ? kCrowdedSlots * tiles_of((int64_t)n, kLaunchSeqs) : 0;
+        some = part_groups(ids, counts, n, a, groups);
         saved_slots = 0;
-        for (Group& x : groups) {
-            int64_t rows = 0, alone = 0;  // of the group; workgroups of many rows of its sequences
-            for (uint32_t i : x.members) rows += counts[i] * a.G, alone += tiles_of(counts[i] * a.G, chunk_rows);
-            const bool many = many_shared(dev, a.q.type, rows, tiles_of(rows, 16) * dev.H * ((x.slots - x.low) / KV_TILE));
-            const bool far = x.slots - x.low >= kLongSlots;
-            const bool fuller = 3 * alone >= 4 * tiles_of(rows, chunk_rows);
-            const auto apart = [&](uint32_t i) {
-                const int64_t own = counts[i] * a.G;
-                const bool chunk = chunks && own > chunk_rows * 3 / 4;
-                if (own <= kTileRows) return x.slots - x.low < least;
-                if (many && (chunk ? fuller : far)) return false;
-                return wide > (chunk && !kv_shared_many(dev.Dp, parts) ? 4 : 1) * kApartWorkgroups;
-            };
-            x.members.erase(std::remove_if(x.members.begin(), x.members.end(), apart), x.members.end());
+        for (const Group& x : groups)
             if (x.members.size() > 1) saved_slots += (x.slots - x.low) * (int64_t)(x.members.size() - 1);
-        }
     }
+    groups.erase(std::remove_if(groups.begin(), groups.end(), [](const Group& x) { return x.members.size() < 2; }), groups.end());
     if (saved_slots * dev.H * 2 * dev.Dp < shared_bytes) groups.clear();
+    if (!groups.empty() && !some) add_singles(ids, counts, n, a, groups);
     // Groups in pieces of as many sequences as one launch takes: each has an entry of its own and
     // the piece one more, and every row leaves partial results of both.
     const int64_t row_bytes = (int64_t)dev.Dp * 4 + 12, room = kPartBytes / 2 / row_bytes / dev.H;
@@ -1008,7 +1109,7 @@ void KvCache::attend_shared(const int32_t* ids, const int64_t* counts, const std
                 p.rows += more, p.end = j + 1;
                 continue;
             }
-            if (p.end - p.first > 1) pieces.push_back(p);
+            if (p.end - p.first > 1 || (p.end > p.first && !x.slots)) pieces.push_back(p);
             p = Piece{&x, j, j, 0};
             if (more && more <= room) p.rows = more, p.end = j + 1;
             else p.first = p.end = j + 1;  // too many rows for any launch
@@ -1038,14 +1139,15 @@ void KvCache::attend_shared(const int32_t* ids, const int64_t* counts, const std
                 mem.tok0[m] = (int)tok0[i], mem.len[m] = (int)q.len, mem.count[m] = (int)counts[i];
                 mem.row0[m + 1] = mem.row0[m] + count;
                 shares.row0[m] = mem.row0[m] - mem.row0[first];
-                shares.unit[1][m] = shares.tiles[1][m] = shares.splits[1][m] = 0;
+                for (int z = 0; z < 2; z++) shares.unit[z][m] = shares.tiles[z][m] = shares.splits[z][m] = 0;
                 const int64_t low = a.window ? std::max<int64_t>(q.len - counts[i] + 1 - a.window, 0) : 0;
                 const int64_t t0 = std::max(p.group->slots, low) / KV_TILE;
                 if (t0 * KV_TILE < q.len) entries[1].push_back({ids[i], m, count, 1, t0, q.len});
                 done[i] = 1;
             }
-            entries[0].push_back({ids[p.group->members[p.first]], first, mem.row0[mem.n] - mem.row0[first], (int)many,
-                                  p.group->low / KV_TILE, p.group->slots});
+            if (p.group->slots)
+                entries[0].push_back({ids[p.group->members[p.first]], first, mem.row0[mem.n] - mem.row0[first], (int)many,
+                                      p.group->low / KV_TILE, p.group->slots});
         }
         // the kernel that suits the rows, for each kind of slots; one launch where it is the same
         bool by_rows[2];

@@ -397,13 +397,16 @@ struct KvCache {
     size_t blocks_of(int64_t slots) const { return (size_t)((slots + dev.B - 1) >> dev.shift); }
     void check_call(hipStream_t s);
     KvTensor tensor(const vgpu_tensor3& t, const char* name) const;
-    // Sequences of a call that are taken together over the slots low .. slots - 1.
+    // Sequences of a call that are taken together over the slots low .. slots - 1; one alone over 0.
     struct Group {
         std::vector<uint32_t> members;
         int64_t low, slots;
     };
     void find_groups(const int32_t* ids, const int64_t* counts, const KvAttend& a, std::vector<uint32_t>& members,
                      size_t from, int depth, std::vector<Group>& groups, int64_t& saved) const;
+    bool part_groups(const int32_t* ids, const int64_t* counts, size_t n, const KvAttend& a, std::vector<Group>& groups) const;
+    void add_singles(const int32_t* ids, const int64_t* counts, size_t n, const KvAttend& a, std::vector<Group>& groups) const;
+    bool whole_steps(const int32_t* ids, const int64_t* counts, size_t n, const KvAttend& a) const;
     // Attends for the sequences that share slots; rest: the others.
     void attend_shared(const int32_t* ids, const int64_t* counts, const std::vector<int64_t>& tok0, size_t n, KvAttend a,
                        std::vector<size_t>& rest, hipStream_t s);
