@@ -146,3 +146,23 @@ def test_prefixes_of_very_different_lengths(dim, dtype):
     cache.append(k, v, seqs=range(72))
     q = _rand((72, 32, dim), dtype, 5)
     _check_large(cache, q, list(range(72)), [1] * 72)
+
+
+@pytest.mark.parametrize("forks,empty", [(126, 3), (127, 1), (120, 9), (253, 200)])
+def test_launches_of_sequences_without_slots(forks, empty):
+    """Beyond the sequences of a launch only empty ones are left."""
+    import torch
+
+    import vicinity_amd as va
+
+    cache = share(va.KVCache(forks + empty + 1, 2, 64, forks + 12, block_tokens=64))
+    k, v = (_rand((640, 2, 64), "bfloat16", i) for i in (1, 2))
+    cache.append(k, v, seqs=[forks + empty])
+    cache.fork([forks + empty] * forks, range(forks))
+    k, v = (_rand((forks, 2, 64), "bfloat16", i) for i in (3, 4))
+    cache.append(k, v, seqs=range(forks))
+    n = forks + empty
+    q = _rand((n, 8, 64), "bfloat16", 5)
+    out, lse = cache.attend(q, seqs=range(n), return_lse=True)
+    assert (out[forks:] == 0).all() and torch.isneginf(lse[forks:]).all()
+    _check_large(cache, q[:forks], list(range(forks)), [1] * forks)

@@ -141,7 +141,7 @@ void launch_kv_shared(const KvDev& c, const KvBatch& b, const KvAttend& a, const
 }
 
 void launch_kv_shared_join(const KvDev& c, const KvAttend& a, const KvMembers& mem, const KvShares& j, hipStream_t s) {
-    int most = 0;
+    int most = 1;  // (none, where all sequences are empty)
     for (int m = 0; m < mem.n; m++) most = j.splits[0][m] + j.splits[1][m] > most ? j.splits[0][m] + j.splits[1][m] : most;
     // A group of threads for every four parts, up to 768 workgroups (48 tokens of 64 query
     // heads, 22 parts each: 10 us with two, 14 with six; 512 rows in all of 25 parts: 8.5 and 6.4).
