@@ -76,9 +76,9 @@ constexpr int BEAM_PIECES = 512;  // pieces that are looked through for them
 
 // One workgroup: one slice of one row, loaded at once.  Bound by the vector unit where rows are
 // many: a conversion, a comparison, a difference, a product, an exponential (four times as
-// long), a conversion to float64 and a sum for each logit (512 rows of 100003 in bfloat16: 30 us, 3.4 TB/s, the vector
-// unit 51% busy and the loads before it not hidden; 4 rows of 32000 in float32: 6 us).  The
-// hits counted by each thread before they are taken to LDS: 40 us.
+// long), a conversion to float64 and a sum for each logit (512 rows of 100003 in bfloat16: 32 us,
+// 3.2 TB/s, the vector unit 52% busy and the loads before it not hidden; 4 rows of 32000 in float32:
+// 6 us).  The hits counted by each thread before they are taken to LDS: 10 us more.
 template <int T, int N>
 __global__ __launch_bounds__(256, T == KV_F32 ? 6 : 7) void beam_slice_kernel(BeamArgs a) {
     constexpr int W = T == KV_F32 ? 4 : 8, HALF = (N + 1) / 2;

@@ -955,7 +955,8 @@ bool KvCache::part_groups(const int32_t* ids, const int64_t* counts, size_t n, c
         const int64_t rows = counts[i] * a.G;
         return rows <= kTileRows ? FEW : chunks && rows > chunk_rows * 3 / 4 ? MANY : MORE;
     };
-    int64_t units[3] = {0, 0, 0}, many_tiles = 0, by_many = 0;  // workgroups of 16 rows; those of MANY: tiles, sequences
+    int64_t units[3] = {0, 0, 0};           // workgroups of 16 rows
+    int64_t many_tiles = 0, by_many = 0;    // of MANY: tiles, sequences
     for (size_t i = 0; i < n; i++) {
         const int64_t own = tiles_of(counts[i] * a.G, 16) * dev.H;
         units[kind_of((uint32_t)i)] += own;
@@ -966,7 +967,8 @@ bool KvCache::part_groups(const int32_t* ids, const int64_t* counts, size_t n, c
     for (const Group& x : groups) {
         int64_t rows = 0;
         for (uint32_t i : x.members) rows += counts[i] * a.G;
-        most = std::max(most, rows), most_slots = std::max(most_slots, x.slots - x.low), tiles += tiles_of(rows, 16) * dev.H * ((x.slots - x.low) / KV_TILE);
+        most = std::max(most, rows), most_slots = std::max(most_slots, x.slots - x.low);
+        tiles += tiles_of(rows, 16) * dev.H * ((x.slots - x.low) / KV_TILE);
         saved += (x.slots - x.low) * (int64_t)(x.members.size() - 1);
         for (uint32_t i : x.members)
             if (kind_of(i) == FEW) few++, few_slots += x.slots - x.low;
@@ -985,10 +987,9 @@ bool KvCache::part_groups(const int32_t* ids, const int64_t* counts, size_t n, c
     // has launches of its own (32 sequences of 5 tokens and 32 of one, 4 x 8 x 128 over 2048 shared
     // slots: 32 us either way, 43 one each).
     const bool more_apart = whole && units[MORE] > kApartWorkgroups && units[MORE] >= 2 * units[FEW];
-    const int64_t launches = tiles_of((int64_t)n, kLaunchSeqs), all_units = units[FEW] + units[MORE] + units[MANY];
-    const int64_t least = kCrowdedSlots * launches * std::min(all_units, kCrowdedUnits * launches) / std::max<int64_t>(all_units, 1);
-    const bool few_apart = (whole && few_slots < few * least) ||
-                           (steps && !others && saved * dev.H * 2 * dev.Dp < kFewBytes);
+    const int64_t launches = tiles_of((int64_t)n, kLaunchSeqs), all = units[FEW] + units[MORE] + units[MANY];
+    const int64_t least = kCrowdedSlots * launches * std::min(all, kCrowdedUnits * launches) / std::max<int64_t>(all, 1);
+    const bool few_apart = (whole && few_slots < few * least) || (steps && !others && saved * dev.H * 2 * dev.Dp < kFewBytes);
     // Rows of the kernel of many stay together where that saves a third of its time, or a quarter over slots
     // that pay for the parts, by how full its workgroups and their last round are (11 sequences of 136
     // rows over 2394 slots of 32 x 96 188 us apart and 127; 12 of 266 over 16224 of 2 x 128 137 and 91, 38
@@ -1004,7 +1005,7 @@ bool KvCache::part_groups(const int32_t* ids, const int64_t* counts, size_t n, c
         for (size_t i = 0; i < n && plan.n < KV_BATCH; i++)
             if (kind_of((uint32_t)i) == MANY) plan.add(seqs[ids[i]].len, counts[i], a.G, chunk_rows, a.causal, a.window);
         plan.split(b, true, kPartBytes / (chunk_rows * ((int64_t)dev.Dp * 4 + 12)));
-        rounds = (double)(tiles_of(plan.groups, kChunkWorkgroups) * kChunkWorkgroups) / (double)std::max<int64_t>(plan.groups, 1);
+        if (plan.groups) rounds = (double)(tiles_of(plan.groups, kChunkWorkgroups) * kChunkWorkgroups) / (double)plan.groups;
     }
     const bool many_apart = units[MORE] + units[MANY] > (can_many ? 1 : 4) * kApartWorkgroups &&
                             (units[FEW] + units[MORE] == 0 || many_tiles >= kManyTiles);
