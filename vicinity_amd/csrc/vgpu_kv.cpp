@@ -84,11 +84,12 @@ constexpr int64_t kApartWorkgroups = kStepWorkgroups / 2;
 // shared slots, which pay for their parts (8 x 128: 32 of 40 rows over 8192 slots 101 us apart, 79
 // together, 32 of 32 over 6560 a fifth faster together; 52 of 48 over 1792 49 and 69; 64 dims, 63 of
 // 16 over 3328 86 and 112).
-constexpr int64_t kLongSlots = 6144;
+constexpr int64_t kLongSlots = 6144, kFullerSlots = 2560;  // (the second: see part_groups)
 // Rows of the kernel of many have so many tiles of 16 to do where they leave sequences of fewer rows,
 // which takes a launch more (28 sequences of which one has 684 rows over 1954 slots of 8 x 96, 34000
-// tiles: 28 us together, 49 not; five of up to 2560 over 417 of 32 x 128, 92000: 151 and 60).
-constexpr int64_t kManyTiles = 65536, kManySlots = 512;
+// tiles: 28 us together, 49 not; four of which one has 272 over 4672 of 32 x 64, 80000: 52 and 98; one
+// of 8192 over 18400 of 8 x 128 beside 16 of 4, 2.4 million: 980 and 600).
+constexpr int64_t kManyTiles = 131072;
 // Levels of branches that are looked at for the best groups.
 constexpr int kSharedDepth = 4;
 
@@ -978,7 +979,7 @@ bool KvCache::part_groups(const int32_t* ids, const int64_t* counts, size_t n, c
     // Beside rows of the kernel of many, where those are nearly all, less than 512 slots are not worth the
     // parts (39 sequences of 8 x 192 over 296 slots, a third with up to 1472 rows: 44 us apart, 116;
     // 39 of 32 x 128 in float32 over 475, a third with up to 147 rows: 162 and 50).
-    if (!steps && most_slots < kManySlots && units[MANY] >= 8 * units[FEW]) {
+    if (!steps && most_slots < 512 && units[MANY] >= 8 * units[FEW]) {
         groups.clear();
         return true;
     }
@@ -1015,7 +1016,7 @@ bool KvCache::part_groups(const int32_t* ids, const int64_t* counts, size_t n, c
         for (uint32_t i : x.members) rows += counts[i] * a.G, alone += tiles_of(counts[i] * a.G, chunk_rows);
         const bool far = many && x.slots - x.low >= kLongSlots;
         const double gain = (double)alone * rounds / (double)tiles_of(rows, chunk_rows);
-        const bool fuller = (many || !can_many) && gain >= (x.slots - x.low >= kLongSlots / 2 ? 4. / 3 : 1.5);
+        const bool fuller = (many || !can_many) && gain >= (x.slots - x.low >= kFullerSlots ? 4. / 3 : 1.5);
         const auto apart = [&](uint32_t i) {
             const auto kind = kind_of(i);
             return kind == MANY ? many_apart && !fuller : (more_apart && !far) || (kind == FEW && few_apart);
